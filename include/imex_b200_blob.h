@@ -80,6 +80,32 @@ extern "C" {
  *                   dims = {threads, payload offset from the start of the blob, payload
  *                   bytes (text without NUL), number of pointer arguments}; pointers = the
  *                   tensor inputs in order, then the outputs.
+ *   ATTENTION       Q, K, V, O, LSE (, key_lens) (, workspace): attention forward that keeps the
+ *                   row statistics a backward pass needs, with shared key heads, masks and
+ *                   strides.  The problem travels as an ImexAttentionShape in the payload
+ *                   (dims[1], dims[2] = its offset and bytes); fparams[0] = sm_scale.
+ *                   Key j is visible to query i of batch b when j < key_lens[b]
+ *                   (IMEX_FLAG_KEY_LENS: int32[batch], values clamped to [0, n_kv]; all keys
+ *                   without) and, with IMEX_FLAG_CAUSAL, j <= i + n_kv - n_q.
+ *                   S = sm_scale Q K^T, LSE = log sum_visible exp S (f32 [batch, q_heads, n_q]),
+ *                   O = exp(S - LSE) V; a row that sees no key gets O = 0, LSE = -inf.
+ *                   Query head h reads key head h / (q_heads / kv_heads).
+ *   ATTENTION_BWD   Q, K, V, O, dO, LSE, dQ, dK, dV (, key_lens) (, workspace): the gradients of
+ *                   the same problem; the probabilities are recomputed from LSE.
+ *                   P = exp(S - LSE), dV = sum_group P^T dO, dS = P (dO V^T - rowsum(dO O)),
+ *                   dQ = sm_scale dS K, dK = sm_scale sum_group dS^T Q.
+ *   GATED_FFN       X[tokens,d_in], W[d_in,2*d_ff], H[tokens,d_ff] (, GU[tokens,2*d_ff] with
+ *                   IMEX_FLAG_SAVE_GU): H = act(X Wg) * (X Wu) with W = [Wg | Wu], act =
+ *                   `epilogue`, f32 accumulation; GU = X W as the backward pass wants it.
+ *                   dims = {tokens, d_in, d_ff, ldx, ldw, ldh}; row pitches, 0 = dense; GU is dense.
+ *   GATED_FFN_BWD   X, W, GU, dH[tokens,d_ff], dX[tokens,d_in], dW[d_in,2*d_ff], workspace:
+ *                   dims = {tokens, d_in, d_ff, ldx, ldw, ldh} (ldx also of dX, ldw of dW, ldh of
+ *                   dH): dU = dH act(G), dG = dH U act'(G), dX = [dG dU] W^T, dW = X^T [dG dU].
+ *   ROTARY          X, positions (int32[tokens]), Y: the first rot_dims of every head turned in
+ *                   pairs by position * frequency, the rest copied; an ImexRotaryShape in the
+ *                   payload; fparams[0] = factor on the turned dimensions.  Pairs are
+ *                   (i, i + rot_dims/2), or (2i, 2i + 1) with IMEX_FLAG_INTERLEAVED;
+ *                   IMEX_FLAG_INVERSE turns the other way (the gradient).  Y may be X.
  *   FILL_UNIFORM    Y[n]  dims = {n, seed, first}; fparams = {lo, hi}
  *   FILL_NORMAL     Y[n]  dims = {n, seed, first}; fparams = {mean, stddev}
  */
@@ -96,7 +122,12 @@ enum ImexOp {
   IMEX_OP_FILL_NORMAL = 10,
   IMEX_OP_EXPR = 11,
   IMEX_OP_ATTENTION_FWD = 12,
-  IMEX_OP_LOOPNEST = 13
+  IMEX_OP_LOOPNEST = 13,
+  IMEX_OP_ATTENTION = 14,
+  IMEX_OP_ATTENTION_BWD = 15,
+  IMEX_OP_GATED_FFN = 16,
+  IMEX_OP_GATED_FFN_BWD = 17,
+  IMEX_OP_ROTARY = 18
 };
 
 /* Postfix code of IMEX_OP_EXPR.  Pushes take the element of input k at the current
@@ -142,7 +173,12 @@ enum ImexFlags {
   IMEX_FLAG_SOFTMAX_NEG_INF = 1u << 2, /* PlaidML form: max starts at -inf, cmpf ogt */
   IMEX_FLAG_TRANS_A = 1u << 3,    /* GEMM: A stored [K,M]                 */
   IMEX_FLAG_TRANS_B = 1u << 4,    /* GEMM: B stored [N,K]                 */
-  IMEX_FLAG_REDUCE_LEADING = 1u << 5 /* EXPR: sum the expression over the rows */
+  IMEX_FLAG_REDUCE_LEADING = 1u << 5, /* EXPR: sum the expression over the rows */
+  IMEX_FLAG_CAUSAL = 1u << 6,      /* ATTENTION*: key j visible to query i iff j <= i + n_kv - n_q */
+  IMEX_FLAG_KEY_LENS = 1u << 7,    /* ATTENTION*: a pointer to int32[batch] key counts follows */
+  IMEX_FLAG_SAVE_GU = 1u << 8,     /* GATED_FFN: X W is kept in a fourth array */
+  IMEX_FLAG_INTERLEAVED = 1u << 9, /* ROTARY: pairs (2i, 2i+1) instead of (i, i + rot_dims/2) */
+  IMEX_FLAG_INVERSE = 1u << 10     /* ROTARY: turn by minus the angle */
 };
 
 typedef struct ImexBlobHeader {
@@ -162,6 +198,26 @@ typedef struct ImexKernelDesc {
   int64_t dims[6];
   float fparams[2];
 } ImexKernelDesc;
+
+/* Payload of IMEX_OP_ATTENTION / IMEX_OP_ATTENTION_BWD.  Strides are in elements, multiples of 8;
+ * the last dimension is dense and every array starts on a 16-byte boundary.  Order of the
+ * arrays: q, k, v, o, dO, dQ, dK, dV (the forward op reads the first four). */
+typedef struct ImexStrides3 {
+  int64_t batch, head, row;
+} ImexStrides3;
+typedef struct ImexAttentionShape {
+  int64_t batch, q_heads, kv_heads, n_q, n_kv, d_head; /* d_head: 64 or 128 */
+  ImexStrides3 strides[8];
+} ImexAttentionShape;
+
+/* Payload of IMEX_OP_ROTARY: strides in elements; turns[i] = frequency of pair i / 2 pi (full
+ * turns per position), rot_dims / 2 of them. */
+#define IMEX_ROTARY_MAX_PAIRS 128
+typedef struct ImexRotaryShape {
+  int64_t tokens, heads, d_head, rot_dims;
+  int64_t x_token, x_head, y_token, y_head;
+  double turns[IMEX_ROTARY_MAX_PAIRS];
+} ImexRotaryShape;
 
 #ifdef __cplusplus
 }

@@ -117,6 +117,12 @@ void *imexStreamStatusWord(void *stream);
 /* Adds n to the launch counter (for kernels launched outside gpuLaunchKernel). */
 void imexNoteLaunches(uint64_t n);
 
+/* Bytes of device scratch the launches of this kernel handle want as their last pointer operand
+ * (0: no such operand).  The scratch is the caller's, like every other operand: launches that may
+ * overlap on the GPU (other streams, graphs that replay side by side) need one each.  Its contents
+ * carry nothing from one launch to the next. */
+size_t imexKernelWorkspaceBytes(void *kernel);
+
 /* ---- peer memory between the processes of one node (one process per GPU).  No reference
  * counterpart: the reference leaves data exchange between ranks to its distributed runtime
  * (the `_idtr_*` calls behind lib/Dialect/DistRuntime).  Used by the row-sharded GEMM to

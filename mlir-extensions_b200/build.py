@@ -36,6 +36,10 @@ RUNTIME_SOURCES = [
     "kernels/expr_jit.cu",
     "kernels/loopnest_jit.cu",
     "kernels/flash_attention.cu",
+    "kernels/attention.cu",
+    "kernels/attention_bwd.cu",
+    "kernels/gated_ffn.cu",
+    "kernels/rotary.cu",
     "kernels/wait_selftest.cu",
     "runtime/cuda_runtime_wrappers.cu",
     "runtime/peer_copy.cu",

@@ -72,6 +72,62 @@ cudaError_t launch_flash_attention_fwd(const void *q, const void *k, const void 
                                        int64_t n_ctx, int64_t d_head, float sm_scale, int dtype,
                                        unsigned *status, cudaStream_t stream);
 
+// Attention with row statistics, shared key heads, causal and length masks and strides (forward
+// and backward).  Element strides; see IMEX_OP_ATTENTION for the definition.
+struct Strides3 {
+  int64_t batch, head, row;
+};
+struct AttentionProblem {
+  int64_t batch, q_heads, kv_heads, n_q, n_kv, d_head;
+  int dtype;                 // kF16 or kBF16
+  float scale;
+  bool causal;
+  const int32_t *key_lens;   // [batch] or nullptr
+  const void *q, *k, *v;
+  void *o;                   // backward: read
+  float *lse;                // backward: read
+  const void *dout;
+  void *dq, *dk, *dv;
+  Strides3 sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  void *workspace;
+};
+// nullptr, or why the problem is refused.  Pointers are looked at only when `pointers`.
+const char *attention_check(const AttentionProblem &p, bool backward, bool pointers);
+size_t attention_workspace_bytes(const AttentionProblem &p, bool backward);
+cudaError_t launch_attention(const AttentionProblem &p, unsigned *status, cudaStream_t stream, int *launched);
+cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cudaStream_t stream, int *launched);
+
+// H = act(X Wg) * (X Wu), W = [Wg | Wu]; pitches in elements, 0 = dense (see IMEX_OP_GATED_FFN).
+struct GatedProblem {
+  int64_t tokens, d_in, d_ff, ldx, ldw, ldh;
+  int dtype;       // kF16 or kBF16
+  int act;         // Epilogue
+  const void *x, *w;
+  void *h;         // forward: written; backward: dH, read
+  void *gu;        // [tokens, 2 * d_ff] dense; forward: written or nullptr; backward: read
+  void *dx, *dw;   // backward
+  void *workspace;
+};
+const char *gated_check(const GatedProblem &p);
+size_t gated_bwd_workspace_bytes(const GatedProblem &p);
+cudaError_t launch_gated(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched);
+cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched);
+
+// Rotary positions (see IMEX_OP_ROTARY).
+struct RotaryProblem {
+  int64_t tokens, heads, d_head, rot_dims;
+  int64_t x_token, x_head, y_token, y_head;  // strides in elements
+  int dtype;
+  bool interleaved, inverse;
+  float factor;
+  const void *x;
+  const int32_t *positions;
+  void *y;
+  const double *turns;  // host memory, rot_dims / 2
+};
+const char *rotary_check(const RotaryProblem &p);
+cudaError_t launch_rotary(const RotaryProblem &p, cudaStream_t stream);
+
 // One thread waits (bounded, ~1 ms) on a barrier nothing signals and reports
 // kStatusSelfTestTimeout: exercises wait expiry -> status word -> gpuWait error.
 cudaError_t launch_wait_selftest(unsigned *status, cudaStream_t stream);

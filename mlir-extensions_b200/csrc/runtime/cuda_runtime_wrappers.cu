@@ -88,12 +88,12 @@ struct Stream {
 
 struct Kernel {
   ImexKernelDesc desc;
-  const std::string *source = nullptr;  // IMEX_OP_LOOPNEST: kernel text, owned by the module
+  const std::string *source = nullptr;  // the descriptor's payload, owned by the module
 };
 
 struct Module {
   std::vector<ImexKernelDesc> kernels;
-  std::vector<std::string> sources;  // per kernel: the text of an IMEX_OP_LOOPNEST kernel, else empty
+  std::vector<std::string> sources;  // per kernel: its payload (kernel text of IMEX_OP_LOOPNEST, shape structs), else empty
   std::vector<std::unique_ptr<Kernel>> handles;  // one per table row, made on first gpuKernelGet
 };
 
@@ -117,8 +117,17 @@ const char *op_name(uint32_t op) {
   case IMEX_OP_EXPR: return "expr";
   case IMEX_OP_ATTENTION_FWD: return "attention_fwd";
   case IMEX_OP_LOOPNEST: return "loopnest";
+  case IMEX_OP_ATTENTION: return "attention";
+  case IMEX_OP_ATTENTION_BWD: return "attention_bwd";
+  case IMEX_OP_GATED_FFN: return "gated_ffn";
+  case IMEX_OP_GATED_FFN_BWD: return "gated_ffn_bwd";
+  case IMEX_OP_ROTARY: return "rotary";
   }
   return nullptr;
+}
+
+bool has_payload(uint32_t op) {
+  return op == IMEX_OP_LOOPNEST || op == IMEX_OP_ATTENTION || op == IMEX_OP_ATTENTION_BWD || op == IMEX_OP_ROTARY;
 }
 
 size_t dtype_bytes(uint32_t dt) {
@@ -219,7 +228,7 @@ Module *load_module(const void *data, size_t size) {
     if (!op_name(k.op))
       throw std::runtime_error(std::string("gpuModuleLoad: kernel '") + k.name +
                                "' names an unknown op " + std::to_string(k.op));
-    if (k.op == IMEX_OP_LOOPNEST) {  // the kernel's text lies in the payload behind the table
+    if (has_payload(k.op)) {  // kernel text or a shape struct in the payload behind the table
       const int64_t off = k.dims[1], len = k.dims[2];
       if (off < 0 || len <= 0 || static_cast<uint64_t>(off) + static_cast<uint64_t>(len) > size)
         throw std::runtime_error(std::string("gpuModuleLoad: kernel '") + k.name + "' points outside the blob");
@@ -284,6 +293,57 @@ void ensure_scratch(Stream *s, size_t bytes) {
   size_t cap = bytes < (1u << 20) ? (1u << 20) : bytes;
   CHECK_CUDA(cudaMalloc(reinterpret_cast<void **>(&s->scratch), cap));
   s->scratch_bytes = cap;
+}
+
+// ---- ops whose problem travels as a struct in the payload, or whose checks come with a reason
+template <typename T> T payload_as(const ImexKernelDesc &d, const std::string *source) {
+  if (!source || source->size() != sizeof(T))
+    throw std::runtime_error(std::string("gpuLaunchKernel: '") + d.name + "' (" + op_name(d.op) + ") has no shape payload");
+  T v;
+  memcpy(&v, source->data(), sizeof v);
+  return v;
+}
+
+void refuse(const ImexKernelDesc &d, const char *why) {
+  if (why)
+    throw std::runtime_error(std::string("gpuLaunchKernel: '") + d.name + "' (" + op_name(d.op) + "): " + why);
+}
+
+imex::AttentionProblem attention_problem(const ImexKernelDesc &d, const std::string *source) {
+  const ImexAttentionShape s = payload_as<ImexAttentionShape>(d, source);
+  if (d.in_dtype != d.out_dtype) refuse(d, "attention keeps its element type");
+  imex::AttentionProblem p{};
+  p.batch = s.batch, p.q_heads = s.q_heads, p.kv_heads = s.kv_heads;
+  p.n_q = s.n_q, p.n_kv = s.n_kv, p.d_head = s.d_head;
+  p.dtype = static_cast<int>(d.in_dtype);
+  p.scale = d.fparams[0];
+  p.causal = d.flags & IMEX_FLAG_CAUSAL;
+  imex::Strides3 *to[8] = {&p.sq, &p.sk, &p.sv, &p.so, &p.sdo, &p.sdq, &p.sdk, &p.sdv};
+  for (int i = 0; i < 8; ++i) *to[i] = imex::Strides3{s.strides[i].batch, s.strides[i].head, s.strides[i].row};
+  refuse(d, imex::attention_check(p, d.op == IMEX_OP_ATTENTION_BWD, false));
+  return p;
+}
+
+imex::GatedProblem gated_problem(const ImexKernelDesc &d) {
+  if (d.in_dtype != d.out_dtype) refuse(d, "the gated product keeps its element type");
+  imex::GatedProblem p{};
+  p.tokens = d.dims[0], p.d_in = d.dims[1], p.d_ff = d.dims[2];
+  p.ldx = d.dims[3], p.ldw = d.dims[4], p.ldh = d.dims[5];
+  p.dtype = static_cast<int>(d.in_dtype);
+  p.act = static_cast<int>(d.epilogue);
+  refuse(d, imex::gated_check(p));
+  return p;
+}
+
+size_t workspace_bytes(const ImexKernelDesc &d, const std::string *source) {
+  switch (d.op) {
+  case IMEX_OP_ATTENTION:
+  case IMEX_OP_ATTENTION_BWD:
+    return imex::attention_workspace_bytes(attention_problem(d, source), d.op == IMEX_OP_ATTENTION_BWD);
+  case IMEX_OP_GATED_FFN_BWD:
+    return imex::gated_bwd_workspace_bytes(gated_problem(d));
+  }
+  return 0;
 }
 
 // One enqueue of the op a kernel handle stands for.
@@ -478,6 +538,65 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
     if (err == cudaErrorNotSupported)
       throw std::runtime_error(std::string("gpuLaunchKernel: the loop-nest kernel '") + d.name +
                                "' could not be compiled for sm_100a (there is no interpreter behind it): " + log);
+    break;
+  }
+  case IMEX_OP_ATTENTION:
+  case IMEX_OP_ATTENTION_BWD: {
+    const bool backward = d.op == IMEX_OP_ATTENTION_BWD;
+    imex::AttentionProblem p = attention_problem(d, source);
+    const size_t ws = imex::attention_workspace_bytes(p, backward);
+    size_t n = backward ? 9 : 5;
+    need(n + ((d.flags & IMEX_FLAG_KEY_LENS) ? 1 : 0) + (ws ? 1 : 0));
+    p.q = ptrs[0], p.k = ptrs[1], p.v = ptrs[2], p.o = ptrs[3];
+    if (backward) {
+      p.dout = ptrs[4], p.lse = static_cast<float *>(ptrs[5]);
+      p.dq = ptrs[6], p.dk = ptrs[7], p.dv = ptrs[8];
+    } else {
+      p.lse = static_cast<float *>(ptrs[4]);
+    }
+    if (d.flags & IMEX_FLAG_KEY_LENS) p.key_lens = static_cast<const int32_t *>(ptrs[n++]);
+    if (ws) p.workspace = ptrs[n];
+    refuse(d, imex::attention_check(p, backward, true));
+    s->last_kernel = backward ? "attention_bwd" : "attention";
+    err = backward ? imex::launch_attention_bwd(p, s->status_dev, s->stream, &launches)
+                   : imex::launch_attention(p, s->status_dev, s->stream, &launches);
+    break;
+  }
+  case IMEX_OP_GATED_FFN: {
+    const bool save = d.flags & IMEX_FLAG_SAVE_GU;
+    need(save ? 4 : 3);
+    imex::GatedProblem p = gated_problem(d);
+    p.x = ptrs[0], p.w = ptrs[1], p.h = ptrs[2];
+    if (save) p.gu = ptrs[3];
+    s->last_kernel = "gated_ffn";
+    err = imex::launch_gated(p, s->status_dev, s->stream, &launches);
+    break;
+  }
+  case IMEX_OP_GATED_FFN_BWD: {
+    need(7);
+    imex::GatedProblem p = gated_problem(d);
+    p.x = ptrs[0], p.w = ptrs[1], p.gu = ptrs[2], p.h = ptrs[3], p.dx = ptrs[4], p.dw = ptrs[5];
+    p.workspace = ptrs[6];
+    s->last_kernel = "gated_ffn_bwd";
+    err = imex::launch_gated_bwd(p, s->status_dev, s->stream, &launches);
+    break;
+  }
+  case IMEX_OP_ROTARY: {
+    need(3);
+    const ImexRotaryShape r = payload_as<ImexRotaryShape>(d, source);
+    if (d.in_dtype != d.out_dtype) refuse(d, "rotary positions keep the element type");
+    imex::RotaryProblem p{};
+    p.tokens = r.tokens, p.heads = r.heads, p.d_head = r.d_head, p.rot_dims = r.rot_dims;
+    p.x_token = r.x_token, p.x_head = r.x_head, p.y_token = r.y_token, p.y_head = r.y_head;
+    p.dtype = static_cast<int>(d.in_dtype);
+    p.interleaved = d.flags & IMEX_FLAG_INTERLEAVED;
+    p.inverse = d.flags & IMEX_FLAG_INVERSE;
+    p.factor = d.fparams[0];
+    p.x = ptrs[0], p.positions = static_cast<const int32_t *>(ptrs[1]), p.y = ptrs[2];
+    p.turns = r.turns;
+    refuse(d, imex::rotary_check(p));
+    s->last_kernel = "rotary";
+    err = imex::launch_rotary(p, s->stream);
     break;
   }
   case IMEX_OP_FILL_UNIFORM:
@@ -754,6 +873,14 @@ void *imexStreamNative(void *stream) {
 
 void *imexStreamStatusWord(void *stream) {
   return stream ? static_cast<void *>(static_cast<Stream *>(stream)->status_dev) : nullptr;
+}
+
+size_t imexKernelWorkspaceBytes(void *kernel) {
+  return catchAll([&]() -> size_t {
+    auto *k = static_cast<Kernel *>(kernel);
+    if (!k) throw std::runtime_error("imexKernelWorkspaceBytes: null kernel");
+    return workspace_bytes(k->desc, k->source);
+  });
 }
 
 void imexNoteLaunches(uint64_t n) { g_launches.fetch_add(n, std::memory_order_relaxed); }

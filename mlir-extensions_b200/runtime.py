@@ -61,6 +61,7 @@ def _load():
         "imexSelfTestWaitTimeout": (None, [vp]),
         "imexStreamStatusWord": (vp, [vp]),
         "imexNoteLaunches": (None, [C.c_uint64]),
+        "imexKernelWorkspaceBytes": (sz, [vp]),
         "imexIpcExport": (C.c_int, [vp, vp]),
         "imexIpcOpen": (vp, [vp]),
         "imexIpcClose": (None, [vp]),
@@ -88,6 +89,7 @@ imexStreamNative = _lib.imexStreamNative
 imexEventRecord = _lib.imexEventRecord
 imexEventElapsedMs = _lib.imexEventElapsedMs
 imexLaunchCount = _lib.imexLaunchCount
+imexKernelWorkspaceBytes = _lib.imexKernelWorkspaceBytes
 imexShardSize = _lib.imexShardSize
 imexShardOffset = _lib.imexShardOffset
 
@@ -128,6 +130,17 @@ def gpuLaunchKernel(stream, kernel, grid, block, shared_mem_bytes, pointer_args,
                               C.cast(params, C.c_void_p), C.cast(deps, C.c_void_p))
     del keep
     return ev
+
+
+def bind_launch(stream, kernel, pointer_args):
+    """A callable that issues this gpuLaunchKernel again and again: the argument list is built once."""
+    params, keep = make_params(pointer_args)
+    args = (stream, kernel, 1, 1, 1, 1, 1, 1, 0, C.cast(params, C.c_void_p), C.cast(_NO_EVENTS, C.c_void_p))
+    fn = _lib.gpuLaunchKernel
+
+    def launch(_keep=(params, keep)):
+        return fn(*args)
+    return launch
 
 
 def last_kernel_name(stream):

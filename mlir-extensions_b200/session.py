@@ -19,6 +19,9 @@ _NP_TO_DTYPE = {np.dtype(np.float32): B.F32, np.dtype(np.int32): B.I32}
 
 
 class Session:
+    """adopt_stream: a cudaStream_t of the caller's to launch on instead of a new stream (1, CUDA's
+    handle of the legacy default stream, where the caller's work runs on that)."""
+
     def __init__(self, device=None, adopt_stream=None):
         dev = None
         if device is not None:
@@ -66,6 +69,15 @@ class Session:
         if wait:
             rt.gpuWait(self.stream)
         return ev
+
+    def bind(self, kernel, pointer_args):
+        """The launch of `kernel` on these pointers as a callable (asynchronous; `wait()` waits), for
+        programs that repeat it: the argument list is built once."""
+        return rt.bind_launch(self.stream, kernel, pointer_args)
+
+    def workspace_bytes(self, kernel):
+        """Device scratch a launch of `kernel` wants as its last pointer (0: none)."""
+        return int(rt.imexKernelWorkspaceBytes(kernel))
 
     def wait(self):
         rt.gpuWait(self.stream)

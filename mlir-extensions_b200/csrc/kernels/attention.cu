@@ -1,65 +1,513 @@
-// Attention forward with row statistics (IMEX_OP_ATTENTION): checks and a plain kernel, one block
-// per query row, one pass over its visible keys with the running maximum and sum.
-#include "attention_common.cuh"
+// Attention forward with row statistics (IMEX_OP_ATTENTION) on the 5th-generation tensor cores:
+// S = Q K^T, P = 2^(scale log2(e) S - m), O += P V in one pass over the visible keys, with a reference
+// maximum m per row that moves only when the row's maximum outgrows it by more than 2^8 (only then are O, in
+// TMEM, and the running sum l rescaled); at the end O / l and LSE = ln 2 (m + log2 l).
+//
+// A CTA runs two streams, each with its own scores S (128 x 128 f32 in TMEM, P takes its place as 16-bit
+// pairs) and its own accumulator O, so that the tensor core works for one stream while the other computes
+// exponentials.  Both masks leave every row a prefix of the keys, so a tile stops at the last key any of its
+// rows sees and only the blocks behind the first row's prefix compare indices.
+//
+//   paired   the streams are two neighbouring tiles of 128 query rows of one head; they share every K and V
+//            tile (tiles [256 t, 256 t + 256)).
+//   packed   all n_q rows of all query heads of one key head fit into one tile (n_q * group <= 128: decoding,
+//            short chunks): both streams hold that tile and take every other key block; merged at the end.
+//
+// When there are fewer tiles than SMs the key blocks of a tile are shared out between `splits` CTAs, which
+// leave O (unnormalised), m and l in the workspace; attention_join_kernel adds them up in order.
+//
+//   warp 0      TMA producer: Q, then K and V tiles through one ring in the order the products use them.
+//   warp 1      issues the products.  Per stream and block: wait for P, O += P V, S = Q K^T of the next
+//               block.  Products run in the order they are issued, so one barrier (`scores`) tells the stream
+//               that its next scores are there AND that P V before them is done.
+//   warps 4-11  stream (warp - 4) / 4, one query row per thread: no shuffles, no exchange.  A row's 128 scores
+//               sit in registers, so these two warpgroups take registers over from the first one
+//               (72 + 2 * 216 = 3 * 168 a thread at launch).
+//
+// Rounding: P once to the 16-bit type (l and LSE add up the unrounded values), O once at the end.
+// V rows between key_lens[b] and the end of its tile are zeroed in shared memory, so that padding may hold
+// anything (0 * NaN would reach the sum); masked scores are selected away.
+// Every wait is bounded; one that runs out records a status code and the role leaves its loop.
+#include "attention_tc.cuh"
 
 namespace imex {
 namespace {
 
 using namespace attn;
+using namespace tc;
 
-struct FwdArgs {
-  const uint16_t *q, *k, *v;
+constexpr int THREADS = 384;
+constexpr unsigned kPollSleepNs = 40;
+// TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512)
+constexpr int TMEM_COLS = 512;
+constexpr int O_COL = 256;
+
+__host__ __device__ constexpr int tile_bytes(int dh) { return TILE * dh * 2; }
+__host__ __device__ constexpr int stages(int dh) { return dh == 128 ? 5 : 8; }
+__host__ __device__ constexpr int q_tiles(bool packed) { return packed ? 1 : 2; }
+constexpr int MERGE_BYTES = 2 * TILE * 8;
+constexpr int smem_bytes(int dh, bool packed) {
+  return 1024 + (q_tiles(packed) + stages(dh)) * tile_bytes(dh) + 256 + (packed ? MERGE_BYTES : 0);
+}
+
+struct FwdParams {
   uint16_t *o;
   float *lse;
   const int32_t *key_lens;
-  Strides3 sq, sk, sv, so;
-  int q_heads, group, n_q, n_kv, d, causal;
-  float scale;
+  float *part_o;   // [splits][rows of the problem][DH], unnormalised
+  float2 *part_ml; // [splits][rows of the problem]
+  unsigned *status;
+  Strides3 so;
+  int q_heads, group, n_q, n_kv, causal;
+  int heads_batch, heads, tiles_q, splits;  // heads: q_heads (paired) or kv_heads (packed)
+  int64_t rows;                             // batch * q_heads * n_q
+  float scale_log2e;
+  uint32_t idesc_s, idesc_o;
 };
 
-template <bool BF16> __global__ void __launch_bounds__(128) attention_rows_kernel(const FwdArgs a) {
-  __shared__ float qs[128], ps[128], red[4];
-  const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  const uint16_t *q = a.q + b * a.sq.batch + h * a.sq.head + i * a.sq.row;
-  const uint16_t *k = a.k + b * a.sk.batch + (h / a.group) * a.sk.head;
-  const uint16_t *v = a.v + b * a.sv.batch + (h / a.group) * a.sv.head;
-  if (t < a.d) qs[t] = to_f32<BF16>(q[t]);
-  __syncthreads();
-  const int limit = visible_keys(i, key_count(a.key_lens, b, a.n_kv), a.n_q, a.n_kv, a.causal);
-  float m = -INFINITY, l = 0.0f, acc = 0.0f;
-  for (int j0 = 0; j0 < limit; j0 += 128) {
-    float s = -INFINITY;
-    if (j0 + t < limit) {
-      s = 0.0f;
-      const uint16_t *kr = k + (j0 + t) * a.sk.row;
-      for (int c = 0; c < a.d; ++c) s = fmaf(qs[c], to_f32<BF16>(kr[c]), s);
-      s *= a.scale;
-    }
-    float x = s;
-    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-    if ((t & 31) == 0) red[t >> 5] = x;
-    __syncthreads();
-    const float m1 = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float p = expf(s - m1), r = expf(m - m1);
-    ps[t] = p;
-    __syncthreads();
-    acc *= r;
-    l *= r;
-    m = m1;
-    const int n = min(128, limit - j0);
-    for (int j = 0; j < n; ++j) {
-      l += ps[j];
-      if (t < a.d) acc = fmaf(ps[j], to_f32<BF16>(v[(j0 + j) * a.sv.row + t]), acc);
-    }
-    __syncthreads();
+// What one CTA does.
+struct Work {
+  int b, head, qt, split;
+  int keys;       // keys of the sequence
+  int kb0;        // first key block
+  int n[2];       // blocks of each stream
+};
+
+template <bool PACKED> __device__ __forceinline__ Work work_of(const FwdParams &p) {
+  Work w;
+  const int hb = blockIdx.x % p.heads_batch, rest = blockIdx.x / p.heads_batch;
+  w.b = hb / p.heads;
+  w.head = hb % p.heads;
+  w.split = rest % p.splits;
+  w.qt = p.tiles_q - 1 - rest / p.splits;  // under the causal mask the long tiles come first
+  w.keys = key_count(p.key_lens, w.b, p.n_kv);
+  auto blocks = [&](int row0, int rows) {  // key blocks that rows [row0, row0 + rows) see
+    if (row0 >= p.n_q) return 0;
+    return (visible_keys(min(row0 + rows, p.n_q) - 1, w.keys, p.n_q, p.n_kv, p.causal) + TILE - 1) / TILE;
+  };
+  if (PACKED) {
+    const int nb = blocks(0, p.n_q);
+    w.kb0 = static_cast<int>(static_cast<int64_t>(nb) * w.split / p.splits);
+    const int mine = static_cast<int>(static_cast<int64_t>(nb) * (w.split + 1) / p.splits) - w.kb0;
+    w.n[0] = (mine + 1) / 2;
+    w.n[1] = mine / 2;
+  } else {
+    const int n0 = blocks(w.qt * 2 * TILE, TILE), n1 = blocks(w.qt * 2 * TILE + TILE, TILE), nb = max(n0, n1);
+    w.kb0 = static_cast<int>(static_cast<int64_t>(nb) * w.split / p.splits);
+    const int kb1 = static_cast<int>(static_cast<int64_t>(nb) * (w.split + 1) / p.splits);
+    w.n[0] = max(0, min(n0, kb1) - w.kb0);
+    w.n[1] = max(0, min(n1, kb1) - w.kb0);
   }
-  if (t < a.d)
-    a.o[b * a.so.batch + h * a.so.head + i * a.so.row + t] = from_f32<BF16>(limit > 0 ? acc / l : 0.0f);
-  if (t == 0)
-    a.lse[(static_cast<int64_t>(b) * a.q_heads + h) * a.n_q + i] = limit > 0 ? m + logf(l) : -INFINITY;
+  return w;
+}
+
+template <bool BF16, int DH, bool PACKED>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                 const __grid_constant__ CUtensorMap tmap_v, const FwdParams p) {
+  constexpr int STAGES = stages(DH);
+  constexpr int TB = tile_bytes(DH);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  auto q_smem = [&](int g) { return smem_base + (PACKED ? 0 : g * TB); };
+  auto kv_smem = [&](int pos) { return smem_base + (q_tiles(PACKED) + pos % STAGES) * TB; };
+  const uint32_t bars = smem_base + (q_tiles(PACKED) + STAGES) * TB;
+  const uint32_t q_full = bars;
+  auto kv_full = [&](int pos) { return bars + 8u * (1 + pos % STAGES); };
+  auto kv_empty = [&](int pos) { return bars + 8u * (1 + STAGES + pos % STAGES); };
+  auto kv_phase = [&](int pos) { return static_cast<uint32_t>(pos / STAGES) & 1u; };
+  auto scores = [&](int g) { return bars + 8u * (1 + 2 * STAGES + g); };
+  auto probs = [&](int g) { return bars + 8u * (3 + 2 * STAGES + g); };
+  const uint32_t merge_bar = bars + 8u * (5 + 2 * STAGES);
+  const uint32_t tmem_slot = bars + 8u * (6 + 2 * STAGES);
+  static_assert(8 * (7 + 2 * STAGES) <= 256, "the barriers fit");
+  uint8_t *smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
+  volatile uint32_t *tmem_slot_ptr = reinterpret_cast<volatile uint32_t *>(smem_aligned + (tmem_slot - smem_base));
+  float2 *merge = reinterpret_cast<float2 *>(smem_aligned + (bars + 256 - smem_base));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Work w = work_of<PACKED>(p);
+  const int n_max = max(w.n[0], w.n[1]);
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(scores(g), 1);
+      mbar_init(probs(g), 4);
+    }
+    mbar_init(merge_bar, 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot_ptr;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------------------ TMA producer
+      if (lane == 0 && n_max > 0) {
+        const int kv_head = PACKED ? w.head : w.head / p.group;
+        if (PACKED) {
+          mbar_expect_tx(q_full, p.n_q * p.group * DH * 2);
+          load_tile<DH>(q_smem(0), &tmap_q, 0, w.head * p.group, w.b, q_full);
+        } else {
+          const int row0 = w.qt * 2 * TILE;
+          const bool second = row0 + TILE < p.n_q;
+          mbar_expect_tx(q_full, second ? 2 * TB : TB);
+          load_tile<DH>(q_smem(0), &tmap_q, row0, w.head, w.b, q_full);
+          if (second) load_tile<DH>(q_smem(1), &tmap_q, row0 + TILE, w.head, w.b, q_full);
+        }
+        int pos = 0;
+        bool ok = true;
+        auto load = [&](const CUtensorMap *map, int block) {
+          if (!ok) return;
+          if (pos >= STAGES && !mbar_wait_relaxed(kv_empty(pos), kv_phase(pos) ^ 1u, kPollSleepNs)) {
+            report(p.status, kStatusTmaWaitTimeout);
+            ok = false;
+            return;
+          }
+          mbar_expect_tx(kv_full(pos), TB);
+          load_tile<DH>(kv_smem(pos), map, (w.kb0 + block) * TILE, kv_head, w.b, kv_full(pos));
+          ++pos;
+        };
+        // the order in which the products below use them
+        if (PACKED) {
+          const int nb = w.n[0] + w.n[1];
+          load(&tmap_k, 0);
+          if (nb > 1) load(&tmap_k, 1);
+          for (int j = 0; j < nb; ++j) {
+            load(&tmap_v, j);
+            if (j + 2 < nb) load(&tmap_k, j + 2);
+          }
+        } else {
+          load(&tmap_k, 0);
+          for (int j = 0; j < n_max; ++j) {
+            load(&tmap_v, j);
+            if (j + 1 < n_max) load(&tmap_k, j + 1);
+          }
+        }
+        // every tile has been used before the CTA may go
+        for (int q = max(0, pos - STAGES); q < pos; ++q)
+          if (!mbar_wait_relaxed(kv_empty(q), kv_phase(q), kPollSleepNs)) break;
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ products
+      // the whole warp walks the loop (it zeroes padded V rows together), lane 0 issues
+      if (n_max > 0) {
+        bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
+        int pos = 0;
+        const int pad_block = w.keys < p.n_kv && w.keys % TILE ? w.keys / TILE - w.kb0 : -1;
+        auto wait_tile = [&](int q) {
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(kv_full(q), kv_phase(q)));
+        };
+        auto issue_scores = [&](int g, int q) {
+          if (lane == 0 && ok) {
+            tcgen05_fence_after();
+            mma_scores<DH>(tmem + g * TILE, q_smem(g), kv_smem(q), p.idesc_s);
+            tcgen05_commit(scores(g));
+          }
+        };
+        auto release = [&](int q) {
+          if (lane == 0 && ok) tcgen05_commit(kv_empty(q));
+        };
+        // O_g += P V of the stream's block jl; the last one signals the stream through its scores barrier
+        auto issue_rows = [&](int g, int jl, int q) {
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g), jl & 1));
+          if (lane == 0 && ok) {
+            tcgen05_fence_after();
+            mma_rows(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0);
+            if (jl + 1 == w.n[g]) tcgen05_commit(scores(g));
+          }
+        };
+        auto wait_v = [&](int q, int block) {
+          wait_tile(q);
+          if (block == pad_block) {  // rows of V behind the sequence's last key
+            const int first = w.keys % TILE, count = (TILE - first) * 8;  // 16-byte units per box
+            for (int e = lane; e < count * (DH / 64); e += 32) {
+              const uint32_t at = kv_smem(q) + (e / count) * BOX_BYTES + first * 128 + (e % count) * 16;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+            }
+            fence_async_smem();
+            __syncwarp();
+          }
+        };
+        if (PACKED) {
+          const int nb = w.n[0] + w.n[1];
+          for (int g = 0; g < 2 && g < nb; ++g) {
+            wait_tile(pos);
+            issue_scores(g, pos);
+            release(pos++);
+          }
+          for (int j = 0; j < nb && ok; ++j) {
+            const int g = j & 1;
+            wait_v(pos, j);
+            issue_rows(g, j >> 1, pos);
+            release(pos++);
+            if (j + 2 < nb) {
+              wait_tile(pos);
+              issue_scores(g, pos);
+              release(pos++);
+            }
+          }
+        } else {
+          wait_tile(0);
+          for (int g = 0; g < 2; ++g)
+            if (w.n[g] > 0) issue_scores(g, 0);
+          release(pos++);
+          for (int j = 0; j < n_max && ok; ++j) {
+            const int v = pos++, k = j + 1 < n_max ? pos++ : -1;
+            wait_v(v, j);
+            for (int g = 0; g < 2; ++g) {
+              if (j < w.n[g]) issue_rows(g, j, v);
+              if (g == 1) release(v);
+              if (g == 0 && k >= 0) wait_tile(k);
+              if (j + 1 < w.n[g]) issue_scores(g, k);
+            }
+            if (k >= 0) release(k);
+          }
+        }
+        if (!ok && lane == 0) report(p.status, kStatusMmaWaitTimeout);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax and output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int g = (warp - 4) >> 2;
+    const int lane_group = warp & 3;
+    const int r = lane_group * 32 + lane;  // row of the tile = TMEM lane
+    const int n = w.n[g];
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
+    const uint32_t s_addr = t_row + g * TILE;
+    const uint32_t o_addr = t_row + O_COL + g * TILE;
+    int head = w.head, i;  // the query this thread's row stands for
+    if (PACKED) {
+      head = w.head * p.group + r / p.n_q;
+      i = r < p.n_q * p.group ? r % p.n_q : p.n_q;
+    } else {
+      i = w.qt * 2 * TILE + g * TILE + r;
+    }
+    const bool exists = i < p.n_q;
+    // rows that do not exist compute on whatever is there and are not written
+    const int limit = exists ? visible_keys(i, w.keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
+    const float neg_inf = -INFINITY;
+    float m = neg_inf, l = 0.0f;  // m: the reference maximum, in units of log2
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = mbar_wait(scores(g), j & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + 32 * c, s[c]);
+      tmem_ld_wait();
+      const int seen = limit - (w.kb0 + (PACKED ? 2 * j + g : j)) * TILE;  // of this block's keys
+      if (__any_sync(0xffffffffu, seen < TILE)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e >= seen) s[c][e] = __float_as_uint(neg_inf);
+      }
+      float top[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          top[c] = max3(top[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+      const float row_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2e;
+      if (j == 0) {
+        m = row_max;
+      } else {
+        const bool move = row_max > m + 8.0f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float a = move ? ex2(m - row_max) : 1.0f;
+#pragma unroll 1
+          for (int c = 0; c < DH; c += 16) {
+            uint32_t v[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "r"(o_addr + c)
+                : "memory");
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * a);
+            tmem_st_16(o_addr + c, v);
+          }
+          l *= a;
+          if (move) m = row_max;
+        }
+      }
+      const float m_safe = m == neg_inf ? 0.0f : m;  // a row without a visible key: every exponent is -inf
+      const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_m2 = pack_f32x2(-m_safe, -m_safe);
+      uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pw[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x0, x1;
+          unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2), x0, x1);
+          const float e0 = ex2(x0), e1 = ex2(x1);
+          sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(e0, e1));
+          pw[e] = pack2<BF16>(e0, e1);
+        }
+        tmem_st_16(s_addr + 16 * c, pw);
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(probs(g));
+      float lo, hi;
+      unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
+      l += lo + hi;
+    }
+    if (ok && n > 0) {
+      ok = mbar_wait(scores(g), n & 1);  // the last P V
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    const int64_t row = exists ? (static_cast<int64_t>(w.b) * p.q_heads + head) * p.n_q + i : 0;
+    // factors of the two streams' accumulators (paired: only this stream's), first column and number of
+    // columns this thread writes
+    float a0 = 1.0f, a1 = 0.0f;
+    int col0 = 0;
+    constexpr int COLS = PACKED ? DH / 2 : DH;
+    if (PACKED) {
+      merge[g * TILE + r] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(merge_bar);
+      ok = ok && mbar_wait(merge_bar, 0);
+      ok = __all_sync(0xffffffffu, ok);
+      const float2 x = merge[r], y = merge[TILE + r];
+      m = fmaxf(x.x, y.x);
+      const float m_safe = m == neg_inf ? 0.0f : m;
+      a0 = ex2(x.x - m_safe), a1 = ex2(y.x - m_safe);
+      l = x.y * a0 + y.y * a1;
+      col0 = g * COLS;
+    }
+    if (!ok) {
+      if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
+    } else {
+      tcgen05_fence_after();
+      const bool has0 = PACKED ? w.n[0] > 0 : n > 0, has1 = PACKED && w.n[1] > 0;
+      const bool some = l > 0.0f;
+      const float inv = p.splits > 1 ? 1.0f : (some ? 1.0f / l : 0.0f);
+      a0 *= inv;
+      a1 *= inv;
+      if (exists && (!PACKED || g == 0)) {
+        if (p.splits > 1) p.part_ml[w.split * p.rows + row] = make_float2(m, l);
+        else p.lse[row] = some ? 0.6931471805599453f * (m + log2f(l)) : neg_inf;
+      }
+#pragma unroll 1
+      for (int c = col0; c < col0 + COLS; c += 32) {
+        uint32_t v0[32], v1[32];
+        if (has0) tmem_ld_32x32((PACKED ? t_row + O_COL : o_addr) + c, v0);
+        if (has1) tmem_ld_32x32(t_row + O_COL + TILE + c, v1);
+        tmem_ld_wait();
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          x[e] = has0 && some ? __uint_as_float(v0[e]) * a0 : 0.0f;
+          if (has1 && some) x[e] = fmaf(__uint_as_float(v1[e]), a1, x[e]);
+        }
+        if (exists && p.splits > 1) {
+          float4 *to = reinterpret_cast<float4 *>(p.part_o + (w.split * p.rows + row) * DH + c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        } else if (exists) {
+          uint4 *to = reinterpret_cast<uint4 *>(p.o + w.b * p.so.batch + head * p.so.head + i * p.so.row + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            to[e] = make_uint4(pack2<BF16>(x[8 * e], x[8 * e + 1]), pack2<BF16>(x[8 * e + 2], x[8 * e + 3]),
+                               pack2<BF16>(x[8 * e + 4], x[8 * e + 5]), pack2<BF16>(x[8 * e + 6], x[8 * e + 7]));
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// O and LSE of a row from its splits, in order.  One warp per row.
+template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_join_kernel(const FwdParams p) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= p.rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * p.rows + row].x);
+  const float m_safe = m == -INFINITY ? 0.0f : m;
+  constexpr int V = DH / 32;
+  float l = 0.0f, x[V] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.part_ml[s * p.rows + row];
+    const float a = ex2(ml.x - m_safe);
+    l = fmaf(ml.y, a, l);
+    const float *from = p.part_o + (s * p.rows + row) * DH + lane * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = fmaf(from[e], a, x[e]);
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const int i = static_cast<int>(row % p.n_q);
+  const int64_t bh = row / p.n_q;
+  uint16_t *to = p.o + (bh / p.q_heads) * p.so.batch + (bh % p.q_heads) * p.so.head + i * p.so.row + lane * V;
+  uint32_t w[V / 2];
+#pragma unroll
+  for (int e = 0; e < V; e += 2) w[e / 2] = pack2<BF16>(x[e] * inv, x[e + 1] * inv);
+  if (V == 4) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t *>(to) = w[0];
+  if (lane == 0) p.lse[row] = l > 0.0f ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
+}
+
+constexpr int SMS = 148;
+
+bool is_packed(const AttentionProblem &p) { return p.n_q * (p.q_heads / p.kv_heads) <= TILE; }
+int64_t tile_count(const AttentionProblem &p) {
+  return is_packed(p) ? p.batch * p.kv_heads : p.batch * p.q_heads * ((p.n_q + 2 * TILE - 1) / (2 * TILE));
+}
+// Shares of a tile's key blocks: enough CTAs for every SM, at least four blocks each (a share's set-up and
+// the joining cost about as much as two).
+int split_count(const AttentionProblem &p) {
+  const int64_t blocks = (p.n_kv + TILE - 1) / TILE, tiles = tile_count(p);
+  int64_t s = tiles >= SMS ? 1 : SMS / tiles;
+  if (s > blocks / 4) s = blocks / 4;
+  return static_cast<int>(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
 
 bool aligned(const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+
+template <bool BF16, int DH, bool PACKED>
+cudaError_t launch_variant(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const FwdParams &f,
+                           unsigned grid, cudaStream_t stream) {
+  cudaError_t e = allow_smem(attention_kernel<BF16, DH, PACKED>, smem_bytes(DH, PACKED));
+  if (e != cudaSuccess) return e;
+  attention_kernel<BF16, DH, PACKED><<<grid, THREADS, smem_bytes(DH, PACKED), stream>>>(tq, tk, tv, f);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || f.splits == 1) return e;
+  attention_join_kernel<BF16, DH><<<static_cast<unsigned>((f.rows + 3) / 4), 128, 0, stream>>>(f);
+  return cudaGetLastError();
+}
 
 } // namespace
 
@@ -70,13 +518,20 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
   if (p.q_heads % p.kv_heads) return "q_heads must be a multiple of kv_heads";
   if (p.d_head != 64 && p.d_head != 128) return "d_head is 64 or 128";
   if (!(p.scale > 0.0f) || p.scale > 3.0e38f) return "sm_scale must be positive and finite";
-  if (p.batch > 65535 || p.q_heads > 65535 || p.n_q > (1 << 30) || p.n_kv > (1 << 30))
-    return "at most 65535 sequences and heads, 2^30 rows";
+  if (p.batch > 65535 || p.q_heads > 65535 || p.n_q > (1 << 30) || p.n_kv > (1 << 30) ||
+      p.batch * p.q_heads * ((p.n_q + TILE - 1) / TILE) > INT32_MAX / 64 ||
+      p.batch * p.kv_heads * ((p.n_kv + TILE - 1) / TILE) > INT32_MAX / 64)
+    return "too many sequences, heads or rows";
   const Strides3 *s[8] = {&p.sq, &p.sk, &p.sv, &p.so, &p.sdo, &p.sdq, &p.sdk, &p.sdv};
-  for (int i = 0; i < (backward ? 8 : 4); ++i)
-    if (s[i]->batch < 0 || s[i]->head < 0 || s[i]->row < 0 || s[i]->batch % 8 || s[i]->head % 8 || s[i]->row % 8 ||
-        s[i]->batch >= (1ll << 38) || s[i]->head >= (1ll << 38) || s[i]->row >= (1ll << 38))
-      return "strides are multiples of 8 elements, below 2^38";
+  const bool of_keys[8] = {false, true, true, false, false, false, true, true};
+  for (int i = 0; i < (backward ? 8 : 4); ++i) {
+    const int64_t extent[3] = {p.batch, of_keys[i] ? p.kv_heads : p.q_heads, of_keys[i] ? p.n_kv : p.n_q};
+    const int64_t step[3] = {s[i]->batch, s[i]->head, s[i]->row};
+    for (int j = 0; j < 3; ++j) {
+      if (step[j] < 0 || step[j] % 8 || step[j] >= (1ll << 38)) return "strides are multiples of 8 elements, below 2^38";
+      if (extent[j] > 1 && step[j] == 0) return "strides of extents above 1 are not zero";
+    }
+  }
   if (!pointers) return nullptr;
   if (!aligned(p.q) || !aligned(p.k) || !aligned(p.v) || !aligned(p.o) ||
       (backward && (!aligned(p.dout) || !aligned(p.dq) || !aligned(p.dk) || !aligned(p.dv))))
@@ -85,20 +540,58 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
 }
 
 size_t attention_workspace_bytes(const AttentionProblem &p, bool backward) {
-  if (!backward) return 0;
-  return (static_cast<size_t>(p.batch) * p.q_heads * p.n_q * sizeof(float) + 255) / 256 * 256;
+  const size_t rows = static_cast<size_t>(p.batch) * p.q_heads * p.n_q;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  if (backward) return up(rows * sizeof(float));
+  const size_t splits = split_count(p);
+  return splits == 1 ? 0 : up(splits * rows * sizeof(float2)) + up(splits * rows * p.d_head * sizeof(float));
 }
 
-cudaError_t launch_attention(const AttentionProblem &p, unsigned *, cudaStream_t stream, int *launched) {
-  FwdArgs a{static_cast<const uint16_t *>(p.q), static_cast<const uint16_t *>(p.k), static_cast<const uint16_t *>(p.v),
-            static_cast<uint16_t *>(p.o), p.lse, p.key_lens, p.sq, p.sk, p.sv, p.so, static_cast<int>(p.q_heads),
-            static_cast<int>(p.q_heads / p.kv_heads), static_cast<int>(p.n_q), static_cast<int>(p.n_kv),
-            static_cast<int>(p.d_head), p.causal ? 1 : 0, p.scale};
-  const dim3 grid(static_cast<unsigned>(p.n_q), static_cast<unsigned>(p.q_heads), static_cast<unsigned>(p.batch));
-  if (p.dtype == kBF16) attention_rows_kernel<true><<<grid, 128, 0, stream>>>(a);
-  else attention_rows_kernel<false><<<grid, 128, 0, stream>>>(a);
-  *launched = 1;
-  return cudaGetLastError();
+cudaError_t launch_attention(const AttentionProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  const bool packed = is_packed(p), bf16 = p.dtype == kBF16;
+  const int64_t group = p.q_heads / p.kv_heads;
+  CUtensorMap tq, tk, tv;
+  if (!make_map_4d(&tq, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq,
+                   packed ? static_cast<int>(p.n_q) : TILE, packed ? static_cast<int>(group) : 1) ||
+      !make_map_4d(&tk, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, TILE, 1) ||
+      !make_map_4d(&tv, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, TILE, 1))
+    return cudaErrorNotSupported;
+  FwdParams f{};
+  f.o = static_cast<uint16_t *>(p.o);
+  f.lse = p.lse;
+  f.key_lens = p.key_lens;
+  f.status = status;
+  f.so = p.so;
+  f.q_heads = static_cast<int>(p.q_heads);
+  f.group = static_cast<int>(group);
+  f.n_q = static_cast<int>(p.n_q);
+  f.n_kv = static_cast<int>(p.n_kv);
+  f.causal = p.causal ? 1 : 0;
+  f.heads = static_cast<int>(packed ? p.kv_heads : p.q_heads);
+  f.heads_batch = f.heads * static_cast<int>(p.batch);
+  f.tiles_q = packed ? 1 : static_cast<int>((p.n_q + 2 * TILE - 1) / (2 * TILE));
+  f.splits = split_count(p);
+  f.rows = p.batch * p.q_heads * p.n_q;
+  f.scale_log2e = p.scale * 1.4426950408889634f;
+  f.idesc_s = instruction_desc(bf16, false, TILE);
+  f.idesc_o = instruction_desc(bf16, true, static_cast<int>(p.d_head));
+  if (f.splits > 1) {
+    f.part_ml = static_cast<float2 *>(p.workspace);
+    const size_t ml = (static_cast<size_t>(f.splits) * f.rows * sizeof(float2) + 255) / 256 * 256;
+    f.part_o = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + ml);
+  }
+  const unsigned grid = static_cast<unsigned>(tile_count(p) * f.splits);
+  *launched = f.splits > 1 ? 2 : 1;
+  if (p.d_head == 64) {
+    if (bf16) return packed ? launch_variant<true, 64, true>(tq, tk, tv, f, grid, stream)
+                            : launch_variant<true, 64, false>(tq, tk, tv, f, grid, stream);
+    return packed ? launch_variant<false, 64, true>(tq, tk, tv, f, grid, stream)
+                  : launch_variant<false, 64, false>(tq, tk, tv, f, grid, stream);
+  }
+  if (bf16) return packed ? launch_variant<true, 128, true>(tq, tk, tv, f, grid, stream)
+                          : launch_variant<true, 128, false>(tq, tk, tv, f, grid, stream);
+  return packed ? launch_variant<false, 128, true>(tq, tk, tv, f, grid, stream)
+                : launch_variant<false, 128, false>(tq, tk, tv, f, grid, stream);
 }
 
 } // namespace imex

@@ -47,7 +47,7 @@ __host__ __device__ constexpr int stages(int dh) { return dh == 128 ? 5 : 8; }
 __host__ __device__ constexpr int q_tiles(bool packed) { return packed ? 1 : 2; }
 constexpr int MERGE_BYTES = 2 * TILE * 8;
 constexpr int smem_bytes(int dh, bool packed) {
-  return 1024 + (q_tiles(packed) + stages(dh)) * tile_bytes(dh) + 256 + (packed ? MERGE_BYTES : 0);
+  return (q_tiles(packed) + stages(dh)) * tile_bytes(dh) + 256 + (packed ? MERGE_BYTES : 0);
 }
 
 struct FwdParams {
@@ -107,8 +107,8 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                  const __grid_constant__ CUtensorMap tmap_v, const FwdParams p) {
   constexpr int STAGES = stages(DH);
   constexpr int TB = tile_bytes(DH);
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
+  const uint32_t smem_base = smem_u32(smem_raw);
   auto q_smem = [&](int g) { return smem_base + (PACKED ? 0 : g * TB); };
   auto kv_smem = [&](int pos) { return smem_base + (q_tiles(PACKED) + pos % STAGES) * TB; };
   const uint32_t bars = smem_base + (q_tiles(PACKED) + STAGES) * TB;
@@ -121,9 +121,8 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   const uint32_t merge_bar = bars + 8u * (5 + 2 * STAGES);
   const uint32_t tmem_slot = bars + 8u * (6 + 2 * STAGES);
   static_assert(8 * (7 + 2 * STAGES) <= 256, "the barriers fit");
-  uint8_t *smem_aligned = smem_raw + (smem_base - smem_u32(smem_raw));
-  volatile uint32_t *tmem_slot_ptr = reinterpret_cast<volatile uint32_t *>(smem_aligned + (tmem_slot - smem_base));
-  float2 *merge = reinterpret_cast<float2 *>(smem_aligned + (bars + 256 - smem_base));
+  volatile uint32_t *tmem_slot_ptr = reinterpret_cast<volatile uint32_t *>(smem_raw + (tmem_slot - smem_base));
+  float2 *merge = reinterpret_cast<float2 *>(smem_raw + (bars + 256 - smem_base));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Work w = work_of<PACKED>(p);
@@ -227,7 +226,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g), jl & 1));
           if (lane == 0 && ok) {
             tcgen05_fence_after();
-            mma_rows(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0);
+            mma_rows<32>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0);
             if (jl + 1 == w.n[g]) tcgen05_commit(scores(g));
           }
         };

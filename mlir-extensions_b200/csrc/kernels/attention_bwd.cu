@@ -1,131 +1,626 @@
-// Attention backward (IMEX_OP_ATTENTION_BWD), plain kernels: one block per query row for dQ (which also
-// leaves delta = rowsum(dO O) in the workspace), one block per key for dK and dV.  The probabilities are
-// recomputed from LSE.
-#include "attention_common.cuh"
+// Attention backward (IMEX_OP_ATTENTION_BWD) on the 5th-generation tensor cores.
+//
+//   P = 2^(scale log2(e) Q K^T - log2(e) LSE)       dV = sum_group P^T dO
+//   dS = P (dO V^T - delta), delta = rowsum(dO O)   dQ = scale dS K,  dK = scale sum_group dS^T Q
+//
+// Two kernels, each with its accumulators in TMEM to the end, so that nothing is added up in memory: no
+// atomics, no f32 copy of dQ, and the same bits in every run.  The price is that Q K^T and dO V^T are
+// computed twice (7 products instead of 5).
+//
+//   attention_dq_kernel    a CTA owns 128 queries (Q, dO stay in shared memory) and walks the key blocks they
+//                          see; it also leaves delta in the workspace for the other kernel.
+//   attention_dkv_kernel   a CTA owns 128 keys (K, V stay) and walks the query blocks that see them, of every
+//                          query head that shares the key head.  It works on the transposed products
+//                          S^T = K Q^T, dP^T = V dO^T (a thread's row is a key), so that P^T and dS^T are A
+//                          operands from TMEM and dO and Q are used as they lie.
+//
+// Roles as in the forward kernel: warp 0 loads tiles (TMA), warp 1 issues products, warps 4-11 compute: two
+// warpgroups share every row's 128 columns, 64 each.  P and dS take the places of S and dP in TMEM as 16-bit
+// pairs (each half in front of its own 64 columns, so that no thread overwrites what another still reads);
+// products run in the order they are issued, so overwriting a score tile is ordered by issuing the
+// next product behind the one that reads it.  While the warps compute P the tensor core runs the
+// previous block's last product and this block's dP; while they compute dS it runs the next block's S.
+//
+// Rounding: P and dS once to the 16-bit type, results once.  Masked entries are selected away, padded K rows
+// zeroed in shared memory where they are a B operand, so padding may hold anything.
+#include "attention_tc.cuh"
 
 namespace imex {
 namespace {
 
 using namespace attn;
+using namespace tc;
 
-struct BwdArgs {
-  const uint16_t *q, *k, *v, *o, *dout;
+constexpr int THREADS = 384;
+constexpr unsigned kPollSleepNs = 40;
+constexpr int TMEM_COLS = 512;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__host__ __device__ constexpr int tile_bytes(int dh) { return TILE * dh * 2; }
+__host__ __device__ constexpr int stages_a(int dh) { return dh == 128 ? 3 : 4; }  // Q (dkv) or K (dq)
+__host__ __device__ constexpr int stages_b(int dh) { return dh == 128 ? 2 : 4; }  // dO (dkv) or V (dq)
+constexpr int STAT_STAGES = 2;
+constexpr int STAT_BYTES = STAT_STAGES * 2 * TILE * 4;
+constexpr int BAR_BYTES = 256;
+constexpr int smem_bytes(int dh) {
+  return (2 + stages_a(dh) + stages_b(dh)) * tile_bytes(dh) + BAR_BYTES + STAT_BYTES;
+}
+
+struct BwdParams {
+  const uint16_t *o, *dout;
   const float *lse;
   float *delta;
   uint16_t *dq, *dk, *dv;
   const int32_t *key_lens;
-  Strides3 sq, sk, sv, so, sdo, sdq, sdk, sdv;
-  int q_heads, group, n_q, n_kv, d, causal;
-  float scale;
+  unsigned *status;
+  Strides3 so, sdo, sdq, sdk, sdv;
+  int q_heads, kv_heads, group, n_q, n_kv, causal, heads_batch, tiles;
+  float scale, scale_log2e;
+  uint32_t idesc_s, idesc_o;
 };
 
-template <bool BF16> __global__ void __launch_bounds__(128) attention_dq_rows_kernel(const BwdArgs a) {
-  __shared__ float qs[128], gs[128], ds[128], red[4];
-  const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  const uint16_t *k = a.k + b * a.sk.batch + (h / a.group) * a.sk.head;
-  const uint16_t *v = a.v + b * a.sv.batch + (h / a.group) * a.sv.head;
-  float part = 0.0f;
-  if (t < a.d) {
-    qs[t] = to_f32<BF16>(a.q[b * a.sq.batch + h * a.sq.head + i * a.sq.row + t]);
-    gs[t] = to_f32<BF16>(a.dout[b * a.sdo.batch + h * a.sdo.head + i * a.sdo.row + t]);
-    part = gs[t] * to_f32<BF16>(a.o[b * a.so.batch + h * a.so.head + i * a.so.row + t]);
-  }
-  for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  if ((t & 31) == 0) red[t >> 5] = part;
-  __syncthreads();
-  const float delta = red[0] + red[1] + red[2] + red[3];
-  const int64_t row = (static_cast<int64_t>(b) * a.q_heads + h) * a.n_q + i;
-  if (t == 0) a.delta[row] = delta;
-  const float lse = a.lse[row];
-  const int limit = visible_keys(i, key_count(a.key_lens, b, a.n_kv), a.n_q, a.n_kv, a.causal);
-  float acc = 0.0f;
-  for (int j0 = 0; j0 < limit; j0 += 128) {
-    float x = 0.0f;
-    if (j0 + t < limit) {
-      const uint16_t *kr = k + (j0 + t) * a.sk.row, *vr = v + (j0 + t) * a.sv.row;
-      float s = 0.0f, dp = 0.0f;
-      for (int c = 0; c < a.d; ++c) {
-        s = fmaf(qs[c], to_f32<BF16>(kr[c]), s);
-        dp = fmaf(gs[c], to_f32<BF16>(vr[c]), dp);
-      }
-      x = expf(s * a.scale - lse) * (dp - delta);
-    }
-    ds[t] = x;
-    __syncthreads();
-    const int n = min(128, limit - j0);
-    if (t < a.d)
-      for (int j = 0; j < n; ++j) acc = fmaf(ds[j], to_f32<BF16>(k[(j0 + j) * a.sk.row + t]), acc);
-    __syncthreads();
-  }
-  if (t < a.d) a.dq[b * a.sdq.batch + h * a.sdq.head + i * a.sdq.row + t] = from_f32<BF16>(acc * a.scale);
+static_assert(smem_bytes(128) <= 232448, "227 KB a CTA");
+
+// Barriers and buffers of one CTA, the same for both kernels: two resident tiles, a ring of A tiles and one
+// of B tiles.
+template <int DH> struct Layout {
+  static constexpr int SA = stages_a(DH), SB = stages_b(DH), TB = tile_bytes(DH);
+  uint32_t base;
+  __device__ uint32_t resident(int i) const { return base + i * TB; }
+  __device__ uint32_t a_tile(int i) const { return base + (2 + i % SA) * TB; }
+  __device__ uint32_t b_tile(int i) const { return base + (2 + SA + i % SB) * TB; }
+  __device__ uint32_t bars() const { return base + (2 + SA + SB) * TB; }
+  __device__ uint32_t res_full() const { return bars(); }
+  __device__ uint32_t a_full(int i) const { return bars() + 8 * (1 + i % SA); }
+  __device__ uint32_t a_empty(int i) const { return bars() + 8 * (1 + SA + i % SA); }
+  __device__ uint32_t a_phase(int i) const { return (i / SA) & 1; }
+  __device__ uint32_t b_full(int i) const { return bars() + 8 * (1 + 2 * SA + i % SB); }
+  __device__ uint32_t b_empty(int i) const { return bars() + 8 * (1 + 2 * SA + SB + i % SB); }
+  __device__ uint32_t b_phase(int i) const { return (i / SB) & 1; }
+  static constexpr int FIXED = 1 + 2 * SA + 2 * SB;
+  __device__ uint32_t bar(int i) const { return bars() + 8 * (FIXED + i); }
+  static constexpr int S_FULL = 0, DP_FULL = 2, P_READY = 3, DS_READY = 4, DONE = 5, STAT_FULL = 6, STAT_EMPTY = 8;
+  static constexpr int TMEM_SLOT = 10;
+  static_assert(8 * (FIXED + 11) <= BAR_BYTES, "the barriers fit");
+  __device__ uint32_t stats() const { return bars() + BAR_BYTES; }
+};
+
+template <int DH> __device__ __forceinline__ void init_barriers(const Layout<DH> &L) {
+  using T = Layout<DH>;
+  mbar_init(L.res_full(), 1);
+  for (int i = 0; i < T::SA; ++i) mbar_init(L.a_full(i), 1), mbar_init(L.a_empty(i), 1);
+  for (int i = 0; i < T::SB; ++i) mbar_init(L.b_full(i), 1), mbar_init(L.b_empty(i), 1);
+  mbar_init(L.bar(T::S_FULL), 1);
+  mbar_init(L.bar(T::S_FULL + 1), 1);
+  mbar_init(L.bar(T::DP_FULL), 1);
+  mbar_init(L.bar(T::P_READY), 8);
+  mbar_init(L.bar(T::DS_READY), 8);
+  mbar_init(L.bar(T::DONE), 1);
+  for (int i = 0; i < STAT_STAGES; ++i) mbar_init(L.bar(T::STAT_FULL + i), 32), mbar_init(L.bar(T::STAT_EMPTY + i), 8);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-template <bool BF16> __global__ void __launch_bounds__(128) attention_dkv_rows_kernel(const BwdArgs a) {
-  __shared__ float ks[128], vs[128], ps[128], ds[128];
-  const int j = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  const int keys = key_count(a.key_lens, b, a.n_kv);
-  float dk = 0.0f, dv = 0.0f;
-  if (j < keys) {
-    if (t < a.d) {
-      ks[t] = to_f32<BF16>(a.k[b * a.sk.batch + hk * a.sk.head + j * a.sk.row + t]);
-      vs[t] = to_f32<BF16>(a.v[b * a.sv.batch + hk * a.sv.head + j * a.sv.row + t]);
+__device__ __forceinline__ void tmem_alloc(uint32_t slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(TMEM_COLS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ld_shared_2x2(uint32_t addr, uint64_t &a, uint64_t &b) {
+  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// The producer's two streams of tiles, in the order the products use them.
+template <int DH, typename LoadA, typename LoadB>
+__device__ __forceinline__ void produce(const Layout<DH> &L, int n, int ahead, unsigned *status, LoadA &&load_a, LoadB &&load_b) {
+  using T = Layout<DH>;
+  bool ok = true;
+  int na = 0, nb = 0;
+  auto a = [&]() {
+    if (!ok || na >= n) return;
+    if (na >= T::SA && !mbar_wait_relaxed(L.a_empty(na), L.a_phase(na) ^ 1u, kPollSleepNs)) {
+      ok = false;
+      return;
     }
-    __syncthreads();
-    for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
-      const uint16_t *q = a.q + b * a.sq.batch + h * a.sq.head;
-      const uint16_t *g = a.dout + b * a.sdo.batch + h * a.sdo.head;
-      for (int i0 = 0; i0 < a.n_q; i0 += 128) {
-        float p = 0.0f, x = 0.0f;
-        const int i = i0 + t;
-        if (i < a.n_q && j < visible_keys(i, keys, a.n_q, a.n_kv, a.causal)) {
-          float s = 0.0f, dp = 0.0f;
-          for (int c = 0; c < a.d; ++c) {
-            s = fmaf(to_f32<BF16>(q[i * a.sq.row + c]), ks[c], s);
-            dp = fmaf(to_f32<BF16>(g[i * a.sdo.row + c]), vs[c], dp);
+    mbar_expect_tx(L.a_full(na), T::TB);
+    load_a(na, L.a_tile(na), L.a_full(na));
+    ++na;
+  };
+  auto b = [&]() {
+    if (!ok || nb >= n) return;
+    if (nb >= T::SB && !mbar_wait_relaxed(L.b_empty(nb), L.b_phase(nb) ^ 1u, kPollSleepNs)) {
+      ok = false;
+      return;
+    }
+    mbar_expect_tx(L.b_full(nb), T::TB);
+    load_b(nb, L.b_tile(nb), L.b_full(nb));
+    ++nb;
+  };
+  for (int j = 0; j < ahead; ++j) a();  // A tiles are used `ahead` blocks earlier than the B tile of the same step
+  for (int j = 0; j < n; ++j) {
+    b();
+    a();
+  }
+  if (!ok) report(status, kStatusTmaWaitTimeout);
+  // every tile has been used before the CTA may go
+  for (int q = max(0, na - T::SA); q < na; ++q)
+    if (!mbar_wait_relaxed(L.a_empty(q), L.a_phase(q), kPollSleepNs)) break;
+  for (int q = max(0, nb - T::SB); q < nb; ++q)
+    if (!mbar_wait_relaxed(L.b_empty(q), L.b_phase(q), kPollSleepNs)) break;
+}
+
+// 16-bit results of one row from TMEM: COLS columns from `taddr`, times `factor` (0 where nothing was added up)
+template <bool BF16, int COLS>
+__device__ __forceinline__ void store_row(uint32_t taddr, bool has, float factor, uint16_t *to, bool exists) {
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t v[32];
+    if (has) {
+      tmem_ld_32x32(taddr + c, v);
+      tmem_ld_wait();
+    }
+    if (exists) {
+      float x[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = has ? __uint_as_float(v[e]) * factor : 0.0f;
+      uint4 *q = reinterpret_cast<uint4 *>(to + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        q[e] = make_uint4(pack2<BF16>(x[8 * e], x[8 * e + 1]), pack2<BF16>(x[8 * e + 2], x[8 * e + 3]),
+                          pack2<BF16>(x[8 * e + 4], x[8 * e + 5]), pack2<BF16>(x[8 * e + 6], x[8 * e + 7]));
+    }
+    __syncwarp();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ dQ
+// TMEM: S_0 [0,128) S_1 [128,256) dP / dS [256,384) dQ [384,512)
+template <bool BF16, int DH>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
+                    const BwdParams p) {
+  using T = Layout<DH>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
+  const T L{smem_u32(smem_raw)};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hb = blockIdx.x % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
+  const int qt = p.tiles - 1 - blockIdx.x / p.heads_batch;  // under the causal mask the long tiles come first
+  const int row0 = qt * TILE;
+  const int keys = key_count(p.key_lens, b, p.n_kv);
+  const int n = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + TILE - 1) / TILE;
+
+  if (threadIdx.x == 0) init_barriers<DH>(L);
+  if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT));
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = ld_shared_u32(L.bar(T::TMEM_SLOT));
+  const uint32_t dp_tmem = tmem + 2 * TILE, dq_tmem = tmem + 3 * TILE;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      if (lane == 0 && n > 0) {
+        mbar_expect_tx(L.res_full(), 2 * T::TB);
+        load_tile<DH>(L.resident(0), &tmap_q, row0, head, b, L.res_full());
+        load_tile<DH>(L.resident(1), &tmap_do, row0, head, b, L.res_full());
+        const int kv_head = head / p.group;
+        produce<DH>(L, n, 1, p.status,
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_k, j * TILE, kv_head, b, bar); },
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_v, j * TILE, kv_head, b, bar); });
+      }
+    } else if (warp == 1 && n > 0) {
+      bool ok = wait_all(L.res_full(), 0);
+      const int pad_block = keys < p.n_kv && keys % TILE ? keys / TILE : -1;
+      auto scores = [&](int j) {  // S_(j & 1) = Q K_j^T
+        ok = ok && wait_all(L.a_full(j), L.a_phase(j));
+        if (j == pad_block) {  // rows of K behind the sequence's last key: a B operand of dS K
+          const int first = keys % TILE, count = (TILE - first) * 8;  // 16-byte units per box
+          for (int e = lane; e < count * (DH / 64); e += 32) {
+            const uint32_t at = L.a_tile(j) + (e / count) * BOX_BYTES + first * 128 + (e % count) * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
-          const int64_t row = (static_cast<int64_t>(b) * a.q_heads + h) * a.n_q + i;
-          p = expf(s * a.scale - a.lse[row]);
-          x = p * (dp - a.delta[row]);
+          fence_async_smem();
+          __syncwarp();
         }
-        ps[t] = p;
-        ds[t] = x;
-        __syncthreads();
-        const int n = min(128, a.n_q - i0);
-        if (t < a.d)
-          for (int r = 0; r < n; ++r) {
-            dv = fmaf(ps[r], to_f32<BF16>(g[(i0 + r) * a.sdo.row + t]), dv);
-            dk = fmaf(ds[r], to_f32<BF16>(q[(i0 + r) * a.sq.row + t]), dk);
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_scores<DH>(tmem + (j & 1) * TILE, L.resident(0), L.a_tile(j), p.idesc_s);
+          tcgen05_commit(L.bar(T::S_FULL + (j & 1)));
+        }
+      };
+      auto products = [&](int j) {  // dP = dO V_j^T
+        ok = ok && wait_all(L.b_full(j), L.b_phase(j));
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s);
+          tcgen05_commit(L.bar(T::DP_FULL));
+          tcgen05_commit(L.b_empty(j));
+        }
+      };
+      scores(0);
+      products(0);
+      if (n > 1) scores(1);
+      for (int j = 0; j < n && ok; ++j) {
+        ok = wait_all(L.bar(T::DS_READY), j & 1);
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_rows<64>(dq_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0);
+          tcgen05_commit(L.a_empty(j));
+        }
+        if (j + 1 < n) products(j + 1);
+        if (j + 2 < n) scores(j + 2);
+      }
+      if (lane == 0 && ok) tcgen05_commit(L.bar(T::DONE));
+      if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int half = (warp - 4) >> 2, lane_group = warp & 3;
+    const int r = lane_group * 32 + lane, i = row0 + r;
+    const bool exists = i < p.n_q;
+    const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
+    // delta of this row (both halves add it up; the first one writes it)
+    float delta = 0.0f, lse2 = INFINITY;
+    if (exists) {
+      const uint4 *o = reinterpret_cast<const uint4 *>(p.o + b * p.so.batch + head * p.so.head + i * p.so.row);
+      const uint4 *g = reinterpret_cast<const uint4 *>(p.dout + b * p.sdo.batch + head * p.sdo.head + i * p.sdo.row);
+#pragma unroll 4
+      for (int c = 0; c < DH / 8; ++c) {
+        const uint4 x = o[c], y = g[c];
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 u = unpack2<BF16>(xs[e]), w = unpack2<BF16>(ys[e]);
+          delta = fmaf(u.x, w.x, delta);
+          delta = fmaf(u.y, w.y, delta);
+        }
+      }
+      const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head) * p.n_q + i;
+      const float lse = p.lse[row];
+      if (lse != -INFINITY) lse2 = lse * LOG2E;  // a row that sees no key: every probability is 2^-inf
+      if (half == 0) p.delta[row] = delta;
+    }
+    const int limit = exists ? visible_keys(i, keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
+    const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_lse2 = pack_f32x2(-lse2, -lse2);
+    const uint64_t neg_delta = pack_f32x2(-delta, -delta);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = wait_all(L.bar(T::S_FULL + (j & 1)), (j >> 1) & 1);
+      if (!ok) break;
+      tcgen05_fence_after();
+      uint64_t pr[32];
+      {
+        uint32_t s[2][32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32(tmem + lanes + (j & 1) * TILE + half * 64 + 32 * c, s[c]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_lse2), x0, x1);
+            pr[16 * c + e] = pack_f32x2(ex2(x0), ex2(x1));
           }
-        __syncthreads();
+      }
+      ok = wait_all(L.bar(T::DP_FULL), j & 1);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const int seen = limit - j * TILE - half * 64;  // of this thread's 64 keys
+      const bool masked = __any_sync(0xffffffffu, seen < 64);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t d[32], w[16];
+        tmem_ld_32x32(dp_tmem + lanes + half * 64 + 32 * c, d);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x0, x1;
+          unpack_f32x2(mul_f32x2(pr[16 * c + e], add_f32x2(pack_u32x2(d[2 * e], d[2 * e + 1]), neg_delta)), x0, x1);
+          if (masked) {
+            x0 = 32 * c + 2 * e < seen ? x0 : 0.0f;
+            x1 = 32 * c + 2 * e + 1 < seen ? x1 : 0.0f;
+          }
+          w[e] = pack2<BF16>(x0, x1);
+        }
+        // dS takes the place of this thread's own part of dP
+        tmem_st_16(dp_tmem + lanes + half * 64 + 16 * c, w);
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(L.bar(T::DS_READY));
+    }
+    if (ok && n > 0) ok = wait_all(L.bar(T::DONE), 0);
+    if (!ok) {
+      if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
+    } else {
+      tcgen05_fence_after();
+      uint16_t *to = p.dq + b * p.sdq.batch + head * p.sdq.head + i * p.sdq.row + half * (DH / 2);
+      store_row<BF16, DH / 2>(dq_tmem + lanes + half * (DH / 2), n > 0, p.scale, to, exists);
+    }
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_free(tmem);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- dK and dV
+// TMEM: S^T / P^T [0,128) dP^T / dS^T [128,256) dV [256,384) dK [384,512)
+template <bool BF16, int DH>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                     const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
+                     const BwdParams p) {
+  using T = Layout<DH>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
+  const T L{smem_u32(smem_raw)};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hb = blockIdx.x % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
+  const int key0 = blockIdx.x / p.heads_batch * TILE;  // under the causal mask the first keys have the most queries
+  const int keys = key_count(p.key_lens, b, p.n_kv);
+  // query i sees key j from i = j - (n_kv - n_q) on
+  const int shift = p.causal ? p.n_kv - p.n_q : 0;
+  const int tiles_q = (p.n_q + TILE - 1) / TILE;
+  const int first_tile = p.causal ? max(0, key0 - shift) / TILE : 0;
+  const int per_head = key0 < keys ? max(0, tiles_q - first_tile) : 0;
+  const int n = per_head * p.group;
+  auto head_of = [&](int j) { return kv_head * p.group + j / per_head; };
+  auto row_of = [&](int j) { return (first_tile + j % per_head) * TILE; };
+
+  if (threadIdx.x == 0) init_barriers<DH>(L);
+  if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT));
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = ld_shared_u32(L.bar(T::TMEM_SLOT));
+  const uint32_t dp_tmem = tmem + TILE, dv_tmem = tmem + 2 * TILE, dk_tmem = tmem + 3 * TILE;
+  auto stat_addr = [&](int j, int which) { return L.stats() + ((j % STAT_STAGES) * 2 + which) * TILE * 4; };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      if (lane == 0 && n > 0) {
+        mbar_expect_tx(L.res_full(), 2 * T::TB);
+        load_tile<DH>(L.resident(0), &tmap_k, key0, kv_head, b, L.res_full());
+        load_tile<DH>(L.resident(1), &tmap_v, key0, kv_head, b, L.res_full());
+        produce<DH>(L, n, 1, p.status,
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_q, row_of(j), head_of(j), b, bar); },
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_do, row_of(j), head_of(j), b, bar); });
+      }
+    } else if (warp == 1 && n > 0) {
+      bool ok = wait_all(L.res_full(), 0);
+      auto scores = [&](int j) {  // S^T = K Q_j^T
+        ok = ok && wait_all(L.a_full(j), L.a_phase(j));
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_scores<DH>(tmem, L.resident(0), L.a_tile(j), p.idesc_s);
+          tcgen05_commit(L.bar(T::S_FULL));
+        }
+      };
+      auto products = [&](int j) {  // dP^T = V dO_j^T
+        ok = ok && wait_all(L.b_full(j), L.b_phase(j));
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s);
+          tcgen05_commit(L.bar(T::DP_FULL));
+        }
+      };
+      scores(0);
+      products(0);
+      for (int j = 0; j < n && ok; ++j) {
+        ok = wait_all(L.bar(T::P_READY), j & 1);
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_rows<64>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0);
+          tcgen05_commit(L.b_empty(j));
+        }
+        if (j + 1 < n) scores(j + 1);
+        ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
+        if (lane == 0 && ok) {
+          tcgen05_fence_after();
+          mma_rows<64>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0);
+          tcgen05_commit(L.a_empty(j));
+        }
+        if (j + 1 < n) products(j + 1);
+      }
+      if (lane == 0 && ok) tcgen05_commit(L.bar(T::DONE));
+      if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
+    } else if (warp == 2) {
+      // row statistics of the query blocks: -log2(e) LSE and -delta.  Queries that do not exist or see no key
+      // get -inf for the first, which makes their probabilities 2^-inf.
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        if (j >= STAT_STAGES) ok = wait_all(L.bar(T::STAT_EMPTY + j % STAT_STAGES), (j / STAT_STAGES - 1) & 1);
+        if (!ok) break;
+        const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head_of(j)) * p.n_q;
+        const int i0 = row_of(j);
+#pragma unroll
+        for (int e = lane; e < TILE; e += 32) {
+          float s = -INFINITY, d = 0.0f;
+          if (i0 + e < p.n_q) {
+            const float lse = p.lse[row + i0 + e];
+            if (lse != -INFINITY) s = -lse * LOG2E;
+            d = -p.delta[row + i0 + e];
+          }
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_addr(j, 0) + e * 4), "f"(s) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_addr(j, 1) + e * 4), "f"(d) : "memory");
+        }
+        mbar_arrive(L.bar(T::STAT_FULL + j % STAT_STAGES));
       }
     }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int half = (warp - 4) >> 2, lane_group = warp & 3;
+    const int r = lane_group * 32 + lane, key = key0 + r;
+    const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
+    // first query that sees this thread's key
+    const int from = key < keys ? (p.causal ? max(0, key - shift) : 0) : INT32_MAX;
+    const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = wait_all(L.bar(T::STAT_FULL + j % STAT_STAGES), (j / STAT_STAGES) & 1) && wait_all(L.bar(T::S_FULL), j & 1);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const int i0 = row_of(j) + half * 64;
+      const bool masked = __any_sync(0xffffffffu, from > i0);
+      const int hidden = from - i0;  // of this thread's 64 queries, the first ones (0 or less: none)
+      uint64_t pr[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], w[16];
+        tmem_ld_32x32(tmem + lanes + half * 64 + 32 * c, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          uint64_t st[2];
+          ld_shared_2x2(stat_addr(j, 0) + (half * 64 + 32 * c + 2 * e) * 4, st[0], st[1]);
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_u32x2(s[2 * (e + f)], s[2 * (e + f) + 1]), scale2, st[f]), x0, x1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            if (masked) {
+              x0 = 32 * c + 2 * (e + f) >= hidden ? x0 : 0.0f;
+              x1 = 32 * c + 2 * (e + f) + 1 >= hidden ? x1 : 0.0f;
+            }
+            pr[16 * c + e + f] = pack_f32x2(x0, x1);
+            w[e + f] = pack2<BF16>(x0, x1);
+          }
+        }
+        tmem_st_16(tmem + lanes + half * 64 + 16 * c, w);
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(L.bar(T::P_READY));
+      ok = wait_all(L.bar(T::DP_FULL), j & 1);
+      if (!ok) break;
+      tcgen05_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t d[32], w[16];
+        tmem_ld_32x32(dp_tmem + lanes + half * 64 + 32 * c, d);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          uint64_t st[2];
+          ld_shared_2x2(stat_addr(j, 1) + (half * 64 + 32 * c + 2 * e) * 4, st[0], st[1]);
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            float x0, x1;
+            unpack_f32x2(mul_f32x2(pr[16 * c + e + f], add_f32x2(pack_u32x2(d[2 * (e + f)], d[2 * (e + f) + 1]), st[f])), x0, x1);
+            if (masked) {  // (P is 0 there, but 0 times the value of a padded row may be NaN)
+              x0 = 32 * c + 2 * (e + f) >= hidden ? x0 : 0.0f;
+              x1 = 32 * c + 2 * (e + f) + 1 >= hidden ? x1 : 0.0f;
+            }
+            w[e + f] = pack2<BF16>(x0, x1);
+          }
+        }
+        tmem_st_16(dp_tmem + lanes + half * 64 + 16 * c, w);
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(L.bar(T::DS_READY));
+        mbar_arrive(L.bar(T::STAT_EMPTY + j % STAT_STAGES));
+      }
+    }
+    if (ok && n > 0) ok = wait_all(L.bar(T::DONE), 0);
+    if (!ok) {
+      if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
+    } else {
+      tcgen05_fence_after();
+      // one warpgroup writes dV, the other dK
+      const bool exists = key < p.n_kv;
+      if (half == 0)
+        store_row<BF16, DH>(dv_tmem + lanes, n > 0, 1.0f, p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key * p.sdv.row, exists);
+      else
+        store_row<BF16, DH>(dk_tmem + lanes, n > 0, p.scale, p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key * p.sdk.row, exists);
+    }
   }
-  if (t < a.d) {
-    a.dk[b * a.sdk.batch + hk * a.sdk.head + j * a.sdk.row + t] = from_f32<BF16>(dk * a.scale);
-    a.dv[b * a.sdv.batch + hk * a.sdv.head + j * a.sdv.row + t] = from_f32<BF16>(dv);
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_free(tmem);
   }
+}
+
+template <bool BF16, int DH>
+cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tdo,
+                        BwdParams f, int64_t batch, cudaStream_t stream) {
+  cudaError_t e = allow_smem(attention_dq_kernel<BF16, DH>, smem_bytes(DH));
+  if (e == cudaSuccess) e = allow_smem(attention_dkv_kernel<BF16, DH>, smem_bytes(DH));
+  if (e != cudaSuccess) return e;
+  f.tiles = (f.n_q + TILE - 1) / TILE;
+  f.heads_batch = static_cast<int>(batch) * f.q_heads;
+  attention_dq_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, THREADS, smem_bytes(DH), stream>>>(tq, tk, tv, tdo, f);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  f.tiles = (f.n_kv + TILE - 1) / TILE;
+  f.heads_batch = static_cast<int>(batch) * f.kv_heads;
+  attention_dkv_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, THREADS, smem_bytes(DH), stream>>>(tq, tk, tv, tdo, f);
+  return cudaGetLastError();
 }
 
 } // namespace
 
-cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *, cudaStream_t stream, int *launched) {
-  auto in = [](const void *x) { return static_cast<const uint16_t *>(x); };
-  auto out = [](void *x) { return static_cast<uint16_t *>(x); };
-  BwdArgs a{in(p.q), in(p.k), in(p.v), in(p.o), in(p.dout), p.lse, static_cast<float *>(p.workspace),
-            out(p.dq), out(p.dk), out(p.dv), p.key_lens, p.sq, p.sk, p.sv, p.so, p.sdo, p.sdq, p.sdk, p.sdv,
-            static_cast<int>(p.q_heads), static_cast<int>(p.q_heads / p.kv_heads), static_cast<int>(p.n_q),
-            static_cast<int>(p.n_kv), static_cast<int>(p.d_head), p.causal ? 1 : 0, p.scale};
-  const dim3 gq(static_cast<unsigned>(p.n_q), static_cast<unsigned>(p.q_heads), static_cast<unsigned>(p.batch));
-  const dim3 gk(static_cast<unsigned>(p.n_kv), static_cast<unsigned>(p.kv_heads), static_cast<unsigned>(p.batch));
-  if (p.dtype == kBF16) {
-    attention_dq_rows_kernel<true><<<gq, 128, 0, stream>>>(a);
-    attention_dkv_rows_kernel<true><<<gk, 128, 0, stream>>>(a);
-  } else {
-    attention_dq_rows_kernel<false><<<gq, 128, 0, stream>>>(a);
-    attention_dkv_rows_kernel<false><<<gk, 128, 0, stream>>>(a);
-  }
+cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  const bool bf16 = p.dtype == kBF16;
+  CUtensorMap tq, tk, tv, tdo;
+  if (!make_map_4d(&tq, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq, TILE, 1) ||
+      !make_map_4d(&tdo, p.dout, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sdo, TILE, 1) ||
+      !make_map_4d(&tk, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, TILE, 1) ||
+      !make_map_4d(&tv, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, TILE, 1))
+    return cudaErrorNotSupported;
+  BwdParams f{};
+  f.o = static_cast<const uint16_t *>(p.o);
+  f.dout = static_cast<const uint16_t *>(p.dout);
+  f.lse = p.lse;
+  f.delta = static_cast<float *>(p.workspace);
+  f.dq = static_cast<uint16_t *>(p.dq);
+  f.dk = static_cast<uint16_t *>(p.dk);
+  f.dv = static_cast<uint16_t *>(p.dv);
+  f.key_lens = p.key_lens;
+  f.status = status;
+  f.so = p.so, f.sdo = p.sdo, f.sdq = p.sdq, f.sdk = p.sdk, f.sdv = p.sdv;
+  f.q_heads = static_cast<int>(p.q_heads);
+  f.kv_heads = static_cast<int>(p.kv_heads);
+  f.group = static_cast<int>(p.q_heads / p.kv_heads);
+  f.n_q = static_cast<int>(p.n_q);
+  f.n_kv = static_cast<int>(p.n_kv);
+  f.causal = p.causal ? 1 : 0;
+  f.scale = p.scale;
+  f.scale_log2e = p.scale * LOG2E;
+  f.idesc_s = instruction_desc(bf16, false, TILE);
+  f.idesc_o = instruction_desc(bf16, true, static_cast<int>(p.d_head));
   *launched = 2;
-  return cudaGetLastError();
+  if (p.d_head == 64)
+    return bf16 ? launch_both<true, 64>(tq, tk, tv, tdo, f, p.batch, stream)
+                : launch_both<false, 64>(tq, tk, tv, tdo, f, p.batch, stream);
+  return bf16 ? launch_both<true, 128>(tq, tk, tv, tdo, f, p.batch, stream)
+              : launch_both<false, 128>(tq, tk, tv, tdo, f, p.batch, stream);
 }
 
 } // namespace imex

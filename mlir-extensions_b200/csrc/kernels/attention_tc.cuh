@@ -53,12 +53,14 @@ __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_smem, uin
                     k ? 1u : 0u);
   }
 }
-// D[128 x DH] (+)= P . B over 128, P 16-bit pairs in TMEM, B a tile in shared memory as it lies (MN-major)
+// D[128 x DH] (+)= P . B over 128, P 16-bit pairs in TMEM (the second 64 values of a row HALF columns behind
+// the first), B a tile in shared memory as it lies (MN-major)
+template <int HALF>
 __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, uint32_t idesc,
                                          bool accumulate) {
 #pragma unroll
   for (int k = 0; k < TILE / 16; ++k)
-    mma_a_tmem(d_tmem, p_tmem + k * 8, make_smem_desc(b_smem + k * 2048, BOX_BYTES, 1024), idesc,
+    mma_a_tmem(d_tmem, p_tmem + (k >> 2) * HALF + (k & 3) * 8, make_smem_desc(b_smem + k * 2048, BOX_BYTES, 1024), idesc,
                (accumulate || k) ? 1u : 0u);
 }
 // c = f32; a, b formats; bit 16: B is MN-major; N >> 3; M >> 4

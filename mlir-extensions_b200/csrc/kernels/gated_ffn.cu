@@ -4,14 +4,31 @@
 // Backward: with [G U] = X W kept by the forward pass, one pass over G, U and dH writes
 // [dG dU] = [dH U act'(G), dH act(G)] into the workspace; because W holds both projections side by side,
 // dX = [dG dU] W^T and dW = X^T [dG dU] are then one product each of the framework's GEMM.
+//
+// Forward, by the number of tokens:
+//   gated_pair_kernel    more than 128 tokens: the CTA-pair GEMM's arrangement (gemm_tcgen05_2cta.cu) with a
+//                        256 x 256 accumulator whose left half is the gate and whose right half is the up
+//                        projection of the same 128 columns of H: CTA 0 of the pair loads the gate's 128
+//                        columns of W, CTA 1 the up projection's, and every thread of the epilogue has both
+//                        values of its elements in its own TMEM lane.
+//   gated_few_kernel     up to 128 tokens, where W's bytes are the time: W^T is the M operand (128 columns of
+//                        a projection per tile, as they lie), the tokens are the N operand, so that no
+//                        part of a tensor-core tile is wasted on rows that do not exist; k is shared out
+//                        between the CTAs of a cluster, which add their parts up through distributed
+//                        shared memory, in order.
+//   gated_tile_kernel    extents, pitches or addresses TMA cannot take (not multiples of 16 bytes).
 #include "attention_common.cuh"
 #include "epilogue.cuh"
+#include "tcgen05_host.h"
+#include "tcgen05_ptx.cuh"
 
 namespace imex {
 namespace {
 
 using attn::from_f32;
 using attn::to_f32;
+using namespace tc;
+using namespace tc_host;
 
 struct GatedArgs {
   const uint16_t *x, *w;
@@ -63,6 +80,351 @@ template <bool BF16> __global__ void __launch_bounds__(256) gated_tile_kernel(co
         a.gu[r * 2 * a.d_ff + a.d_ff + c] = from_f32<BF16>(u[i][j]);
       }
     }
+}
+
+// Eight consecutive results of a row.
+template <bool BF16> __device__ __forceinline__ void store8(uint16_t *to, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] = static_cast<uint32_t>(from_f32<BF16>(v[2 * e])) | (static_cast<uint32_t>(from_f32<BF16>(v[2 * e + 1])) << 16);
+  *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void tmem_alloc_one(uint32_t slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+
+// ------------------------------------------------------------------------------------------ many tokens
+namespace pair {
+constexpr int BM = 128;   // rows per CTA, 256 per pair
+constexpr int BF = 128;   // columns of H per tile
+constexpr int BK = 128;
+constexpr int STAGES = 3;
+constexpr int BOX = 128 * 128;        // 128 rows x 64 k of X, or 128 k x 64 columns of W
+constexpr int STAGE_BYTES = 4 * BOX;  // two boxes of each
+constexpr int THREADS = 192;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 256;
+struct Params {
+  uint16_t *h, *gu;
+  unsigned *status;
+  long long ldh;
+  int tokens, d_ff, act, tiles_m, tiles_f, num_tiles, k_blocks;
+  uint32_t idesc;
+};
+// Bands of eight row blocks: the tiles in flight share few columns of W and few rows of X.
+__device__ __forceinline__ void coords(int tile, const Params &p, int &mb, int &fb) {
+  const int band_tiles = 8 * p.tiles_f, band = tile / band_tiles, first = band * 8;
+  const int rows = min(8, p.tiles_m - first), t = tile - band * band_tiles;
+  fb = t / rows;
+  mb = first + t % rows;
+}
+} // namespace pair
+
+template <bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
+gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const pair::Params p) {
+  using namespace pair;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw), bars = base + STAGES * STAGE_BYTES;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  auto acc_full = [&](int a) { return bars + 8u * (2 * STAGES + a); };
+  auto acc_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
+  const uint32_t slot = bars + 8u * (2 * STAGES + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);   // used in CTA 0: its own expect-tx arrival
+      mbar_init(empty_bar(s), 1);  // one multicast commit per round
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 8);  // used in CTA 0: four epilogue warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers exist before anything signals them
+  tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (slot - base));
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < p.num_tiles && ok; tile += clusters) {
+        int mb, fb;
+        coords(tile, p, mb, fb);
+        const int row0 = mb * 2 * BM + static_cast<int>(rank) * BM;
+        const int col0 = fb * BF + (rank ? p.d_ff : 0);  // CTA 0: the gate's columns, CTA 1: the up projection's
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u)) {
+            report(p.status, kStatusTmaWaitTimeout);
+            ok = false;
+            break;
+          }
+          const uint32_t bar = map_to_cta(full_bar(stage), 0);
+          if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
+          const uint32_t x = base + stage * STAGE_BYTES, w = x + 2 * BOX;
+          tma_load_2d_pair(x, &tmap_x, kb * BK, row0, bar);
+          tma_load_2d_pair(x + BOX, &tmap_x, kb * BK + 64, row0, bar);
+          tma_load_2d_pair(w, &tmap_w, col0, kb * BK, bar);
+          tma_load_2d_pair(w + BOX, &tmap_w, col0 + 64, kb * BK, bar);
+          if (++stage == STAGES) stage = 0, phase ^= 1u;
+        }
+      }
+      // everything this CTA loaded has been used before it may go
+      for (int s = 0; s < STAGES; ++s) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1u)) break;
+        if (++stage == STAGES) stage = 0, phase ^= 1u;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = cluster; tile < p.num_tiles && ok; tile += clusters) {
+        ok = mbar_wait(acc_empty(acc), acc_phase ^ 1u);
+        tcgen05_fence_after();
+        for (int kb = 0; kb < p.k_blocks && ok; ++kb) {
+          ok = mbar_wait(full_bar(stage), phase);
+          if (!ok) break;
+          tcgen05_fence_after();
+          const uint32_t x = base + stage * STAGE_BYTES, w = x + 2 * BOX;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            tcgen05_mma_f16_pair(tmem + acc * 256, make_smem_desc(x + (k >> 2) * BOX + (k & 3) * 32, 16, 1024),
+                                 make_smem_desc(w + k * 2048, BOX, 1024), p.idesc, (kb | k) ? 1u : 0u);
+          tcgen05_commit_pair(empty_bar(stage), 3);
+          if (++stage == STAGES) stage = 0, phase ^= 1u;
+        }
+        if (ok) tcgen05_commit_pair(acc_full(acc), 3);
+        if (++acc == 2) acc = 0, acc_phase ^= 1u;
+      }
+      if (!ok) report(p.status, kStatusMmaWaitTimeout);
+    }
+  } else {
+    const int lane_group = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = cluster; tile < p.num_tiles; tile += clusters) {
+      int mb, fb;
+      coords(tile, p, mb, fb);
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full(acc), acc_phase))) {
+        if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
+        break;
+      }
+      tcgen05_fence_after();
+      const int row = mb * 2 * BM + static_cast<int>(rank) * BM + lane_group * 32 + lane;
+      const uint32_t t = tmem + (static_cast<uint32_t>(lane_group * 32) << 16) + acc * 256;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BF; c0 += 32) {
+        uint32_t g[32], u[32];
+        tmem_ld_32x32(t + c0, g);
+        tmem_ld_32x32(t + BF + c0, u);
+        tmem_ld_wait();
+        if (row < p.tokens) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            const int col = fb * BF + c0 + j;
+            if (col < p.d_ff) {  // d_ff is a multiple of 8 here
+              float x[8], y[8], v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                x[e] = __uint_as_float(g[j + e]);
+                y[e] = __uint_as_float(u[j + e]);
+                v[e] = apply_epilogue_fast(x[e], p.act) * y[e];
+              }
+              store8<BF16>(p.h + row * p.ldh + col, v);
+              if (p.gu) {
+                uint16_t *gu = p.gu + static_cast<long long>(row) * 2 * p.d_ff + col;
+                store8<BF16>(gu, x);
+                store8<BF16>(gu + p.d_ff, y);
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty(acc), 0));
+      if (++acc == 2) acc = 0, acc_phase ^= 1u;
+    }
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other may still touch its memory
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------- few tokens
+namespace few {
+constexpr int BF = 128;                 // columns of H per tile: the M of both products
+constexpr int BK = 64;
+constexpr int W_BOX = BK * 128;         // 64 k x 64 columns
+constexpr int W_BYTES = 4 * W_BOX;      // gate and up, two boxes each
+__host__ __device__ constexpr int stage_bytes(int nt) { return W_BYTES + nt * 128; }
+// two CTAs per SM up to 32 tokens (102 and 108 KB), one above
+__host__ __device__ constexpr int stages(int nt) { return nt <= 32 ? 3 : nt == 64 ? 5 : 4; }
+__host__ __device__ constexpr int smem_bytes(int nt) { return stages(nt) * stage_bytes(nt) + 256; }
+constexpr int THREADS = 192;
+struct Params {
+  uint16_t *h, *gu;
+  unsigned *status;
+  long long ldh;
+  int tokens, d_ff, act, k_blocks, shares;
+  uint32_t idesc;
+};
+} // namespace few
+
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(few::THREADS, NT <= 32 ? 2 : 1)
+gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const few::Params p) {
+  using namespace few;
+  constexpr int STAGES = stages(NT), STAGE_BYTES = stage_bytes(NT);
+  static_assert(2 * NT * BF * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw), bars = base + STAGES * STAGE_BYTES;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  const uint32_t acc_full = bars + 8u * (2 * STAGES), slot = acc_full + 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int f0 = blockIdx.x / p.shares * BF;
+  const int kb0 = p.k_blocks * rank / p.shares, kb1 = p.k_blocks * (rank + 1) / p.shares;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(acc_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc_one(slot, 2 * NT);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (slot - base));
+  float *sums = reinterpret_cast<float *>(smem_raw);  // [gate, up][NT][BF] once the ring is done with
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % STAGES;
+        if (i >= STAGES && !mbar_wait(empty_bar(s), (i / STAGES - 1) & 1)) {
+          report(p.status, kStatusTmaWaitTimeout);
+          break;
+        }
+        mbar_expect_tx(full_bar(s), STAGE_BYTES);
+        const uint32_t w = base + s * STAGE_BYTES;
+        tma_load_2d(w, &tmap_w, f0, kb * BK, full_bar(s));
+        tma_load_2d(w + W_BOX, &tmap_w, f0 + 64, kb * BK, full_bar(s));
+        tma_load_2d(w + 2 * W_BOX, &tmap_w, p.d_ff + f0, kb * BK, full_bar(s));
+        tma_load_2d(w + 3 * W_BOX, &tmap_w, p.d_ff + f0 + 64, kb * BK, full_bar(s));
+        tma_load_2d(w + W_BYTES, &tmap_x, kb * BK, 0, full_bar(s));
+      }
+      for (int i = max(0, kb1 - kb0 - STAGES); i < kb1 - kb0; ++i)  // everything has been used
+        if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1)) break;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % STAGES;
+        ok = mbar_wait(full_bar(s), (i / STAGES) & 1);
+        if (!ok) break;
+        tcgen05_fence_after();
+        const uint32_t w = base + s * STAGE_BYTES;
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) {
+          const uint64_t x = make_smem_desc(w + W_BYTES + k * 32, 16, 1024);
+          tcgen05_mma_f16(tmem, make_smem_desc(w + k * 2048, W_BOX, 1024), x, p.idesc, (i | k) ? 1u : 0u);
+          tcgen05_mma_f16(tmem + NT, make_smem_desc(w + 2 * W_BOX + k * 2048, W_BOX, 1024), x, p.idesc, (i | k) ? 1u : 0u);
+        }
+        tcgen05_commit(empty_bar(s));
+      }
+      if (ok) tcgen05_commit(acc_full);
+      else report(p.status, kStatusMmaWaitTimeout);
+    }
+  }
+  __syncwarp();
+  // sums of this CTA's share of k: lane = column of H, a row of `sums` per token
+  bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
+  if (warp >= 2) {
+    if (ok) {
+      tcgen05_fence_after();
+      const int lane_group = warp & 3;
+      const uint32_t t = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
+#pragma unroll 1
+      for (int c0 = 0; c0 < 2 * NT; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32(t + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) sums[(c0 + e) * BF + lane_group * 32 + lane] = __uint_as_float(v[e]);
+      }
+    } else if (lane == 0) {
+      report(p.status, kStatusEpiWaitTimeout);
+    }
+  }
+  if (p.shares > 1) cluster_sync_all();
+  else __syncthreads();
+  if (warp >= 2 && ok) {
+    const int c = threadIdx.x - 64, col = f0 + c;
+    if (col < p.d_ff) {
+      const uint32_t mine = base + c * 4;
+      for (int token = rank; token < p.tokens; token += p.shares) {
+        float g = 0.0f, u = 0.0f;
+        for (int r = 0; r < p.shares; ++r) {
+          const uint32_t from = p.shares > 1 ? map_to_cta(mine, r) : mine;
+          float x, y;
+          if (p.shares > 1) {
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from + token * BF * 4) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(from + (NT + token) * BF * 4) : "memory");
+          } else {
+            x = sums[token * BF + c];
+            y = sums[(NT + token) * BF + c];
+          }
+          g += x;
+          u += y;
+        }
+        p.h[token * p.ldh + col] = from_f32<BF16>(apply_epilogue_fast(g, p.act) * u);
+        if (p.gu) {
+          p.gu[static_cast<long long>(token) * 2 * p.d_ff + col] = from_f32<BF16>(g);
+          p.gu[static_cast<long long>(token) * 2 * p.d_ff + p.d_ff + col] = from_f32<BF16>(u);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  if (p.shares > 1) cluster_sync_all();  // the others may still read this CTA's sums
+  else __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT) : "memory");
+  }
 }
 
 struct GradArgs {
@@ -137,14 +499,110 @@ const char *gated_check(const GatedProblem &p) {
 
 size_t gated_bwd_workspace_bytes(const GatedProblem &p) { return dgu_bytes(p) + gemm_tcgen05_workspace_bytes(); }
 
-cudaError_t launch_gated(const GatedProblem &p, unsigned *, cudaStream_t stream, int *launched) {
+namespace {
+
+bool tma_takes(const GatedProblem &p) {
+  auto on16 = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  return p.d_in % 8 == 0 && p.d_ff % 8 == 0 && p.ldx % 8 == 0 && p.ldw % 8 == 0 && p.ldh % 8 == 0 && on16(p.x) &&
+         on16(p.w) && on16(p.h) && (!p.gu || on16(p.gu));
+}
+
+template <bool BF16, int NT>
+cudaError_t launch_few(const GatedProblem &p, const few::Params &f, cudaStream_t stream) {
+  CUtensorMap tx, tw;
+  if (!make_map(&tx, p.x, p.dtype, p.d_in, p.tokens, NT, pitch(p.ldx, p.d_in)) ||
+      !make_map(&tw, p.w, p.dtype, 2 * p.d_ff, p.d_in, few::BK, pitch(p.ldw, 2 * p.d_ff)))
+    return cudaErrorNotSupported;
+  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(gated_few_kernel<BF16, NT>),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, few::smem_bytes(NT));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.d_ff + few::BF - 1) / few::BF) * f.shares);
+  cfg.blockDim = dim3(few::THREADS);
+  cfg.dynamicSmemBytes = few::smem_bytes(NT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(f.shares);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, gated_few_kernel<BF16, NT>, tx, tw, f);
+}
+
+template <bool BF16> cudaError_t launch_few_tokens(const GatedProblem &p, unsigned *status, cudaStream_t stream) {
+  few::Params f{};
+  f.h = static_cast<uint16_t *>(p.h);
+  f.gu = static_cast<uint16_t *>(p.gu);
+  f.status = status;
+  f.ldh = pitch(p.ldh, p.d_ff);
+  f.tokens = static_cast<int>(p.tokens);
+  f.d_ff = static_cast<int>(p.d_ff);
+  f.act = p.act;
+  f.k_blocks = static_cast<int>((p.d_in + few::BK - 1) / few::BK);
+  const int nt = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
+  // Shares of k per tile: as many CTAs as run at once, at least two k blocks each.  One token of 4096 x 11264
+  // (88 tiles): 36.9 us with one share, 32.8 with 3 (what fits at once), 37.3 with 4; 8192 x 1024 (8 tiles): 55,
+  // 24.6 (3), 14.0 (8).
+  const int64_t tiles = (p.d_ff + few::BF - 1) / few::BF, slots = nt <= 32 ? 2 * 148 : 148;
+  int64_t shares = slots / tiles;
+  if (shares > 8) shares = 8;
+  if (shares > f.k_blocks / 2) shares = f.k_blocks / 2;
+  f.shares = shares < 1 ? 1 : static_cast<int>(shares);
+  const uint32_t fmt = BF16 ? 1u : 0u;
+  // f32 accumulator; A (W) is MN-major, B (X) K-major; N >> 3, M >> 4
+  f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (static_cast<uint32_t>(nt >> 3) << 17) |
+            (static_cast<uint32_t>(few::BF >> 4) << 24);
+  if (nt == 16) return launch_few<BF16, 16>(p, f, stream);
+  if (nt == 32) return launch_few<BF16, 32>(p, f, stream);
+  if (nt == 64) return launch_few<BF16, 64>(p, f, stream);
+  return launch_few<BF16, 128>(p, f, stream);
+}
+
+template <bool BF16> cudaError_t launch_many_tokens(const GatedProblem &p, unsigned *status, cudaStream_t stream) {
+  CUtensorMap tx, tw;
+  if (!make_map(&tx, p.x, p.dtype, p.d_in, p.tokens, pair::BM, pitch(p.ldx, p.d_in)) ||
+      !make_map(&tw, p.w, p.dtype, 2 * p.d_ff, p.d_in, pair::BK, pitch(p.ldw, 2 * p.d_ff)))
+    return cudaErrorNotSupported;
+  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(gated_pair_kernel<BF16>),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM_BYTES);
+  if (e != cudaSuccess) return e;
+  pair::Params f{};
+  f.h = static_cast<uint16_t *>(p.h);
+  f.gu = static_cast<uint16_t *>(p.gu);
+  f.status = status;
+  f.ldh = pitch(p.ldh, p.d_ff);
+  f.tokens = static_cast<int>(p.tokens);
+  f.d_ff = static_cast<int>(p.d_ff);
+  f.act = p.act;
+  f.tiles_m = static_cast<int>((p.tokens + 2 * pair::BM - 1) / (2 * pair::BM));
+  f.tiles_f = static_cast<int>((p.d_ff + pair::BF - 1) / pair::BF);
+  f.num_tiles = f.tiles_m * f.tiles_f;
+  f.k_blocks = static_cast<int>((p.d_in + pair::BK - 1) / pair::BK);
+  const uint32_t fmt = BF16 ? 1u : 0u;
+  // f32 accumulator; B (W) is MN-major; N = 256, M = 256
+  f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+  const int clusters = f.num_tiles < 74 ? f.num_tiles : 74;  // a pair of SMs each
+  gated_pair_kernel<BF16><<<2 * clusters, pair::THREADS, pair::SMEM_BYTES, stream>>>(tx, tw, f);
+  return cudaGetLastError();
+}
+
+} // namespace
+
+cudaError_t launch_gated(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  *launched = 1;
+  const bool bf16 = p.dtype == kBF16;
+  if (tma_takes(p)) {
+    if (p.tokens <= 128)
+      return bf16 ? launch_few_tokens<true>(p, status, stream) : launch_few_tokens<false>(p, status, stream);
+    return bf16 ? launch_many_tokens<true>(p, status, stream) : launch_many_tokens<false>(p, status, stream);
+  }
   GatedArgs a{static_cast<const uint16_t *>(p.x), static_cast<const uint16_t *>(p.w), static_cast<uint16_t *>(p.h),
               static_cast<uint16_t *>(p.gu), pitch(p.ldx, p.d_in), pitch(p.ldw, 2 * p.d_ff), pitch(p.ldh, p.d_ff),
               p.tokens, p.d_in, p.d_ff, p.act};
   const dim3 grid(static_cast<unsigned>((p.d_ff + 63) / 64), static_cast<unsigned>((p.tokens + 63) / 64));
-  if (p.dtype == kBF16) gated_tile_kernel<true><<<grid, 256, 0, stream>>>(a);
+  if (bf16) gated_tile_kernel<true><<<grid, 256, 0, stream>>>(a);
   else gated_tile_kernel<false><<<grid, 256, 0, stream>>>(a);
-  *launched = 1;
   return cudaGetLastError();
 }
 

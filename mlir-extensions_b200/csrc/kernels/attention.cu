@@ -30,6 +30,8 @@
 // Every wait is bounded; one that runs out records a status code and the role leaves its loop.
 #include "attention_tc.cuh"
 
+#include <type_traits>
+
 namespace imex {
 namespace {
 
@@ -38,6 +40,10 @@ using namespace tc;
 
 constexpr int THREADS = 384;
 constexpr unsigned kPollSleepNs = 40;
+#ifndef FMA8
+#define FMA8 2
+#endif
+constexpr int FMA_OF_8 = FMA8;
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512)
 constexpr int TMEM_COLS = 512;
 constexpr int O_COL = 256;
@@ -117,14 +123,14 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   auto kv_empty = [&](int pos) { return bars + 8u * (1 + STAGES + pos % STAGES); };
   auto kv_phase = [&](int pos) { return static_cast<uint32_t>(pos / STAGES) & 1u; };
   auto scores = [&](int g) { return bars + 8u * (1 + 2 * STAGES + g); };
-  auto probs = [&](int g) { return bars + 8u * (3 + 2 * STAGES + g); };
-  const uint32_t merge_bar = bars + 8u * (5 + 2 * STAGES);
-  const uint32_t tmem_slot = bars + 8u * (6 + 2 * STAGES);
-  static_assert(8 * (7 + 2 * STAGES) <= 256, "the barriers fit");
+  auto probs = [&](int g, int half) { return bars + 8u * (3 + 2 * STAGES + 2 * g + half); };
+  const uint32_t merge_bar = bars + 8u * (7 + 2 * STAGES);
+  const uint32_t tmem_slot = bars + 8u * (8 + 2 * STAGES);
+  static_assert(8 * (9 + 2 * STAGES) <= 256, "the barriers fit");
   volatile uint32_t *tmem_slot_ptr = reinterpret_cast<volatile uint32_t *>(smem_raw + (tmem_slot - smem_base));
   float2 *merge = reinterpret_cast<float2 *>(smem_raw + (bars + 256 - smem_base));
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const Work w = work_of<PACKED>(p);
   const int n_max = max(w.n[0], w.n[1]);
 
@@ -136,7 +142,8 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(scores(g), 1);
-      mbar_init(probs(g), 4);
+      mbar_init(probs(g, 0), 4);
+      mbar_init(probs(g, 1), 4);
     }
     mbar_init(merge_bar, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -206,28 +213,35 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       // the whole warp walks the loop (it zeroes padded V rows together), lane 0 issues
       if (n_max > 0) {
         bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
+        const uint32_t leader = elect_one();
         int pos = 0;
         const int pad_block = w.keys < p.n_kv && w.keys % TILE ? w.keys / TILE - w.kb0 : -1;
         auto wait_tile = [&](int q) {
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(kv_full(q), kv_phase(q)));
         };
         auto issue_scores = [&](int g, int q) {
-          if (lane == 0 && ok) {
+          if (ok) {
             tcgen05_fence_after();
-            mma_scores<DH>(tmem + g * TILE, q_smem(g), kv_smem(q), p.idesc_s);
-            tcgen05_commit(scores(g));
+            mma_scores<DH>(tmem + g * TILE, q_smem(g), kv_smem(q), p.idesc_s, leader);
+            commit(scores(g), leader);
           }
         };
         auto release = [&](int q) {
-          if (lane == 0 && ok) tcgen05_commit(kv_empty(q));
+          if (ok) commit(kv_empty(q), leader);
         };
         // O_g += P V of the stream's block jl; the last one signals the stream through its scores barrier
         auto issue_rows = [&](int g, int jl, int q) {
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g), jl & 1));
-          if (lane == 0 && ok) {
+          // in two halves, the first while the stream still computes the second
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g, 0), jl & 1));
+          if (ok) {
             tcgen05_fence_after();
-            mma_rows<32>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0);
-            if (jl + 1 == w.n[g]) tcgen05_commit(scores(g));
+            mma_rows<32, 0, 4>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0, leader);
+          }
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g, 1), jl & 1));
+          if (ok) {
+            tcgen05_fence_after();
+            mma_rows<32, 4, 8>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, true, leader);
+            if (jl + 1 == w.n[g]) commit(scores(g), leader);
           }
         };
         auto wait_v = [&](int q, int block) {
@@ -313,7 +327,8 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + 32 * c, s[c]);
       tmem_ld_wait();
       const int seen = limit - (w.kb0 + (PACKED ? 2 * j + g : j)) * TILE;  // of this block's keys
-      if (__any_sync(0xffffffffu, seen < TILE)) {
+      const bool masked = __any_sync(0xffffffffu, seen < TILE);
+      if (masked) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -355,23 +370,30 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       const float m_safe = m == neg_inf ? 0.0f : m;  // a row without a visible key: every exponent is -inf
       const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_m2 = pack_f32x2(-m_safe, -m_safe);
       uint64_t sum[2] = {0ull, 0ull};
+      auto exponentials = [&](auto fma_of_8) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pw[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pw[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x0, x1;
-          unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2), x0, x1);
-          const float e0 = ex2(x0), e1 = ex2(x1);
-          sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(e0, e1));
-          pw[e] = pack2<BF16>(e0, e1);
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t x = fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2);
+            const uint64_t y = ex2_pair<decltype(fma_of_8)::value>(x, e);
+            sum[e & 1] = add_f32x2(sum[e & 1], y);
+            float e0, e1;
+            unpack_f32x2(y, e0, e1);
+            pw[e] = pack2<BF16>(e0, e1);
+          }
+          tmem_st_16(s_addr + 16 * c, pw);
+          if (c & 1) {
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(probs(g, c >> 1));
+          }
         }
-        tmem_st_16(s_addr + 16 * c, pw);
-      }
-      tmem_st_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(probs(g));
+      };
+      if (masked) exponentials(std::integral_constant<int, 0>());
+      else exponentials(std::integral_constant<int, FMA_OF_8>());
       float lo, hi;
       unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
       l += lo + hi;

@@ -193,7 +193,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   using T = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
   const T L{smem_u32(smem_raw)};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hb = blockIdx.x % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
   const int qt = p.tiles - 1 - blockIdx.x / p.heads_batch;  // under the causal mask the long tiles come first
   const int row0 = qt * TILE;
@@ -222,6 +222,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       }
     } else if (warp == 1 && n > 0) {
       bool ok = wait_all(L.res_full(), 0);
+      const uint32_t leader = elect_one();
       const int pad_block = keys < p.n_kv && keys % TILE ? keys / TILE : -1;
       auto scores = [&](int j) {  // S_(j & 1) = Q K_j^T
         ok = ok && wait_all(L.a_full(j), L.a_phase(j));
@@ -234,19 +235,19 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           fence_async_smem();
           __syncwarp();
         }
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(tmem + (j & 1) * TILE, L.resident(0), L.a_tile(j), p.idesc_s);
-          tcgen05_commit(L.bar(T::S_FULL + (j & 1)));
+          mma_scores<DH>(tmem + (j & 1) * TILE, L.resident(0), L.a_tile(j), p.idesc_s, leader);
+          commit(L.bar(T::S_FULL + (j & 1)), leader);
         }
       };
       auto products = [&](int j) {  // dP = dO V_j^T
         ok = ok && wait_all(L.b_full(j), L.b_phase(j));
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s);
-          tcgen05_commit(L.bar(T::DP_FULL));
-          tcgen05_commit(L.b_empty(j));
+          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s, leader);
+          commit(L.bar(T::DP_FULL), leader);
+          commit(L.b_empty(j), leader);
         }
       };
       scores(0);
@@ -254,15 +255,15 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (n > 1) scores(1);
       for (int j = 0; j < n && ok; ++j) {
         ok = wait_all(L.bar(T::DS_READY), j & 1);
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_rows<64>(dq_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0);
-          tcgen05_commit(L.a_empty(j));
+          mma_rows<64>(dq_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
+          commit(L.a_empty(j), leader);
         }
         if (j + 1 < n) products(j + 1);
         if (j + 2 < n) scores(j + 2);
       }
-      if (lane == 0 && ok) tcgen05_commit(L.bar(T::DONE));
+      if (ok) commit(L.bar(T::DONE), leader);
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
     }
   } else {
@@ -372,7 +373,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   using T = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
   const T L{smem_u32(smem_raw)};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hb = blockIdx.x % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
   const int key0 = blockIdx.x / p.heads_batch * TILE;  // under the causal mask the first keys have the most queries
   const int keys = key_count(p.key_lens, b, p.n_kv);
@@ -407,41 +408,42 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       }
     } else if (warp == 1 && n > 0) {
       bool ok = wait_all(L.res_full(), 0);
+      const uint32_t leader = elect_one();
       auto scores = [&](int j) {  // S^T = K Q_j^T
         ok = ok && wait_all(L.a_full(j), L.a_phase(j));
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(tmem, L.resident(0), L.a_tile(j), p.idesc_s);
-          tcgen05_commit(L.bar(T::S_FULL));
+          mma_scores<DH>(tmem, L.resident(0), L.a_tile(j), p.idesc_s, leader);
+          commit(L.bar(T::S_FULL), leader);
         }
       };
       auto products = [&](int j) {  // dP^T = V dO_j^T
         ok = ok && wait_all(L.b_full(j), L.b_phase(j));
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s);
-          tcgen05_commit(L.bar(T::DP_FULL));
+          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s, leader);
+          commit(L.bar(T::DP_FULL), leader);
         }
       };
       scores(0);
       products(0);
       for (int j = 0; j < n && ok; ++j) {
         ok = wait_all(L.bar(T::P_READY), j & 1);
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_rows<64>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0);
-          tcgen05_commit(L.b_empty(j));
+          mma_rows<64>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0, leader);
+          commit(L.b_empty(j), leader);
         }
         if (j + 1 < n) scores(j + 1);
         ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
-        if (lane == 0 && ok) {
+        if (ok) {
           tcgen05_fence_after();
-          mma_rows<64>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0);
-          tcgen05_commit(L.a_empty(j));
+          mma_rows<64>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
+          commit(L.a_empty(j), leader);
         }
         if (j + 1 < n) products(j + 1);
       }
-      if (lane == 0 && ok) tcgen05_commit(L.bar(T::DONE));
+      if (ok) commit(L.bar(T::DONE), leader);
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
     } else if (warp == 2) {
       // row statistics of the query blocks: -log2(e) LSE and -delta.  Queries that do not exist or see no key

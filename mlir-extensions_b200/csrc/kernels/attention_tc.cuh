@@ -34,34 +34,63 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, 
 }
 
 // ---- products -----------------------------------------------------------------------------------
-__device__ __forceinline__ void mma_a_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// One thread issues.  The whole warp walks the code with the issuing thread as a predicate: behind a branch on
+// the lane every descriptor would be moved into uniform registers one at a time, which costs more than a
+// 128 x 128 x 16 product takes.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(leader)
       : "memory");
 }
 // D[128 x 128] = A . B^T over DH, both tiles in shared memory, rows of d_head values (K-major)
 template <int DH>
-__device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem, uint32_t idesc) {
+__device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem, uint32_t idesc,
+                                           uint32_t leader) {
+  const uint64_t a = make_smem_desc(a_smem, 16, 1024), b = make_smem_desc(b_smem, 16, 1024);
 #pragma unroll
   for (int k = 0; k < DH / 16; ++k) {
-    const uint32_t off = (k >> 2) * BOX_BYTES + (k & 3) * 32;
-    tcgen05_mma_f16(d_tmem, make_smem_desc(a_smem + off, 16, 1024), make_smem_desc(b_smem + off, 16, 1024), idesc,
-                    k ? 1u : 0u);
+    const uint64_t off = ((k >> 2) * BOX_BYTES + (k & 3) * 32) >> 4;
+    mma_ss(d_tmem, a + off, b + off, idesc, k ? 1u : 0u, leader);
   }
 }
 // D[128 x DH] (+)= P . B over 128, P 16-bit pairs in TMEM (the second 64 values of a row HALF columns behind
-// the first), B a tile in shared memory as it lies (MN-major)
-template <int HALF>
+// the first), B a tile in shared memory as it lies (MN-major); the 16-row steps [K0, K1) of it
+template <int HALF, int K0 = 0, int K1 = TILE / 16>
 __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, uint32_t idesc,
-                                         bool accumulate) {
+                                         bool accumulate, uint32_t leader) {
+  const uint64_t b = make_smem_desc(b_smem, BOX_BYTES, 1024);
 #pragma unroll
-  for (int k = 0; k < TILE / 16; ++k)
-    mma_a_tmem(d_tmem, p_tmem + (k >> 2) * HALF + (k & 3) * 8, make_smem_desc(b_smem + k * 2048, BOX_BYTES, 1024), idesc,
-               (accumulate || k) ? 1u : 0u);
+  for (int k = K0; k < K1; ++k)
+    mma_ts(d_tmem, p_tmem + (k >> 2) * HALF + (k & 3) * 8, b + static_cast<uint64_t>(k * 2048 >> 4), idesc,
+           (accumulate || k) ? 1u : 0u, leader);
 }
 // c = f32; a, b formats; bit 16: B is MN-major; N >> 3; M >> 4
 inline uint32_t instruction_desc(bool bf16, bool b_mn_major, int n) {
@@ -130,6 +159,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// 2^x for two values in [-125, 127) on the FMA pipe: n = x to the nearest integer (by adding 1.5 * 2^23),
+// 2^(x - n) from a polynomial of degree 4 on [-1/2, 1/2] (minimax in relative error with p(0) = 1: 2.9e-6), n
+// added to the exponent.  The special-function unit gives 16 exponentials a cycle and SM, which is less than the
+// tensor core needs; a part of them is taken here.
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t x) {
+  const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f);
+  const uint64_t t = add_f32x2(x, magic);
+  const uint64_t f = fma_f32x2(add_f32x2(t, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), x);
+  uint64_t p = fma_f32x2(pack_f32x2(0.009582852944731712f, 0.009582852944731712f), f,
+                         pack_f32x2(0.055906426161527634f, 0.055906426161527634f));
+  p = fma_f32x2(p, f, pack_f32x2(0.24024099111557007f, 0.24024099111557007f));
+  p = fma_f32x2(p, f, pack_f32x2(0.6931241750717163f, 0.6931241750717163f));
+  p = fma_f32x2(p, f, pack_f32x2(1.0f, 1.0f));
+  uint32_t lo, hi, n0, n1;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(p));
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(n0), "=r"(n1) : "l"(t));
+  return pack_u32x2(lo + (n0 << 23), hi + (n1 << 23));
+}
+// 2^x of a pair whose place in its row is `pair`; FMA_OF_8 of eight pairs on the FMA pipe (-inf only where that
+// is 0: the polynomial's smallest result is 2^-125)
+template <int FMA_OF_8> __device__ __forceinline__ uint64_t ex2_pair(uint64_t x, int pair) {
+  float x0, x1;
+  unpack_f32x2(x, x0, x1);
+  if ((pair * FMA_OF_8) % 8 < FMA_OF_8) return ex2_fma(pack_f32x2(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f)));
+  return pack_f32x2(ex2(x0), ex2(x1));
 }
 
 // ---- host ---------------------------------------------------------------------------------------

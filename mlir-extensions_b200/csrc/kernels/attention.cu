@@ -30,8 +30,6 @@
 // Every wait is bounded; one that runs out records a status code and the role leaves its loop.
 #include "attention_tc.cuh"
 
-#include <type_traits>
-
 namespace imex {
 namespace {
 
@@ -40,10 +38,6 @@ using namespace tc;
 
 constexpr int THREADS = 384;
 constexpr unsigned kPollSleepNs = 40;
-#ifndef FMA8
-#define FMA8 2
-#endif
-constexpr int FMA_OF_8 = FMA8;
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512)
 constexpr int TMEM_COLS = 512;
 constexpr int O_COL = 256;
@@ -327,8 +321,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + 32 * c, s[c]);
       tmem_ld_wait();
       const int seen = limit - (w.kb0 + (PACKED ? 2 * j + g : j)) * TILE;  // of this block's keys
-      const bool masked = __any_sync(0xffffffffu, seen < TILE);
-      if (masked) {
+      if (__any_sync(0xffffffffu, seen < TILE)) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -370,30 +363,25 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       const float m_safe = m == neg_inf ? 0.0f : m;  // a row without a visible key: every exponent is -inf
       const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_m2 = pack_f32x2(-m_safe, -m_safe);
       uint64_t sum[2] = {0ull, 0ull};
-      auto exponentials = [&](auto fma_of_8) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pw[16];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pw[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint64_t x = fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2);
-            const uint64_t y = ex2_pair<decltype(fma_of_8)::value>(x, e);
-            sum[e & 1] = add_f32x2(sum[e & 1], y);
-            float e0, e1;
-            unpack_f32x2(y, e0, e1);
-            pw[e] = pack2<BF16>(e0, e1);
-          }
-          tmem_st_16(s_addr + 16 * c, pw);
-          if (c & 1) {
-            tmem_st_wait();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(probs(g, c >> 1));
-          }
+        for (int e = 0; e < 16; ++e) {
+          float x0, x1;
+          unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2), x0, x1);
+          const float e0 = ex2(x0), e1 = ex2(x1);
+          sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(e0, e1));
+          pw[e] = pack2<BF16>(e0, e1);
         }
-      };
-      if (masked) exponentials(std::integral_constant<int, 0>());
-      else exponentials(std::integral_constant<int, FMA_OF_8>());
+        tmem_st_16(s_addr + 16 * c, pw);
+        if (c & 1) {
+          tmem_st_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(probs(g, c >> 1));
+        }
+      }
       float lo, hi;
       unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
       l += lo + hi;

@@ -79,9 +79,9 @@ template <int DH> struct Layout {
   __device__ uint32_t b_phase(int i) const { return (i / SB) & 1; }
   static constexpr int FIXED = 1 + 2 * SA + 2 * SB;
   __device__ uint32_t bar(int i) const { return bars() + 8 * (FIXED + i); }
-  static constexpr int S_FULL = 0, DP_FULL = 2, P_READY = 3, DS_READY = 4, DONE = 5, STAT_FULL = 6, STAT_EMPTY = 8;
-  static constexpr int TMEM_SLOT = 10;
-  static_assert(8 * (FIXED + 11) <= BAR_BYTES, "the barriers fit");
+  static constexpr int S_FULL = 0, S_READ = 1, DP_FULL = 2, P_READY = 4, DS_READY = 6, DONE = 8, STAT_FULL = 9, STAT_EMPTY = 11;
+  static constexpr int TMEM_SLOT = 13;
+  static_assert(8 * (FIXED + 14) <= BAR_BYTES, "the barriers fit");
   __device__ uint32_t stats() const { return bars() + BAR_BYTES; }
 };
 
@@ -91,10 +91,8 @@ template <int DH> __device__ __forceinline__ void init_barriers(const Layout<DH>
   for (int i = 0; i < T::SA; ++i) mbar_init(L.a_full(i), 1), mbar_init(L.a_empty(i), 1);
   for (int i = 0; i < T::SB; ++i) mbar_init(L.b_full(i), 1), mbar_init(L.b_empty(i), 1);
   mbar_init(L.bar(T::S_FULL), 1);
-  mbar_init(L.bar(T::S_FULL + 1), 1);
-  mbar_init(L.bar(T::DP_FULL), 1);
-  mbar_init(L.bar(T::P_READY), 8);
-  mbar_init(L.bar(T::DS_READY), 8);
+  mbar_init(L.bar(T::S_READ), 8);
+  for (int i = 0; i < 2; ++i) mbar_init(L.bar(T::DP_FULL + i), 1), mbar_init(L.bar(T::P_READY + i), 8), mbar_init(L.bar(T::DS_READY + i), 8);
   mbar_init(L.bar(T::DONE), 1);
   for (int i = 0; i < STAT_STAGES; ++i) mbar_init(L.bar(T::STAT_FULL + i), 32), mbar_init(L.bar(T::STAT_EMPTY + i), 8);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -184,7 +182,9 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bool has, float factor
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
-// TMEM: S_0 [0,128) S_1 [128,256) dP / dS [256,384) dQ [384,512)
+// TMEM: S [0,128), dP / dS of even and odd blocks [128,256) [256,384), dQ [384,512).  S is free for the next
+// block as soon as it has been read, dP has two places: the scores and products of block j + 1 run while the
+// warps still work on block j, so that the warps only ever wait for each other.
 template <bool BF16, int DH>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -206,7 +206,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = ld_shared_u32(L.bar(T::TMEM_SLOT));
-  const uint32_t dp_tmem = tmem + 2 * TILE, dq_tmem = tmem + 3 * TILE;
+  const uint32_t dq_tmem = tmem + 3 * TILE;
+  auto dp_tmem = [&](int j) { return tmem + TILE + (j & 1) * TILE; };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -224,7 +225,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       bool ok = wait_all(L.res_full(), 0);
       const uint32_t leader = elect_one();
       const int pad_block = keys < p.n_kv && keys % TILE ? keys / TILE : -1;
-      auto scores = [&](int j) {  // S_(j & 1) = Q K_j^T
+      auto scores = [&](int j) {  // S = Q K_j^T
         ok = ok && wait_all(L.a_full(j), L.a_phase(j));
         if (j == pad_block) {  // rows of K behind the sequence's last key: a B operand of dS K
           const int first = keys % TILE, count = (TILE - first) * 8;  // 16-byte units per box
@@ -237,31 +238,33 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(tmem + (j & 1) * TILE, L.resident(0), L.a_tile(j), p.idesc_s, leader);
-          commit(L.bar(T::S_FULL + (j & 1)), leader);
+          mma_scores<DH>(tmem, L.resident(0), L.a_tile(j), p.idesc_s, leader);
+          commit(L.bar(T::S_FULL), leader);
         }
       };
       auto products = [&](int j) {  // dP = dO V_j^T
         ok = ok && wait_all(L.b_full(j), L.b_phase(j));
         if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s, leader);
-          commit(L.bar(T::DP_FULL), leader);
+          mma_scores<DH>(dp_tmem(j), L.resident(1), L.b_tile(j), p.idesc_s, leader);
+          commit(L.bar(T::DP_FULL + (j & 1)), leader);
           commit(L.b_empty(j), leader);
         }
       };
       scores(0);
       products(0);
-      if (n > 1) scores(1);
       for (int j = 0; j < n && ok; ++j) {
-        ok = wait_all(L.bar(T::DS_READY), j & 1);
+        if (j + 1 < n) {
+          ok = wait_all(L.bar(T::S_READ), j & 1);
+          scores(j + 1);
+          products(j + 1);
+        }
+        ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
         if (ok) {
           tcgen05_fence_after();
-          mma_rows<64>(dq_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
+          mma_rows<64>(dq_tmem, dp_tmem(j), L.a_tile(j), p.idesc_o, j > 0, leader);
           commit(L.a_empty(j), leader);
         }
-        if (j + 1 < n) products(j + 1);
-        if (j + 2 < n) scores(j + 2);
       }
       if (ok) commit(L.bar(T::DONE), leader);
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
@@ -298,15 +301,18 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const uint64_t neg_delta = pack_f32x2(-delta, -delta);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = wait_all(L.bar(T::S_FULL + (j & 1)), (j >> 1) & 1);
+      ok = wait_all(L.bar(T::S_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
       uint64_t pr[32];
       {
         uint32_t s[2][32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld_32x32(tmem + lanes + (j & 1) * TILE + half * 64 + 32 * c, s[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32(tmem + lanes + half * 64 + 32 * c, s[c]);
         tmem_ld_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(L.bar(T::S_READ));
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -316,7 +322,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             pr[16 * c + e] = pack_f32x2(ex2(x0), ex2(x1));
           }
       }
-      ok = wait_all(L.bar(T::DP_FULL), j & 1);
+      ok = wait_all(L.bar(T::DP_FULL + (j & 1)), (j >> 1) & 1);
       if (!ok) break;
       tcgen05_fence_after();
       const int seen = limit - j * TILE - half * 64;  // of this thread's 64 keys
@@ -324,7 +330,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t d[32], w[16];
-        tmem_ld_32x32(dp_tmem + lanes + half * 64 + 32 * c, d);
+        tmem_ld_32x32(dp_tmem(j) + lanes + half * 64 + 32 * c, d);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -337,7 +343,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           w[e] = pack2<BF16>(x0, x1);
         }
         // dS takes the place of this thread's own part of dP
-        tmem_st_16(dp_tmem + lanes + half * 64 + 16 * c, w);
+        tmem_st_16(dp_tmem(j) + lanes + half * 64 + 16 * c, w);
       }
       tmem_st_wait();
       tcgen05_fence_before();
@@ -427,20 +433,27 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       };
       scores(0);
       products(0);
+      // a product over P or dS in two parts: both halves' first 32 columns, then their second ones
+      auto in_parts = [&](int ready, int j, uint32_t d, uint32_t a, uint32_t tile) {
+        ok = ok && wait_all(L.bar(ready), j & 1);
+        if (ok) {
+          tcgen05_fence_after();
+          mma_rows<64, 0, 2>(d, a, tile, p.idesc_o, j > 0, leader);
+          mma_rows<64, 4, 6>(d, a, tile, p.idesc_o, true, leader);
+        }
+        ok = ok && wait_all(L.bar(ready + 1), j & 1);
+        if (ok) {
+          tcgen05_fence_after();
+          mma_rows<64, 2, 4>(d, a, tile, p.idesc_o, true, leader);
+          mma_rows<64, 6, 8>(d, a, tile, p.idesc_o, true, leader);
+        }
+      };
       for (int j = 0; j < n && ok; ++j) {
-        ok = wait_all(L.bar(T::P_READY), j & 1);
-        if (ok) {
-          tcgen05_fence_after();
-          mma_rows<64>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0, leader);
-          commit(L.b_empty(j), leader);
-        }
+        in_parts(T::P_READY, j, dv_tmem, tmem, L.b_tile(j));
+        if (ok) commit(L.b_empty(j), leader);
         if (j + 1 < n) scores(j + 1);
-        ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
-        if (ok) {
-          tcgen05_fence_after();
-          mma_rows<64>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
-          commit(L.a_empty(j), leader);
-        }
+        in_parts(T::DS_READY, j, dk_tmem, dp_tmem, L.a_tile(j));
+        if (ok) commit(L.a_empty(j), leader);
         if (j + 1 < n) products(j + 1);
       }
       if (ok) commit(L.bar(T::DONE), leader);
@@ -509,11 +522,11 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
         }
         tmem_st_16(tmem + lanes + half * 64 + 16 * c, w);
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(L.bar(T::P_READY + c));
       }
-      tmem_st_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(L.bar(T::P_READY));
       ok = wait_all(L.bar(T::DP_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
@@ -538,14 +551,12 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           }
         }
         tmem_st_16(dp_tmem + lanes + half * 64 + 16 * c, w);
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(L.bar(T::DS_READY + c));
       }
-      tmem_st_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(L.bar(T::DS_READY));
-        mbar_arrive(L.bar(T::STAT_EMPTY + j % STAT_STAGES));
-      }
+      if (lane == 0) mbar_arrive(L.bar(T::STAT_EMPTY + j % STAT_STAGES));
     }
     if (ok && n > 0) ok = wait_all(L.bar(T::DONE), 0);
     if (!ok) {

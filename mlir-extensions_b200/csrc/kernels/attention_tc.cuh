@@ -161,33 +161,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x for two values in [-125, 127) on the FMA pipe: n = x to the nearest integer (by adding 1.5 * 2^23),
-// 2^(x - n) from a polynomial of degree 4 on [-1/2, 1/2] (minimax in relative error with p(0) = 1: 2.9e-6), n
-// added to the exponent.  The special-function unit gives 16 exponentials a cycle and SM, which is less than the
-// tensor core needs; a part of them is taken here.
-__device__ __forceinline__ uint64_t ex2_fma(uint64_t x) {
-  const uint64_t magic = pack_f32x2(12582912.0f, 12582912.0f);
-  const uint64_t t = add_f32x2(x, magic);
-  const uint64_t f = fma_f32x2(add_f32x2(t, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), x);
-  uint64_t p = fma_f32x2(pack_f32x2(0.009582852944731712f, 0.009582852944731712f), f,
-                         pack_f32x2(0.055906426161527634f, 0.055906426161527634f));
-  p = fma_f32x2(p, f, pack_f32x2(0.24024099111557007f, 0.24024099111557007f));
-  p = fma_f32x2(p, f, pack_f32x2(0.6931241750717163f, 0.6931241750717163f));
-  p = fma_f32x2(p, f, pack_f32x2(1.0f, 1.0f));
-  uint32_t lo, hi, n0, n1;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(p));
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(n0), "=r"(n1) : "l"(t));
-  return pack_u32x2(lo + (n0 << 23), hi + (n1 << 23));
-}
-// 2^x of a pair whose place in its row is `pair`; FMA_OF_8 of eight pairs on the FMA pipe (-inf only where that
-// is 0: the polynomial's smallest result is 2^-125)
-template <int FMA_OF_8> __device__ __forceinline__ uint64_t ex2_pair(uint64_t x, int pair) {
-  float x0, x1;
-  unpack_f32x2(x, x0, x1);
-  if ((pair * FMA_OF_8) % 8 < FMA_OF_8) return ex2_fma(pack_f32x2(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f)));
-  return pack_f32x2(ex2(x0), ex2(x1));
-}
-
 // ---- host ---------------------------------------------------------------------------------------
 // (d, row, head, batch) map of a 16-bit array with element strides, box [1, box_heads, box_rows, 64].
 inline bool make_map_4d(CUtensorMap *m, const void *base, int dtype, int64_t d, int64_t rows, int64_t heads,

@@ -216,7 +216,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         auto issue_scores = [&](int g, int q) {
           if (ok) {
             tcgen05_fence_after();
-            mma_scores<DH>(tmem + g * TILE, q_smem(g), kv_smem(q), p.idesc_s, leader);
+            mma_scores<DH, TILE>(tmem + g * TILE, q_smem(g), kv_smem(q), p.idesc_s, leader);
             commit(scores(g), leader);
           }
         };
@@ -229,12 +229,12 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g, 0), jl & 1));
           if (ok) {
             tcgen05_fence_after();
-            mma_rows<32, 0, 4>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0, leader);
+            mma_rows<TILE, 32, 0, 4>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0, leader);
           }
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g, 1), jl & 1));
           if (ok) {
             tcgen05_fence_after();
-            mma_rows<32, 4, 8>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, true, leader);
+            mma_rows<TILE, 32, 4, 8>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, true, leader);
             if (jl + 1 == w.n[g]) commit(scores(g), leader);
           }
         };
@@ -509,7 +509,7 @@ bool aligned(const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 template <bool BF16, int DH, bool PACKED>
 cudaError_t launch_variant(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const FwdParams &f,
                            unsigned grid, cudaStream_t stream) {
-  cudaError_t e = allow_smem(attention_kernel<BF16, DH, PACKED>, smem_bytes(DH, PACKED));
+  cudaError_t e = allow_smem<attention_kernel<BF16, DH, PACKED>>(smem_bytes(DH, PACKED));
   if (e != cudaSuccess) return e;
   attention_kernel<BF16, DH, PACKED><<<grid, THREADS, smem_bytes(DH, PACKED), stream>>>(tq, tk, tv, f);
   e = cudaGetLastError();

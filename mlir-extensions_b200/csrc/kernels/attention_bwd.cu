@@ -14,8 +14,11 @@
 //                          S^T = K Q^T, dP^T = V dO^T (a thread's row is a key), so that P^T and dS^T are A
 //                          operands from TMEM and dO and Q are used as they lie.
 //
-// Roles as in the forward kernel: warp 0 loads tiles (TMA), warp 1 issues products, warps 4-11 compute: two
-// warpgroups share every row's 128 columns, 64 each.  P and dS take the places of S and dP in TMEM as 16-bit
+// The walked blocks are as long as the head is wide: 128 rows for d_head 128; 64 rows for d_head 64, where a CTA
+// then needs half of the TMEM and of the shared memory, so that two run on an SM and fill each other's waits.
+//
+// Roles as in the forward kernel: warp 0 loads tiles (TMA), warp 1 issues products, warps 4 and up compute, 64
+// columns of a row per thread (with 128-row blocks two warpgroups share the rows).  P and dS take the places of S and dP in TMEM as 16-bit
 // pairs (each half in front of its own 64 columns, so that no thread overwrites what another still reads);
 // products run in the order they are issued, so overwriting a score tile is ordered by issuing the
 // next product behind the one that reads it.  While the warps compute P the tensor core runs the
@@ -31,20 +34,25 @@ namespace {
 using namespace attn;
 using namespace tc;
 
-constexpr int THREADS = 384;
 constexpr unsigned kPollSleepNs = 40;
-constexpr int TMEM_COLS = 512;
 constexpr float LOG2E = 1.4426950408889634f;
 
-__host__ __device__ constexpr int tile_bytes(int dh) { return TILE * dh * 2; }
-__host__ __device__ constexpr int stages_a(int dh) { return dh == 128 ? 3 : 4; }  // Q (dkv) or K (dq)
-__host__ __device__ constexpr int stages_b(int dh) { return dh == 128 ? 2 : 4; }  // dO (dkv) or V (dq)
-constexpr int STAT_STAGES = 2;
-constexpr int STAT_BYTES = STAT_STAGES * 2 * TILE * 4;
-constexpr int BAR_BYTES = 256;
-constexpr int smem_bytes(int dh) {
-  return (2 + stages_a(dh) + stages_b(dh)) * tile_bytes(dh) + BAR_BYTES + STAT_BYTES;
-}
+// Sizes by d_head.  BN: rows of a walked block.
+template <int DH> struct Sizes {
+  static constexpr int BN = DH;
+  static constexpr int CTAS = DH == 128 ? 1 : 2;           // per SM
+  static constexpr int THREADS = 128 + 2 * BN;             // a thread per row and 64 columns
+  static constexpr int WARPS = 2 * BN / 32;                // that compute
+  static constexpr int TMEM_COLS = 4 * BN;
+  static constexpr int RB = TILE * DH * 2, TB = BN * DH * 2;  // bytes of a resident tile and of a walked one
+  static constexpr int SA = DH == 128 ? 3 : 4, SB = DH == 128 ? 2 : 3;  // stages: Q (dkv) or K (dq); dO or V
+  static constexpr int STAT_STAGES = 2;
+  static constexpr int STAT_BYTES = STAT_STAGES * 2 * BN * 4;
+  static constexpr int BAR_BYTES = 256;
+  static constexpr int SMEM = 2 * RB + (SA + SB) * TB + BAR_BYTES + STAT_BYTES;
+};
+static_assert(Sizes<128>::SMEM <= 232448, "227 KB a CTA");
+static_assert(2 * (Sizes<64>::SMEM + 1024) <= 233472, "two CTAs per SM");
 
 struct BwdParams {
   const uint16_t *o, *dout;
@@ -59,17 +67,17 @@ struct BwdParams {
   uint32_t idesc_s, idesc_o;
 };
 
-static_assert(smem_bytes(128) <= 232448, "227 KB a CTA");
-
 // Barriers and buffers of one CTA, the same for both kernels: two resident tiles, a ring of A tiles and one
 // of B tiles.
-template <int DH> struct Layout {
-  static constexpr int SA = stages_a(DH), SB = stages_b(DH), TB = tile_bytes(DH);
+template <int DH> struct Layout : Sizes<DH> {
+  using Z = Sizes<DH>;
+  static constexpr int SA = Z::SA, SB = Z::SB, TB = Z::TB, RB = Z::RB;
   uint32_t base;
-  __device__ uint32_t resident(int i) const { return base + i * TB; }
-  __device__ uint32_t a_tile(int i) const { return base + (2 + i % SA) * TB; }
-  __device__ uint32_t b_tile(int i) const { return base + (2 + SA + i % SB) * TB; }
-  __device__ uint32_t bars() const { return base + (2 + SA + SB) * TB; }
+  __device__ explicit Layout(uint32_t b) : base(b) {}
+  __device__ uint32_t resident(int i) const { return base + i * RB; }
+  __device__ uint32_t a_tile(int i) const { return base + 2 * RB + (i % SA) * TB; }
+  __device__ uint32_t b_tile(int i) const { return base + 2 * RB + (SA + i % SB) * TB; }
+  __device__ uint32_t bars() const { return base + 2 * RB + (SA + SB) * TB; }
   __device__ uint32_t res_full() const { return bars(); }
   __device__ uint32_t a_full(int i) const { return bars() + 8 * (1 + i % SA); }
   __device__ uint32_t a_empty(int i) const { return bars() + 8 * (1 + SA + i % SA); }
@@ -79,10 +87,10 @@ template <int DH> struct Layout {
   __device__ uint32_t b_phase(int i) const { return (i / SB) & 1; }
   static constexpr int FIXED = 1 + 2 * SA + 2 * SB;
   __device__ uint32_t bar(int i) const { return bars() + 8 * (FIXED + i); }
-  static constexpr int S_FULL = 0, S_READ = 1, DP_FULL = 2, P_READY = 4, DS_READY = 6, DONE = 8, STAT_FULL = 9, STAT_EMPTY = 11;
-  static constexpr int TMEM_SLOT = 13;
-  static_assert(8 * (FIXED + 14) <= BAR_BYTES, "the barriers fit");
-  __device__ uint32_t stats() const { return bars() + BAR_BYTES; }
+  static constexpr int S_FULL = 0, S_READ = 1, DP_FULL = 2, P_READY = 4, DS_READY = 5, DONE = 6, STAT_FULL = 7, STAT_EMPTY = 9;
+  static constexpr int TMEM_SLOT = 11;
+  static_assert(8 * (FIXED + 12) <= Z::BAR_BYTES, "the barriers fit");
+  __device__ uint32_t stats() const { return bars() + Z::BAR_BYTES; }
 };
 
 template <int DH> __device__ __forceinline__ void init_barriers(const Layout<DH> &L) {
@@ -91,31 +99,41 @@ template <int DH> __device__ __forceinline__ void init_barriers(const Layout<DH>
   for (int i = 0; i < T::SA; ++i) mbar_init(L.a_full(i), 1), mbar_init(L.a_empty(i), 1);
   for (int i = 0; i < T::SB; ++i) mbar_init(L.b_full(i), 1), mbar_init(L.b_empty(i), 1);
   mbar_init(L.bar(T::S_FULL), 1);
-  mbar_init(L.bar(T::S_READ), 8);
-  for (int i = 0; i < 2; ++i) mbar_init(L.bar(T::DP_FULL + i), 1), mbar_init(L.bar(T::P_READY + i), 8), mbar_init(L.bar(T::DS_READY + i), 8);
+  mbar_init(L.bar(T::S_READ), T::WARPS);
+  for (int i = 0; i < 2; ++i) mbar_init(L.bar(T::DP_FULL + i), 1);
+  mbar_init(L.bar(T::P_READY), T::WARPS);
+  mbar_init(L.bar(T::DS_READY), T::WARPS);
   mbar_init(L.bar(T::DONE), 1);
-  for (int i = 0; i < STAT_STAGES; ++i) mbar_init(L.bar(T::STAT_FULL + i), 32), mbar_init(L.bar(T::STAT_EMPTY + i), 8);
+  for (int i = 0; i < T::STAT_STAGES; ++i) mbar_init(L.bar(T::STAT_FULL + i), 32), mbar_init(L.bar(T::STAT_EMPTY + i), T::WARPS);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_alloc(uint32_t slot) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(TMEM_COLS) : "memory");
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_free(uint32_t tmem) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void ld_shared_2x2(uint32_t addr, uint64_t &a, uint64_t &b) {
-  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr) : "memory");
-}
 __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// The computing warpgroups take registers over from the first one: 168 a thread at launch with three
+// warpgroups (72 + 2 * 216), 128 with two and two CTAs per SM (56 + 200).
+template <int DH> __device__ __forceinline__ void give_registers() {
+  if (DH == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+}
+template <int DH> __device__ __forceinline__ void take_registers() {
+  if (DH == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
 }
 
 // The producer's two streams of tiles, in the order the products use them.
@@ -157,6 +175,16 @@ __device__ __forceinline__ void produce(const Layout<DH> &L, int n, int ahead, u
     if (!mbar_wait_relaxed(L.b_empty(q), L.b_phase(q), kPollSleepNs)) break;
 }
 
+// 64 columns of this thread's row
+__device__ __forceinline__ void load_64(uint32_t taddr, uint32_t (&v)[64]) {
+  uint32_t lo[32], hi[32];
+  tmem_ld_32x32(taddr, lo);
+  tmem_ld_32x32(taddr + 32, hi);
+  tmem_ld_wait();
+#pragma unroll
+  for (int e = 0; e < 32; ++e) v[e] = lo[e], v[32 + e] = hi[e];
+}
+
 // 16-bit results of one row from TMEM: COLS columns from `taddr`, times `factor` (0 where nothing was added up)
 template <bool BF16, int COLS>
 __device__ __forceinline__ void store_row(uint32_t taddr, bool has, float factor, uint16_t *to, bool exists) {
@@ -182,55 +210,56 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bool has, float factor
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
-// TMEM: S [0,128), dP / dS of even and odd blocks [128,256) [256,384), dQ [384,512).  S is free for the next
+// TMEM, in units of BN columns: S [0,1), dP / dS of even and odd blocks [1,2) [2,3), dQ [3,4).  S is free for the next
 // block as soon as it has been read, dP has two places: the scores and products of block j + 1 run while the
 // warps still work on block j, so that the warps only ever wait for each other.
 template <bool BF16, int DH>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Sizes<DH>::THREADS, Sizes<DH>::CTAS)
 attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                     const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                     const BwdParams p) {
   using T = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
-  const T L{smem_u32(smem_raw)};
+  const T L(smem_u32(smem_raw));
+  constexpr int BN = T::BN;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hb = blockIdx.x % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
   const int qt = p.tiles - 1 - blockIdx.x / p.heads_batch;  // under the causal mask the long tiles come first
   const int row0 = qt * TILE;
   const int keys = key_count(p.key_lens, b, p.n_kv);
-  const int n = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + TILE - 1) / TILE;
+  const int n = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + BN - 1) / BN;
 
   if (threadIdx.x == 0) init_barriers<DH>(L);
-  if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT));
+  if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT), T::TMEM_COLS);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = ld_shared_u32(L.bar(T::TMEM_SLOT));
-  const uint32_t dq_tmem = tmem + 3 * TILE;
-  auto dp_tmem = [&](int j) { return tmem + TILE + (j & 1) * TILE; };
+  const uint32_t dq_tmem = tmem + 3 * BN;
+  auto dp_tmem = [&](int j) { return tmem + BN + (j & 1) * BN; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    give_registers<DH>();
     if (warp == 0) {
       if (lane == 0 && n > 0) {
-        mbar_expect_tx(L.res_full(), 2 * T::TB);
+        mbar_expect_tx(L.res_full(), 2 * T::RB);
         load_tile<DH>(L.resident(0), &tmap_q, row0, head, b, L.res_full());
         load_tile<DH>(L.resident(1), &tmap_do, row0, head, b, L.res_full());
         const int kv_head = head / p.group;
         produce<DH>(L, n, 1, p.status,
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_k, j * TILE, kv_head, b, bar); },
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_v, j * TILE, kv_head, b, bar); });
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_k, j * BN, kv_head, b, bar); },
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_v, j * BN, kv_head, b, bar); });
       }
     } else if (warp == 1 && n > 0) {
       bool ok = wait_all(L.res_full(), 0);
       const uint32_t leader = elect_one();
-      const int pad_block = keys < p.n_kv && keys % TILE ? keys / TILE : -1;
+      const int pad_block = keys < p.n_kv && keys % BN ? keys / BN : -1;
       auto scores = [&](int j) {  // S = Q K_j^T
         ok = ok && wait_all(L.a_full(j), L.a_phase(j));
         if (j == pad_block) {  // rows of K behind the sequence's last key: a B operand of dS K
-          const int first = keys % TILE, count = (TILE - first) * 8;  // 16-byte units per box
+          const int first = keys % BN, count = (BN - first) * 8;  // 16-byte units per box
           for (int e = lane; e < count * (DH / 64); e += 32) {
-            const uint32_t at = L.a_tile(j) + (e / count) * BOX_BYTES + first * 128 + (e % count) * 16;
+            const uint32_t at = L.a_tile(j) + (e / count) * (BN * 128) + first * 128 + (e % count) * 16;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
           fence_async_smem();
@@ -238,7 +267,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(tmem, L.resident(0), L.a_tile(j), p.idesc_s, leader);
+          mma_scores<DH, BN>(tmem, L.resident(0), L.a_tile(j), p.idesc_s, leader);
           commit(L.bar(T::S_FULL), leader);
         }
       };
@@ -246,7 +275,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         ok = ok && wait_all(L.b_full(j), L.b_phase(j));
         if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(dp_tmem(j), L.resident(1), L.b_tile(j), p.idesc_s, leader);
+          mma_scores<DH, BN>(dp_tmem(j), L.resident(1), L.b_tile(j), p.idesc_s, leader);
           commit(L.bar(T::DP_FULL + (j & 1)), leader);
           commit(L.b_empty(j), leader);
         }
@@ -262,7 +291,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
         if (ok) {
           tcgen05_fence_after();
-          mma_rows<64>(dq_tmem, dp_tmem(j), L.a_tile(j), p.idesc_o, j > 0, leader);
+          mma_rows<BN, 64>(dq_tmem, dp_tmem(j), L.a_tile(j), p.idesc_o, j > 0, leader);
           commit(L.a_empty(j), leader);
         }
       }
@@ -270,8 +299,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int half = (warp - 4) >> 2, lane_group = warp & 3;
+    take_registers<DH>();
+    const int half = BN == 128 ? (warp - 4) >> 2 : 0, lane_group = warp & 3;
     const int r = lane_group * 32 + lane, i = row0 + r;
     const bool exists = i < p.n_q;
     const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
@@ -304,46 +333,47 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       ok = wait_all(L.bar(T::S_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
+      const int seen = limit - j * BN - half * 64;  // of this thread's 64 keys
+      const bool masked = __any_sync(0xffffffffu, seen < 64);
       uint64_t pr[32];
       {
-        uint32_t s[2][32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld_32x32(tmem + lanes + half * 64 + 32 * c, s[c]);
-        tmem_ld_wait();
+        uint32_t s[64];
+        load_64(tmem + lanes + half * 64, s);
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(L.bar(T::S_READ));
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int e = 0; e < 64; ++e)
+            if (e >= seen) s[e] = __float_as_uint(-INFINITY);
+        }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_lse2), x0, x1);
-            pr[16 * c + e] = pack_f32x2(ex2(x0), ex2(x1));
-          }
+        for (int e = 0; e < 32; ++e) {
+          float x0, x1;
+          unpack_f32x2(fma_f32x2(pack_u32x2(s[2 * e], s[2 * e + 1]), scale2, neg_lse2), x0, x1);
+          pr[e] = pack_f32x2(ex2(x0), ex2(x1));
+        }
       }
       ok = wait_all(L.bar(T::DP_FULL + (j & 1)), (j >> 1) & 1);
       if (!ok) break;
       tcgen05_fence_after();
-      const int seen = limit - j * TILE - half * 64;  // of this thread's 64 keys
-      const bool masked = __any_sync(0xffffffffu, seen < 64);
+      {
+        uint32_t d[64], w[32];
+        load_64(dp_tmem(j) + lanes + half * 64, d);
+        if (masked) {  // (P is 0 there, but 0 times the product with a padded row may be NaN)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t d[32], w[16];
-        tmem_ld_32x32(dp_tmem(j) + lanes + half * 64 + 32 * c, d);
-        tmem_ld_wait();
+          for (int e = 0; e < 64; ++e)
+            if (e >= seen) d[e] = 0u;
+        }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 32; ++e) {
           float x0, x1;
-          unpack_f32x2(mul_f32x2(pr[16 * c + e], add_f32x2(pack_u32x2(d[2 * e], d[2 * e + 1]), neg_delta)), x0, x1);
-          if (masked) {
-            x0 = 32 * c + 2 * e < seen ? x0 : 0.0f;
-            x1 = 32 * c + 2 * e + 1 < seen ? x1 : 0.0f;
-          }
+          unpack_f32x2(mul_f32x2(pr[e], add_f32x2(pack_u32x2(d[2 * e], d[2 * e + 1]), neg_delta)), x0, x1);
           w[e] = pack2<BF16>(x0, x1);
         }
         // dS takes the place of this thread's own part of dP
-        tmem_st_16(dp_tmem(j) + lanes + half * 64 + 16 * c, w);
+        tmem_st_16(dp_tmem(j) + lanes + half * 64, w);
+        tmem_st_16(dp_tmem(j) + lanes + half * 64 + 16, w + 16);
       }
       tmem_st_wait();
       tcgen05_fence_before();
@@ -355,8 +385,9 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
     } else {
       tcgen05_fence_after();
-      uint16_t *to = p.dq + b * p.sdq.batch + head * p.sdq.head + i * p.sdq.row + half * (DH / 2);
-      store_row<BF16, DH / 2>(dq_tmem + lanes + half * (DH / 2), n > 0, p.scale, to, exists);
+      constexpr int COLS = DH * 4 / T::WARPS;  // a warpgroup's share of the columns
+      uint16_t *to = p.dq + b * p.sdq.batch + head * p.sdq.head + i * p.sdq.row + half * COLS;
+      store_row<BF16, COLS>(dq_tmem + lanes + half * COLS, n > 0, p.scale, to, exists);
     }
   }
 
@@ -365,52 +396,54 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_free(tmem);
+    tmem_free(tmem, T::TMEM_COLS);
   }
 }
 
 // ------------------------------------------------------------------------------------------- dK and dV
-// TMEM: S^T / P^T [0,128) dP^T / dS^T [128,256) dV [256,384) dK [384,512)
+// TMEM, in units of BN columns: S^T / P^T, dP^T / dS^T, dV, dK
 template <bool BF16, int DH>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Sizes<DH>::THREADS, Sizes<DH>::CTAS)
 attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                      const BwdParams p) {
   using T = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
-  const T L{smem_u32(smem_raw)};
+  const T L(smem_u32(smem_raw));
+  constexpr int BN = T::BN;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hb = blockIdx.x % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
   const int key0 = blockIdx.x / p.heads_batch * TILE;  // under the causal mask the first keys have the most queries
   const int keys = key_count(p.key_lens, b, p.n_kv);
   // query i sees key j from i = j - (n_kv - n_q) on
   const int shift = p.causal ? p.n_kv - p.n_q : 0;
-  const int tiles_q = (p.n_q + TILE - 1) / TILE;
-  const int first_tile = p.causal ? max(0, key0 - shift) / TILE : 0;
+  const int tiles_q = (p.n_q + BN - 1) / BN;
+  const int first_tile = p.causal ? max(0, key0 - shift) / BN : 0;
   const int per_head = key0 < keys ? max(0, tiles_q - first_tile) : 0;
   const int n = per_head * p.group;
   auto head_of = [&](int j) { return kv_head * p.group + j / per_head; };
-  auto row_of = [&](int j) { return (first_tile + j % per_head) * TILE; };
+  auto row_of = [&](int j) { return (first_tile + j % per_head) * BN; };
 
   if (threadIdx.x == 0) init_barriers<DH>(L);
-  if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT));
+  if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT), T::TMEM_COLS);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = ld_shared_u32(L.bar(T::TMEM_SLOT));
-  const uint32_t dp_tmem = tmem + TILE, dv_tmem = tmem + 2 * TILE, dk_tmem = tmem + 3 * TILE;
-  auto stat_addr = [&](int j, int which) { return L.stats() + ((j % STAT_STAGES) * 2 + which) * TILE * 4; };
+  const uint32_t dp_tmem = tmem + BN, dv_tmem = tmem + 2 * BN, dk_tmem = tmem + 3 * BN;
+  float *stats = reinterpret_cast<float *>(smem_raw + (L.stats() - L.base));
+  auto stat_of = [&](int j, int which) { return stats + ((j % T::STAT_STAGES) * 2 + which) * BN; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    give_registers<DH>();
     if (warp == 0) {
       if (lane == 0 && n > 0) {
-        mbar_expect_tx(L.res_full(), 2 * T::TB);
+        mbar_expect_tx(L.res_full(), 2 * T::RB);
         load_tile<DH>(L.resident(0), &tmap_k, key0, kv_head, b, L.res_full());
         load_tile<DH>(L.resident(1), &tmap_v, key0, kv_head, b, L.res_full());
         produce<DH>(L, n, 1, p.status,
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_q, row_of(j), head_of(j), b, bar); },
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH>(dst, &tmap_do, row_of(j), head_of(j), b, bar); });
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_q, row_of(j), head_of(j), b, bar); },
+                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_do, row_of(j), head_of(j), b, bar); });
       }
     } else if (warp == 1 && n > 0) {
       bool ok = wait_all(L.res_full(), 0);
@@ -419,7 +452,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         ok = ok && wait_all(L.a_full(j), L.a_phase(j));
         if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(tmem, L.resident(0), L.a_tile(j), p.idesc_s, leader);
+          mma_scores<DH, BN>(tmem, L.resident(0), L.a_tile(j), p.idesc_s, leader);
           commit(L.bar(T::S_FULL), leader);
         }
       };
@@ -427,33 +460,26 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         ok = ok && wait_all(L.b_full(j), L.b_phase(j));
         if (ok) {
           tcgen05_fence_after();
-          mma_scores<DH>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s, leader);
+          mma_scores<DH, BN>(dp_tmem, L.resident(1), L.b_tile(j), p.idesc_s, leader);
           commit(L.bar(T::DP_FULL), leader);
         }
       };
       scores(0);
       products(0);
-      // a product over P or dS in two parts: both halves' first 32 columns, then their second ones
-      auto in_parts = [&](int ready, int j, uint32_t d, uint32_t a, uint32_t tile) {
-        ok = ok && wait_all(L.bar(ready), j & 1);
-        if (ok) {
-          tcgen05_fence_after();
-          mma_rows<64, 0, 2>(d, a, tile, p.idesc_o, j > 0, leader);
-          mma_rows<64, 4, 6>(d, a, tile, p.idesc_o, true, leader);
-        }
-        ok = ok && wait_all(L.bar(ready + 1), j & 1);
-        if (ok) {
-          tcgen05_fence_after();
-          mma_rows<64, 2, 4>(d, a, tile, p.idesc_o, true, leader);
-          mma_rows<64, 6, 8>(d, a, tile, p.idesc_o, true, leader);
-        }
-      };
       for (int j = 0; j < n && ok; ++j) {
-        in_parts(T::P_READY, j, dv_tmem, tmem, L.b_tile(j));
-        if (ok) commit(L.b_empty(j), leader);
+        ok = wait_all(L.bar(T::P_READY), j & 1);
+        if (ok) {
+          tcgen05_fence_after();
+          mma_rows<BN, 64>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0, leader);
+          commit(L.b_empty(j), leader);
+        }
         if (j + 1 < n) scores(j + 1);
-        in_parts(T::DS_READY, j, dk_tmem, dp_tmem, L.a_tile(j));
-        if (ok) commit(L.a_empty(j), leader);
+        ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
+        if (ok) {
+          tcgen05_fence_after();
+          mma_rows<BN, 64>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
+          commit(L.a_empty(j), leader);
+        }
         if (j + 1 < n) products(j + 1);
       }
       if (ok) commit(L.bar(T::DONE), leader);
@@ -463,27 +489,31 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       // get -inf for the first, which makes their probabilities 2^-inf.
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
-        if (j >= STAT_STAGES) ok = wait_all(L.bar(T::STAT_EMPTY + j % STAT_STAGES), (j / STAT_STAGES - 1) & 1);
-        if (!ok) break;
         const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head_of(j)) * p.n_q;
         const int i0 = row_of(j);
+        float s[BN / 32], d[BN / 32];  // fetched before the wait for a free place
 #pragma unroll
-        for (int e = lane; e < TILE; e += 32) {
-          float s = -INFINITY, d = 0.0f;
-          if (i0 + e < p.n_q) {
-            const float lse = p.lse[row + i0 + e];
-            if (lse != -INFINITY) s = -lse * LOG2E;
-            d = -p.delta[row + i0 + e];
+        for (int e = 0; e < BN / 32; ++e) {
+          const int i = i0 + 32 * e + lane;
+          s[e] = -INFINITY, d[e] = 0.0f;
+          if (i < p.n_q) {
+            const float lse = p.lse[row + i];
+            if (lse != -INFINITY) s[e] = -lse * LOG2E;
+            d[e] = -p.delta[row + i];
           }
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_addr(j, 0) + e * 4), "f"(s) : "memory");
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_addr(j, 1) + e * 4), "f"(d) : "memory");
         }
-        mbar_arrive(L.bar(T::STAT_FULL + j % STAT_STAGES));
+        if (j >= T::STAT_STAGES) ok = wait_all(L.bar(T::STAT_EMPTY + j % T::STAT_STAGES), (j / T::STAT_STAGES - 1) & 1);
+#pragma unroll
+        for (int e = 0; e < BN / 32; ++e) {
+          stat_of(j, 0)[32 * e + lane] = s[e];
+          stat_of(j, 1)[32 * e + lane] = d[e];
+        }
+        mbar_arrive(L.bar(T::STAT_FULL + j % T::STAT_STAGES));
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int half = (warp - 4) >> 2, lane_group = warp & 3;
+    take_registers<DH>();
+    const int half = BN == 128 ? (warp - 4) >> 2 : 0, lane_group = warp & 3;
     const int r = lane_group * 32 + lane, key = key0 + r;
     const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
     // first query that sees this thread's key
@@ -491,83 +521,75 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = wait_all(L.bar(T::STAT_FULL + j % STAT_STAGES), (j / STAT_STAGES) & 1) && wait_all(L.bar(T::S_FULL), j & 1);
+      ok = wait_all(L.bar(T::STAT_FULL + j % T::STAT_STAGES), (j / T::STAT_STAGES) & 1) && wait_all(L.bar(T::S_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
       const int i0 = row_of(j) + half * 64;
       const bool masked = __any_sync(0xffffffffu, from > i0);
       const int hidden = from - i0;  // of this thread's 64 queries, the first ones (0 or less: none)
       uint64_t pr[32];
+      {
+        uint32_t s[64], w[32];
+        load_64(tmem + lanes + half * 64, s);
+        if (masked) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], w[16];
-        tmem_ld_32x32(tmem + lanes + half * 64 + 32 * c, s);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          uint64_t st[2];
-          ld_shared_2x2(stat_addr(j, 0) + (half * 64 + 32 * c + 2 * e) * 4, st[0], st[1]);
-#pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_u32x2(s[2 * (e + f)], s[2 * (e + f) + 1]), scale2, st[f]), x0, x1);
-            x0 = ex2(x0);
-            x1 = ex2(x1);
-            if (masked) {
-              x0 = 32 * c + 2 * (e + f) >= hidden ? x0 : 0.0f;
-              x1 = 32 * c + 2 * (e + f) + 1 >= hidden ? x1 : 0.0f;
-            }
-            pr[16 * c + e + f] = pack_f32x2(x0, x1);
-            w[e + f] = pack2<BF16>(x0, x1);
-          }
+          for (int e = 0; e < 64; ++e)
+            if (e < hidden) s[e] = __float_as_uint(-INFINITY);
         }
-        tmem_st_16(tmem + lanes + half * 64 + 16 * c, w);
-        tmem_st_wait();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(L.bar(T::P_READY + c));
+        const ulonglong2 *st = reinterpret_cast<const ulonglong2 *>(stat_of(j, 0) + half * 64);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float x0, x1;
+          unpack_f32x2(fma_f32x2(pack_u32x2(s[2 * e], s[2 * e + 1]), scale2, e & 1 ? st[e / 2].y : st[e / 2].x), x0, x1);
+          x0 = ex2(x0);
+          x1 = ex2(x1);
+          pr[e] = pack_f32x2(x0, x1);
+          w[e] = pack2<BF16>(x0, x1);
+        }
+        tmem_st_16(tmem + lanes + half * 64, w);
+        tmem_st_16(tmem + lanes + half * 64 + 16, w + 16);
       }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(L.bar(T::P_READY));
       ok = wait_all(L.bar(T::DP_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
+      {
+        uint32_t d[64], w[32];
+        load_64(dp_tmem + lanes + half * 64, d);
+        if (masked) {  // (P is 0 there, but 0 times the product with a padded row may be NaN)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t d[32], w[16];
-        tmem_ld_32x32(dp_tmem + lanes + half * 64 + 32 * c, d);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          uint64_t st[2];
-          ld_shared_2x2(stat_addr(j, 1) + (half * 64 + 32 * c + 2 * e) * 4, st[0], st[1]);
-#pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            float x0, x1;
-            unpack_f32x2(mul_f32x2(pr[16 * c + e + f], add_f32x2(pack_u32x2(d[2 * (e + f)], d[2 * (e + f) + 1]), st[f])), x0, x1);
-            if (masked) {  // (P is 0 there, but 0 times the value of a padded row may be NaN)
-              x0 = 32 * c + 2 * (e + f) >= hidden ? x0 : 0.0f;
-              x1 = 32 * c + 2 * (e + f) + 1 >= hidden ? x1 : 0.0f;
-            }
-            w[e + f] = pack2<BF16>(x0, x1);
-          }
+          for (int e = 0; e < 64; ++e)
+            if (e < hidden) d[e] = 0u;
         }
-        tmem_st_16(dp_tmem + lanes + half * 64 + 16 * c, w);
-        tmem_st_wait();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(L.bar(T::DS_READY + c));
+        const ulonglong2 *st = reinterpret_cast<const ulonglong2 *>(stat_of(j, 1) + half * 64);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float x0, x1;
+          unpack_f32x2(mul_f32x2(pr[e], add_f32x2(pack_u32x2(d[2 * e], d[2 * e + 1]), e & 1 ? st[e / 2].y : st[e / 2].x)), x0, x1);
+          w[e] = pack2<BF16>(x0, x1);
+        }
+        tmem_st_16(dp_tmem + lanes + half * 64, w);
+        tmem_st_16(dp_tmem + lanes + half * 64 + 16, w + 16);
       }
-      if (lane == 0) mbar_arrive(L.bar(T::STAT_EMPTY + j % STAT_STAGES));
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(L.bar(T::DS_READY));
+      if (lane == 0) mbar_arrive(L.bar(T::STAT_EMPTY + j % T::STAT_STAGES));
     }
     if (ok && n > 0) ok = wait_all(L.bar(T::DONE), 0);
     if (!ok) {
       if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
     } else {
       tcgen05_fence_after();
-      // one warpgroup writes dV, the other dK
+      // with two warpgroups one writes dV, the other dK
       const bool exists = key < p.n_kv;
       if (half == 0)
         store_row<BF16, DH>(dv_tmem + lanes, n > 0, 1.0f, p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key * p.sdv.row, exists);
-      else
+      if (half == 1 || BN == 64)
         store_row<BF16, DH>(dk_tmem + lanes, n > 0, p.scale, p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key * p.sdk.row, exists);
     }
   }
@@ -577,23 +599,25 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    tmem_free(tmem);
+    tmem_free(tmem, T::TMEM_COLS);
   }
 }
 
 template <bool BF16, int DH>
 cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tdo,
+                        const CUtensorMap &tqb, const CUtensorMap &tdob, const CUtensorMap &tkb, const CUtensorMap &tvb,
                         BwdParams f, int64_t batch, cudaStream_t stream) {
-  cudaError_t e = allow_smem(attention_dq_kernel<BF16, DH>, smem_bytes(DH));
-  if (e == cudaSuccess) e = allow_smem(attention_dkv_kernel<BF16, DH>, smem_bytes(DH));
+  using Z = Sizes<DH>;
+  cudaError_t e = allow_smem<attention_dq_kernel<BF16, DH>>(Z::SMEM);
+  if (e == cudaSuccess) e = allow_smem<attention_dkv_kernel<BF16, DH>>(Z::SMEM);
   if (e != cudaSuccess) return e;
   f.tiles = (f.n_q + TILE - 1) / TILE;
   f.heads_batch = static_cast<int>(batch) * f.q_heads;
-  attention_dq_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, THREADS, smem_bytes(DH), stream>>>(tq, tk, tv, tdo, f);
+  attention_dq_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, Z::THREADS, Z::SMEM, stream>>>(tq, tkb, tvb, tdo, f);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   f.tiles = (f.n_kv + TILE - 1) / TILE;
   f.heads_batch = static_cast<int>(batch) * f.kv_heads;
-  attention_dkv_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, THREADS, smem_bytes(DH), stream>>>(tq, tk, tv, tdo, f);
+  attention_dkv_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, Z::THREADS, Z::SMEM, stream>>>(tqb, tk, tv, tdob, f);
   return cudaGetLastError();
 }
 
@@ -601,11 +625,18 @@ cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUte
 
 cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
   const bool bf16 = p.dtype == kBF16;
-  CUtensorMap tq, tk, tv, tdo;
+  CUtensorMap tq, tk, tv, tdo, tqb, tkb, tvb, tdob;  // resident tiles, walked blocks
   if (!make_map_4d(&tq, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq, TILE, 1) ||
       !make_map_4d(&tdo, p.dout, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sdo, TILE, 1) ||
       !make_map_4d(&tk, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, TILE, 1) ||
       !make_map_4d(&tv, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, TILE, 1))
+    return cudaErrorNotSupported;
+  tqb = tq, tkb = tk, tvb = tv, tdob = tdo;
+  if (p.d_head == 64 &&
+      (!make_map_4d(&tqb, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq, 64, 1) ||
+       !make_map_4d(&tdob, p.dout, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sdo, 64, 1) ||
+       !make_map_4d(&tkb, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, 64, 1) ||
+       !make_map_4d(&tvb, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, 64, 1)))
     return cudaErrorNotSupported;
   BwdParams f{};
   f.o = static_cast<const uint16_t *>(p.o);
@@ -626,14 +657,14 @@ cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cu
   f.causal = p.causal ? 1 : 0;
   f.scale = p.scale;
   f.scale_log2e = p.scale * LOG2E;
-  f.idesc_s = instruction_desc(bf16, false, TILE);
+  f.idesc_s = instruction_desc(bf16, false, static_cast<int>(p.d_head));  // BN is d_head
   f.idesc_o = instruction_desc(bf16, true, static_cast<int>(p.d_head));
   *launched = 2;
   if (p.d_head == 64)
-    return bf16 ? launch_both<true, 64>(tq, tk, tv, tdo, f, p.batch, stream)
-                : launch_both<false, 64>(tq, tk, tv, tdo, f, p.batch, stream);
-  return bf16 ? launch_both<true, 128>(tq, tk, tv, tdo, f, p.batch, stream)
-              : launch_both<false, 128>(tq, tk, tv, tdo, f, p.batch, stream);
+    return bf16 ? launch_both<true, 64>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream)
+                : launch_both<false, 64>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream);
+  return bf16 ? launch_both<true, 128>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream)
+              : launch_both<false, 128>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream);
 }
 
 } // namespace imex

@@ -9,6 +9,8 @@
 #include "tcgen05_host.h"
 #include "tcgen05_ptx.cuh"
 
+#include <atomic>
+
 namespace imex {
 namespace attn {
 
@@ -26,11 +28,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
       "l"(map), "r"(x), "r"(row), "r"(head), "r"(batch), "r"(bar)
       : "memory");
 }
-template <int DH>
+template <int DH, int ROWS = TILE>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, int row, int head, int batch,
                                           uint32_t bar) {
 #pragma unroll
-  for (int j = 0; j < DH / 64; ++j) tma_load_4d(dst + j * BOX_BYTES, map, j * 64, row, head, batch, bar);
+  for (int j = 0; j < DH / 64; ++j) tma_load_4d(dst + j * (ROWS * 128), map, j * 64, row, head, batch, bar);
 }
 
 // ---- products -----------------------------------------------------------------------------------
@@ -70,23 +72,23 @@ __device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
       "r"(leader)
       : "memory");
 }
-// D[128 x 128] = A . B^T over DH, both tiles in shared memory, rows of d_head values (K-major)
-template <int DH>
+// D[128 x BN] = A . B^T over DH, both tiles in shared memory, rows of d_head values (K-major)
+template <int DH, int BN>
 __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem, uint32_t idesc,
                                            uint32_t leader) {
   const uint64_t a = make_smem_desc(a_smem, 16, 1024), b = make_smem_desc(b_smem, 16, 1024);
 #pragma unroll
   for (int k = 0; k < DH / 16; ++k) {
-    const uint64_t off = ((k >> 2) * BOX_BYTES + (k & 3) * 32) >> 4;
-    mma_ss(d_tmem, a + off, b + off, idesc, k ? 1u : 0u, leader);
+    const uint64_t ao = ((k >> 2) * BOX_BYTES + (k & 3) * 32) >> 4, bo = ((k >> 2) * (BN * 128) + (k & 3) * 32) >> 4;
+    mma_ss(d_tmem, a + ao, b + bo, idesc, k ? 1u : 0u, leader);
   }
 }
-// D[128 x DH] (+)= P . B over 128, P 16-bit pairs in TMEM (the second 64 values of a row HALF columns behind
+// D[128 x DH] (+)= P . B over BN, P 16-bit pairs in TMEM (the second 64 values of a row HALF columns behind
 // the first), B a tile in shared memory as it lies (MN-major); the 16-row steps [K0, K1) of it
-template <int HALF, int K0 = 0, int K1 = TILE / 16>
+template <int BN, int HALF, int K0 = 0, int K1 = BN / 16>
 __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, uint32_t idesc,
                                          bool accumulate, uint32_t leader) {
-  const uint64_t b = make_smem_desc(b_smem, BOX_BYTES, 1024);
+  const uint64_t b = make_smem_desc(b_smem, BN * 128, 1024);
 #pragma unroll
   for (int k = K0; k < K1; ++k)
     mma_ts(d_tmem, p_tmem + (k >> 2) * HALF + (k & 3) * 8, b + static_cast<uint64_t>(k * 2048 >> 4), idesc,
@@ -181,8 +183,17 @@ inline bool make_map_4d(CUtensorMap *m, const void *base, int dtype, int64_t d, 
 }
 
 // Dynamic shared memory beyond 48 KB has to be asked for on every device a kernel runs on.
-template <typename K> cudaError_t allow_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// `kernel` is a template argument so that each has its own record of where that was done.
+template <auto kernel> cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 } // namespace attn

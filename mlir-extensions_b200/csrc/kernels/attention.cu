@@ -3,15 +3,21 @@
 // maximum m per row that moves only when the row's maximum outgrows it by more than 2^8 (only then are O, in
 // TMEM, and the running sum l rescaled); at the end O / l and LSE = ln 2 (m + log2 l).
 //
-// A CTA runs two streams, each with its own scores S (128 x 128 f32 in TMEM, P takes its place as 16-bit
+// Three arrangements:
+//
+//   solo     d_head 64: a CTA holds one tile of 128 query rows and half of the SM's TMEM and shared memory, so that
+//            two run on an SM.  P has TMEM columns of its own, so the next block's scores are computed while the
+//            warps still work on this one.
+//
+// With d_head 128 S, P and O leave no such room; a CTA runs two streams instead, each with its own scores S (128 x 128 f32 in TMEM, P takes its place as 16-bit
 // pairs) and its own accumulator O, so that the tensor core works for one stream while the other computes
 // exponentials.  Both masks leave every row a prefix of the keys, so a tile stops at the last key any of its
 // rows sees and only the blocks behind the first row's prefix compare indices.
 //
-//   paired   the streams are two neighbouring tiles of 128 query rows of one head; they share every K and V
+//   paired   more than 128 rows per key head: the streams are two neighbouring tiles of 128 query rows of one head; they share every K and V
 //            tile (tiles [256 t, 256 t + 256)).
 //   packed   all n_q rows of all query heads of one key head fit into one tile (n_q * group <= 128: decoding,
-//            short chunks): both streams hold that tile and take every other key block; merged at the end.
+//            short chunks; also with d_head 64): both streams hold that tile and take every other key block; merged at the end.
 //
 // When there are fewer tiles than SMs the key blocks of a tile are shared out between `splits` CTAs, which
 // leave O (unnormalised), m and l in the workspace; attention_join_kernel adds them up in order.
@@ -99,6 +105,103 @@ template <bool PACKED> __device__ __forceinline__ Work work_of(const FwdParams &
     w.n[1] = max(0, min(n1, kb1) - w.kb0);
   }
   return w;
+}
+
+// ---- one block of a row's keys, a row per thread -----------------------------------------------------
+// Scores of keys the row does not see become -inf; seen: of this block's keys, may be negative or large.
+__device__ __forceinline__ void mask_scores(uint32_t (&s)[4][32], int seen) {
+  if (__any_sync(0xffffffffu, seen < TILE)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (32 * c + e >= seen) s[c][e] = __float_as_uint(-INFINITY);
+  }
+}
+__device__ __forceinline__ float row_maximum(const uint32_t (&s)[4][32]) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) top[c] = max3(top[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+// Moves the reference maximum where the row's outgrows it by more than 2^8: O and l shrink by 2^(m - row_max).
+// O must not be in use by a product.
+template <int DH> __device__ __forceinline__ void move_reference(float &m, float &l, float row_max, uint32_t o_addr) {
+  const bool move = row_max > m + 8.0f;
+  if (!__any_sync(0xffffffffu, move)) return;
+  const float a = move ? ex2(m - row_max) : 1.0f;
+#pragma unroll 1
+  for (int c = 0; c < DH; c += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32(o_addr + c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * a);
+    tmem_st_16(o_addr + c, v);
+    tmem_st_16(o_addr + c + 16, v + 16);
+  }
+  l *= a;
+  if (move) m = row_max;
+}
+// P = 2^(scale s - m) as 16-bit pairs to p_addr; ready(half) after each 64 keys; returns the sum of P.
+template <bool BF16, typename Ready>
+__device__ __forceinline__ float exponentials(const uint32_t (&s)[4][32], float scale_log2e, float m, uint32_t p_addr,
+                                              Ready &&ready) {
+  const float m_safe = m == -INFINITY ? 0.0f : m;  // a row without a visible key: every exponent is -inf
+  const uint64_t scale2 = pack_f32x2(scale_log2e, scale_log2e), neg_m2 = pack_f32x2(-m_safe, -m_safe);
+  uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pw[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float x0, x1;
+      unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2), x0, x1);
+      const float e0 = ex2(x0), e1 = ex2(x1);
+      sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(e0, e1));
+      pw[e] = pack2<BF16>(e0, e1);
+    }
+    tmem_st_16(p_addr + 16 * c, pw);
+    if (c & 1) {
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      ready(c >> 1);
+    }
+  }
+  float lo, hi;
+  unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l > 0.0f ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
+}
+// 32 results of a row: f32 into the workspace (splits) or rounded into O
+template <bool BF16, int DH>
+__device__ __forceinline__ void store_32(const FwdParams &p, const float (&x)[32], int split, int64_t row, uint16_t *o, int c) {
+  if (p.splits > 1) {
+    float4 *to = reinterpret_cast<float4 *>(p.part_o + (split * p.rows + row) * DH + c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+  } else {
+    uint4 *to = reinterpret_cast<uint4 *>(o + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      to[e] = make_uint4(pack2<BF16>(x[8 * e], x[8 * e + 1]), pack2<BF16>(x[8 * e + 2], x[8 * e + 3]),
+                         pack2<BF16>(x[8 * e + 4], x[8 * e + 5]), pack2<BF16>(x[8 * e + 6], x[8 * e + 7]));
+  }
+}
+// Rows [first, TILE) of a tile in shared memory to zero, by a whole warp, before products read them
+template <int DH> __device__ __forceinline__ void zero_rows(uint32_t tile, int first, int lane) {
+  const int count = (TILE - first) * 8;  // 16-byte units per box
+  for (int e = lane; e < count * (DH / 64); e += 32) {
+    const uint32_t at = tile + (e / count) * BOX_BYTES + first * 128 + (e % count) * 16;
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+  }
+  fence_async_smem();
+  __syncwarp();
 }
 
 template <bool BF16, int DH, bool PACKED>
@@ -240,17 +343,9 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         };
         auto wait_v = [&](int q, int block) {
           wait_tile(q);
-          if (block == pad_block) {  // rows of V behind the sequence's last key
-            const int first = w.keys % TILE, count = (TILE - first) * 8;  // 16-byte units per box
-            for (int e = lane; e < count * (DH / 64); e += 32) {
-              const uint32_t at = kv_smem(q) + (e / count) * BOX_BYTES + first * 128 + (e % count) * 16;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-            }
-            fence_async_smem();
-            __syncwarp();
-          }
+          if (block == pad_block) zero_rows<DH>(kv_smem(q), w.keys % TILE, lane);  // V behind the sequence's last key
         };
-        if (PACKED) {
+      if (PACKED) {
           const int nb = w.n[0] + w.n[1];
           for (int g = 0; g < 2 && g < nb; ++g) {
             wait_tile(pos);
@@ -321,70 +416,13 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + 32 * c, s[c]);
       tmem_ld_wait();
       const int seen = limit - (w.kb0 + (PACKED ? 2 * j + g : j)) * TILE;  // of this block's keys
-      if (__any_sync(0xffffffffu, seen < TILE)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * c + e >= seen) s[c][e] = __float_as_uint(neg_inf);
-      }
-      float top[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; e += 2)
-          top[c] = max3(top[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-      const float row_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2e;
-      if (j == 0) {
-        m = row_max;
-      } else {
-        const bool move = row_max > m + 8.0f;
-        if (__any_sync(0xffffffffu, move)) {
-          const float a = move ? ex2(m - row_max) : 1.0f;
-#pragma unroll 1
-          for (int c = 0; c < DH; c += 16) {
-            uint32_t v[16];
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                : "r"(o_addr + c)
-                : "memory");
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * a);
-            tmem_st_16(o_addr + c, v);
-          }
-          l *= a;
-          if (move) m = row_max;
-        }
-      }
-      const float m_safe = m == neg_inf ? 0.0f : m;  // a row without a visible key: every exponent is -inf
-      const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_m2 = pack_f32x2(-m_safe, -m_safe);
-      uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pw[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x0, x1;
-          unpack_f32x2(fma_f32x2(pack_u32x2(s[c][2 * e], s[c][2 * e + 1]), scale2, neg_m2), x0, x1);
-          const float e0 = ex2(x0), e1 = ex2(x1);
-          sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(e0, e1));
-          pw[e] = pack2<BF16>(e0, e1);
-        }
-        tmem_st_16(s_addr + 16 * c, pw);
-        if (c & 1) {
-          tmem_st_wait();
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(probs(g, c >> 1));
-        }
-      }
-      float lo, hi;
-      unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
-      l += lo + hi;
+      mask_scores(s, seen);
+      const float row_max = row_maximum(s) * p.scale_log2e;
+      if (j == 0) m = row_max;
+      else move_reference<DH>(m, l, row_max, o_addr);  // (P V of the block before is done: it was issued before these scores)
+      l += exponentials<BF16>(s, p.scale_log2e, m, s_addr, [&](int half) {
+        if (lane == 0) mbar_arrive(probs(g, half));
+      });
     }
     if (ok && n > 0) {
       ok = mbar_wait(scores(g), n & 1);  // the last P V
@@ -420,7 +458,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       a1 *= inv;
       if (exists && (!PACKED || g == 0)) {
         if (p.splits > 1) p.part_ml[w.split * p.rows + row] = make_float2(m, l);
-        else p.lse[row] = some ? 0.6931471805599453f * (m + log2f(l)) : neg_inf;
+        else p.lse[row] = row_lse(m, l);
       }
 #pragma unroll 1
       for (int c = col0; c < col0 + COLS; c += 32) {
@@ -434,17 +472,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
           x[e] = has0 && some ? __uint_as_float(v0[e]) * a0 : 0.0f;
           if (has1 && some) x[e] = fmaf(__uint_as_float(v1[e]), a1, x[e]);
         }
-        if (exists && p.splits > 1) {
-          float4 *to = reinterpret_cast<float4 *>(p.part_o + (w.split * p.rows + row) * DH + c);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) to[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-        } else if (exists) {
-          uint4 *to = reinterpret_cast<uint4 *>(p.o + w.b * p.so.batch + head * p.so.head + i * p.so.row + c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            to[e] = make_uint4(pack2<BF16>(x[8 * e], x[8 * e + 1]), pack2<BF16>(x[8 * e + 2], x[8 * e + 3]),
-                               pack2<BF16>(x[8 * e + 4], x[8 * e + 5]), pack2<BF16>(x[8 * e + 6], x[8 * e + 7]));
-        }
+        if (exists) store_32<BF16, DH>(p, x, w.split, row, p.o + w.b * p.so.batch + head * p.so.head + i * p.so.row, c);
         __syncwarp();
       }
     }
@@ -456,6 +484,203 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   if (warp == 1) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// ---- solo: d_head 64, one tile per CTA, two CTAs per SM
+namespace solo {
+constexpr int DH = 64, STAGES = 5, TB = TILE * DH * 2;
+constexpr int THREADS = 256;
+constexpr int TMEM_COLS = 256;  // S [0,128) P [128,192) O [192,256)
+constexpr int P_COL = 128, O_COL = 192;
+constexpr int SMEM = (1 + STAGES) * TB + 256;
+// registers: 128 a thread at launch with two CTAs per SM, handed over as 56 + 200
+static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+} // namespace solo
+
+template <bool BF16>
+__global__ void __launch_bounds__(solo::THREADS, 2)
+attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                      const __grid_constant__ CUtensorMap tmap_v, const FwdParams p) {
+  constexpr int DH = solo::DH, STAGES = solo::STAGES, TB = solo::TB;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t q_smem = smem_u32(smem_raw);
+  auto kv_smem = [&](int pos) { return q_smem + (1 + pos % STAGES) * TB; };
+  const uint32_t bars = q_smem + (1 + STAGES) * TB;
+  const uint32_t q_full = bars;
+  auto kv_full = [&](int pos) { return bars + 8u * (1 + pos % STAGES); };
+  auto kv_empty = [&](int pos) { return bars + 8u * (1 + STAGES + pos % STAGES); };
+  auto kv_phase = [&](int pos) { return static_cast<uint32_t>(pos / STAGES) & 1u; };
+  const uint32_t scores = bars + 8u * (1 + 2 * STAGES), read = scores + 8, probs = scores + 16, rows_done = scores + 32;
+  const uint32_t tmem_slot = scores + 40;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  const int hb = blockIdx.x % p.heads_batch, rest = blockIdx.x / p.heads_batch;
+  const int b = hb / p.heads, head = hb % p.heads, split = rest % p.splits;
+  const int row0 = (p.tiles_q - 1 - rest / p.splits) * TILE;  // under the causal mask the long tiles come first
+  const int keys = key_count(p.key_lens, b, p.n_kv);
+  const int nb = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + TILE - 1) / TILE;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(nb) * split / p.splits);
+  const int n = static_cast<int>(static_cast<int64_t>(nb) * (split + 1) / p.splits) - kb0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+    }
+    mbar_init(scores, 1);
+    mbar_init(read, 4);
+    mbar_init(probs, 4);
+    mbar_init(probs + 8, 4);
+    mbar_init(rows_done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(solo::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (tmem_slot - q_smem));
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      if (lane == 0 && n > 0) {
+        mbar_expect_tx(q_full, TB);
+        load_tile<DH>(q_smem, &tmap_q, row0, head, b, q_full);
+        const int kv_head = head / p.group;
+        int pos = 0;
+        bool ok = true;
+        auto load = [&](const CUtensorMap *map, int block) {
+          if (!ok) return;
+          if (pos >= STAGES && !mbar_wait_relaxed(kv_empty(pos), kv_phase(pos) ^ 1u, kPollSleepNs)) {
+            report(p.status, kStatusTmaWaitTimeout);
+            ok = false;
+            return;
+          }
+          mbar_expect_tx(kv_full(pos), TB);
+          load_tile<DH>(kv_smem(pos), map, (kb0 + block) * TILE, kv_head, b, kv_full(pos));
+          ++pos;
+        };
+        load(&tmap_k, 0);
+        for (int j = 0; j < n; ++j) {
+          if (j + 1 < n) load(&tmap_k, j + 1);
+          load(&tmap_v, j);
+        }
+        for (int q = max(0, pos - STAGES); q < pos; ++q)  // every tile has been used
+          if (!mbar_wait_relaxed(kv_empty(q), kv_phase(q), kPollSleepNs)) break;
+      }
+    } else if (warp == 1 && n > 0) {
+      const uint32_t leader = elect_one();
+      bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
+      int pos = 0;
+      const int pad_block = keys < p.n_kv && keys % TILE ? keys / TILE - kb0 : -1;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+      };
+      auto next_scores = [&]() {
+        wait(kv_full(pos), kv_phase(pos));
+        if (ok) {
+          tcgen05_fence_after();
+          mma_scores<DH, TILE>(tmem, q_smem, kv_smem(pos), p.idesc_s, leader);
+          commit(scores, leader);
+          commit(kv_empty(pos), leader);
+        }
+        ++pos;
+      };
+      next_scores();
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) {
+          wait(read, j & 1);
+          next_scores();
+        }
+        wait(kv_full(pos), kv_phase(pos));
+        if (j == pad_block) zero_rows<DH>(kv_smem(pos), keys % TILE, lane);  // V behind the sequence's last key
+        for (int half = 0; half < 2; ++half) {
+          wait(probs + 8 * half, j & 1);
+          if (!ok) break;
+          tcgen05_fence_after();
+          const uint32_t o = tmem + solo::O_COL, q = tmem + solo::P_COL;
+          if (half == 0) mma_rows<TILE, 32, 0, 4>(o, q, kv_smem(pos), p.idesc_o, j > 0, leader);
+          else mma_rows<TILE, 32, 4, 8>(o, q, kv_smem(pos), p.idesc_o, true, leader);
+        }
+        if (ok) {
+          commit(rows_done, leader);
+          commit(kv_empty(pos), leader);
+        }
+        ++pos;
+      }
+      if (!ok && lane == 0) report(p.status, kStatusMmaWaitTimeout);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int lane_group = warp & 3, r = lane_group * 32 + lane, i = row0 + r;
+    const bool exists = i < p.n_q;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
+    const int limit = exists ? visible_keys(i, keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+    for (int j = 0; j < n; ++j) {
+      if (!(ok = wait(scores, j & 1))) break;
+      tcgen05_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(t_row + 32 * c, s[c]);
+      tmem_ld_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(read);
+      mask_scores(s, limit - (kb0 + j) * TILE);
+      const float row_max = row_maximum(s) * p.scale_log2e;
+      if (j == 0) {
+        m = row_max;
+      } else {
+        if (!(ok = wait(rows_done, (j - 1) & 1))) break;  // P and O are free
+        tcgen05_fence_after();
+        move_reference<DH>(m, l, row_max, t_row + solo::O_COL);
+      }
+      l += exponentials<BF16>(s, p.scale_log2e, m, t_row + solo::P_COL, [&](int half) {
+        if (lane == 0) mbar_arrive(probs + 8 * half);
+      });
+    }
+    if (ok && n > 0) ok = wait(rows_done, (n - 1) & 1);
+    if (!ok) {
+      if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
+    } else {
+      tcgen05_fence_after();
+      const int64_t row = exists ? (static_cast<int64_t>(b) * p.q_heads + head) * p.n_q + i : 0;
+      const bool some = l > 0.0f;
+      const float f = p.splits > 1 ? 1.0f : (some ? 1.0f / l : 0.0f);
+      if (exists) {
+        if (p.splits > 1) p.part_ml[split * p.rows + row] = make_float2(m, l);
+        else p.lse[row] = row_lse(m, l);
+      }
+#pragma unroll 1
+      for (int c = 0; c < DH; c += 32) {
+        uint32_t v[32];
+        if (n > 0) tmem_ld_32x32(t_row + solo::O_COL + c, v);
+        tmem_ld_wait();
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = n > 0 && some ? __uint_as_float(v[e]) * f : 0.0f;
+        if (exists) store_32<BF16, DH>(p, x, split, row, p.o + b * p.so.batch + head * p.so.head + i * p.so.row, c);
+        __syncwarp();
+      }
+    }
+  }
+
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(solo::TMEM_COLS) : "memory");
   }
 }
 
@@ -486,32 +711,46 @@ template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_jo
   for (int e = 0; e < V; e += 2) w[e / 2] = pack2<BF16>(x[e] * inv, x[e + 1] * inv);
   if (V == 4) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[V / 2 - 1]);
   else *reinterpret_cast<uint32_t *>(to) = w[0];
-  if (lane == 0) p.lse[row] = l > 0.0f ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
+  if (lane == 0) p.lse[row] = row_lse(m, l);
 }
 
 constexpr int SMS = 148;
 
 bool is_packed(const AttentionProblem &p) { return p.n_q * (p.q_heads / p.kv_heads) <= TILE; }
+int64_t tiles_per_head(const AttentionProblem &p) {
+  if (is_packed(p)) return 1;
+  const int64_t rows = p.d_head == 64 ? TILE : 2 * TILE;
+  return (p.n_q + rows - 1) / rows;
+}
 int64_t tile_count(const AttentionProblem &p) {
-  return is_packed(p) ? p.batch * p.kv_heads : p.batch * p.q_heads * ((p.n_q + 2 * TILE - 1) / (2 * TILE));
+  return p.batch * (is_packed(p) ? p.kv_heads : p.q_heads) * tiles_per_head(p);
 }
 // Shares of a tile's key blocks: enough CTAs for every SM, at least four blocks each (a share's set-up and
 // the joining cost about as much as two).
 int split_count(const AttentionProblem &p) {
   const int64_t blocks = (p.n_kv + TILE - 1) / TILE, tiles = tile_count(p);
-  int64_t s = tiles >= SMS ? 1 : SMS / tiles;
+  const int64_t slots = !is_packed(p) && p.d_head == 64 ? 2 * SMS : SMS;
+  int64_t s = tiles >= slots ? 1 : slots / tiles;
   if (s > blocks / 4) s = blocks / 4;
   return static_cast<int>(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
 
 bool aligned(const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
-template <bool BF16, int DH, bool PACKED>
-cudaError_t launch_variant(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const FwdParams &f,
-                           unsigned grid, cudaStream_t stream) {
-  cudaError_t e = allow_smem<attention_kernel<BF16, DH, PACKED>>(smem_bytes(DH, PACKED));
-  if (e != cudaSuccess) return e;
-  attention_kernel<BF16, DH, PACKED><<<grid, THREADS, smem_bytes(DH, PACKED), stream>>>(tq, tk, tv, f);
+template <bool BF16, int DH>
+cudaError_t launch_typed(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const FwdParams &f,
+                         unsigned grid, bool packed, cudaStream_t stream) {
+  cudaError_t e;
+  if (packed) {
+    if ((e = allow_smem<attention_kernel<BF16, DH, true>>(smem_bytes(DH, true))) != cudaSuccess) return e;
+    attention_kernel<BF16, DH, true><<<grid, THREADS, smem_bytes(DH, true), stream>>>(tq, tk, tv, f);
+  } else if constexpr (DH == 64) {
+    if ((e = allow_smem<attention_solo_kernel<BF16>>(solo::SMEM)) != cudaSuccess) return e;
+    attention_solo_kernel<BF16><<<grid, solo::THREADS, solo::SMEM, stream>>>(tq, tk, tv, f);
+  } else {
+    if ((e = allow_smem<attention_kernel<BF16, DH, false>>(smem_bytes(DH, false))) != cudaSuccess) return e;
+    attention_kernel<BF16, DH, false><<<grid, THREADS, smem_bytes(DH, false), stream>>>(tq, tk, tv, f);
+  }
   e = cudaGetLastError();
   if (e != cudaSuccess || f.splits == 1) return e;
   attention_join_kernel<BF16, DH><<<static_cast<unsigned>((f.rows + 3) / 4), 128, 0, stream>>>(f);
@@ -578,7 +817,7 @@ cudaError_t launch_attention(const AttentionProblem &p, unsigned *status, cudaSt
   f.causal = p.causal ? 1 : 0;
   f.heads = static_cast<int>(packed ? p.kv_heads : p.q_heads);
   f.heads_batch = f.heads * static_cast<int>(p.batch);
-  f.tiles_q = packed ? 1 : static_cast<int>((p.n_q + 2 * TILE - 1) / (2 * TILE));
+  f.tiles_q = static_cast<int>(tiles_per_head(p));
   f.splits = split_count(p);
   f.rows = p.batch * p.q_heads * p.n_q;
   f.scale_log2e = p.scale * 1.4426950408889634f;
@@ -591,16 +830,11 @@ cudaError_t launch_attention(const AttentionProblem &p, unsigned *status, cudaSt
   }
   const unsigned grid = static_cast<unsigned>(tile_count(p) * f.splits);
   *launched = f.splits > 1 ? 2 : 1;
-  if (p.d_head == 64) {
-    if (bf16) return packed ? launch_variant<true, 64, true>(tq, tk, tv, f, grid, stream)
-                            : launch_variant<true, 64, false>(tq, tk, tv, f, grid, stream);
-    return packed ? launch_variant<false, 64, true>(tq, tk, tv, f, grid, stream)
-                  : launch_variant<false, 64, false>(tq, tk, tv, f, grid, stream);
-  }
-  if (bf16) return packed ? launch_variant<true, 128, true>(tq, tk, tv, f, grid, stream)
-                          : launch_variant<true, 128, false>(tq, tk, tv, f, grid, stream);
-  return packed ? launch_variant<false, 128, true>(tq, tk, tv, f, grid, stream)
-                : launch_variant<false, 128, false>(tq, tk, tv, f, grid, stream);
+  if (p.d_head == 64)
+    return bf16 ? launch_typed<true, 64>(tq, tk, tv, f, grid, packed, stream)
+                : launch_typed<false, 64>(tq, tk, tv, f, grid, packed, stream);
+  return bf16 ? launch_typed<true, 128>(tq, tk, tv, f, grid, packed, stream)
+              : launch_typed<false, 128>(tq, tk, tv, f, grid, packed, stream);
 }
 
 } // namespace imex

@@ -36,6 +36,8 @@
 // Every wait is bounded; one that runs out records a status code and the role leaves its loop.
 #include "attention_tc.cuh"
 
+#include <cstdlib>
+
 namespace imex {
 namespace {
 
@@ -732,6 +734,7 @@ int split_count(const AttentionProblem &p) {
   const int64_t slots = !is_packed(p) && p.d_head == 64 ? 2 * SMS : SMS;
   int64_t s = tiles >= slots ? 1 : slots / tiles;
   if (s > blocks / 4) s = blocks / 4;
+  if (const char *e = getenv("SPL")) s = atoi(e);
   return static_cast<int>(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
 

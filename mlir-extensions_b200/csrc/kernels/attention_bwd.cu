@@ -24,6 +24,10 @@
 // next product behind the one that reads it.  While the warps compute P the tensor core runs the
 // previous block's last product and this block's dP; while they compute dS it runs the next block's S.
 //
+// Where there are fewer tiles than SMs, or few long ones (shared key heads make the blocks of a key tile many,
+// the causal mask makes them uneven), the blocks of a tile are shared out between the CTAs of a cluster; each
+// leaves its sums in its shared memory, and each adds up a part of the rows over all of them, in order.
+//
 // Rounding: P and dS once to the 16-bit type, results once.  Masked entries are selected away, padded K rows
 // zeroed in shared memory where they are a B operand, so padding may hold anything.
 #include "attention_tc.cuh"
@@ -63,6 +67,7 @@ struct BwdParams {
   unsigned *status;
   Strides3 so, sdo, sdq, sdk, sdv;
   int q_heads, kv_heads, group, n_q, n_kv, causal, heads_batch, tiles;
+  int shares;  // CTAs (one cluster) among which a tile's blocks are shared out: 1, 2, 4 or 8
   float scale, scale_log2e;
   uint32_t idesc_s, idesc_o;
 };
@@ -136,12 +141,15 @@ template <int DH> __device__ __forceinline__ void take_registers() {
   else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
 }
 
+// Blocks [share_of(n, r, s), share_of(n, r + 1, s)) are those of share r of s
+__device__ __forceinline__ int share_of(int n, int r, int s) { return static_cast<int>(static_cast<int64_t>(n) * r / s); }
+
 // The producer's two streams of tiles, in the order the products use them.
 template <int DH, typename LoadA, typename LoadB>
-__device__ __forceinline__ void produce(const Layout<DH> &L, int n, int ahead, unsigned *status, LoadA &&load_a, LoadB &&load_b) {
+__device__ __forceinline__ void produce(const Layout<DH> &L, int n, unsigned *status, LoadA &&load_a, LoadB &&load_b) {
   using T = Layout<DH>;
   bool ok = true;
-  int na = 0, nb = 0;
+  int na = n > 0, nb = n > 0;  // the first of each is on its way already
   auto a = [&]() {
     if (!ok || na >= n) return;
     if (na >= T::SA && !mbar_wait_relaxed(L.a_empty(na), L.a_phase(na) ^ 1u, kPollSleepNs)) {
@@ -162,10 +170,9 @@ __device__ __forceinline__ void produce(const Layout<DH> &L, int n, int ahead, u
     load_b(nb, L.b_tile(nb), L.b_full(nb));
     ++nb;
   };
-  for (int j = 0; j < ahead; ++j) a();  // A tiles are used `ahead` blocks earlier than the B tile of the same step
-  for (int j = 0; j < n; ++j) {
-    b();
+  for (int j = 1; j < n; ++j) {
     a();
+    b();
   }
   if (!ok) report(status, kStatusTmaWaitTimeout);
   // every tile has been used before the CTA may go
@@ -173,6 +180,39 @@ __device__ __forceinline__ void produce(const Layout<DH> &L, int n, int ahead, u
     if (!mbar_wait_relaxed(L.a_empty(q), L.a_phase(q), kPollSleepNs)) break;
   for (int q = max(0, nb - T::SB); q < nb; ++q)
     if (!mbar_wait_relaxed(L.b_empty(q), L.b_phase(q), kPollSleepNs)) break;
+}
+
+// -rowsum(dO O) of ROWS rows into `to`: DH / 8 lanes read a row together (a lane per row would touch 32 lines with
+// every access: 14000 cycles a tile)
+template <bool BF16, int DH, int ROWS>
+__device__ __forceinline__ void row_deltas(const uint16_t *o, int64_t o_step, const uint16_t *g, int64_t g_step, int row0,
+                                           int rows, int lane, float *to) {
+  constexpr int GROUP = DH / 8, AT_ONCE = 32 / GROUP, N = ROWS / AT_ONCE;  // lanes per row, rows per access, accesses
+  const int sub = lane / GROUP, c = lane % GROUP * 8;
+  uint4 x[N], y[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int row = row0 + k * AT_ONCE + sub;
+    x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) {
+      x[k] = *reinterpret_cast<const uint4 *>(o + row * o_step + c);
+      y[k] = *reinterpret_cast<const uint4 *>(g + row * g_step + c);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const uint32_t xs[4] = {x[k].x, x[k].y, x[k].z, x[k].w}, ys[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+    float d = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 u = unpack2<BF16>(xs[e]), w = unpack2<BF16>(ys[e]);
+      d = fmaf(u.x, w.x, d);
+      d = fmaf(u.y, w.y, d);
+    }
+#pragma unroll
+    for (int s = 1; s < GROUP; s *= 2) d += __shfl_xor_sync(0xffffffffu, d, s);
+    if (lane % GROUP == 0) to[k * AT_ONCE + sub] = -d;
+  }
 }
 
 // 64 columns of this thread's row
@@ -185,9 +225,12 @@ __device__ __forceinline__ void load_64(uint32_t taddr, uint32_t (&v)[64]) {
   for (int e = 0; e < 32; ++e) v[e] = lo[e], v[32 + e] = hi[e];
 }
 
-// 16-bit results of one row from TMEM: COLS columns from `taddr`, times `factor` (0 where nothing was added up)
-template <bool BF16, int COLS>
-__device__ __forceinline__ void store_row(uint32_t taddr, bool has, float factor, uint16_t *to, bool exists) {
+// ---- sums of a share: f32 rows of DH values in shared memory, 16-byte units swizzled by the row
+template <int DH> __device__ __forceinline__ uint32_t sum_offset(int row, int unit) {
+  return row * (DH * 4) + ((unit ^ (row & 7)) * 16);
+}
+template <int DH, int COLS>
+__device__ __forceinline__ void leave_row(uint32_t taddr, bool has, uint32_t sums, int row, int col0) {
 #pragma unroll 1
   for (int c = 0; c < COLS; c += 32) {
     uint32_t v[32];
@@ -195,18 +238,64 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bool has, float factor
       tmem_ld_32x32(taddr + c, v);
       tmem_ld_wait();
     }
-    if (exists) {
-      float x[32];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = has ? __uint_as_float(v[e]) * factor : 0.0f;
-      uint4 *q = reinterpret_cast<uint4 *>(to + c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        q[e] = make_uint4(pack2<BF16>(x[8 * e], x[8 * e + 1]), pack2<BF16>(x[8 * e + 2], x[8 * e + 3]),
-                          pack2<BF16>(x[8 * e + 4], x[8 * e + 5]), pack2<BF16>(x[8 * e + 6], x[8 * e + 7]));
-    }
-    __syncwarp();
+    for (int e = 0; e < 8; ++e)
+      st_shared_v4(sums + sum_offset<DH>(row, (col0 + c) / 4 + e),
+                   has ? make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                     __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]))
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
   }
+}
+// This CTA's part of the rows over all shares, in order, to 16 bits: neighbouring threads write neighbouring
+// 16 bytes of a row.  `thread` of THREADS; the loads of two steps are in flight together.
+template <bool BF16, int DH, int S, int THREADS>
+__device__ __forceinline__ void add_up_of(uint32_t sums, int rank, float factor, uint16_t *to, int64_t step, int rows_left,
+                                          int thread) {
+  constexpr int UNITS = TILE / S * (DH / 8), STEPS = (UNITS + THREADS - 1) / THREADS;
+#pragma unroll 2
+  for (int k = 0; k < STEPS; ++k) {
+    const int u = thread + k * THREADS;
+    const int row = rank * (TILE / S) + u / (DH / 8), unit = u % (DH / 8) * 2;
+    float4 v[S][2];
+#pragma unroll
+    for (int r = 0; r < S; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = sums + sum_offset<DH>(u < UNITS ? row : 0, unit + h);
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[r][h].x), "=f"(v[r][h].y), "=f"(v[r][h].z), "=f"(v[r][h].w)
+                     : "r"(S > 1 ? map_to_cta(at, r) : at));
+      }
+#pragma unroll
+    for (int r = 1; r < S; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v[0][h].x += v[r][h].x;
+        v[0][h].y += v[r][h].y;
+        v[0][h].z += v[r][h].z;
+        v[0][h].w += v[r][h].w;
+      }
+    const float4 x = v[0][0], y = v[0][1];
+    if (u < UNITS && row < rows_left)
+      *reinterpret_cast<uint4 *>(to + row * step + unit * 4) =
+          make_uint4(pack2<BF16>(x.x * factor, x.y * factor), pack2<BF16>(x.z * factor, x.w * factor),
+                     pack2<BF16>(y.x * factor, y.y * factor), pack2<BF16>(y.z * factor, y.w * factor));
+  }
+}
+template <bool BF16, int DH, int THREADS>
+__device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, float factor, uint16_t *to, int64_t step,
+                                       int rows_left, int thread) {
+  if (shares == 1) add_up_of<BF16, DH, 1, THREADS>(sums, rank, factor, to, step, rows_left, thread);
+  else if (shares == 2) add_up_of<BF16, DH, 2, THREADS>(sums, rank, factor, to, step, rows_left, thread);
+  else if (shares == 4) add_up_of<BF16, DH, 4, THREADS>(sums, rank, factor, to, step, rows_left, thread);
+  else add_up_of<BF16, DH, 8, THREADS>(sums, rank, factor, to, step, rows_left, thread);
+}
+// The computing warps' sums are in place everywhere / have been read everywhere.  The first warpgroup takes part
+// when there are several CTAs.
+template <int THREADS> __device__ __forceinline__ void sums_barrier(int shares) {
+  __syncwarp();
+  if (shares > 1) cluster_sync_all();
+  else asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
@@ -223,17 +312,40 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   const T L(smem_u32(smem_raw));
   constexpr int BN = T::BN;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int hb = blockIdx.x % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
-  const int qt = p.tiles - 1 - blockIdx.x / p.heads_batch;  // under the causal mask the long tiles come first
+  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
+  const int hb = tile % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
+  const int qt = p.tiles - 1 - tile / p.heads_batch;  // under the causal mask the long tiles come first
   const int row0 = qt * TILE;
   const int keys = key_count(p.key_lens, b, p.n_kv);
-  const int n = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + BN - 1) / BN;
+  const int n_all = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + BN - 1) / BN;
+  const int first = share_of(n_all, rank, p.shares), n = share_of(n_all, rank + 1, p.shares) - first;  // key blocks
 
-  if (threadIdx.x == 0) init_barriers<DH>(L);
+  auto load_a = [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_k, (first + j) * BN, head / p.group, b, bar); };
+  auto load_b = [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_v, (first + j) * BN, head / p.group, b, bar); };
+  if (threadIdx.x == 0) {
+    init_barriers<DH>(L);
+    if (n > 0) {  // the first tiles, while the others set up
+      mbar_expect_tx(L.res_full(), 2 * T::RB);
+      load_tile<DH>(L.resident(0), &tmap_q, row0, head, b, L.res_full());
+      load_tile<DH>(L.resident(1), &tmap_do, row0, head, b, L.res_full());
+      mbar_expect_tx(L.a_full(0), T::TB);
+      load_a(0, L.a_tile(0), L.a_full(0));
+      mbar_expect_tx(L.b_full(0), T::TB);
+      load_b(0, L.b_tile(0), L.b_full(0));
+    }
+  }
   if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT), T::TMEM_COLS);
+  float *neg_deltas = reinterpret_cast<float *>(smem_raw + (L.stats() - L.base));
+  if (warp >= 4) {
+    constexpr int ROWS = TILE / T::WARPS;
+    row_deltas<BF16, DH, ROWS>(p.o + b * p.so.batch + head * p.so.head, p.so.row,
+                               p.dout + b * p.sdo.batch + head * p.sdo.head, p.sdo.row, row0 + (warp - 4) * ROWS, p.n_q,
+                               lane, neg_deltas + (warp - 4) * ROWS);
+  }
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = ld_shared_u32(L.bar(T::TMEM_SLOT));
   const uint32_t dq_tmem = tmem + 3 * BN;
   auto dp_tmem = [&](int j) { return tmem + BN + (j & 1) * BN; };
@@ -241,25 +353,17 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   if (warp < 4) {
     give_registers<DH>();
     if (warp == 0) {
-      if (lane == 0 && n > 0) {
-        mbar_expect_tx(L.res_full(), 2 * T::RB);
-        load_tile<DH>(L.resident(0), &tmap_q, row0, head, b, L.res_full());
-        load_tile<DH>(L.resident(1), &tmap_do, row0, head, b, L.res_full());
-        const int kv_head = head / p.group;
-        produce<DH>(L, n, 1, p.status,
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_k, j * BN, kv_head, b, bar); },
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_v, j * BN, kv_head, b, bar); });
-      }
+      if (lane == 0) produce<DH>(L, n, p.status, load_a, load_b);
     } else if (warp == 1 && n > 0) {
       bool ok = wait_all(L.res_full(), 0);
       const uint32_t leader = elect_one();
-      const int pad_block = keys < p.n_kv && keys % BN ? keys / BN : -1;
+      const int pad_block = keys < p.n_kv && keys % BN ? keys / BN - first : -1;
       auto scores = [&](int j) {  // S = Q K_j^T
         ok = ok && wait_all(L.a_full(j), L.a_phase(j));
         if (j == pad_block) {  // rows of K behind the sequence's last key: a B operand of dS K
-          const int first = keys % BN, count = (BN - first) * 8;  // 16-byte units per box
+          const int row = keys % BN, count = (BN - row) * 8;  // 16-byte units per box
           for (int e = lane; e < count * (DH / 64); e += 32) {
-            const uint32_t at = L.a_tile(j) + (e / count) * (BN * 128) + first * 128 + (e % count) * 16;
+            const uint32_t at = L.a_tile(j) + (e / count) * (BN * 128) + row * 128 + (e % count) * 16;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
           fence_async_smem();
@@ -298,42 +402,34 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (ok) commit(L.bar(T::DONE), leader);
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
     }
+    __syncwarp();
+    if (p.shares > 1) {  // the computing warps' two barriers
+      cluster_sync_all();
+      cluster_sync_all();
+    }
   } else {
     take_registers<DH>();
     const int half = BN == 128 ? (warp - 4) >> 2 : 0, lane_group = warp & 3;
     const int r = lane_group * 32 + lane, i = row0 + r;
     const bool exists = i < p.n_q;
     const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
-    // delta of this row (both halves add it up; the first one writes it)
-    float delta = 0.0f, lse2 = INFINITY;
+    const float neg_d = neg_deltas[r];
+    float lse2 = INFINITY;
     if (exists) {
-      const uint4 *o = reinterpret_cast<const uint4 *>(p.o + b * p.so.batch + head * p.so.head + i * p.so.row);
-      const uint4 *g = reinterpret_cast<const uint4 *>(p.dout + b * p.sdo.batch + head * p.sdo.head + i * p.sdo.row);
-#pragma unroll 4
-      for (int c = 0; c < DH / 8; ++c) {
-        const uint4 x = o[c], y = g[c];
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 u = unpack2<BF16>(xs[e]), w = unpack2<BF16>(ys[e]);
-          delta = fmaf(u.x, w.x, delta);
-          delta = fmaf(u.y, w.y, delta);
-        }
-      }
       const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head) * p.n_q + i;
       const float lse = p.lse[row];
       if (lse != -INFINITY) lse2 = lse * LOG2E;  // a row that sees no key: every probability is 2^-inf
-      if (half == 0) p.delta[row] = delta;
+      if (half == 0 && rank == 0) p.delta[row] = -neg_d;
     }
     const int limit = exists ? visible_keys(i, keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
     const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_lse2 = pack_f32x2(-lse2, -lse2);
-    const uint64_t neg_delta = pack_f32x2(-delta, -delta);
+    const uint64_t neg_delta = pack_f32x2(neg_d, neg_d);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       ok = wait_all(L.bar(T::S_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
-      const int seen = limit - j * BN - half * 64;  // of this thread's 64 keys
+      const int seen = limit - (first + j) * BN - half * 64;  // of this thread's 64 keys
       const bool masked = __any_sync(0xffffffffu, seen < 64);
       uint64_t pr[32];
       {
@@ -386,9 +482,13 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     } else {
       tcgen05_fence_after();
       constexpr int COLS = DH * 4 / T::WARPS;  // a warpgroup's share of the columns
-      uint16_t *to = p.dq + b * p.sdq.batch + head * p.sdq.head + i * p.sdq.row + half * COLS;
-      store_row<BF16, COLS>(dq_tmem + lanes + half * COLS, n > 0, p.scale, to, exists);
+      leave_row<DH, COLS>(dq_tmem + lanes + half * COLS, n > 0, L.base, r, half * COLS);
     }
+    constexpr int CT = T::THREADS - 128;
+    sums_barrier<CT>(p.shares);
+    add_up<BF16, DH, CT>(L.base, rank, p.shares, p.scale, p.dq + b * p.sdq.batch + head * p.sdq.head + row0 * p.sdq.row,
+                         p.sdq.row, p.n_q - row0, threadIdx.x - 128);
+    sums_barrier<CT>(p.shares);
   }
 
   __syncwarp();
@@ -412,19 +512,33 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const T L(smem_u32(smem_raw));
   constexpr int BN = T::BN;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int hb = blockIdx.x % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
-  const int key0 = blockIdx.x / p.heads_batch * TILE;  // under the causal mask the first keys have the most queries
+  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
+  const int hb = tile % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
+  const int key0 = tile / p.heads_batch * TILE;  // under the causal mask the first keys have the most queries
   const int keys = key_count(p.key_lens, b, p.n_kv);
   // query i sees key j from i = j - (n_kv - n_q) on
   const int shift = p.causal ? p.n_kv - p.n_q : 0;
   const int tiles_q = (p.n_q + BN - 1) / BN;
   const int first_tile = p.causal ? max(0, key0 - shift) / BN : 0;
   const int per_head = key0 < keys ? max(0, tiles_q - first_tile) : 0;
-  const int n = per_head * p.group;
-  auto head_of = [&](int j) { return kv_head * p.group + j / per_head; };
-  auto row_of = [&](int j) { return (first_tile + j % per_head) * BN; };
+  const int n_all = per_head * p.group, first = share_of(n_all, rank, p.shares), n = share_of(n_all, rank + 1, p.shares) - first;
+  auto head_of = [&](int j) { return kv_head * p.group + (first + j) / per_head; };
+  auto row_of = [&](int j) { return (first_tile + (first + j) % per_head) * BN; };
 
-  if (threadIdx.x == 0) init_barriers<DH>(L);
+  auto load_a = [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_q, row_of(j), head_of(j), b, bar); };
+  auto load_b = [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_do, row_of(j), head_of(j), b, bar); };
+  if (threadIdx.x == 0) {
+    init_barriers<DH>(L);
+    if (n > 0) {  // the first tiles, while the others set up
+      mbar_expect_tx(L.res_full(), 2 * T::RB);
+      load_tile<DH>(L.resident(0), &tmap_k, key0, kv_head, b, L.res_full());
+      load_tile<DH>(L.resident(1), &tmap_v, key0, kv_head, b, L.res_full());
+      mbar_expect_tx(L.a_full(0), T::TB);
+      load_a(0, L.a_tile(0), L.a_full(0));
+      mbar_expect_tx(L.b_full(0), T::TB);
+      load_b(0, L.b_tile(0), L.b_full(0));
+    }
+  }
   if (warp == 1) tmem_alloc(L.bar(T::TMEM_SLOT), T::TMEM_COLS);
   tcgen05_fence_before();
   __syncthreads();
@@ -437,14 +551,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   if (warp < 4) {
     give_registers<DH>();
     if (warp == 0) {
-      if (lane == 0 && n > 0) {
-        mbar_expect_tx(L.res_full(), 2 * T::RB);
-        load_tile<DH>(L.resident(0), &tmap_k, key0, kv_head, b, L.res_full());
-        load_tile<DH>(L.resident(1), &tmap_v, key0, kv_head, b, L.res_full());
-        produce<DH>(L, n, 1, p.status,
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_q, row_of(j), head_of(j), b, bar); },
-                    [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_do, row_of(j), head_of(j), b, bar); });
-      }
+      if (lane == 0) produce<DH>(L, n, p.status, load_a, load_b);
     } else if (warp == 1 && n > 0) {
       bool ok = wait_all(L.res_full(), 0);
       const uint32_t leader = elect_one();
@@ -486,7 +593,9 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
     } else if (warp == 2) {
       // row statistics of the query blocks: -log2(e) LSE and -delta.  Queries that do not exist or see no key
-      // get -inf for the first, which makes their probabilities 2^-inf.
+      // get -inf for the first, which makes their probabilities 2^-inf.  The kernel may have been started while the
+      // last CTAs of the dQ kernel, which writes delta, still run.
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
         const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head_of(j)) * p.n_q;
@@ -510,6 +619,11 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         }
         mbar_arrive(L.bar(T::STAT_FULL + j % T::STAT_STAGES));
       }
+    }
+    __syncwarp();
+    if (p.shares > 1) {  // the computing warps' two barriers
+      cluster_sync_all();
+      cluster_sync_all();
     }
   } else {
     take_registers<DH>();
@@ -585,13 +699,18 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
     } else {
       tcgen05_fence_after();
-      // with two warpgroups one writes dV, the other dK
-      const bool exists = key < p.n_kv;
-      if (half == 0)
-        store_row<BF16, DH>(dv_tmem + lanes, n > 0, 1.0f, p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key * p.sdv.row, exists);
-      if (half == 1 || BN == 64)
-        store_row<BF16, DH>(dk_tmem + lanes, n > 0, p.scale, p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key * p.sdk.row, exists);
+      // with two warpgroups one takes dV, the other dK
+      if (half == 0) leave_row<DH, DH>(dv_tmem + lanes, n > 0, L.base, r, 0);
+      if (half == 1 || BN == 64) leave_row<DH, DH>(dk_tmem + lanes, n > 0, L.base + TILE * DH * 4, r, 0);
     }
+    constexpr int CT = T::THREADS - 128;
+    sums_barrier<CT>(p.shares);
+    add_up<BF16, DH, CT>(L.base, rank, p.shares, 1.0f, p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row,
+                         p.sdv.row, p.n_kv - key0, threadIdx.x - 128);
+    add_up<BF16, DH, CT>(L.base + TILE * DH * 4, rank, p.shares, p.scale,
+                         p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key0 * p.sdk.row, p.sdk.row, p.n_kv - key0,
+                         threadIdx.x - 128);
+    sums_barrier<CT>(p.shares);
   }
 
   __syncwarp();
@@ -603,22 +722,56 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   }
 }
 
+// `early`: may start while the last CTAs of the kernel before it still run.
+template <auto kernel, int DH, typename... Maps>
+cudaError_t launch_shared(const BwdParams &f, int64_t tiles, bool early, cudaStream_t stream, const Maps &...maps) {
+  using Z = Sizes<DH>;
+  const cudaError_t e = allow_smem<kernel>(Z::SMEM);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * f.shares));
+  cfg.blockDim = dim3(Z::THREADS);
+  cfg.dynamicSmemBytes = Z::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(f.shares);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, maps..., f);
+}
+
+// CTAs a tile's `blocks` are shared out between: as many as fit on the GPU at once, at least `least` blocks each,
+// at most four (clusters of eight CTAs that fill their SMs wait long for a place); one doubling more for the
+// uneven tiles of the causal mask as long as the tiles alone do not fill the GPU.  dK / dV with 1 and 2 shares:
+// 128 tiles of up to 32 blocks (d_head 128) 109 and 99 us, 256 tiles of up to 128 blocks 474 and 497 us; 16 tiles of
+// up to 64 blocks with 1, 2, 4 and 8: 128, 84, 62 and 62 us.
+int share_count(int64_t tiles, int64_t blocks, int64_t slots, int least, bool uneven) {
+  int s = 1;
+  while (s < 4 && blocks >= least * 2 * s && (tiles * s * 2 <= slots || (uneven && s == 1 && tiles <= slots))) s *= 2;
+  return s;
+}
+
 template <bool BF16, int DH>
 cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tdo,
                         const CUtensorMap &tqb, const CUtensorMap &tdob, const CUtensorMap &tkb, const CUtensorMap &tvb,
                         BwdParams f, int64_t batch, cudaStream_t stream) {
   using Z = Sizes<DH>;
-  cudaError_t e = allow_smem<attention_dq_kernel<BF16, DH>>(Z::SMEM);
-  if (e == cudaSuccess) e = allow_smem<attention_dkv_kernel<BF16, DH>>(Z::SMEM);
-  if (e != cudaSuccess) return e;
+  const int64_t slots = 148 * Z::CTAS;
   f.tiles = (f.n_q + TILE - 1) / TILE;
   f.heads_batch = static_cast<int>(batch) * f.q_heads;
-  attention_dq_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, Z::THREADS, Z::SMEM, stream>>>(tq, tkb, tvb, tdo, f);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  int64_t tiles = static_cast<int64_t>(f.tiles) * f.heads_batch;
+  f.shares = share_count(tiles, (f.n_kv + Z::BN - 1) / Z::BN, slots, DH == 64 ? 2 : 4, f.causal);
+  cudaError_t e = launch_shared<attention_dq_kernel<BF16, DH>, DH>(f, tiles, false, stream, tq, tkb, tvb, tdo);
+  if (e != cudaSuccess) return e;
   f.tiles = (f.n_kv + TILE - 1) / TILE;
   f.heads_batch = static_cast<int>(batch) * f.kv_heads;
-  attention_dkv_kernel<BF16, DH><<<static_cast<unsigned>(f.tiles) * f.heads_batch, Z::THREADS, Z::SMEM, stream>>>(tqb, tk, tv, tdob, f);
-  return cudaGetLastError();
+  tiles = static_cast<int64_t>(f.tiles) * f.heads_batch;
+  f.shares = share_count(tiles, static_cast<int64_t>((f.n_q + Z::BN - 1) / Z::BN) * f.group, slots, DH == 64 ? 2 : 4, f.causal);
+  return launch_shared<attention_dkv_kernel<BF16, DH>, DH>(f, tiles, true, stream, tqb, tk, tv, tdob);
 }
 
 } // namespace

@@ -418,6 +418,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       i = w.qt * 2 * TILE + g * TILE + r;
     }
     const bool exists = i < p.n_q;
+    const bool idle = PACKED && lane_group * 32 >= p.n_q * p.group;  // a warp without rows only keeps step
     // rows that do not exist compute on whatever is there and are not written
     const int limit = exists ? visible_keys(i, w.keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
     const float neg_inf = -INFINITY;
@@ -427,6 +428,13 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       ok = mbar_wait(scores(g), j & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      if (idle) {
+        if (lane == 0) {
+          mbar_arrive(probs(g, 0));
+          mbar_arrive(probs(g, 1));
+        }
+        continue;
+      }
       tcgen05_fence_after();
       uint32_t s[4][32];
 #pragma unroll
@@ -543,6 +551,9 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
   const int hb = blockIdx.x % p.heads_batch, rest = blockIdx.x / p.heads_batch;
   const int b = hb / p.heads, head = hb % p.heads, split = rest % p.splits;
   const int row0 = (p.tiles_q - 1 - rest / p.splits) * TILE;  // under the causal mask the long tiles come first
+  // Packed rows that fit into one warp start in another quarter of the tile from CTA to CTA: the warp that has them
+  // then sits on another scheduler than that of the SM's other CTA.
+  const int rows = PACKED ? p.n_q * p.group : TILE, base = PACKED && rows <= 32 ? blockIdx.x % 4 * 32 : 0;
   const int keys = key_count(p.key_lens, b, p.n_kv);
   const int nb = (visible_keys((PACKED ? p.n_q : min(row0 + TILE, p.n_q)) - 1, keys, p.n_q, p.n_kv, p.causal) + TILE - 1) / TILE;
   const int kb0 = static_cast<int>(static_cast<int64_t>(nb) * split / p.splits);
@@ -562,8 +573,8 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (n > 0) {  // Q and the first keys, while the others set up
-      mbar_expect_tx(q_full, PACKED ? p.n_q * p.group * DH * 2 : TB);
-      load_tile<DH>(q_smem, &tmap_q, row0, PACKED ? head * p.group : head, b, q_full);
+      mbar_expect_tx(q_full, rows * DH * 2);
+      load_tile<DH>(q_smem + base * (DH * 2), &tmap_q, row0, PACKED ? head * p.group : head, b, q_full);
       mbar_expect_tx(kv_full(0), TB);
       load_tile<DH>(kv_smem(0), &tmap_k, kb0 * TILE, PACKED ? head : head / p.group, b, kv_full(0));
     }
@@ -649,10 +660,13 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int lane_group = warp & 3, r = lane_group * 32 + lane;
     // head and query of a row of the tile; rows that do not exist compute on whatever is there and are not written
-    auto head_of = [&](int row) { return PACKED ? head * p.group + row / p.n_q : head; };
-    auto query_of = [&](int row) { return PACKED ? (row < p.n_q * p.group ? row % p.n_q : p.n_q) : row0 + row; };
+    auto head_of = [&](int row) { return PACKED ? head * p.group + (row - base) / p.n_q : head; };
+    auto query_of = [&](int row) {
+      return PACKED ? (row >= base && row - base < rows ? (row - base) % p.n_q : p.n_q) : row0 + row;
+    };
     const int i = query_of(r);
     const bool exists = i < p.n_q;
+    const bool idle = PACKED && !__any_sync(0xffffffffu, exists);  // a warp without rows only keeps step
     const uint32_t t_row = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
     const int limit = exists ? visible_keys(i, keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
     float m = -INFINITY, l = 0.0f;
@@ -660,6 +674,15 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
     for (int j = 0; j < n; ++j) {
       if (!(ok = wait(scores, j & 1))) break;
+      if (idle) {
+        if (lane == 0) mbar_arrive(read);
+        if (j > 0 && !(ok = wait(rows_done, (j - 1) & 1))) break;
+        if (lane == 0) {
+          mbar_arrive(probs);
+          mbar_arrive(probs + 8);
+        }
+        continue;
+      }
       tcgen05_fence_after();
       uint32_t s[4][32];
 #pragma unroll

@@ -275,6 +275,8 @@ def rotary(name, tokens, heads, d_head, frequencies, dtype=BF16, interleaved=Fal
     freqs = [float(f) for f in frequencies]
     if min(tokens, heads, d_head) < 1:
         raise ValueError("rotary: extents are at least 1")
+    if d_head > 512:
+        raise ValueError("rotary: d_head is at most 512")
     if not 1 <= len(freqs) <= ROTARY_MAX_PAIRS or 2 * len(freqs) > d_head:
         raise ValueError("rotary: 1..%d frequencies, two dimensions of the head each" % ROTARY_MAX_PAIRS)
     if not all(math.isfinite(f) for f in freqs) or not math.isfinite(factor):

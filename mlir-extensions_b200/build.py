@@ -39,6 +39,7 @@ RUNTIME_SOURCES = [
     "kernels/attention.cu",
     "kernels/attention_bwd.cu",
     "kernels/gated_ffn.cu",
+    "kernels/gated_bwd.cu",
     "kernels/rotary.cu",
     "kernels/wait_selftest.cu",
     "runtime/cuda_runtime_wrappers.cu",

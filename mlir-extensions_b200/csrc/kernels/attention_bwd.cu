@@ -31,6 +31,7 @@
 // Rounding: P and dS once to the 16-bit type, results once.  Masked entries are selected away, padded K rows
 // zeroed in shared memory where they are a B operand, so padding may hold anything.
 #include "attention_tc.cuh"
+#include "tile_sums.cuh"
 
 namespace imex {
 namespace {
@@ -92,9 +93,9 @@ template <int DH> struct Layout : Sizes<DH> {
   __device__ uint32_t b_phase(int i) const { return (i / SB) & 1; }
   static constexpr int FIXED = 1 + 2 * SA + 2 * SB;
   __device__ uint32_t bar(int i) const { return bars() + 8 * (FIXED + i); }
-  static constexpr int S_FULL = 0, S_READ = 1, DP_FULL = 2, P_READY = 4, DS_READY = 5, DONE = 6, STAT_FULL = 7, STAT_EMPTY = 9;
-  static constexpr int TMEM_SLOT = 11;
-  static_assert(8 * (FIXED + 12) <= Z::BAR_BYTES, "the barriers fit");
+  static constexpr int S_FULL = 0, S_READ = 1, DP_FULL = 2, P_READY = 4, DS_READY = 5, DONE = 7, STAT_FULL = 8, STAT_EMPTY = 10;
+  static constexpr int TMEM_SLOT = 12;
+  static_assert(8 * (FIXED + 13) <= Z::BAR_BYTES, "the barriers fit");
   __device__ uint32_t stats() const { return bars() + Z::BAR_BYTES; }
 };
 
@@ -107,7 +108,7 @@ template <int DH> __device__ __forceinline__ void init_barriers(const Layout<DH>
   mbar_init(L.bar(T::S_READ), T::WARPS);
   for (int i = 0; i < 2; ++i) mbar_init(L.bar(T::DP_FULL + i), 1);
   mbar_init(L.bar(T::P_READY), T::WARPS);
-  mbar_init(L.bar(T::DS_READY), T::WARPS);
+  for (int i = 0; i < 2; ++i) mbar_init(L.bar(T::DS_READY + i), T::WARPS);
   mbar_init(L.bar(T::DONE), 1);
   for (int i = 0; i < T::STAT_STAGES; ++i) mbar_init(L.bar(T::STAT_FULL + i), 32), mbar_init(L.bar(T::STAT_EMPTY + i), T::WARPS);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -225,83 +226,12 @@ __device__ __forceinline__ void load_64(uint32_t taddr, uint32_t (&v)[64]) {
   for (int e = 0; e < 32; ++e) v[e] = lo[e], v[32 + e] = hi[e];
 }
 
-// ---- sums of a share: f32 rows of DH values in shared memory, 16-byte units swizzled by the row
-template <int DH> __device__ __forceinline__ uint32_t sum_offset(int row, int unit) {
-  return row * (DH * 4) + ((unit ^ (row & 7)) * 16);
-}
-template <int DH, int COLS>
-__device__ __forceinline__ void leave_row(uint32_t taddr, bool has, uint32_t sums, int row, int col0) {
-#pragma unroll 1
-  for (int c = 0; c < COLS; c += 32) {
-    uint32_t v[32];
-    if (has) {
-      tmem_ld_32x32(taddr + c, v);
-      tmem_ld_wait();
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      st_shared_v4(sums + sum_offset<DH>(row, (col0 + c) / 4 + e),
-                   has ? make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
-                                     __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]))
-                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-  }
-}
-// This CTA's part of the rows over all shares, in order, to 16 bits: neighbouring threads write neighbouring
-// 16 bytes of a row.  `thread` of THREADS; the loads of two steps are in flight together.
-template <bool BF16, int DH, int S, int THREADS>
-__device__ __forceinline__ void add_up_of(uint32_t sums, int rank, float factor, uint16_t *to, int64_t step, int rows_left,
-                                          int thread) {
-  constexpr int UNITS = TILE / S * (DH / 8), STEPS = (UNITS + THREADS - 1) / THREADS;
-#pragma unroll 2
-  for (int k = 0; k < STEPS; ++k) {
-    const int u = thread + k * THREADS;
-    const int row = rank * (TILE / S) + u / (DH / 8), unit = u % (DH / 8) * 2;
-    float4 v[S][2];
-#pragma unroll
-    for (int r = 0; r < S; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t at = sums + sum_offset<DH>(u < UNITS ? row : 0, unit + h);
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[r][h].x), "=f"(v[r][h].y), "=f"(v[r][h].z), "=f"(v[r][h].w)
-                     : "r"(S > 1 ? map_to_cta(at, r) : at));
-      }
-#pragma unroll
-    for (int r = 1; r < S; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v[0][h].x += v[r][h].x;
-        v[0][h].y += v[r][h].y;
-        v[0][h].z += v[r][h].z;
-        v[0][h].w += v[r][h].w;
-      }
-    const float4 x = v[0][0], y = v[0][1];
-    if (u < UNITS && row < rows_left)
-      *reinterpret_cast<uint4 *>(to + row * step + unit * 4) =
-          make_uint4(pack2<BF16>(x.x * factor, x.y * factor), pack2<BF16>(x.z * factor, x.w * factor),
-                     pack2<BF16>(y.x * factor, y.y * factor), pack2<BF16>(y.z * factor, y.w * factor));
-  }
-}
-template <bool BF16, int DH, int THREADS>
-__device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, float factor, uint16_t *to, int64_t step,
-                                       int rows_left, int thread) {
-  if (shares == 1) add_up_of<BF16, DH, 1, THREADS>(sums, rank, factor, to, step, rows_left, thread);
-  else if (shares == 2) add_up_of<BF16, DH, 2, THREADS>(sums, rank, factor, to, step, rows_left, thread);
-  else if (shares == 4) add_up_of<BF16, DH, 4, THREADS>(sums, rank, factor, to, step, rows_left, thread);
-  else add_up_of<BF16, DH, 8, THREADS>(sums, rank, factor, to, step, rows_left, thread);
-}
-// The computing warps' sums are in place everywhere / have been read everywhere.  The first warpgroup takes part
-// when there are several CTAs.
-template <int THREADS> __device__ __forceinline__ void sums_barrier(int shares) {
-  __syncwarp();
-  if (shares > 1) cluster_sync_all();
-  else asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
-}
-
 // ------------------------------------------------------------------------------------------------ dQ
 // TMEM, in units of BN columns: S [0,1), dP / dS of even and odd blocks [1,2) [2,3), dQ [3,4).  S is free for the next
 // block as soon as it has been read, dP has two places: the scores and products of block j + 1 run while the
-// warps still work on block j, so that the warps only ever wait for each other.
+// warps still work on block j, so that the warps only ever wait for each other.  A warp may then be a block ahead
+// of another one, hence a barrier each for the dS of even and odd blocks; two ahead it cannot be, because the dP of
+// block j + 2 comes behind the product over all of dS j.
 template <bool BF16, int DH>
 __global__ void __launch_bounds__(Sizes<DH>::THREADS, Sizes<DH>::CTAS)
 attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -392,7 +322,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           scores(j + 1);
           products(j + 1);
         }
-        ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
+        ok = ok && wait_all(L.bar(T::DS_READY + (j & 1)), (j >> 1) & 1);
         if (ok) {
           tcgen05_fence_after();
           mma_rows<BN, 64>(dq_tmem, dp_tmem(j), L.a_tile(j), p.idesc_o, j > 0, leader);
@@ -474,7 +404,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(L.bar(T::DS_READY));
+      if (lane == 0) mbar_arrive(L.bar(T::DS_READY + (j & 1)));
     }
     if (ok && n > 0) ok = wait_all(L.bar(T::DONE), 0);
     if (!ok) {

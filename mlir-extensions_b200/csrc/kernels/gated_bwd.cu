@@ -1,0 +1,322 @@
+// Backward pass of the gated feed-forward product (IMEX_OP_GATED_FFN_BWD).
+//
+// With [G U] = X W kept by the forward pass, one pass over G, U and dH writes [dG dU] = [dH U act'(G), dH act(G)]
+// into the workspace, rounded once to the 16-bit type; because W holds both projections side by side,
+// dX = [dG dU] W^T and dW = X^T [dG dU] are then one product each.  Large ones go to the framework's CTA-pair GEMM;
+// small ones to gated_product_kernel: 128 x 128 tiles, two CTAs per SM, k shared out between the CTAs of a cluster
+// where there are few tiles.
+#include "attention_common.cuh"
+#include "epilogue.cuh"
+#include "tile_sums.cuh"
+
+namespace imex {
+namespace {
+
+using namespace attn;
+using namespace tc;
+using namespace tc_host;
+
+struct GradArgs {
+  const uint16_t *gu, *dh;
+  uint16_t *dgu;
+  int64_t ldh, tokens, d_ff;
+  int act;
+};
+
+// act(g) and its derivative
+__device__ __forceinline__ void act_both(float g, int act, float &value, float &slope) {
+  if (act == kEpiSilu) {
+    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+    value = g * s;
+    slope = s * (1.0f + g * (1.0f - s));
+  } else if (act == kEpiRelu) {
+    value = relu_ugt(g);
+    slope = !(g <= 0.0f) ? 1.0f : 0.0f;
+  } else {
+    value = g;
+    slope = 1.0f;
+  }
+}
+
+// 10 bytes per element of H and few operations: bound by memory.  V columns per thread.
+template <bool BF16, int V> __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
+  struct alignas(2 * V) Pack {
+    uint16_t v[V];
+  };
+  const int64_t per_row = a.d_ff / V, n = a.tokens * per_row;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
+       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = e / per_row, c = (e - r * per_row) * V, at = r * 2 * a.d_ff + c;
+    Pack g = *reinterpret_cast<const Pack *>(a.gu + at), u = *reinterpret_cast<const Pack *>(a.gu + at + a.d_ff);
+    const Pack d = *reinterpret_cast<const Pack *>(a.dh + r * a.ldh + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float value, slope;
+      act_both(to_f32<BF16>(g.v[i]), a.act, value, slope);
+      const float dh = to_f32<BF16>(d.v[i]);
+      g.v[i] = from_f32<BF16>(dh * to_f32<BF16>(u.v[i]) * slope);
+      u.v[i] = from_f32<BF16>(dh * value);
+    }
+    *reinterpret_cast<Pack *>(a.dgu + at) = g;
+    *reinterpret_cast<Pack *>(a.dgu + at + a.d_ff) = u;
+  }
+}
+
+
+// ---- D[128 x 128 tiles] = A . B, f32 sums, 16-bit results
+namespace prod {
+constexpr int BK = 64, STAGES = 3;
+constexpr int TILE_BYTES = 128 * 128;          // 128 rows or columns x 64 k
+constexpr int STAGE_BYTES = 2 * TILE_BYTES;
+constexpr int SMEM = STAGES * STAGE_BYTES + 256;
+constexpr int THREADS = 256;                   // TMA, products, two idle warps, four that hand the sums over
+static_assert(128 * 128 * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
+static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+struct Params {
+  uint16_t *d;
+  unsigned *status;
+  long long ldd;
+  int rows, cols, tiles_n, k_blocks, shares;
+  uint32_t idesc;
+};
+} // namespace prod
+
+// MN_MAJOR: A is stored [k, rows] and B [k, cols] (X^T dGU); else [rows, k] and [cols, k] (dGU W^T).
+// FIRST: dX's product, which may start while the kernel that writes dGU still runs and lets dW's start beside it once
+// that has ended.
+template <bool BF16, bool MN_MAJOR, bool FIRST>
+__global__ void __launch_bounds__(prod::THREADS, 2)
+gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const prod::Params p) {
+  using namespace prod;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw), bars = base + STAGES * STAGE_BYTES;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  const uint32_t done = bars + 8u * (2 * STAGES), slot = done + 8;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
+  const int row0 = tile / p.tiles_n * 128, col0 = tile % p.tiles_n * 128;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.shares);
+  const int n = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / p.shares) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(128) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (slot - base));
+
+  if (warp == 0) {
+    if (FIRST) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+    if (lane == 0) {
+      for (int i = 0; i < n; ++i) {
+        const int s = i % STAGES, k = (kb0 + i) * BK;
+        if (i >= STAGES && !mbar_wait(empty_bar(s), (i / STAGES - 1) & 1)) {
+          report(p.status, kStatusTmaWaitTimeout);
+          break;
+        }
+        mbar_expect_tx(full_bar(s), STAGE_BYTES);
+        const uint32_t a = base + s * STAGE_BYTES, b = a + TILE_BYTES;
+        if (MN_MAJOR) {
+          tma_load_2d(a, &tmap_a, row0, k, full_bar(s));
+          tma_load_2d(a + TILE_BYTES / 2, &tmap_a, row0 + 64, k, full_bar(s));
+          tma_load_2d(b, &tmap_b, col0, k, full_bar(s));
+          tma_load_2d(b + TILE_BYTES / 2, &tmap_b, col0 + 64, k, full_bar(s));
+        } else {
+          tma_load_2d(a, &tmap_a, k, row0, full_bar(s));
+          tma_load_2d(b, &tmap_b, k, col0, full_bar(s));
+        }
+      }
+      for (int i = max(0, n - STAGES); i < n; ++i)  // everything has been used
+        if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1)) break;
+      // this kernel's end then also stands for the end of the one it was started beside
+      if (!FIRST) asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
+  } else if (warp == 1) {
+    const uint32_t leader = elect_one();
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const int s = i % STAGES;
+      ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (i / STAGES) & 1));
+      if (!ok) break;
+      tcgen05_fence_after();
+      const uint32_t at = base + s * STAGE_BYTES;
+      const uint64_t a = make_smem_desc(at, MN_MAJOR ? TILE_BYTES / 2 : 16, 1024);
+      const uint64_t b = make_smem_desc(at + TILE_BYTES, MN_MAJOR ? TILE_BYTES / 2 : 16, 1024);
+#pragma unroll
+      for (int k = 0; k < BK / 16; ++k) {
+        const uint64_t off = (MN_MAJOR ? k * 2048 : k * 32) >> 4;
+        mma_ss(tmem, a + off, b + off, p.idesc, (i | k) ? 1u : 0u, leader);
+      }
+      commit(empty_bar(s), leader);
+    }
+    if (ok) commit(done, leader);
+    else if (lane == 0) report(p.status, kStatusMmaWaitTimeout);
+  }
+  if (warp < 4) {
+    if (p.shares > 1) {  // the other warps' two barriers
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
+    }
+  } else {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0));
+    if (ok) {
+      tcgen05_fence_after();
+      const int lane_group = warp & 3;
+      leave_row<128, 128>(tmem + (static_cast<uint32_t>(lane_group * 32) << 16), true, base, lane_group * 32 + lane, 0);
+    } else if (lane == 0) {
+      report(p.status, kStatusEpiWaitTimeout);
+    }
+    sums_barrier<128>(p.shares);
+    add_up<BF16, 128, 128>(base, rank, p.shares, 1.0f, p.d + static_cast<long long>(row0) * p.ldd + col0, p.ldd, p.rows - row0,
+                           threadIdx.x - 128, (p.cols - col0 + 7) / 8);
+    sums_barrier<128>(p.shares);
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128) : "memory");
+  }
+}
+
+int64_t pitch(int64_t ld, int64_t width) { return ld > 0 ? ld : width; }
+size_t dgu_bytes(const GatedProblem &p) { return (static_cast<size_t>(p.tokens) * 2 * p.d_ff * 2 + 255) / 256 * 256; }
+
+// The framework's GEMM on the kernel its shapes ask for.
+cudaError_t product(GemmProblem &g, unsigned *status, cudaStream_t stream) {
+  if (gemm_tcgen05_2cta_preferred(g)) {
+    const cudaError_t e = launch_gemm_tcgen05_2cta(g, status, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
+  return launch_gemm_simt(g, stream);
+}
+
+// The pair GEMM's 256 x 256 tiles move half as much through shared memory per operation, but they need many tiles and
+// a long k to pay: 4096 tokens of 4096 x 11264 (256 and 1408 tiles, k 22528 and 4096): 1.20 ms, 1.38 and 1.57 with dX
+// or dW by the small kernel.  300 of 1000 x 2720: 58 us and 30; one of 4096 x 11264 (k of dW 1): 397 and 137; 2048 of
+// 4096 x 4096 (512 tiles, k 2048): dW saves 40 of 300 us; 4096 of 2048 x 2048 (128 tiles, k 4096): the same.
+bool small_product(const GemmProblem &g) {
+  const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
+  return tiles <= 64 || g.K <= 2048 || (tiles <= 148 && g.K <= 4096);
+}
+
+template <auto kernel>
+cudaError_t launch_product(const GemmProblem &g, unsigned *status, cudaStream_t stream) {
+  const bool mn = g.trans_a;
+  CUtensorMap ta, tb;
+  if (!(mn ? make_map(&ta, g.A, g.in_dtype, g.M, g.K, prod::BK, g.lda) : make_map(&ta, g.A, g.in_dtype, g.K, g.M, 128, g.lda)) ||
+      !(mn ? make_map(&tb, g.B, g.in_dtype, g.N, g.K, prod::BK, g.ldb) : make_map(&tb, g.B, g.in_dtype, g.K, g.N, 128, g.ldb)))
+    return cudaErrorNotSupported;
+  const cudaError_t e = allow_smem<kernel>(prod::SMEM);
+  if (e != cudaSuccess) return e;
+  prod::Params p{};
+  p.d = reinterpret_cast<uint16_t *>(g.C);
+  p.status = status;
+  p.ldd = g.ldc;
+  p.rows = static_cast<int>(g.M);
+  p.cols = static_cast<int>(g.N);
+  p.tiles_n = static_cast<int>((g.N + 127) / 128);
+  p.k_blocks = static_cast<int>((g.K + prod::BK - 1) / prod::BK);
+  const int64_t tiles = (g.M + 127) / 128 * p.tiles_n;
+  // shares of k: as many CTAs as run at once, at least four k blocks each
+  p.shares = 1;
+  while (p.shares < 8 && tiles * p.shares * 2 <= 2 * 148 && p.k_blocks >= 8 * p.shares) p.shares *= 2;
+  const uint32_t fmt = g.in_dtype == kBF16 ? 1u : 0u;
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 3u << 15 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.shares));
+  cfg.blockDim = dim3(prod::THREADS);
+  cfg.dynamicSmemBytes = prod::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.shares);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+}
+
+} // namespace
+
+size_t gated_bwd_workspace_bytes(const GatedProblem &p) { return dgu_bytes(p) + gemm_tcgen05_workspace_bytes(); }
+
+cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  const int64_t ldx = pitch(p.ldx, p.d_in), ldw = pitch(p.ldw, 2 * p.d_ff), ldh = pitch(p.ldh, p.d_ff);
+  uint16_t *dgu = static_cast<uint16_t *>(p.workspace);
+  GradArgs a{static_cast<const uint16_t *>(p.gu), static_cast<const uint16_t *>(p.h), dgu, ldh, p.tokens, p.d_ff, p.act};
+  auto on16 = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  const bool wide = p.d_ff % 8 == 0 && ldh % 8 == 0 && on16(p.gu) && on16(p.h) && on16(dgu);
+  const int64_t items = p.tokens * (wide ? p.d_ff / 8 : p.d_ff);
+  const int64_t most = 148 * 8 * 4;  // resident blocks, four rounds each at the most
+  const unsigned blocks = static_cast<unsigned>((items + 255) / 256 < most ? (items + 255) / 256 : most);
+  if (p.dtype == kBF16) {
+    if (wide) gated_grad_kernel<true, 8><<<blocks, 256, 0, stream>>>(a);
+    else gated_grad_kernel<true, 1><<<blocks, 256, 0, stream>>>(a);
+  } else {
+    if (wide) gated_grad_kernel<false, 8><<<blocks, 256, 0, stream>>>(a);
+    else gated_grad_kernel<false, 1><<<blocks, 256, 0, stream>>>(a);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  *launched = 1;
+  // dX[tokens, d_in] = dGU[tokens, 2 d_ff] . W^T, W stored [d_in, 2 d_ff]
+  int n = 1;
+  GemmProblem g;
+  g.in_dtype = g.out_dtype = p.dtype;
+  g.epilogue = kEpiNone;
+  g.accumulate = false;
+  g.bias = nullptr;
+  g.workspace = reinterpret_cast<char *>(p.workspace) + dgu_bytes(p);
+  g.workspace_bytes = gemm_tcgen05_workspace_bytes();
+  g.launched = &n;
+  g.A = dgu, g.B = p.w, g.C = static_cast<float *>(p.dx);
+  g.M = p.tokens, g.N = p.d_in, g.K = 2 * p.d_ff;
+  g.lda = 2 * p.d_ff, g.ldb = ldw, g.ldc = ldx;
+  g.trans_a = false, g.trans_b = true;
+  const bool fits = gemm_tcgen05_2cta_supported(g) && p.d_in % 8 == 0 && ldx % 8 == 0 && on16(p.x) && on16(p.dw);
+  const bool bf16 = p.dtype == kBF16;
+  if (fits && small_product(g))
+    e = bf16 ? launch_product<gated_product_kernel<true, false, true>>(g, status, stream)
+             : launch_product<gated_product_kernel<false, false, true>>(g, status, stream);
+  else
+    e = product(g, status, stream);
+  if (e != cudaSuccess) return e;
+  *launched += n;
+  // dW[d_in, 2 d_ff] = X^T . dGU, X stored [tokens, d_in]
+  n = 1;
+  g.A = p.x, g.B = dgu, g.C = static_cast<float *>(p.dw);
+  g.M = p.d_in, g.N = 2 * p.d_ff, g.K = p.tokens;
+  g.lda = ldx, g.ldb = 2 * p.d_ff, g.ldc = ldw;
+  g.trans_a = true, g.trans_b = false;
+  if (fits && small_product(g))
+    e = bf16 ? launch_product<gated_product_kernel<true, true, false>>(g, status, stream)
+             : launch_product<gated_product_kernel<false, true, false>>(g, status, stream);
+  else
+    e = product(g, status, stream);
+  if (e != cudaSuccess) return e;
+  *launched += n;
+  return cudaSuccess;
+}
+
+} // namespace imex

@@ -1,11 +1,6 @@
-// The gated feed-forward product H = act(X Wg) * (X Wu) with W = [Wg | Wu] (IMEX_OP_GATED_FFN) and its
-// backward pass (IMEX_OP_GATED_FFN_BWD).
+// The gated feed-forward product H = act(X Wg) * (X Wu) with W = [Wg | Wu] (IMEX_OP_GATED_FFN), by the number
+// of tokens:
 //
-// Backward: with [G U] = X W kept by the forward pass, one pass over G, U and dH writes
-// [dG dU] = [dH U act'(G), dH act(G)] into the workspace; because W holds both projections side by side,
-// dX = [dG dU] W^T and dW = X^T [dG dU] are then one product each of the framework's GEMM.
-//
-// Forward, by the number of tokens:
 //   gated_pair_kernel    more than 128 tokens: the CTA-pair GEMM's arrangement (gemm_tcgen05_2cta.cu) with a
 //                        256 x 256 accumulator whose left half is the gate and whose right half is the up
 //                        projection of the same 128 columns of H: CTA 0 of the pair loads the gate's 128
@@ -427,63 +422,7 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   }
 }
 
-struct GradArgs {
-  const uint16_t *gu, *dh;
-  uint16_t *dgu;
-  int64_t ldh, tokens, d_ff;
-  int act;
-};
-
-// act(g) and its derivative
-__device__ __forceinline__ void act_both(float g, int act, float &value, float &slope) {
-  if (act == kEpiSilu) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-    value = g * s;
-    slope = s * (1.0f + g * (1.0f - s));
-  } else if (act == kEpiRelu) {
-    value = relu_ugt(g);
-    slope = !(g <= 0.0f) ? 1.0f : 0.0f;
-  } else {
-    value = g;
-    slope = 1.0f;
-  }
-}
-
-// 10 bytes per element of H and few operations: bound by memory.  V columns per thread.
-template <bool BF16, int V> __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
-  struct alignas(2 * V) Pack {
-    uint16_t v[V];
-  };
-  const int64_t per_row = a.d_ff / V, n = a.tokens * per_row;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
-       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = e / per_row, c = (e - r * per_row) * V, at = r * 2 * a.d_ff + c;
-    Pack g = *reinterpret_cast<const Pack *>(a.gu + at), u = *reinterpret_cast<const Pack *>(a.gu + at + a.d_ff);
-    const Pack d = *reinterpret_cast<const Pack *>(a.dh + r * a.ldh + c);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float value, slope;
-      act_both(to_f32<BF16>(g.v[i]), a.act, value, slope);
-      const float dh = to_f32<BF16>(d.v[i]);
-      g.v[i] = from_f32<BF16>(dh * to_f32<BF16>(u.v[i]) * slope);
-      u.v[i] = from_f32<BF16>(dh * value);
-    }
-    *reinterpret_cast<Pack *>(a.dgu + at) = g;
-    *reinterpret_cast<Pack *>(a.dgu + at + a.d_ff) = u;
-  }
-}
-
 int64_t pitch(int64_t ld, int64_t width) { return ld > 0 ? ld : width; }
-size_t dgu_bytes(const GatedProblem &p) { return (static_cast<size_t>(p.tokens) * 2 * p.d_ff * 2 + 255) / 256 * 256; }
-
-// The framework's GEMM on the kernel its shapes ask for.
-cudaError_t product(GemmProblem &g, unsigned *status, cudaStream_t stream) {
-  if (gemm_tcgen05_2cta_preferred(g)) {
-    const cudaError_t e = launch_gemm_tcgen05_2cta(g, status, stream);
-    if (e != cudaErrorNotSupported) return e;
-  }
-  return launch_gemm_simt(g, stream);
-}
 
 } // namespace
 
@@ -496,8 +435,6 @@ const char *gated_check(const GatedProblem &p) {
     return "row pitch smaller than the row";
   return nullptr;
 }
-
-size_t gated_bwd_workspace_bytes(const GatedProblem &p) { return dgu_bytes(p) + gemm_tcgen05_workspace_bytes(); }
 
 namespace {
 
@@ -604,52 +541,6 @@ cudaError_t launch_gated(const GatedProblem &p, unsigned *status, cudaStream_t s
   if (bf16) gated_tile_kernel<true><<<grid, 256, 0, stream>>>(a);
   else gated_tile_kernel<false><<<grid, 256, 0, stream>>>(a);
   return cudaGetLastError();
-}
-
-cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
-  const int64_t ldx = pitch(p.ldx, p.d_in), ldw = pitch(p.ldw, 2 * p.d_ff), ldh = pitch(p.ldh, p.d_ff);
-  uint16_t *dgu = static_cast<uint16_t *>(p.workspace);
-  GradArgs a{static_cast<const uint16_t *>(p.gu), static_cast<const uint16_t *>(p.h), dgu, ldh, p.tokens, p.d_ff, p.act};
-  auto on16 = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
-  const bool wide = p.d_ff % 8 == 0 && ldh % 8 == 0 && on16(p.gu) && on16(p.h) && on16(dgu);
-  const int64_t items = p.tokens * (wide ? p.d_ff / 8 : p.d_ff);
-  const int64_t most = 148 * 8 * 4;  // resident blocks, four rounds each at the most
-  const unsigned blocks = static_cast<unsigned>((items + 255) / 256 < most ? (items + 255) / 256 : most);
-  if (p.dtype == kBF16) {
-    if (wide) gated_grad_kernel<true, 8><<<blocks, 256, 0, stream>>>(a);
-    else gated_grad_kernel<true, 1><<<blocks, 256, 0, stream>>>(a);
-  } else {
-    if (wide) gated_grad_kernel<false, 8><<<blocks, 256, 0, stream>>>(a);
-    else gated_grad_kernel<false, 1><<<blocks, 256, 0, stream>>>(a);
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  *launched = 1;
-  // dX[tokens, d_in] = dGU[tokens, 2 d_ff] . W^T, W stored [d_in, 2 d_ff]
-  int n = 1;
-  GemmProblem g;
-  g.in_dtype = g.out_dtype = p.dtype;
-  g.epilogue = kEpiNone;
-  g.accumulate = false;
-  g.bias = nullptr;
-  g.workspace = reinterpret_cast<char *>(p.workspace) + dgu_bytes(p);
-  g.workspace_bytes = gemm_tcgen05_workspace_bytes();
-  g.launched = &n;
-  g.A = dgu, g.B = p.w, g.C = static_cast<float *>(p.dx);
-  g.M = p.tokens, g.N = p.d_in, g.K = 2 * p.d_ff;
-  g.lda = 2 * p.d_ff, g.ldb = ldw, g.ldc = ldx;
-  g.trans_a = false, g.trans_b = true;
-  if ((e = product(g, status, stream)) != cudaSuccess) return e;
-  *launched += n;
-  // dW[d_in, 2 d_ff] = X^T . dGU, X stored [tokens, d_in]
-  n = 1;
-  g.A = p.x, g.B = dgu, g.C = static_cast<float *>(p.dw);
-  g.M = p.d_in, g.N = 2 * p.d_ff, g.K = p.tokens;
-  g.lda = ldx, g.ldb = 2 * p.d_ff, g.ldc = ldw;
-  g.trans_a = true, g.trans_b = false;
-  if ((e = product(g, status, stream)) != cudaSuccess) return e;
-  *launched += n;
-  return cudaSuccess;
 }
 
 } // namespace imex

@@ -1,0 +1,84 @@
+// How CTAs hand over a 128-row tile of f32 sums in TMEM: through their shared memory, where the CTAs of a cluster
+// that hold parts of the same sums add them up in order, and out as 16-bit rows with neighbouring threads on
+// neighbouring addresses.
+#pragma once
+#include "attention_tc.cuh"
+
+namespace imex {
+namespace attn {
+
+// f32 rows of DH values in shared memory, 16-byte units swizzled by the row
+template <int DH> __device__ __forceinline__ uint32_t sum_offset(int row, int unit) {
+  return row * (DH * 4) + ((unit ^ (row & 7)) * 16);
+}
+template <int DH, int COLS>
+__device__ __forceinline__ void leave_row(uint32_t taddr, bool has, uint32_t sums, int row, int col0) {
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 32) {
+    uint32_t v[32];
+    if (has) {
+      tmem_ld_32x32(taddr + c, v);
+      tmem_ld_wait();
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      st_shared_v4(sums + sum_offset<DH>(row, (col0 + c) / 4 + e),
+                   has ? make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                     __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]))
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+  }
+}
+// This CTA's part of the rows over all shares, in order, to 16 bits: neighbouring threads write neighbouring
+// 16 bytes of a row.  `thread` of THREADS; rows_left rows and units_left units of eight columns exist; the loads of two steps are in flight together.
+template <bool BF16, int DH, int S, int THREADS>
+__device__ __forceinline__ void add_up_of(uint32_t sums, int rank, float factor, uint16_t *to, int64_t step, int rows_left,
+                                          int units_left, int thread) {
+  constexpr int UNITS = TILE / S * (DH / 8), STEPS = (UNITS + THREADS - 1) / THREADS;
+#pragma unroll 2
+  for (int k = 0; k < STEPS; ++k) {
+    const int u = thread + k * THREADS;
+    const int row = rank * (TILE / S) + u / (DH / 8), unit = u % (DH / 8) * 2;
+    float4 v[S][2];
+#pragma unroll
+    for (int r = 0; r < S; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t at = sums + sum_offset<DH>(u < UNITS ? row : 0, unit + h);
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[r][h].x), "=f"(v[r][h].y), "=f"(v[r][h].z), "=f"(v[r][h].w)
+                     : "r"(S > 1 ? map_to_cta(at, r) : at));
+      }
+#pragma unroll
+    for (int r = 1; r < S; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v[0][h].x += v[r][h].x;
+        v[0][h].y += v[r][h].y;
+        v[0][h].z += v[r][h].z;
+        v[0][h].w += v[r][h].w;
+      }
+    const float4 x = v[0][0], y = v[0][1];
+    if (u < UNITS && row < rows_left && unit / 2 < units_left)
+      *reinterpret_cast<uint4 *>(to + row * step + unit * 4) =
+          make_uint4(pack2<BF16>(x.x * factor, x.y * factor), pack2<BF16>(x.z * factor, x.w * factor),
+                     pack2<BF16>(y.x * factor, y.y * factor), pack2<BF16>(y.z * factor, y.w * factor));
+  }
+}
+template <bool BF16, int DH, int THREADS>
+__device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, float factor, uint16_t *to, int64_t step,
+                                       int rows_left, int thread, int units_left = DH / 8) {
+  if (shares == 1) add_up_of<BF16, DH, 1, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
+  else if (shares == 2) add_up_of<BF16, DH, 2, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
+  else if (shares == 4) add_up_of<BF16, DH, 4, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
+  else add_up_of<BF16, DH, 8, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
+}
+// The computing warps' sums are in place everywhere / have been read everywhere.  The first warpgroup takes part
+// when there are several CTAs.
+template <int THREADS> __device__ __forceinline__ void sums_barrier(int shares) {
+  __syncwarp();
+  if (shares > 1) cluster_sync_all();
+  else asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+
+} // namespace attn
+} // namespace imex

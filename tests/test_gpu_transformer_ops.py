@@ -307,6 +307,41 @@ def test_attention_runs_give_the_same_bits(pkg, sess):
             assert torch.equal(first[n].contiguous().view(torch.int16), again[n].contiguous().view(torch.int16)), n
 
 
+@pytest.mark.parametrize("d,kind", [(64, "f16"), (128, "bf16")])
+def test_attention_gradients_with_warps_out_of_step(pkg, d, kind):
+    """Many CTAs, short and long ones beside each other, every launch behind other work that leaves the caches cold:
+    the gradients of the first and of later launches are the same bits, none of them NaN."""
+    torch.manual_seed(3)
+    dims = (4, 16, 16, 1000, 1000, d)
+    new = lambda: torch.randn((4, 1000, 16, d), device="cuda").to(TORCH[kind])  # noqa: E731
+    with pkg.Session(device=0, adopt_stream=1) as sess:
+        B = pkg.blob
+        q, k, v, do, o = new(), new(), new(), new(), torch.empty((4, 1000, 16, d), dtype=TORCH[kind], device="cuda")
+        lse, lens = torch.empty((4, 16, 1000), device="cuda"), torch.tensor([0, 1000, 777, 850], dtype=torch.int32, device="cuda")
+        kw = dict(dtype=_dt(pkg, kind), key_lens=True, layout="tokens")
+        grads = [torch.empty_like(q) for _ in range(3)]
+
+        def bind(desc, args):
+            kernel = sess.kernel(desc)
+            need = sess.workspace_bytes(kernel)
+            if need:
+                args = args + [torch.empty(need, dtype=torch.uint8, device="cuda")]
+            return sess.bind(kernel, [t.data_ptr() for t in args]), args
+        forward, keep = bind(B.attention("a", *dims, **kw), [q, k, v, o, lse, lens])
+        backward, keep2 = bind(B.attention_bwd("b", *dims, **kw), [q, k, v, o, do, lse] + grads + [lens])
+        forward()
+        first, spoil = None, torch.empty(64 << 20, device="cuda")
+        for _ in range(25):
+            spoil.fill_(1.0)
+            for g in grads:
+                g.fill_(float("nan"))
+            backward()
+            got = [g.clone() for g in grads]
+            assert all(torch.isfinite(g).all() for g in got)
+            first = first or got
+            assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(first, got))
+
+
 # --------------------------------------------------------------------------------------- gated product
 def _act(g, act):
     return {0: g, 1: g.clamp(min=0), 2: torch.nn.functional.silu(g)}[act]
@@ -418,7 +453,8 @@ def _rotary_tolerance(x, want, n, kind, interleaved, factor):
 @pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "interleaved"])
 @pytest.mark.parametrize("inverse", [False, True], ids=["", "inverse"])
 @pytest.mark.parametrize("case", [(1, 1, 2, 2, "f32"), (7, 3, 64, 64, "bf16"), (300, 2, 128, 64, "f16"), (5, 40, 80, 20, "bf16"),
-                                  (33, 5, 96, 24, "f32"), (2, 9, 256, 256, "f16"), (600, 1, 66, 6, "bf16")],
+                                  (33, 5, 96, 24, "f32"), (2, 9, 256, 256, "f16"), (600, 1, 66, 6, "bf16"),
+                                  (3, 2, 511, 18, "f16"), (2000, 3, 16, 8, "f32"), (40, 7, 512, 256, "bf16")],
                          ids=lambda c: "-".join(str(x) for x in c))
 def test_rotary(pkg, sess, case, interleaved, inverse):
     tokens, heads, d, rot, kind = case
@@ -441,23 +477,24 @@ def test_rotary(pkg, sess, case, interleaved, inverse):
     assert np.array_equal(back.view(np.int32 if kind == "f32" else np.int16), _bits(got))
 
 
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "interleaved"])
 @pytest.mark.parametrize("step", [1, 2, 8])
-def test_rotary_strides_and_alignment(pkg, sess, step):
+def test_rotary_strides_and_alignment(pkg, sess, step, interleaved):
     """Heads inside a wider row, starting on any element."""
     tokens, heads, d, held = 20, 3, 64, 3 * 72 + step
     x = _rand((tokens * held + 16,), "f16", 8)
     pos = torch.arange(tokens, dtype=torch.int32)
     y = Output(sess, tokens * held, "f16")
     freqs = pkg.blob.rotary_frequencies(32)
-    _launch(sess, pkg.blob.rotary("r", tokens, heads, d, freqs, pkg.blob.F16, x_strides=(held, 72), y_strides=(held, 72)),
+    _launch(sess, pkg.blob.rotary("r", tokens, heads, d, freqs, pkg.blob.F16, interleaved, x_strides=(held, 72), y_strides=(held, 72)),
             [sess.upload(_bits(x)) + 2 * step, sess.upload(pos.numpy()), y.ptr])
     xs = x[step:step + tokens * held].reshape(tokens, held)[:, :3 * 72].reshape(tokens, 3, 72)[..., :d]
     got = y.get((tokens, held))
     assert (got[:, 3 * 72:].contiguous().view(torch.int16) == SENTINEL).all()
     got = got[:, :3 * 72].reshape(tokens, 3, 72)
     assert (got[..., d:].contiguous().view(torch.int16) == SENTINEL).all()
-    want = _rotate(xs, pos, freqs, False, False, 1.0)
-    assert ((got[..., :d].double() - want).abs() <= _rotary_tolerance(xs, want, 16, "f16", False, 1.0)).all()
+    want = _rotate(xs, pos, freqs, interleaved, False, 1.0)
+    assert ((got[..., :d].double() - want).abs() <= _rotary_tolerance(xs, want, 16, "f16", interleaved, 1.0)).all()
 
 
 # ------------------------------------------------------------------------------------- a block of them

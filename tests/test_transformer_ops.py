@@ -60,7 +60,7 @@ def test_rotary_descriptor_and_refusals():
     assert struct.unpack("<8q", d.payload[:64]) == (5, 2, 64, 4, 200, 70, 128, 64)
     for bad in (dict(tokens=0), dict(frequencies=[]), dict(frequencies=[1.0] * 33), dict(frequencies=[float("inf")]),
                 dict(dtype=B.I32), dict(y_strides=(200, 63)), dict(y_strides=(100, 64)), dict(x_strides=(1, 2, 3)),
-                dict(x_strides=(-64, 64))):
+                dict(x_strides=(-64, 64)), dict(d_head=513)):
         args = dict(tokens=5, heads=2, d_head=64, frequencies=[1.0])
         args.update(bad)
         with pytest.raises(ValueError):

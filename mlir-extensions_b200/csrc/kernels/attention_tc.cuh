@@ -72,6 +72,26 @@ __device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
       "r"(leader)
       : "memory");
 }
+// The same for CTA pairs: M 256, both CTAs' shared memory; the commit signals the barrier of both.
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t leader) {
+  const uint16_t both = 3;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+      "h"(both), "r"(leader)
+      : "memory");
+}
 // D[128 x BN] = A . B^T over DH, both tiles in shared memory, rows of d_head values (K-major)
 template <int DH, int BN>
 __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_smem, uint32_t b_smem, uint32_t idesc,

@@ -14,8 +14,7 @@
 //   gated_tile_kernel    extents, pitches or addresses TMA cannot take (not multiples of 16 bytes).
 #include "attention_common.cuh"
 #include "epilogue.cuh"
-#include "tcgen05_host.h"
-#include "tcgen05_ptx.cuh"
+#include "attention_tc.cuh"
 
 namespace imex {
 namespace {
@@ -128,7 +127,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   auto acc_full = [&](int a) { return bars + 8u * (2 * STAGES + a); };
   auto acc_empty = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
   const uint32_t slot = bars + 8u * (2 * STAGES + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
 
@@ -187,29 +186,36 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
       }
     }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
+      // the whole warp walks the loop, one thread issues (see attention_tc.cuh)
+      const uint32_t leader = attn::elect_one();
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+        return ok;
+      };
       for (int tile = cluster; tile < p.num_tiles && ok; tile += clusters) {
-        ok = mbar_wait(acc_empty(acc), acc_phase ^ 1u);
+        if (!wait(acc_empty(acc), acc_phase ^ 1u)) break;
         tcgen05_fence_after();
-        for (int kb = 0; kb < p.k_blocks && ok; ++kb) {
-          ok = mbar_wait(full_bar(stage), phase);
-          if (!ok) break;
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!wait(full_bar(stage), phase)) break;
           tcgen05_fence_after();
-          const uint32_t x = base + stage * STAGE_BYTES, w = x + 2 * BOX;
+          const uint32_t x = base + stage * STAGE_BYTES;
+          const uint64_t a = make_smem_desc(x, 16, 1024), w = make_smem_desc(x + 2 * BOX, BOX, 1024);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            tcgen05_mma_f16_pair(tmem + acc * 256, make_smem_desc(x + (k >> 2) * BOX + (k & 3) * 32, 16, 1024),
-                                 make_smem_desc(w + k * 2048, BOX, 1024), p.idesc, (kb | k) ? 1u : 0u);
-          tcgen05_commit_pair(empty_bar(stage), 3);
+            attn::mma_pair(tmem + acc * 256, a + (((k >> 2) * BOX + (k & 3) * 32) >> 4), w + (k * 2048 >> 4), p.idesc,
+                           (kb | k) ? 1u : 0u, leader);
+          attn::commit_pair(empty_bar(stage), leader);
           if (++stage == STAGES) stage = 0, phase ^= 1u;
         }
-        if (ok) tcgen05_commit_pair(acc_full(acc), 3);
+        if (!ok) break;
+        attn::commit_pair(acc_full(acc), leader);
         if (++acc == 2) acc = 0, acc_phase ^= 1u;
       }
-      if (!ok) report(p.status, kStatusMmaWaitTimeout);
+      if (!ok && lane == 0) report(p.status, kStatusMmaWaitTimeout);
     }
   } else {
     const int lane_group = warp & 3;
@@ -302,7 +308,7 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
   const uint32_t acc_full = bars + 8u * (2 * STAGES), slot = acc_full + 8;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int f0 = blockIdx.x / p.shares * BF;
   const int kb0 = p.k_blocks * rank / p.shares, kb1 = p.k_blocks * (rank + 1) / p.shares;
@@ -343,25 +349,25 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1)) break;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, s = i % STAGES;
-        ok = mbar_wait(full_bar(s), (i / STAGES) & 1);
-        if (!ok) break;
-        tcgen05_fence_after();
-        const uint32_t w = base + s * STAGE_BYTES;
+    const uint32_t leader = attn::elect_one();
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int i = kb - kb0, s = i % STAGES;
+      ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (i / STAGES) & 1));
+      if (!ok) break;
+      tcgen05_fence_after();
+      const uint32_t at = base + s * STAGE_BYTES;
+      const uint64_t g = make_smem_desc(at, W_BOX, 1024), u = make_smem_desc(at + 2 * W_BOX, W_BOX, 1024);
+      const uint64_t x = make_smem_desc(at + W_BYTES, 16, 1024);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k) {
-          const uint64_t x = make_smem_desc(w + W_BYTES + k * 32, 16, 1024);
-          tcgen05_mma_f16(tmem, make_smem_desc(w + k * 2048, W_BOX, 1024), x, p.idesc, (i | k) ? 1u : 0u);
-          tcgen05_mma_f16(tmem + NT, make_smem_desc(w + 2 * W_BOX + k * 2048, W_BOX, 1024), x, p.idesc, (i | k) ? 1u : 0u);
-        }
-        tcgen05_commit(empty_bar(s));
+      for (int k = 0; k < BK / 16; ++k) {
+        attn::mma_ss(tmem, g + (k * 2048 >> 4), x + (k * 32 >> 4), p.idesc, (i | k) ? 1u : 0u, leader);
+        attn::mma_ss(tmem + NT, u + (k * 2048 >> 4), x + (k * 32 >> 4), p.idesc, (i | k) ? 1u : 0u, leader);
       }
-      if (ok) tcgen05_commit(acc_full);
-      else report(p.status, kStatusMmaWaitTimeout);
+      attn::commit(empty_bar(s), leader);
     }
+    if (ok) attn::commit(acc_full, leader);
+    else if (lane == 0) report(p.status, kStatusMmaWaitTimeout);
   }
   __syncwarp();
   // sums of this CTA's share of k: lane = column of H, a row of `sums` per token
@@ -450,8 +456,7 @@ cudaError_t launch_few(const GatedProblem &p, const few::Params &f, cudaStream_t
   if (!make_map(&tx, p.x, p.dtype, p.d_in, p.tokens, NT, pitch(p.ldx, p.d_in)) ||
       !make_map(&tw, p.w, p.dtype, 2 * p.d_ff, p.d_in, few::BK, pitch(p.ldw, 2 * p.d_ff)))
     return cudaErrorNotSupported;
-  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(gated_few_kernel<BF16, NT>),
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, few::smem_bytes(NT));
+  const cudaError_t e = attn::allow_smem<gated_few_kernel<BF16, NT>>(few::smem_bytes(NT));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.d_ff + few::BF - 1) / few::BF) * f.shares);
@@ -501,8 +506,7 @@ template <bool BF16> cudaError_t launch_many_tokens(const GatedProblem &p, unsig
   if (!make_map(&tx, p.x, p.dtype, p.d_in, p.tokens, pair::BM, pitch(p.ldx, p.d_in)) ||
       !make_map(&tw, p.w, p.dtype, 2 * p.d_ff, p.d_in, pair::BK, pitch(p.ldw, 2 * p.d_ff)))
     return cudaErrorNotSupported;
-  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(gated_pair_kernel<BF16>),
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM_BYTES);
+  const cudaError_t e = attn::allow_smem<gated_pair_kernel<BF16>>(pair::SMEM_BYTES);
   if (e != cudaSuccess) return e;
   pair::Params f{};
   f.h = static_cast<uint16_t *>(p.h);

@@ -6,9 +6,10 @@
 //                        projection of the same 128 columns of H: CTA 0 of the pair loads the gate's 128
 //                        columns of W, CTA 1 the up projection's, and every thread of the epilogue has both
 //                        values of its elements in its own TMEM lane.
-//   gated_few_kernel     up to 128 tokens, where W's bytes are the time: W^T is the M operand (128 columns of
-//                        a projection per tile, as they lie), the tokens are the N operand, so that no
-//                        part of a tensor-core tile is wasted on rows that do not exist; k is shared out
+//   gated_few_kernel     up to 128 tokens, where W's bytes are the time: W^T is the M operand (the gate's and
+//                        the up projection's columns of 64 columns of H per tile, as they lie), the tokens
+//                        are the N operand, so that no part of a tensor-core tile is wasted on rows that do
+//                        not exist; k is shared out
 //                        between the CTAs of a cluster, which add their parts up through distributed
 //                        shared memory, in order.
 //   gated_tile_kernel    extents, pitches or addresses TMA cannot take (not multiples of 16 bytes).
@@ -279,14 +280,15 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 
 // ------------------------------------------------------------------------------------------- few tokens
 namespace few {
-constexpr int BF = 128;                 // columns of H per tile: the M of both products
+constexpr int BF = 64;                  // columns of H per tile; the M of the product is their gate and up columns
 constexpr int BK = 64;
 constexpr int W_BOX = BK * 128;         // 64 k x 64 columns
-constexpr int W_BYTES = 4 * W_BOX;      // gate and up, two boxes each
+constexpr int W_BYTES = 2 * W_BOX;      // gate, up
 __host__ __device__ constexpr int stage_bytes(int nt) { return W_BYTES + nt * 128; }
-// two CTAs per SM up to 32 tokens (102 and 108 KB), one above
-__host__ __device__ constexpr int stages(int nt) { return nt <= 32 ? 3 : nt == 64 ? 5 : 4; }
+// 90 to 100 KB of loads in flight; two CTAs per SM
+__host__ __device__ constexpr int stages(int nt) { return nt <= 32 ? 5 : nt == 64 ? 4 : 3; }
 __host__ __device__ constexpr int smem_bytes(int nt) { return stages(nt) * stage_bytes(nt) + 256; }
+static_assert(2 * (smem_bytes(32) + 1024) <= 233472 && 2 * (smem_bytes(128) + 1024) <= 233472, "two CTAs per SM");
 constexpr int THREADS = 192;
 struct Params {
   uint16_t *h, *gu;
@@ -298,11 +300,12 @@ struct Params {
 } // namespace few
 
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(few::THREADS, NT <= 32 ? 2 : 1)
+__global__ void __launch_bounds__(few::THREADS, 2)
 gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const few::Params p) {
   using namespace few;
   constexpr int STAGES = stages(NT), STAGE_BYTES = stage_bytes(NT);
-  static_assert(2 * NT * BF * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
+  static_assert(NT * 2 * BF * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
+  constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw), bars = base + STAGES * STAGE_BYTES;
   auto full_bar = [&](int s) { return bars + 8u * s; };
@@ -322,12 +325,12 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc_one(slot, 2 * NT);
+  if (warp == 1) tmem_alloc_one(slot, TMEM_COLS);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (slot - base));
-  float *sums = reinterpret_cast<float *>(smem_raw);  // [gate, up][NT][BF] once the ring is done with
+  float *sums = reinterpret_cast<float *>(smem_raw);  // [NT][gate BF, up BF] once the ring is done with
 
   if (warp == 0) {
     if (lane == 0) {
@@ -340,9 +343,7 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         mbar_expect_tx(full_bar(s), STAGE_BYTES);
         const uint32_t w = base + s * STAGE_BYTES;
         tma_load_2d(w, &tmap_w, f0, kb * BK, full_bar(s));
-        tma_load_2d(w + W_BOX, &tmap_w, f0 + 64, kb * BK, full_bar(s));
-        tma_load_2d(w + 2 * W_BOX, &tmap_w, p.d_ff + f0, kb * BK, full_bar(s));
-        tma_load_2d(w + 3 * W_BOX, &tmap_w, p.d_ff + f0 + 64, kb * BK, full_bar(s));
+        tma_load_2d(w + W_BOX, &tmap_w, p.d_ff + f0, kb * BK, full_bar(s));
         tma_load_2d(w + W_BYTES, &tmap_x, kb * BK, 0, full_bar(s));
       }
       for (int i = max(0, kb1 - kb0 - STAGES); i < kb1 - kb0; ++i)  // everything has been used
@@ -357,13 +358,10 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       if (!ok) break;
       tcgen05_fence_after();
       const uint32_t at = base + s * STAGE_BYTES;
-      const uint64_t g = make_smem_desc(at, W_BOX, 1024), u = make_smem_desc(at + 2 * W_BOX, W_BOX, 1024);
-      const uint64_t x = make_smem_desc(at + W_BYTES, 16, 1024);
+      const uint64_t w = make_smem_desc(at, W_BOX, 1024), x = make_smem_desc(at + W_BYTES, 16, 1024);
 #pragma unroll
-      for (int k = 0; k < BK / 16; ++k) {
-        attn::mma_ss(tmem, g + (k * 2048 >> 4), x + (k * 32 >> 4), p.idesc, (i | k) ? 1u : 0u, leader);
-        attn::mma_ss(tmem + NT, u + (k * 2048 >> 4), x + (k * 32 >> 4), p.idesc, (i | k) ? 1u : 0u, leader);
-      }
+      for (int k = 0; k < BK / 16; ++k)
+        attn::mma_ss(tmem, w + (k * 2048 >> 4), x + (k * 32 >> 4), p.idesc, (i | k) ? 1u : 0u, leader);
       attn::commit(empty_bar(s), leader);
     }
     if (ok) attn::commit(acc_full, leader);
@@ -378,12 +376,13 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
       const int lane_group = warp & 3;
       const uint32_t t = tmem + (static_cast<uint32_t>(lane_group * 32) << 16);
 #pragma unroll 1
-      for (int c0 = 0; c0 < 2 * NT; c0 += 32) {
+      for (int c0 = 0; c0 < NT; c0 += 32) {
         uint32_t v[32];
         tmem_ld_32x32(t + c0, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sums[(c0 + e) * BF + lane_group * 32 + lane] = __uint_as_float(v[e]);
+        for (int e = 0; e < 32; ++e)
+          if (c0 + e < NT) sums[(c0 + e) * 2 * BF + lane_group * 32 + lane] = __uint_as_float(v[e]);
       }
     } else if (lane == 0) {
       report(p.status, kStatusEpiWaitTimeout);
@@ -392,21 +391,18 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   if (p.shares > 1) cluster_sync_all();
   else __syncthreads();
   if (warp >= 2 && ok) {
-    const int c = threadIdx.x - 64, col = f0 + c;
+    // two tokens at a time
+    const int c = threadIdx.x % BF, col = f0 + c;
     if (col < p.d_ff) {
-      const uint32_t mine = base + c * 4;
-      for (int token = rank; token < p.tokens; token += p.shares) {
+      for (int token = rank * 2 + (threadIdx.x - 64) / BF; token < p.tokens; token += 2 * p.shares) {
+        const uint32_t mine = base + (token * 2 * BF + c) * 4;
         float g = 0.0f, u = 0.0f;
+#pragma unroll 4
         for (int r = 0; r < p.shares; ++r) {
           const uint32_t from = p.shares > 1 ? map_to_cta(mine, r) : mine;
           float x, y;
-          if (p.shares > 1) {
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from + token * BF * 4) : "memory");
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(from + (NT + token) * BF * 4) : "memory");
-          } else {
-            x = sums[token * BF + c];
-            y = sums[(NT + token) * BF + c];
-          }
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(from + BF * 4));
           g += x;
           u += y;
         }
@@ -424,7 +420,7 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   else __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * NT) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }
 }
 
@@ -483,18 +479,17 @@ template <bool BF16> cudaError_t launch_few_tokens(const GatedProblem &p, unsign
   f.act = p.act;
   f.k_blocks = static_cast<int>((p.d_in + few::BK - 1) / few::BK);
   const int nt = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
+  const int64_t tiles = (p.d_ff + few::BF - 1) / few::BF;
   // Shares of k per tile: as many CTAs as run at once, at least two k blocks each.  One token of 4096 x 11264
-  // (88 tiles): 36.9 us with one share, 32.8 with 3 (what fits at once), 37.3 with 4; 8192 x 1024 (8 tiles): 55,
-  // 24.6 (3), 14.0 (8).
-  const int64_t tiles = (p.d_ff + few::BF - 1) / few::BF, slots = nt <= 32 ? 2 * 148 : 148;
-  int64_t shares = slots / tiles;
+  // (176 tiles): 31.5 us with one share, 38 with 2; of 8192 x 1024 (16 tiles): 35 us with one, 10.3 with 8.
+  int64_t shares = 2 * 148 / tiles;
   if (shares > 8) shares = 8;
   if (shares > f.k_blocks / 2) shares = f.k_blocks / 2;
   f.shares = shares < 1 ? 1 : static_cast<int>(shares);
   const uint32_t fmt = BF16 ? 1u : 0u;
   // f32 accumulator; A (W) is MN-major, B (X) K-major; N >> 3, M >> 4
   f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (static_cast<uint32_t>(nt >> 3) << 17) |
-            (static_cast<uint32_t>(few::BF >> 4) << 24);
+            ((128u >> 4) << 24);
   if (nt == 16) return launch_few<BF16, 16>(p, f, stream);
   if (nt == 32) return launch_few<BF16, 32>(p, f, stream);
   if (nt == 64) return launch_few<BF16, 64>(p, f, stream);

@@ -145,6 +145,14 @@ template <int DH> __device__ __forceinline__ void take_registers() {
 // Blocks [share_of(n, r, s), share_of(n, r + 1, s)) are those of share r of s
 __device__ __forceinline__ int share_of(int n, int r, int s) { return static_cast<int>(static_cast<int64_t>(n) * r / s); }
 
+// A resident tile of 128 rows, by the boxes of BN rows that the walked blocks use.
+template <int DH>
+__device__ __forceinline__ void load_resident(uint32_t dst, const CUtensorMap *map, int row, int head, int batch, uint32_t bar) {
+  constexpr int BN = Sizes<DH>::BN;
+#pragma unroll
+  for (int r = 0; r < TILE; r += BN) load_tile<DH, BN>(dst + r * 128, map, row + r, head, batch, bar);
+}
+
 // The producer's two streams of tiles, in the order the products use them.
 template <int DH, typename LoadA, typename LoadB>
 __device__ __forceinline__ void produce(const Layout<DH> &L, int n, unsigned *status, LoadA &&load_a, LoadB &&load_b) {
@@ -256,8 +264,8 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     init_barriers<DH>(L);
     if (n > 0) {  // the first tiles, while the others set up
       mbar_expect_tx(L.res_full(), 2 * T::RB);
-      load_tile<DH>(L.resident(0), &tmap_q, row0, head, b, L.res_full());
-      load_tile<DH>(L.resident(1), &tmap_do, row0, head, b, L.res_full());
+      load_resident<DH>(L.resident(0), &tmap_q, row0, head, b, L.res_full());
+      load_resident<DH>(L.resident(1), &tmap_do, row0, head, b, L.res_full());
       mbar_expect_tx(L.a_full(0), T::TB);
       load_a(0, L.a_tile(0), L.a_full(0));
       mbar_expect_tx(L.b_full(0), T::TB);
@@ -461,8 +469,8 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     init_barriers<DH>(L);
     if (n > 0) {  // the first tiles, while the others set up
       mbar_expect_tx(L.res_full(), 2 * T::RB);
-      load_tile<DH>(L.resident(0), &tmap_k, key0, kv_head, b, L.res_full());
-      load_tile<DH>(L.resident(1), &tmap_v, key0, kv_head, b, L.res_full());
+      load_resident<DH>(L.resident(0), &tmap_k, key0, kv_head, b, L.res_full());
+      load_resident<DH>(L.resident(1), &tmap_v, key0, kv_head, b, L.res_full());
       mbar_expect_tx(L.a_full(0), T::TB);
       load_a(0, L.a_tile(0), L.a_full(0));
       mbar_expect_tx(L.b_full(0), T::TB);
@@ -687,7 +695,6 @@ int share_count(int64_t tiles, int64_t blocks, int64_t slots, int least, bool un
 
 template <bool BF16, int DH>
 cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tdo,
-                        const CUtensorMap &tqb, const CUtensorMap &tdob, const CUtensorMap &tkb, const CUtensorMap &tvb,
                         BwdParams f, int64_t batch, cudaStream_t stream) {
   using Z = Sizes<DH>;
   const int64_t slots = 148 * Z::CTAS;
@@ -695,31 +702,25 @@ cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUte
   f.heads_batch = static_cast<int>(batch) * f.q_heads;
   int64_t tiles = static_cast<int64_t>(f.tiles) * f.heads_batch;
   f.shares = share_count(tiles, (f.n_kv + Z::BN - 1) / Z::BN, slots, DH == 64 ? 2 : 4, f.causal);
-  cudaError_t e = launch_shared<attention_dq_kernel<BF16, DH>, DH>(f, tiles, false, stream, tq, tkb, tvb, tdo);
+  cudaError_t e = launch_shared<attention_dq_kernel<BF16, DH>, DH>(f, tiles, false, stream, tq, tk, tv, tdo);
   if (e != cudaSuccess) return e;
   f.tiles = (f.n_kv + TILE - 1) / TILE;
   f.heads_batch = static_cast<int>(batch) * f.kv_heads;
   tiles = static_cast<int64_t>(f.tiles) * f.heads_batch;
   f.shares = share_count(tiles, static_cast<int64_t>((f.n_q + Z::BN - 1) / Z::BN) * f.group, slots, DH == 64 ? 2 : 4, f.causal);
-  return launch_shared<attention_dkv_kernel<BF16, DH>, DH>(f, tiles, true, stream, tqb, tk, tv, tdob);
+  return launch_shared<attention_dkv_kernel<BF16, DH>, DH>(f, tiles, true, stream, tq, tk, tv, tdo);
 }
 
 } // namespace
 
 cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
   const bool bf16 = p.dtype == kBF16;
-  CUtensorMap tq, tk, tv, tdo, tqb, tkb, tvb, tdob;  // resident tiles, walked blocks
-  if (!make_map_4d(&tq, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq, TILE, 1) ||
-      !make_map_4d(&tdo, p.dout, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sdo, TILE, 1) ||
-      !make_map_4d(&tk, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, TILE, 1) ||
-      !make_map_4d(&tv, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, TILE, 1))
-    return cudaErrorNotSupported;
-  tqb = tq, tkb = tk, tvb = tv, tdob = tdo;
-  if (p.d_head == 64 &&
-      (!make_map_4d(&tqb, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq, 64, 1) ||
-       !make_map_4d(&tdob, p.dout, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sdo, 64, 1) ||
-       !make_map_4d(&tkb, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, 64, 1) ||
-       !make_map_4d(&tvb, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, 64, 1)))
+  const int rows = static_cast<int>(p.d_head);  // BN
+  CUtensorMap tq, tk, tv, tdo;
+  if (!make_map_4d(&tq, p.q, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sq, rows, 1) ||
+      !make_map_4d(&tdo, p.dout, p.dtype, p.d_head, p.n_q, p.q_heads, p.batch, p.sdo, rows, 1) ||
+      !make_map_4d(&tk, p.k, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sk, rows, 1) ||
+      !make_map_4d(&tv, p.v, p.dtype, p.d_head, p.n_kv, p.kv_heads, p.batch, p.sv, rows, 1))
     return cudaErrorNotSupported;
   BwdParams f{};
   f.o = static_cast<const uint16_t *>(p.o);
@@ -744,10 +745,10 @@ cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cu
   f.idesc_o = instruction_desc(bf16, true, static_cast<int>(p.d_head));
   *launched = 2;
   if (p.d_head == 64)
-    return bf16 ? launch_both<true, 64>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream)
-                : launch_both<false, 64>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream);
-  return bf16 ? launch_both<true, 128>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream)
-              : launch_both<false, 128>(tq, tk, tv, tdo, tqb, tdob, tkb, tvb, f, p.batch, stream);
+    return bf16 ? launch_both<true, 64>(tq, tk, tv, tdo, f, p.batch, stream)
+                : launch_both<false, 64>(tq, tk, tv, tdo, f, p.batch, stream);
+  return bf16 ? launch_both<true, 128>(tq, tk, tv, tdo, f, p.batch, stream)
+              : launch_both<false, 128>(tq, tk, tv, tdo, f, p.batch, stream);
 }
 
 } // namespace imex

@@ -35,6 +35,8 @@
 // Every wait is bounded; one that runs out records a status code and the role leaves its loop.
 #include "attention_tc.cuh"
 
+#include <type_traits>
+
 namespace imex {
 namespace {
 
@@ -284,6 +286,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot_ptr;
+  if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -588,6 +591,7 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (tmem_slot - q_smem));
+  if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -745,23 +749,44 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
   }
 }
 
-// O and LSE of a row from its splits, in order.  One warp per row.
+// O and LSE of a row from its splits (64 at most).  One warp per row: a lane has the maximum and sum of two splits, then
+// the warp adds up the rows in order, eight loads in flight.
 template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_join_kernel(const FwdParams p) {
+  // started while the last tiles still run
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= p.rows) return;
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[s * p.rows + row].x);
-  const float m_safe = m == -INFINITY ? 0.0f : m;
-  constexpr int V = DH / 32;
-  float l = 0.0f, x[V] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = p.part_ml[s * p.rows + row];
-    const float a = ex2(ml.x - m_safe);
-    l = fmaf(ml.y, a, l);
-    const float *from = p.part_o + (s * p.rows + row) * DH + lane * V;
+  float2 ml[2];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = fmaf(from[e], a, x[e]);
+  for (int k = 0; k < 2; ++k)
+    ml[k] = lane + 32 * k < p.splits ? p.part_ml[(lane + 32 * k) * p.rows + row] : make_float2(-INFINITY, 0.0f);
+  float m = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+  for (int s = 16; s; s /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+  const float m_safe = m == -INFINITY ? 0.0f : m;
+  const float a0 = ex2(ml[0].x - m_safe), a1 = ex2(ml[1].x - m_safe);
+  float l = fmaf(ml[0].y, a0, ml[1].y * a1);
+#pragma unroll
+  for (int s = 16; s; s /= 2) l += __shfl_xor_sync(0xffffffffu, l, s);
+  constexpr int V = DH / 32;
+  using Vec = typename std::conditional<V == 4, float4, float2>::type;
+  float x[V] = {};
+  const float *from = p.part_o + row * DH + lane * V;
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+    Vec v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (s0 + k < p.splits) v[k] = *reinterpret_cast<const Vec *>(from + (s0 + k) * p.rows * DH);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (s0 + k < p.splits) {
+        const int s = s0 + k;
+        const float a = __shfl_sync(0xffffffffu, s < 32 ? a0 : a1, s & 31);
+        const float *e = reinterpret_cast<const float *>(&v[k]);
+#pragma unroll
+        for (int c = 0; c < V; ++c) x[c] = fmaf(e[c], a, x[c]);
+      }
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   const int i = static_cast<int>(row % p.n_q);
@@ -817,8 +842,16 @@ cudaError_t launch_typed(const CUtensorMap &tq, const CUtensorMap &tk, const CUt
   else
     e = launch_tiles<attention_kernel<BF16, PACKED>>(tq, tk, tv, f, grid, THREADS, smem_bytes(PACKED), stream);
   if (e != cudaSuccess || f.splits == 1) return e;
-  attention_join_kernel<BF16, DH><<<static_cast<unsigned>((f.rows + 3) / 4), 128, 0, stream>>>(f);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((f.rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<BF16, DH>, f);
 }
 template <bool BF16, int DH>
 cudaError_t launch_rows(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const FwdParams &f,

@@ -352,12 +352,12 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g, 0), jl & 1));
           if (ok) {
             tcgen05_fence_after();
-            mma_rows<TILE, 32, 0, 4>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0, leader);
+            mma_rows<TILE, TILE, 0, 4>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, jl > 0, leader);
           }
           if (ok) ok = __all_sync(0xffffffffu, mbar_wait(probs(g, 1), jl & 1));
           if (ok) {
             tcgen05_fence_after();
-            mma_rows<TILE, 32, 4, 8>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, true, leader);
+            mma_rows<TILE, TILE, 4, 8>(tmem + O_COL + g * TILE, tmem + g * TILE, kv_smem(q), p.idesc_o, true, leader);
             if (jl + 1 == w.n[g]) commit(scores(g), leader);
           }
         };
@@ -649,8 +649,8 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
           if (!ok) break;
           tcgen05_fence_after();
           const uint32_t o = tmem + solo::O_COL, q = tmem + solo::P_COL;
-          if (half == 0) mma_rows<TILE, 32, 0, 4>(o, q, kv_smem(pos), p.idesc_o, j > 0, leader);
-          else mma_rows<TILE, 32, 4, 8>(o, q, kv_smem(pos), p.idesc_o, true, leader);
+          if (half == 0) mma_rows<TILE, TILE, 0, 4>(o, q, kv_smem(pos), p.idesc_o, j > 0, leader);
+          else mma_rows<TILE, TILE, 4, 8>(o, q, kv_smem(pos), p.idesc_o, true, leader);
         }
         if (ok) {
           commit(rows_done, leader);

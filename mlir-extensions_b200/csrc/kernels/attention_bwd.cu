@@ -17,9 +17,10 @@
 // The walked blocks are as long as the head is wide: 128 rows for d_head 128; 64 rows for d_head 64, where a CTA
 // then needs half of the TMEM and of the shared memory, so that two run on an SM and fill each other's waits.
 //
-// Roles as in the forward kernel: warp 0 loads tiles (TMA), warp 1 issues products, warps 4 and up compute, 64
-// columns of a row per thread (with 128-row blocks two warpgroups share the rows).  P and dS take the places of S and dP in TMEM as 16-bit
-// pairs (each half in front of its own 64 columns, so that no thread overwrites what another still reads);
+// Roles as in the forward kernel: warp 0 loads tiles (TMA), warp 1 issues products, warps 4 and up compute, 32
+// columns of a row per thread: four warps per scheduler fill each other's waits better than two with 64 columns each
+// (4096 causal, d_head 128: 393 us instead of 425).  P and dS take the places of S and dP in TMEM as 16-bit
+// pairs (each thread's in front of its own columns, so that no thread overwrites what another still reads);
 // products run in the order they are issued, so overwriting a score tile is ordered by issuing the
 // next product behind the one that reads it.  While the warps compute P the tensor core runs the
 // previous block's last product and this block's dP; while they compute dS it runs the next block's S.
@@ -46,8 +47,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 template <int DH> struct Sizes {
   static constexpr int BN = DH;
   static constexpr int CTAS = DH == 128 ? 1 : 2;           // per SM
-  static constexpr int THREADS = 128 + 2 * BN;             // a thread per row and 64 columns
-  static constexpr int WARPS = 2 * BN / 32;                // that compute
+  static constexpr int CPT = 32;                           // columns of a row per computing thread
+  static constexpr int PARTS = BN / CPT;                   // threads that share a row
+  static constexpr int THREADS = 128 + TILE * PARTS;
+  static constexpr int WARPS = 4 * PARTS;                  // that compute
   static constexpr int TMEM_COLS = 4 * BN;
   static constexpr int RB = TILE * DH * 2, TB = BN * DH * 2;  // bytes of a resident tile and of a walked one
   static constexpr int SA = DH == 128 ? 3 : 4, SB = DH == 128 ? 2 : 3;  // stages: Q (dkv) or K (dq); dO or V
@@ -131,15 +134,20 @@ __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
-// The computing warpgroups take registers over from the first one: 168 a thread at launch with three
-// warpgroups (72 + 2 * 216), 128 with two and two CTAs per SM (56 + 200).
+// The computing warpgroups take registers over from the first one; both shares add up to what the threads have at
+// launch (65536 over threads and CTAs, in eights).
+template <int DH> struct Registers {
+  using Z = Sizes<DH>;
+  static constexpr int LAUNCH = 65536 / (Z::THREADS * Z::CTAS) / 8 * 8;
+  static constexpr int GIVE = 32;
+  static constexpr int TAKE = (LAUNCH + (LAUNCH - GIVE) / Z::PARTS) / 8 * 8;
+  static_assert(GIVE + Z::PARTS * TAKE <= (1 + Z::PARTS) * LAUNCH, "no more than there are");
+};
 template <int DH> __device__ __forceinline__ void give_registers() {
-  if (DH == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers<DH>::GIVE));
 }
 template <int DH> __device__ __forceinline__ void take_registers() {
-  if (DH == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Registers<DH>::TAKE));
 }
 
 // Blocks [share_of(n, r, s), share_of(n, r + 1, s)) are those of share r of s
@@ -224,14 +232,20 @@ __device__ __forceinline__ void row_deltas(const uint16_t *o, int64_t o_step, co
   }
 }
 
-// 64 columns of this thread's row
-__device__ __forceinline__ void load_64(uint32_t taddr, uint32_t (&v)[64]) {
-  uint32_t lo[32], hi[32];
-  tmem_ld_32x32(taddr, lo);
-  tmem_ld_32x32(taddr + 32, hi);
+// N columns of this thread's row
+template <int N> __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[N]) {
+  uint32_t x[N / 32][32];
+#pragma unroll
+  for (int c = 0; c < N / 32; ++c) tmem_ld_32x32(taddr + 32 * c, x[c]);
   tmem_ld_wait();
 #pragma unroll
-  for (int e = 0; e < 32; ++e) v[e] = lo[e], v[32 + e] = hi[e];
+  for (int e = 0; e < N; ++e) v[e] = x[e / 32][e % 32];
+}
+// N / 2 words of pairs in their place
+template <int N> __device__ __forceinline__ void store_pairs(uint32_t taddr, const uint32_t (&w)[N / 2]) {
+#pragma unroll
+  for (int c = 0; c < N / 32; ++c) tmem_st_16(taddr + 16 * c, w + 16 * c);
+  tmem_st_wait();
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
@@ -248,7 +262,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   using T = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
   const T L(smem_u32(smem_raw));
-  constexpr int BN = T::BN;
+  constexpr int BN = T::BN, CPT = T::CPT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
   const int hb = tile % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
@@ -333,7 +347,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         ok = ok && wait_all(L.bar(T::DS_READY + (j & 1)), (j >> 1) & 1);
         if (ok) {
           tcgen05_fence_after();
-          mma_rows<BN, 64>(dq_tmem, dp_tmem(j), L.a_tile(j), p.idesc_o, j > 0, leader);
+          mma_rows<BN, CPT>(dq_tmem, dp_tmem(j), L.a_tile(j), p.idesc_o, j > 0, leader);
           commit(L.a_empty(j), leader);
         }
       }
@@ -347,7 +361,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     }
   } else {
     take_registers<DH>();
-    const int half = BN == 128 ? (warp - 4) >> 2 : 0, lane_group = warp & 3;
+    const int part = (warp - 4) >> 2, lane_group = warp & 3;
     const int r = lane_group * 32 + lane, i = row0 + r;
     const bool exists = i < p.n_q;
     const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
@@ -357,7 +371,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head) * p.n_q + i;
       const float lse = p.lse[row];
       if (lse != -INFINITY) lse2 = lse * LOG2E;  // a row that sees no key: every probability is 2^-inf
-      if (half == 0 && rank == 0) p.delta[row] = -neg_d;
+      if (part == 0 && rank == 0) p.delta[row] = -neg_d;
     }
     const int limit = exists ? visible_keys(i, keys, p.n_q, p.n_kv, p.causal) : INT32_MAX;
     const uint64_t scale2 = pack_f32x2(p.scale_log2e, p.scale_log2e), neg_lse2 = pack_f32x2(-lse2, -lse2);
@@ -367,22 +381,22 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       ok = wait_all(L.bar(T::S_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
-      const int seen = limit - (first + j) * BN - half * 64;  // of this thread's 64 keys
-      const bool masked = __any_sync(0xffffffffu, seen < 64);
-      uint64_t pr[32];
+      const int seen = limit - (first + j) * BN - part * CPT;  // of this thread's keys
+      const bool masked = __any_sync(0xffffffffu, seen < CPT);
+      uint64_t pr[CPT / 2];
       {
-        uint32_t s[64];
-        load_64(tmem + lanes + half * 64, s);
+        uint32_t s[CPT];
+        load_columns<CPT>(tmem + lanes + part * CPT, s);
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(L.bar(T::S_READ));
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < CPT; ++e)
             if (e >= seen) s[e] = __float_as_uint(-INFINITY);
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < CPT / 2; ++e) {
           float x0, x1;
           unpack_f32x2(fma_f32x2(pack_u32x2(s[2 * e], s[2 * e + 1]), scale2, neg_lse2), x0, x1);
           pr[e] = pack_f32x2(ex2(x0), ex2(x1));
@@ -392,24 +406,22 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (!ok) break;
       tcgen05_fence_after();
       {
-        uint32_t d[64], w[32];
-        load_64(dp_tmem(j) + lanes + half * 64, d);
+        uint32_t d[CPT], w[CPT / 2];
+        load_columns<CPT>(dp_tmem(j) + lanes + part * CPT, d);
         if (masked) {  // (P is 0 there, but 0 times the product with a padded row may be NaN)
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < CPT; ++e)
             if (e >= seen) d[e] = 0u;
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < CPT / 2; ++e) {
           float x0, x1;
           unpack_f32x2(mul_f32x2(pr[e], add_f32x2(pack_u32x2(d[2 * e], d[2 * e + 1]), neg_delta)), x0, x1);
           w[e] = pack2<BF16>(x0, x1);
         }
         // dS takes the place of this thread's own part of dP
-        tmem_st_16(dp_tmem(j) + lanes + half * 64, w);
-        tmem_st_16(dp_tmem(j) + lanes + half * 64 + 16, w + 16);
+        store_pairs<CPT>(dp_tmem(j) + lanes + part * CPT, w);
       }
-      tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(L.bar(T::DS_READY + (j & 1)));
@@ -420,7 +432,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     } else {
       tcgen05_fence_after();
       constexpr int COLS = DH * 4 / T::WARPS;  // a warpgroup's share of the columns
-      leave_row<DH, COLS>(dq_tmem + lanes + half * COLS, n > 0, L.base, r, half * COLS);
+      leave_row<DH, COLS>(dq_tmem + lanes + part * COLS, n > 0, L.base, r, part * COLS);
     }
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(p.shares);
@@ -448,7 +460,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   using T = Layout<DH>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
   const T L(smem_u32(smem_raw));
-  constexpr int BN = T::BN;
+  constexpr int BN = T::BN, CPT = T::CPT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
   const int hb = tile % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
@@ -515,14 +527,14 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         ok = wait_all(L.bar(T::P_READY), j & 1);
         if (ok) {
           tcgen05_fence_after();
-          mma_rows<BN, 64>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0, leader);
+          mma_rows<BN, CPT>(dv_tmem, tmem, L.b_tile(j), p.idesc_o, j > 0, leader);
           commit(L.b_empty(j), leader);
         }
         if (j + 1 < n) scores(j + 1);
         ok = ok && wait_all(L.bar(T::DS_READY), j & 1);
         if (ok) {
           tcgen05_fence_after();
-          mma_rows<BN, 64>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
+          mma_rows<BN, CPT>(dk_tmem, dp_tmem, L.a_tile(j), p.idesc_o, j > 0, leader);
           commit(L.a_empty(j), leader);
         }
         if (j + 1 < n) products(j + 1);
@@ -565,7 +577,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
   } else {
     take_registers<DH>();
-    const int half = BN == 128 ? (warp - 4) >> 2 : 0, lane_group = warp & 3;
+    const int part = (warp - 4) >> 2, lane_group = warp & 3;
     const int r = lane_group * 32 + lane, key = key0 + r;
     const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
     // first query that sees this thread's key
@@ -576,21 +588,21 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       ok = wait_all(L.bar(T::STAT_FULL + j % T::STAT_STAGES), (j / T::STAT_STAGES) & 1) && wait_all(L.bar(T::S_FULL), j & 1);
       if (!ok) break;
       tcgen05_fence_after();
-      const int i0 = row_of(j) + half * 64;
+      const int i0 = row_of(j) + part * CPT;
       const bool masked = __any_sync(0xffffffffu, from > i0);
-      const int hidden = from - i0;  // of this thread's 64 queries, the first ones (0 or less: none)
-      uint64_t pr[32];
+      const int hidden = from - i0;  // of this thread's queries, the first ones (0 or less: none)
+      uint64_t pr[CPT / 2];
       {
-        uint32_t s[64], w[32];
-        load_64(tmem + lanes + half * 64, s);
+        uint32_t s[CPT], w[CPT / 2];
+        load_columns<CPT>(tmem + lanes + part * CPT, s);
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < CPT; ++e)
             if (e < hidden) s[e] = __float_as_uint(-INFINITY);
         }
-        const ulonglong2 *st = reinterpret_cast<const ulonglong2 *>(stat_of(j, 0) + half * 64);
+        const ulonglong2 *st = reinterpret_cast<const ulonglong2 *>(stat_of(j, 0) + part * CPT);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < CPT / 2; ++e) {
           float x0, x1;
           unpack_f32x2(fma_f32x2(pack_u32x2(s[2 * e], s[2 * e + 1]), scale2, e & 1 ? st[e / 2].y : st[e / 2].x), x0, x1);
           x0 = ex2(x0);
@@ -598,10 +610,8 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           pr[e] = pack_f32x2(x0, x1);
           w[e] = pack2<BF16>(x0, x1);
         }
-        tmem_st_16(tmem + lanes + half * 64, w);
-        tmem_st_16(tmem + lanes + half * 64 + 16, w + 16);
+        store_pairs<CPT>(tmem + lanes + part * CPT, w);
       }
-      tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(L.bar(T::P_READY));
@@ -609,24 +619,22 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (!ok) break;
       tcgen05_fence_after();
       {
-        uint32_t d[64], w[32];
-        load_64(dp_tmem + lanes + half * 64, d);
+        uint32_t d[CPT], w[CPT / 2];
+        load_columns<CPT>(dp_tmem + lanes + part * CPT, d);
         if (masked) {  // (P is 0 there, but 0 times the product with a padded row may be NaN)
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
+          for (int e = 0; e < CPT; ++e)
             if (e < hidden) d[e] = 0u;
         }
-        const ulonglong2 *st = reinterpret_cast<const ulonglong2 *>(stat_of(j, 1) + half * 64);
+        const ulonglong2 *st = reinterpret_cast<const ulonglong2 *>(stat_of(j, 1) + part * CPT);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < CPT / 2; ++e) {
           float x0, x1;
           unpack_f32x2(mul_f32x2(pr[e], add_f32x2(pack_u32x2(d[2 * e], d[2 * e + 1]), e & 1 ? st[e / 2].y : st[e / 2].x)), x0, x1);
           w[e] = pack2<BF16>(x0, x1);
         }
-        tmem_st_16(dp_tmem + lanes + half * 64, w);
-        tmem_st_16(dp_tmem + lanes + half * 64 + 16, w + 16);
+        store_pairs<CPT>(dp_tmem + lanes + part * CPT, w);
       }
-      tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(L.bar(T::DS_READY));
@@ -637,9 +645,13 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (lane == 0) report(p.status, kStatusEpiWaitTimeout);
     } else {
       tcgen05_fence_after();
-      // with two warpgroups one takes dV, the other dK
-      if (half == 0) leave_row<DH, DH>(dv_tmem + lanes, n > 0, L.base, r, 0);
-      if (half == 1 || BN == 64) leave_row<DH, DH>(dk_tmem + lanes, n > 0, L.base + TILE * DH * 4, r, 0);
+      // the columns of dV and dK, side by side in TMEM, shared out between the warpgroups
+      constexpr int COLS = 2 * DH / T::PARTS;
+#pragma unroll
+      for (int c = 0; c < COLS; c += DH < COLS ? DH : COLS) {
+        const int col = part * COLS + c;
+        leave_row<DH, (DH < COLS ? DH : COLS)>(dv_tmem + lanes + col, n > 0, L.base + col / DH * (TILE * DH * 4), r, col % DH);
+      }
     }
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(p.shares);

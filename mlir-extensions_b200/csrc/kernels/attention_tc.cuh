@@ -103,15 +103,15 @@ __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint32_t a_smem, uin
     mma_ss(d_tmem, a + ao, b + bo, idesc, k ? 1u : 0u, leader);
   }
 }
-// D[128 x DH] (+)= P . B over BN, P 16-bit pairs in TMEM (the second 64 values of a row HALF columns behind
-// the first), B a tile in shared memory as it lies (MN-major); the 16-row steps [K0, K1) of it
-template <int BN, int HALF, int K0 = 0, int K1 = BN / 16>
+// D[128 x DH] (+)= P . B over BN; P 16-bit pairs in TMEM, PART values of a row in front of each run of PART columns
+// (where as many f32 values were); B a tile in shared memory as it lies (MN-major); the 16-row steps [K0, K1) of it
+template <int BN, int PART, int K0 = 0, int K1 = BN / 16>
 __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t p_tmem, uint32_t b_smem, uint32_t idesc,
                                          bool accumulate, uint32_t leader) {
   const uint64_t b = make_smem_desc(b_smem, BN * 128, 1024);
 #pragma unroll
   for (int k = K0; k < K1; ++k)
-    mma_ts(d_tmem, p_tmem + (k >> 2) * HALF + (k & 3) * 8, b + static_cast<uint64_t>(k * 2048 >> 4), idesc,
+    mma_ts(d_tmem, p_tmem + k / (PART / 16) * PART + k % (PART / 16) * 8, b + static_cast<uint64_t>(k * 2048 >> 4), idesc,
            (accumulate || k) ? 1u : 0u, leader);
 }
 // c = f32; a, b formats; bit 16: B is MN-major; N >> 3; M >> 4

@@ -118,7 +118,7 @@ void *imexStreamStatusWord(void *stream);
 void imexNoteLaunches(uint64_t n);
 
 /* Bytes of device scratch the launches of this kernel handle want as their last pointer operand
- * (0: no such operand).  The scratch is the caller's, like every other operand: launches that may
+ * (0: no such operand; else it starts on a 16-byte boundary).  The scratch is the caller's, like every other operand: launches that may
  * overlap on the GPU (other streams, graphs that replay side by side) need one each.  Its contents
  * carry nothing from one launch to the next. */
 size_t imexKernelWorkspaceBytes(void *kernel);

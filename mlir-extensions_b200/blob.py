@@ -166,8 +166,8 @@ def _attention(op, name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype, sm_
     if layout not in ("heads", "tokens"):
         raise ValueError('attention: layout is "heads" ([batch, heads, rows, d]) or "tokens" ([batch, rows, heads, d])')
     sm_scale = d_head ** -0.5 if sm_scale is None else float(sm_scale)
-    if not (math.isfinite(sm_scale) and sm_scale > 0):
-        raise ValueError("attention: sm_scale must be positive and finite")
+    if not 0 < sm_scale <= 1e30:
+        raise ValueError("attention: sm_scale must be positive and at most 1e30")
     strides = dict(strides or {})
     table = []
     for a in _ATTENTION_ARRAYS:
@@ -176,6 +176,8 @@ def _attention(op, name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype, sm_
             s = tuple(int(v) for v in strides.pop(a))
             if len(s) != 3 or any(v % 8 for v in s) or min(s) < 0:
                 raise ValueError("attention: the strides of %r are (batch, head, row) in elements, multiples of 8" % a)
+            if any(step == 0 and n > 1 for step, n in zip(s, (batch, heads, rows))):
+                raise ValueError("attention: a stride of %r is zero" % a)
             if a in ("o", "dq", "dk", "dv") and _rows_overlap(d_head, zip(s, (batch, heads, rows))):
                 raise ValueError("attention: the rows of the output %r overlap" % a)
         elif layout == "heads":
@@ -212,8 +214,9 @@ def attention_bwd(name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype=BF16,
                   key_lens=False, layout="heads", strides=None):
     """The gradients of `attention` for dO, with the probabilities recomputed from LSE.  Pointers Q, K, V,
     O, dO, LSE, dQ, dK, dV, then key_lens and the workspace as in `attention`.  Gradients of shared key
-    heads are summed over their query heads; masked keys and rows that see no key get zeros.  The result
-    does not change from run to run (no atomics).  strides also takes "do", "dq", "dk", "dv"."""
+    heads are summed over their query heads; masked keys and rows that see no key get zeros.  P and
+    dS = P (dO V^T - rowsum(dO O)) are rounded to the element type in between, so with F16 |dS| has to stay
+    below 65504.  The result does not change from run to run (no atomics).  strides also takes "do", "dq", "dk", "dv"."""
     return _attention(OP_ATTENTION_BWD, name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype, sm_scale, causal,
                       key_lens, layout, strides)
 

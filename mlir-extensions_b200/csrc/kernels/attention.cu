@@ -44,6 +44,7 @@ using namespace attn;
 using namespace tc;
 
 constexpr int THREADS = 384;
+constexpr int REGISTERS = 168;  // a thread at launch, handed over as 72 + 2 * 216
 constexpr unsigned kPollSleepNs = 40;
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512)
 constexpr int TMEM_COLS = 512;
@@ -530,7 +531,7 @@ constexpr int THREADS = 256;
 constexpr int TMEM_COLS = 256;  // S [0,128) P [128,192) O [192,256)
 constexpr int P_COL = 128, O_COL = 192;
 constexpr int SMEM = (1 + STAGES) * TB + 256;
-// registers: 128 a thread at launch with two CTAs per SM, handed over as 56 + 200
+constexpr int REGISTERS = 128;  // a thread at launch with two CTAs per SM, handed over as 56 + 200
 static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
 } // namespace solo
 
@@ -827,8 +828,8 @@ bool aligned(const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 
 template <auto kernel>
 cudaError_t launch_tiles(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const FwdParams &f,
-                         unsigned grid, int threads, int smem, cudaStream_t stream) {
-  const cudaError_t e = allow_smem<kernel>(smem);
+                         unsigned grid, int threads, int smem, int registers, cudaStream_t stream) {
+  const cudaError_t e = allow_smem<kernel>(smem, registers);
   if (e != cudaSuccess) return e;
   kernel<<<grid, threads, smem, stream>>>(tq, tk, tv, f);
   return cudaGetLastError();
@@ -838,9 +839,9 @@ cudaError_t launch_typed(const CUtensorMap &tq, const CUtensorMap &tk, const CUt
                          unsigned grid, cudaStream_t stream) {
   cudaError_t e;
   if constexpr (DH == 64)
-    e = launch_tiles<attention_solo_kernel<BF16, PACKED>>(tq, tk, tv, f, grid, solo::THREADS, solo::SMEM, stream);
+    e = launch_tiles<attention_solo_kernel<BF16, PACKED>>(tq, tk, tv, f, grid, solo::THREADS, solo::SMEM, solo::REGISTERS, stream);
   else
-    e = launch_tiles<attention_kernel<BF16, PACKED>>(tq, tk, tv, f, grid, THREADS, smem_bytes(PACKED), stream);
+    e = launch_tiles<attention_kernel<BF16, PACKED>>(tq, tk, tv, f, grid, THREADS, smem_bytes(PACKED), REGISTERS, stream);
   if (e != cudaSuccess || f.splits == 1) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((f.rows + 3) / 4));
@@ -868,7 +869,7 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
     return "batch, heads and lengths are at least 1";
   if (p.q_heads % p.kv_heads) return "q_heads must be a multiple of kv_heads";
   if (p.d_head != 64 && p.d_head != 128) return "d_head is 64 or 128";
-  if (!(p.scale > 0.0f) || p.scale > 3.0e38f) return "sm_scale must be positive and finite";
+  if (!(p.scale > 0.0f) || p.scale > 1.0e30f) return "sm_scale must be positive and at most 1e30";
   if (p.batch > 65535 || p.q_heads > 65535 || p.n_q > (1 << 30) || p.n_kv > (1 << 30) ||
       p.batch * p.q_heads * ((p.n_q + TILE - 1) / TILE) > INT32_MAX / 64 ||
       p.batch * p.kv_heads * ((p.n_kv + TILE - 1) / TILE) > INT32_MAX / 64)
@@ -887,6 +888,7 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
   if (!aligned(p.q) || !aligned(p.k) || !aligned(p.v) || !aligned(p.o) ||
       (backward && (!aligned(p.dout) || !aligned(p.dq) || !aligned(p.dk) || !aligned(p.dv))))
     return "arrays must be 16-byte aligned";
+  if (attention_workspace_bytes(p, backward) && !aligned(p.workspace)) return "the workspace must be 16-byte aligned";
   return nullptr;
 }
 

@@ -676,7 +676,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 template <auto kernel, int DH, typename... Maps>
 cudaError_t launch_shared(const BwdParams &f, int64_t tiles, bool early, cudaStream_t stream, const Maps &...maps) {
   using Z = Sizes<DH>;
-  const cudaError_t e = allow_smem<kernel>(Z::SMEM);
+  const cudaError_t e = allow_smem<kernel>(Z::SMEM, Registers<DH>::LAUNCH);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * f.shares));

@@ -203,8 +203,9 @@ inline bool make_map_4d(CUtensorMap *m, const void *base, int dtype, int64_t d, 
 }
 
 // Dynamic shared memory beyond 48 KB has to be asked for on every device a kernel runs on.
-// `kernel` is a template argument so that each has its own record of where that was done.
-template <auto kernel> cudaError_t allow_smem(int bytes) {
+// `kernel` is a template argument so that each has its own record of where that was done.  registers: what its
+// warpgroups hand over by setmaxnreg adds up to this many a thread, so it must have been built with them.
+template <auto kernel> cudaError_t allow_smem(int bytes, int registers = 0) {
   static std::atomic<uint64_t> done{0};  // a bit per device
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -212,6 +213,11 @@ template <auto kernel> cudaError_t allow_smem(int bytes) {
   const uint64_t bit = device < 64 ? 1ull << device : 0;
   if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
   e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && registers) {
+    cudaFuncAttributes built;
+    e = cudaFuncGetAttributes(&built, reinterpret_cast<const void *>(kernel));
+    if (e == cudaSuccess && built.numRegs != registers) e = cudaErrorInvalidKernelImage;
+  }
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
   return e;
 }

@@ -268,6 +268,7 @@ cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream
   uint16_t *dgu = static_cast<uint16_t *>(p.workspace);
   GradArgs a{static_cast<const uint16_t *>(p.gu), static_cast<const uint16_t *>(p.h), dgu, ldh, p.tokens, p.d_ff, p.act};
   auto on16 = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  if (!on16(p.workspace)) return cudaErrorMisalignedAddress;
   const bool wide = p.d_ff % 8 == 0 && ldh % 8 == 0 && on16(p.gu) && on16(p.h) && on16(dgu);
   const int64_t items = p.tokens * (wide ? p.d_ff / 8 : p.d_ff);
   const int64_t most = 148 * 8 * 4;  // resident blocks, four rounds each at the most

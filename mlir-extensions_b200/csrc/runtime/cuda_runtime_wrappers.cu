@@ -577,6 +577,7 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
     imex::GatedProblem p = gated_problem(d);
     p.x = ptrs[0], p.w = ptrs[1], p.gu = ptrs[2], p.h = ptrs[3], p.dx = ptrs[4], p.dw = ptrs[5];
     p.workspace = ptrs[6];
+    if (reinterpret_cast<uintptr_t>(p.workspace) & 15) refuse(d, "the workspace must be 16-byte aligned");
     s->last_kernel = "gated_ffn_bwd";
     err = imex::launch_gated_bwd(p, s->status_dev, s->stream, &launches);
     break;

@@ -12,12 +12,14 @@ probabilities (and dS) once to the 16-bit type before the second product and eve
 plus what 32-bit arithmetic leaves: F = 2e-5 relative on P (a score is a sum of d_head products, |S| up to ten or so:
 d_head 2^-24 sum |q||k| scale, the exponential 2^-22) and on sums of up to a few thousand terms."""
 import math
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 import torch
 
-from __graft_entry__ import load_package
+from __graft_entry__ import ROOT, load_package
 
 pytestmark = pytest.mark.gpu
 
@@ -342,6 +344,17 @@ def test_attention_gradients_with_warps_out_of_step(pkg, d, kind):
             assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(first, got))
 
 
+@pytest.mark.parametrize("op,arg,message", [("attention", 0, "16-byte aligned"), ("attention", 3, "16-byte aligned"),
+                                            ("attention_bwd", 7, "16-byte aligned"), ("attention_bwd", -1, "the workspace must be")])
+def test_misaligned_arrays_are_refused(op, arg, message):
+    """Before anything is launched, by the error convention: one line on stdout, then abort()."""
+    text = ("from __graft_entry__ import load_package\npkg = load_package()\nB = pkg.blob\ns = pkg.Session(device=0)\n"
+            "k = s.kernel(B.%s('a', 1, 1, 1, 8, 8, 64))\nn = %d\np = [s.alloc(4096) for _ in range(n)]\n"
+            "p[%d] += 8\ns.launch(k, p)\n" % (op, 5 if op == "attention" else 10, arg))
+    r = subprocess.run([sys.executable, "-c", text], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == -6 and message in r.stdout, r.stdout + r.stderr
+
+
 # --------------------------------------------------------------------------------------- gated product
 def _act(g, act):
     return {0: g, 1: g.clamp(min=0), 2: torch.nn.functional.silu(g)}[act]
@@ -564,6 +577,15 @@ def test_captured_block_replays_on_new_inputs(pkg):
                  (B.attention_bwd("b", *dims, causal=True, key_lens=True), [q, k, v, o, do, lse, dq, dk, dv, lens]),
                  (B.gated_ffn("g", 70, 64, 136, save_gu=True), [x, w, h, gu]),
                  (B.gated_ffn_bwd("gb", 70, 64, 136), [x, w, gu, dh, dx, dw])]
+        # one query on a long cache (shares of the keys, joined), its gradients (shares in a cluster), few rows
+        dims1 = (1, 4, 1, 1, 5000, 128)
+        q1, do1, k1, v1 = new(1, 4, 1, 128), new(1, 4, 1, 128), new(1, 1, 5000, 128), new(1, 1, 5000, 128)
+        o1, lse1, dq1, dk1, dv1 = torch.empty_like(q1), torch.empty((1, 4, 1), device="cuda"), torch.empty_like(q1), torch.empty_like(k1), torch.empty_like(k1)
+        x1, w1, h1 = new(3, 1024), new(1024, 256), new(3, 128)
+        calls += [(B.attention("a1", *dims1), [q1, k1, v1, o1, lse1]),
+                  (B.attention_bwd("b1", *dims1), [q1, k1, v1, o1, do1, lse1, dq1, dk1, dv1]),
+                  (B.gated_ffn("g1", 3, 1024, 128), [x1, w1, h1])]
+        outs = [o, lse, dq, dk, dv, h, gu, dx, dw, o1, lse1, dq1, dk1, dv1, h1]
         launches, keep = [], []
         for desc, args in calls:
             kernel = sess.kernel(desc)
@@ -572,7 +594,6 @@ def test_captured_block_replays_on_new_inputs(pkg):
                 args = args + [torch.empty(need, dtype=torch.uint8, device="cuda")]
             keep.append(args)
             launches.append(sess.bind(kernel, [t.data_ptr() for t in args]))
-        outs = [o, lse, dq, dk, dv, h, gu, dx, dw]
         for run in launches:
             run()
         stream.synchronize()
@@ -580,7 +601,7 @@ def test_captured_block_replays_on_new_inputs(pkg):
         with torch.cuda.graph(graph, stream=stream):
             for run in launches:
                 run()
-        for t in (q, k, v, do, x, w, dh):
+        for t in (q, k, v, do, x, w, dh, q1, do1, k1, v1, x1, w1):
             t.copy_(new(*t.shape))
         lens.copy_(torch.tensor([0, 149], dtype=torch.int32))
         for run in launches:

@@ -34,7 +34,7 @@ def test_attention_descriptor():
     ({"d_head": 96}, "64 or 128"), ({"dtype": 1}, "F16 or BF16"), ({"layout": "rows"}, "layout"),
     ({"sm_scale": 0.0}, "positive"), ({"sm_scale": -1.0}, "positive"), ({"sm_scale": float("nan")}, "positive"),
     ({"strides": {"q": (1, 2)}}, "multiples of 8"), ({"strides": {"q": (64, 64, 68)}}, "multiples of 8"),
-    ({"strides": {"x": (64, 64, 64)}}, "unknown"), ({"strides": {"o": (640, 64, 8)}}, "overlap")])
+    ({"strides": {"x": (64, 64, 64)}}, "unknown"), ({"strides": {"k": (0, 64, 128)}}, "zero"), ({"sm_scale": 1e31}, "positive"), ({"strides": {"o": (640, 64, 8)}}, "overlap")])
 def test_attention_refusals(change, message):
     args = dict(batch=2, q_heads=4, kv_heads=2, n_q=10, n_kv=10, d_head=64)
     args.update(change)

@@ -95,7 +95,7 @@ extern "C" {
  *                   P = exp(S - LSE), dV = sum_group P^T dO, dS = P (dO V^T - rowsum(dO O)),
  *                   dQ = sm_scale dS K, dK = sm_scale sum_group dS^T Q.
  *   GATED_FFN       X[tokens,d_in], W[d_in,2*d_ff], H[tokens,d_ff] (, GU[tokens,2*d_ff] with
- *                   IMEX_FLAG_SAVE_GU): H = act(X Wg) * (X Wu) with W = [Wg | Wu], act =
+ *                   IMEX_FLAG_SAVE_GU) (, workspace): H = act(X Wg) * (X Wu) with W = [Wg | Wu], act =
  *                   `epilogue`, f32 accumulation; GU = X W as the backward pass wants it.
  *                   dims = {tokens, d_in, d_ff, ldx, ldw, ldh}; row pitches, 0 = dense; GU is dense.
  *   GATED_FFN_BWD   X, W, GU, dH[tokens,d_ff], dX[tokens,d_in], dW[d_in,2*d_ff], workspace:

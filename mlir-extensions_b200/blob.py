@@ -237,8 +237,9 @@ def _gated(op, name, tokens, d_in, d_ff, dtype, act, flags, ldx, ldw, ldh):
 def gated_ffn(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, save_gu=False, ldx=0, ldw=0, ldh=0):
     """H = act(X Wg) * (X Wu).  Pointers X [tokens, d_in], W [d_in, 2 * d_ff] (the gate's columns, then
     the up projection's), H [tokens, d_ff], and with save_gu GU [tokens, 2 * d_ff] = X W for the backward
-    pass.  f32 accumulation; H and GU are rounded once.  ldx / ldw / ldh: row pitches in elements (0 =
-    dense; GU is dense)."""
+    pass, then the workspace when Session.workspace_bytes says so (extents or pitches that are not multiples
+    of 8).  f32 accumulation; H and GU are rounded once.  ldx / ldw / ldh: row pitches in elements (0 = dense;
+    GU is dense).  Arrays start on 16-byte boundaries unless the extents need the workspace."""
     return _gated(OP_GATED_FFN, name, tokens, d_in, d_ff, dtype, act, FLAG_SAVE_GU if save_gu else 0, ldx, ldw, ldh)
 
 

@@ -436,8 +436,10 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     }
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(p.shares);
-    add_up<BF16, DH, CT>(L.base, rank, p.shares, p.scale, p.dq + b * p.sdq.batch + head * p.sdq.head + row0 * p.sdq.row,
-                         p.sdq.row, p.n_q - row0, threadIdx.x - 128);
+    uint16_t *dq = p.dq + b * p.sdq.batch + head * p.sdq.head + row0 * p.sdq.row;
+    add_up<DH, CT>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+      if (row0 + row < p.n_q) store_unit<BF16>(dq + row * p.sdq.row + unit * 8, x, y, p.scale);
+    });
     sums_barrier<CT>(p.shares);
   }
 
@@ -655,11 +657,14 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(p.shares);
-    add_up<BF16, DH, CT>(L.base, rank, p.shares, 1.0f, p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row,
-                         p.sdv.row, p.n_kv - key0, threadIdx.x - 128);
-    add_up<BF16, DH, CT>(L.base + TILE * DH * 4, rank, p.shares, p.scale,
-                         p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key0 * p.sdk.row, p.sdk.row, p.n_kv - key0,
-                         threadIdx.x - 128);
+    uint16_t *dv = p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row;
+    uint16_t *dk = p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key0 * p.sdk.row;
+    add_up<DH, CT>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+      if (key0 + row < p.n_kv) store_unit<BF16>(dv + row * p.sdv.row + unit * 8, x, y, 1.0f);
+    });
+    add_up<DH, CT>(L.base + TILE * DH * 4, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+      if (key0 + row < p.n_kv) store_unit<BF16>(dk + row * p.sdk.row + unit * 8, x, y, p.scale);
+    });
     sums_barrier<CT>(p.shares);
   }
 

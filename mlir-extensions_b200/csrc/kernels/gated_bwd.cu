@@ -3,11 +3,9 @@
 // With [G U] = X W kept by the forward pass, one pass over G, U and dH writes [dG dU] = [dH U act'(G), dH act(G)]
 // into the workspace, rounded once to the 16-bit type; because W holds both projections side by side,
 // dX = [dG dU] W^T and dW = X^T [dG dU] are then one product each.  Large ones go to the framework's CTA-pair GEMM;
-// small ones to gated_product_kernel: 128 x 128 tiles, two CTAs per SM, k shared out between the CTAs of a cluster
-// where there are few tiles.
-#include "attention_common.cuh"
-#include "epilogue.cuh"
-#include "tile_sums.cuh"
+// small ones, and extents that are not multiples of eight, to gated_product_kernel: 128 x 128 tiles, two CTAs per SM, k
+// shared out between the CTAs of a cluster where there are few tiles.
+#include "gated_common.cuh"
 
 namespace imex {
 namespace {
@@ -20,6 +18,7 @@ struct GradArgs {
   const uint16_t *gu, *dh;
   uint16_t *dgu;
   int64_t ldh, tokens, d_ff;
+  int64_t up;  // first column of dU in dGU, half its row
   int act;
 };
 
@@ -43,26 +42,28 @@ template <bool BF16, int V> __global__ void __launch_bounds__(256) gated_grad_ke
   struct alignas(2 * V) Pack {
     uint16_t v[V];
   };
-  const int64_t per_row = a.d_ff / V, n = a.tokens * per_row;
+  const int64_t per_row = a.up / V, n = a.tokens * per_row;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
        e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t r = e / per_row, c = (e - r * per_row) * V, at = r * 2 * a.d_ff + c;
-    Pack g = *reinterpret_cast<const Pack *>(a.gu + at), u = *reinterpret_cast<const Pack *>(a.gu + at + a.d_ff);
-    const Pack d = *reinterpret_cast<const Pack *>(a.dh + r * a.ldh + c);
+    Pack g{}, u{};
+    if (c < a.d_ff) {
+      g = *reinterpret_cast<const Pack *>(a.gu + at), u = *reinterpret_cast<const Pack *>(a.gu + at + a.d_ff);
+      const Pack d = *reinterpret_cast<const Pack *>(a.dh + r * a.ldh + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float value, slope;
-      act_both(to_f32<BF16>(g.v[i]), a.act, value, slope);
-      const float dh = to_f32<BF16>(d.v[i]);
-      g.v[i] = from_f32<BF16>(dh * to_f32<BF16>(u.v[i]) * slope);
-      u.v[i] = from_f32<BF16>(dh * value);
+      for (int i = 0; i < V; ++i) {
+        float value, slope;
+        act_both(to_f32<BF16>(g.v[i]), a.act, value, slope);
+        const float dh = to_f32<BF16>(d.v[i]);
+        g.v[i] = from_f32<BF16>(dh * to_f32<BF16>(u.v[i]) * slope);
+        u.v[i] = from_f32<BF16>(dh * value);
+      }
     }
-    *reinterpret_cast<Pack *>(a.dgu + at) = g;
-    *reinterpret_cast<Pack *>(a.dgu + at + a.d_ff) = u;
+    *reinterpret_cast<Pack *>(a.dgu + r * 2 * a.up + c) = g;
+    *reinterpret_cast<Pack *>(a.dgu + r * 2 * a.up + c + a.up) = u;
   }
 }
-
 
 // ---- D[128 x 128 tiles] = A . B, f32 sums, 16-bit results
 namespace prod {
@@ -78,6 +79,8 @@ struct Params {
   unsigned *status;
   long long ldd;
   int rows, cols, tiles_n, k_blocks, shares;
+  int wide;        // results may be stored 16 bytes at a time
+  int half, held;  // columns come in halves of `half`, of which `held` exist and are stored side by side
   uint32_t idesc;
 };
 } // namespace prod
@@ -184,8 +187,21 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       report(p.status, kStatusEpiWaitTimeout);
     }
     sums_barrier<128>(p.shares);
-    add_up<BF16, 128, 128>(base, rank, p.shares, 1.0f, p.d + static_cast<long long>(row0) * p.ldd + col0, p.ldd, p.rows - row0,
-                           threadIdx.x - 128, (p.cols - col0 + 7) / 8);
+    add_up<128, 128>(base, rank, p.shares, threadIdx.x - 128, [&](int r, int unit, float4 x, float4 y) {
+      const int col = col0 + unit * 8;
+      if (row0 + r >= p.rows || col >= p.cols) return;
+      uint16_t *to = p.d + (row0 + r) * p.ldd;
+      if (p.wide) {
+        store_unit<BF16>(to + col, x, y, 1.0f);
+      } else {
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int h = col + e < p.half ? 0 : 1, c = col + e - h * p.half;
+          if (c < p.held) to[h * p.held + c] = from_f32<BF16>(v[e]);
+        }
+      }
+    });
     sums_barrier<128>(p.shares);
   }
   __syncwarp();
@@ -195,18 +211,6 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128) : "memory");
   }
-}
-
-int64_t pitch(int64_t ld, int64_t width) { return ld > 0 ? ld : width; }
-size_t dgu_bytes(const GatedProblem &p) { return (static_cast<size_t>(p.tokens) * 2 * p.d_ff * 2 + 255) / 256 * 256; }
-
-// The framework's GEMM on the kernel its shapes ask for.
-cudaError_t product(GemmProblem &g, unsigned *status, cudaStream_t stream) {
-  if (gemm_tcgen05_2cta_preferred(g)) {
-    const cudaError_t e = launch_gemm_tcgen05_2cta(g, status, stream);
-    if (e != cudaErrorNotSupported) return e;
-  }
-  return launch_gemm_simt(g, stream);
 }
 
 // The pair GEMM's 256 x 256 tiles move half as much through shared memory per operation, but they need many tiles and
@@ -219,7 +223,7 @@ bool small_product(const GemmProblem &g) {
 }
 
 template <auto kernel>
-cudaError_t launch_product(const GemmProblem &g, unsigned *status, cudaStream_t stream) {
+cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_t held, unsigned *status, cudaStream_t stream) {
   const bool mn = g.trans_a;
   CUtensorMap ta, tb;
   if (!(mn ? make_map(&ta, g.A, g.in_dtype, g.M, g.K, prod::BK, g.lda) : make_map(&ta, g.A, g.in_dtype, g.K, g.M, 128, g.lda)) ||
@@ -233,6 +237,9 @@ cudaError_t launch_product(const GemmProblem &g, unsigned *status, cudaStream_t 
   p.ldd = g.ldc;
   p.rows = static_cast<int>(g.M);
   p.cols = static_cast<int>(g.N);
+  p.wide = wide;
+  p.half = static_cast<int>(half);
+  p.held = static_cast<int>(held);
   p.tiles_n = static_cast<int>((g.N + 127) / 128);
   p.k_blocks = static_cast<int>((g.K + prod::BK - 1) / prod::BK);
   const int64_t tiles = (g.M + 127) / 128 * p.tiles_n;
@@ -261,65 +268,81 @@ cudaError_t launch_product(const GemmProblem &g, unsigned *status, cudaStream_t 
 
 } // namespace
 
-size_t gated_bwd_workspace_bytes(const GatedProblem &p) { return dgu_bytes(p) + gemm_tcgen05_workspace_bytes(); }
-
-cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
-  const int64_t ldx = pitch(p.ldx, p.d_in), ldw = pitch(p.ldw, 2 * p.d_ff), ldh = pitch(p.ldh, p.d_ff);
-  uint16_t *dgu = static_cast<uint16_t *>(p.workspace);
-  GradArgs a{static_cast<const uint16_t *>(p.gu), static_cast<const uint16_t *>(p.h), dgu, ldh, p.tokens, p.d_ff, p.act};
-  auto on16 = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
-  if (!on16(p.workspace)) return cudaErrorMisalignedAddress;
-  const bool wide = p.d_ff % 8 == 0 && ldh % 8 == 0 && on16(p.gu) && on16(p.h) && on16(dgu);
-  const int64_t items = p.tokens * (wide ? p.d_ff / 8 : p.d_ff);
+namespace {
+// dGU, then the padded copies or the GEMM's scratch
+size_t dgu_bytes(const GatedProblem &p) {
+  return gated::round_up(static_cast<size_t>(p.tokens) * 2 * gated::eights(p.d_ff) * 2);
+}
+template <bool BF16>
+cudaError_t launch_passes(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  const gated::Layout l(p, dgu_bytes(p));
+  int64_t ldx = gated::pitch(p.ldx, p.d_in), ldw = gated::pitch(p.ldw, 2 * p.d_ff);
+  const int64_t ldh = gated::pitch(p.ldh, p.d_ff), ld_dx = ldx, ld_dw = ldw;
+  const void *x = p.x, *w = p.w;
+  char *ws = static_cast<char *>(p.workspace);
+  uint16_t *dgu = reinterpret_cast<uint16_t *>(ws);
+  cudaError_t e;
+  *launched = 0;
+  if (l.padded) {
+    e = gated::launch_pad(x, ldx, ws + l.x, p.tokens, p.d_in, l.d_in, 1, stream);
+    if (e == cudaSuccess) e = gated::launch_pad(w, ldw, ws + l.w, p.d_in, p.d_ff, l.d_ff, 2, stream);
+    if (e != cudaSuccess) return e;
+    *launched = 2;
+    x = ws + l.x, w = ws + l.w;
+    ldx = l.d_in, ldw = 2 * l.d_ff;
+  }
+  const GradArgs a{static_cast<const uint16_t *>(p.gu), static_cast<const uint16_t *>(p.h), dgu, ldh, p.tokens, p.d_ff, l.d_ff, p.act};
+  const int64_t items = p.tokens * (l.padded ? l.d_ff : l.d_ff / 8);
   const int64_t most = 148 * 8 * 4;  // resident blocks, four rounds each at the most
   const unsigned blocks = static_cast<unsigned>((items + 255) / 256 < most ? (items + 255) / 256 : most);
-  if (p.dtype == kBF16) {
-    if (wide) gated_grad_kernel<true, 8><<<blocks, 256, 0, stream>>>(a);
-    else gated_grad_kernel<true, 1><<<blocks, 256, 0, stream>>>(a);
-  } else {
-    if (wide) gated_grad_kernel<false, 8><<<blocks, 256, 0, stream>>>(a);
-    else gated_grad_kernel<false, 1><<<blocks, 256, 0, stream>>>(a);
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  *launched = 1;
-  // dX[tokens, d_in] = dGU[tokens, 2 d_ff] . W^T, W stored [d_in, 2 d_ff]
+  if (l.padded) gated_grad_kernel<BF16, 1><<<blocks, 256, 0, stream>>>(a);
+  else gated_grad_kernel<BF16, 8><<<blocks, 256, 0, stream>>>(a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  ++*launched;
+
   int n = 1;
   GemmProblem g;
   g.in_dtype = g.out_dtype = p.dtype;
   g.epilogue = kEpiNone;
   g.accumulate = false;
   g.bias = nullptr;
-  g.workspace = reinterpret_cast<char *>(p.workspace) + dgu_bytes(p);
+  g.workspace = ws + l.rest;
   g.workspace_bytes = gemm_tcgen05_workspace_bytes();
   g.launched = &n;
-  g.A = dgu, g.B = p.w, g.C = static_cast<float *>(p.dx);
-  g.M = p.tokens, g.N = p.d_in, g.K = 2 * p.d_ff;
-  g.lda = 2 * p.d_ff, g.ldb = ldw, g.ldc = ldx;
+  // dX[tokens, d_in] = dGU[tokens, 2 d_ff] . W^T, W stored [d_in, 2 d_ff]
+  g.A = dgu, g.B = w, g.C = static_cast<float *>(p.dx);
+  g.M = p.tokens, g.N = p.d_in, g.K = 2 * l.d_ff;
+  g.lda = 2 * l.d_ff, g.ldb = ldw, g.ldc = ld_dx;
   g.trans_a = false, g.trans_b = true;
-  const bool fits = gemm_tcgen05_2cta_supported(g) && p.d_in % 8 == 0 && ldx % 8 == 0 && on16(p.x) && on16(p.dw);
-  const bool bf16 = p.dtype == kBF16;
-  if (fits && small_product(g))
-    e = bf16 ? launch_product<gated_product_kernel<true, false, true>>(g, status, stream)
-             : launch_product<gated_product_kernel<false, false, true>>(g, status, stream);
+  if (l.padded || small_product(g))
+    e = launch_product<gated_product_kernel<BF16, false, true>>(g, !l.padded, gated::eights(g.N), g.N, status, stream);
   else
-    e = product(g, status, stream);
+    e = launch_gemm_tcgen05_2cta(g, status, stream);
   if (e != cudaSuccess) return e;
   *launched += n;
   // dW[d_in, 2 d_ff] = X^T . dGU, X stored [tokens, d_in]
   n = 1;
-  g.A = p.x, g.B = dgu, g.C = static_cast<float *>(p.dw);
-  g.M = p.d_in, g.N = 2 * p.d_ff, g.K = p.tokens;
-  g.lda = ldx, g.ldb = 2 * p.d_ff, g.ldc = ldw;
+  g.A = x, g.B = dgu, g.C = static_cast<float *>(p.dw);
+  g.M = p.d_in, g.N = 2 * l.d_ff, g.K = p.tokens;
+  g.lda = ldx, g.ldb = 2 * l.d_ff, g.ldc = ld_dw;
   g.trans_a = true, g.trans_b = false;
-  if (fits && small_product(g))
-    e = bf16 ? launch_product<gated_product_kernel<true, true, false>>(g, status, stream)
-             : launch_product<gated_product_kernel<false, true, false>>(g, status, stream);
+  if (l.padded || small_product(g))
+    e = launch_product<gated_product_kernel<BF16, true, false>>(g, !l.padded, l.d_ff, p.d_ff, status, stream);
   else
-    e = product(g, status, stream);
+    e = launch_gemm_tcgen05_2cta(g, status, stream);
   if (e != cudaSuccess) return e;
   *launched += n;
   return cudaSuccess;
+}
+} // namespace
+
+size_t gated_bwd_workspace_bytes(const GatedProblem &p) {
+  const gated::Layout l(p, dgu_bytes(p));
+  return l.rest + (l.padded ? 0 : gemm_tcgen05_workspace_bytes());
+}
+
+cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  return p.dtype == kBF16 ? launch_passes<true>(p, status, stream, launched) : launch_passes<false>(p, status, stream, launched);
 }
 
 } // namespace imex

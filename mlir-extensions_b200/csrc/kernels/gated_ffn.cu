@@ -6,16 +6,16 @@
 //                        projection of the same 128 columns of H: CTA 0 of the pair loads the gate's 128
 //                        columns of W, CTA 1 the up projection's, and every thread of the epilogue has both
 //                        values of its elements in its own TMEM lane.
+//   gated_tile_kernel    more than 128 tokens, but few such tiles: 128 tokens x 64 columns of H, whose gate and up
+//                        columns are one 128-column operand, two CTAs per SM.
 //   gated_few_kernel     up to 128 tokens, where W's bytes are the time: W^T is the M operand (the gate's and
 //                        the up projection's columns of 64 columns of H per tile, as they lie), the tokens
 //                        are the N operand, so that no part of a tensor-core tile is wasted on rows that do
-//                        not exist; k is shared out
-//                        between the CTAs of a cluster, which add their parts up through distributed
-//                        shared memory, in order.
-//   gated_tile_kernel    extents, pitches or addresses TMA cannot take (not multiples of 16 bytes).
-#include "attention_common.cuh"
-#include "epilogue.cuh"
-#include "attention_tc.cuh"
+//                        not exist.
+//
+// In the last two k is shared out between the CTAs of a cluster where there are few tiles; they add their parts up
+// through distributed shared memory, in order.
+#include "gated_common.cuh"
 
 namespace imex {
 namespace {
@@ -25,60 +25,14 @@ using attn::to_f32;
 using namespace tc;
 using namespace tc_host;
 
-struct GatedArgs {
-  const uint16_t *x, *w;
-  uint16_t *h, *gu;
-  int64_t ldx, ldw, ldh;
-  int64_t tokens, d_in, d_ff;
-  int act;
-};
-
-// Any extents: 64 x 64 outputs per block, 4 x 4 of both projections per thread.
-template <bool BF16> __global__ void __launch_bounds__(256) gated_tile_kernel(const GatedArgs a) {
-  __shared__ float xs[16][64 + 4], gs[16][64 + 4], us[16][64 + 4];
-  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 64, n0 = static_cast<int64_t>(blockIdx.x) * 64;
-  float g[4][4] = {}, u[4][4] = {};
-  for (int64_t k0 = 0; k0 < a.d_in; k0 += 16) {
-    for (int e = tid; e < 64 * 16; e += 256) {
-      const int m = e / 16, k = e % 16;
-      xs[k][m] = m0 + m < a.tokens && k0 + k < a.d_in ? to_f32<BF16>(a.x[(m0 + m) * a.ldx + k0 + k]) : 0.0f;
-    }
-    for (int e = tid; e < 16 * 64; e += 256) {
-      const int k = e / 64, n = e % 64;
-      const bool in = n0 + n < a.d_ff && k0 + k < a.d_in;
-      const uint16_t *w = a.w + (k0 + k) * a.ldw + n0 + n;
-      gs[k][n] = in ? to_f32<BF16>(w[0]) : 0.0f;
-      us[k][n] = in ? to_f32<BF16>(w[a.d_ff]) : 0.0f;
-    }
-    __syncthreads();
+// Eight consecutive results of a row, `count` of which exist; by one access when `wide`.
+template <bool BF16> __device__ __forceinline__ void store8(uint16_t *to, const float (&v)[8], bool wide, int count) {
+  if (!wide) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          g[i][j] = fmaf(xs[k][ty * 4 + i], gs[k][tx * 4 + j], g[i][j]);
-          u[i][j] = fmaf(xs[k][ty * 4 + i], us[k][tx * 4 + j], u[i][j]);
-        }
-    __syncthreads();
+    for (int e = 0; e < 8; ++e)
+      if (e < count) to[e] = from_f32<BF16>(v[e]);
+    return;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = m0 + ty * 4 + i, c = n0 + tx * 4 + j;
-      if (r >= a.tokens || c >= a.d_ff) continue;
-      a.h[r * a.ldh + c] = from_f32<BF16>(apply_epilogue_fast(g[i][j], a.act) * u[i][j]);
-      if (a.gu) {
-        a.gu[r * 2 * a.d_ff + c] = from_f32<BF16>(g[i][j]);
-        a.gu[r * 2 * a.d_ff + a.d_ff + c] = from_f32<BF16>(u[i][j]);
-      }
-    }
-}
-
-// Eight consecutive results of a row.
-template <bool BF16> __device__ __forceinline__ void store8(uint16_t *to, const float (&v)[8]) {
   uint32_t w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -106,6 +60,8 @@ struct Params {
   unsigned *status;
   long long ldh;
   int tokens, d_ff, act, tiles_m, tiles_f, num_tiles, k_blocks;
+  int up;    // first column of the up projection in W
+  int wide;  // results may be stored 16 bytes at a time
   uint32_t idesc;
 };
 // Bands of eight row blocks: the tiles in flight share few columns of W and few rows of X.
@@ -163,7 +119,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         int mb, fb;
         coords(tile, p, mb, fb);
         const int row0 = mb * 2 * BM + static_cast<int>(rank) * BM;
-        const int col0 = fb * BF + (rank ? p.d_ff : 0);  // CTA 0: the gate's columns, CTA 1: the up projection's
+        const int col0 = fb * BF + (rank ? p.up : 0);  // CTA 0: the gate's columns, CTA 1: the up projection's
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u)) {
             report(p.status, kStatusTmaWaitTimeout);
@@ -242,7 +198,8 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             const int col = fb * BF + c0 + j;
-            if (col < p.d_ff) {  // d_ff is a multiple of 8 here
+            if (col < p.d_ff) {
+              const int count = p.d_ff - col;
               float x[8], y[8], v[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
@@ -250,11 +207,11 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
                 y[e] = __uint_as_float(u[j + e]);
                 v[e] = apply_epilogue_fast(x[e], p.act) * y[e];
               }
-              store8<BF16>(p.h + row * p.ldh + col, v);
+              store8<BF16>(p.h + row * p.ldh + col, v, p.wide, count);
               if (p.gu) {
                 uint16_t *gu = p.gu + static_cast<long long>(row) * 2 * p.d_ff + col;
-                store8<BF16>(gu, x);
-                store8<BF16>(gu + p.d_ff, y);
+                store8<BF16>(gu, x, p.wide, count);
+                store8<BF16>(gu + p.d_ff, y, p.wide, count);
               }
             }
           }
@@ -278,6 +235,145 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
   }
 }
 
+// -------------------------------------------------------------------------------- some tokens, few tiles
+namespace mid {
+constexpr int BK = 64, STAGES = 3;
+constexpr int BF = 64;                         // columns of H per tile
+constexpr int TILE_BYTES = 128 * 128;          // 128 tokens x 64 k, or 64 k x (64 gate, 64 up) columns
+constexpr int STAGE_BYTES = 2 * TILE_BYTES;
+constexpr int SMEM = STAGES * STAGE_BYTES + 256;
+constexpr int THREADS = 256;                   // TMA, products, two idle warps, four that hand the sums over
+static_assert(128 * 128 * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
+static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+struct Params {
+  uint16_t *h, *gu;
+  unsigned *status;
+  long long ldh;
+  int tokens, d_ff, act, tiles_f, k_blocks, shares, up, wide;
+  uint32_t idesc;
+};
+} // namespace mid
+
+template <bool BF16>
+__global__ void __launch_bounds__(mid::THREADS, 2)
+gated_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const mid::Params p) {
+  using namespace mid;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw), bars = base + STAGES * STAGE_BYTES;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
+  const uint32_t done = bars + 8u * (2 * STAGES), slot = done + 8;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
+  const int row0 = tile / p.tiles_f * 128, f0 = tile % p.tiles_f * BF;
+  const int kb0 = p.k_blocks * rank / p.shares, n = p.k_blocks * (rank + 1) / p.shares - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc_one(slot, 128);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (slot - base));
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < n; ++i) {
+        const int s = i % STAGES, k = (kb0 + i) * BK;
+        if (i >= STAGES && !mbar_wait(empty_bar(s), (i / STAGES - 1) & 1)) {
+          report(p.status, kStatusTmaWaitTimeout);
+          break;
+        }
+        mbar_expect_tx(full_bar(s), STAGE_BYTES);
+        const uint32_t x = base + s * STAGE_BYTES, w = x + TILE_BYTES;
+        tma_load_2d(x, &tmap_x, k, row0, full_bar(s));
+        tma_load_2d(w, &tmap_w, f0, k, full_bar(s));
+        tma_load_2d(w + TILE_BYTES / 2, &tmap_w, p.up + f0, k, full_bar(s));
+      }
+      for (int i = max(0, n - STAGES); i < n; ++i)  // everything has been used
+        if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1)) break;
+    }
+  } else if (warp == 1) {
+    const uint32_t leader = attn::elect_one();
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const int s = i % STAGES;
+      ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), (i / STAGES) & 1));
+      if (!ok) break;
+      tcgen05_fence_after();
+      const uint32_t at = base + s * STAGE_BYTES;
+      const uint64_t x = make_smem_desc(at, 16, 1024), w = make_smem_desc(at + TILE_BYTES, TILE_BYTES / 2, 1024);
+#pragma unroll
+      for (int k = 0; k < BK / 16; ++k)
+        attn::mma_ss(tmem, x + (k * 32 >> 4), w + (k * 2048 >> 4), p.idesc, (i | k) ? 1u : 0u, leader);
+      attn::commit(empty_bar(s), leader);
+    }
+    if (ok) attn::commit(done, leader);
+    else if (lane == 0) report(p.status, kStatusMmaWaitTimeout);
+  }
+  if (warp < 4) {
+    if (p.shares > 1) {  // the other warps' two barriers
+      __syncwarp();
+      cluster_sync_all();
+      cluster_sync_all();
+    }
+  } else {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0));
+    if (ok) {
+      tcgen05_fence_after();
+      const int lane_group = warp & 3;
+      attn::leave_row<128, 128>(tmem + (static_cast<uint32_t>(lane_group * 32) << 16), true, base, lane_group * 32 + lane, 0);
+    } else if (lane == 0) {
+      report(p.status, kStatusEpiWaitTimeout);
+    }
+    attn::sums_barrier<128>(p.shares);
+    // this CTA's part of the tokens; a thread has eight columns of H, whose up projection lies 64 columns behind
+    for (int u = threadIdx.x - 128; u < 128 / p.shares * (BF / 8); u += 128) {
+      const int r = rank * (128 / p.shares) + u / (BF / 8), unit = u % (BF / 8), token = row0 + r, col = f0 + unit * 8;
+      float g[8] = {}, y[8] = {};
+#pragma unroll 2
+      for (int s = 0; s < p.shares; ++s) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t at = base + attn::sum_offset<128>(r, unit * 2 + (h & 1) + (h >> 1) * 16);
+          float4 v;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                       : "r"(p.shares > 1 ? map_to_cta(at, s) : at));
+          float *to = (h >> 1 ? y : g) + (h & 1) * 4;
+          to[0] += v.x, to[1] += v.y, to[2] += v.z, to[3] += v.w;
+        }
+      }
+      if (token < p.tokens && col < p.d_ff) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = apply_epilogue_fast(g[e], p.act) * y[e];
+        store8<BF16>(p.h + token * p.ldh + col, v, p.wide, p.d_ff - col);
+        if (p.gu) {
+          uint16_t *gu = p.gu + static_cast<long long>(token) * 2 * p.d_ff + col;
+          store8<BF16>(gu, g, p.wide, p.d_ff - col);
+          store8<BF16>(gu + p.d_ff, y, p.wide, p.d_ff - col);
+        }
+      }
+    }
+    attn::sums_barrier<128>(p.shares);
+  }
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128) : "memory");
+  }
+}
+
 // ------------------------------------------------------------------------------------------- few tokens
 namespace few {
 constexpr int BF = 64;                  // columns of H per tile; the M of the product is their gate and up columns
@@ -295,6 +391,7 @@ struct Params {
   unsigned *status;
   long long ldh;
   int tokens, d_ff, act, k_blocks, shares;
+  int up;  // first column of the up projection in W
   uint32_t idesc;
 };
 } // namespace few
@@ -343,7 +440,7 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         mbar_expect_tx(full_bar(s), STAGE_BYTES);
         const uint32_t w = base + s * STAGE_BYTES;
         tma_load_2d(w, &tmap_w, f0, kb * BK, full_bar(s));
-        tma_load_2d(w + W_BOX, &tmap_w, p.d_ff + f0, kb * BK, full_bar(s));
+        tma_load_2d(w + W_BOX, &tmap_w, p.up + f0, kb * BK, full_bar(s));
         tma_load_2d(w + W_BYTES, &tmap_x, kb * BK, 0, full_bar(s));
       }
       for (int i = max(0, kb1 - kb0 - STAGES); i < kb1 - kb0; ++i)  // everything has been used
@@ -424,40 +521,49 @@ gated_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   }
 }
 
-int64_t pitch(int64_t ld, int64_t width) { return ld > 0 ? ld : width; }
-
 } // namespace
 
-const char *gated_check(const GatedProblem &p) {
+const char *gated_check(const GatedProblem &p, bool backward, bool pointers) {
   if (p.dtype != kF16 && p.dtype != kBF16) return "the element type is f16 or bf16";
   if (p.act != kEpiNone && p.act != kEpiRelu && p.act != kEpiSilu) return "unknown activation";
   if (p.tokens < 1 || p.d_in < 1 || p.d_ff < 1) return "extents are at least 1";
   if (p.tokens > (1 << 30) || p.d_in > (1 << 29) || p.d_ff > (1 << 29)) return "extents are at most 2^30 tokens, 2^29 columns";
   if ((p.ldx && p.ldx < p.d_in) || (p.ldw && p.ldw < 2 * p.d_ff) || (p.ldh && p.ldh < p.d_ff))
     return "row pitch smaller than the row";
+  if (!pointers) return nullptr;
+  const bool padded = gated::Layout(p).padded;
+  const uintptr_t unit = padded ? 2 : 16;
+  for (const void *q : {p.x, p.w, static_cast<const void *>(p.h), static_cast<const void *>(p.gu),
+                        static_cast<const void *>(p.dx), static_cast<const void *>(p.dw)})
+    if (reinterpret_cast<uintptr_t>(q) % unit)
+      return padded ? "arrays must be aligned to their elements" : "arrays must be 16-byte aligned";
+  if ((padded || backward) && reinterpret_cast<uintptr_t>(p.workspace) % 16) return "the workspace must be 16-byte aligned";
   return nullptr;
 }
 
+size_t gated_workspace_bytes(const GatedProblem &p) { return gated::Layout(p).rest; }
+
 namespace {
 
-bool tma_takes(const GatedProblem &p) {
-  auto on16 = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
-  return p.d_in % 8 == 0 && p.d_ff % 8 == 0 && p.ldx % 8 == 0 && p.ldw % 8 == 0 && p.ldh % 8 == 0 && on16(p.x) &&
-         on16(p.w) && on16(p.h) && (!p.gu || on16(p.gu));
+// A problem as the kernels get it: extents as the results have them, X and W with rows of whole 16-byte units.
+struct Prepared {
+  const void *x, *w;
+  int64_t ldx, ldw, ldh, up;  // up: first column of the up projection in W
+  bool wide;
+};
+
+bool tiles(CUtensorMap *tx, CUtensorMap *tw, const GatedProblem &p, const Prepared &q, int rows_x, int rows_w) {
+  return make_map(tx, q.x, p.dtype, p.d_in, p.tokens, rows_x, q.ldx) && make_map(tw, q.w, p.dtype, q.up + p.d_ff, p.d_in, rows_w, q.ldw);
 }
 
-template <bool BF16, int NT>
-cudaError_t launch_few(const GatedProblem &p, const few::Params &f, cudaStream_t stream) {
-  CUtensorMap tx, tw;
-  if (!make_map(&tx, p.x, p.dtype, p.d_in, p.tokens, NT, pitch(p.ldx, p.d_in)) ||
-      !make_map(&tw, p.w, p.dtype, 2 * p.d_ff, p.d_in, few::BK, pitch(p.ldw, 2 * p.d_ff)))
-    return cudaErrorNotSupported;
-  const cudaError_t e = attn::allow_smem<gated_few_kernel<BF16, NT>>(few::smem_bytes(NT));
-  if (e != cudaSuccess) return e;
+// `shares` CTAs per cluster
+template <typename Params>
+cudaError_t launch_cluster(void (*kernel)(CUtensorMap, CUtensorMap, Params), const CUtensorMap &tx, const CUtensorMap &tw,
+                           const Params &f, int64_t grid, int threads, int smem, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.d_ff + few::BF - 1) / few::BF) * f.shares);
-  cfg.blockDim = dim3(few::THREADS);
-  cfg.dynamicSmemBytes = few::smem_bytes(NT);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -465,19 +571,35 @@ cudaError_t launch_few(const GatedProblem &p, const few::Params &f, cudaStream_t
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gated_few_kernel<BF16, NT>, tx, tw, f);
+  return cudaLaunchKernelEx(&cfg, kernel, tx, tw, f);
 }
 
-template <bool BF16> cudaError_t launch_few_tokens(const GatedProblem &p, unsigned *status, cudaStream_t stream) {
-  few::Params f{};
+template <typename Params> Params common(const GatedProblem &p, const Prepared &q, int bk, unsigned *status) {
+  Params f{};
   f.h = static_cast<uint16_t *>(p.h);
   f.gu = static_cast<uint16_t *>(p.gu);
   f.status = status;
-  f.ldh = pitch(p.ldh, p.d_ff);
+  f.ldh = q.ldh;
   f.tokens = static_cast<int>(p.tokens);
   f.d_ff = static_cast<int>(p.d_ff);
   f.act = p.act;
-  f.k_blocks = static_cast<int>((p.d_in + few::BK - 1) / few::BK);
+  f.up = static_cast<int>(q.up);
+  f.k_blocks = static_cast<int>((p.d_in + bk - 1) / bk);
+  return f;
+}
+
+template <bool BF16, int NT>
+cudaError_t launch_few(const GatedProblem &p, const Prepared &q, const few::Params &f, int64_t grid, cudaStream_t stream) {
+  CUtensorMap tx, tw;
+  if (!tiles(&tx, &tw, p, q, NT, few::BK)) return cudaErrorNotSupported;
+  const cudaError_t e = attn::allow_smem<gated_few_kernel<BF16, NT>>(few::smem_bytes(NT));
+  if (e != cudaSuccess) return e;
+  return launch_cluster(gated_few_kernel<BF16, NT>, tx, tw, f, grid, few::THREADS, few::smem_bytes(NT), stream);
+}
+
+template <bool BF16>
+cudaError_t launch_few_tokens(const GatedProblem &p, const Prepared &q, unsigned *status, cudaStream_t stream) {
+  few::Params f = common<few::Params>(p, q, few::BK, status);
   const int nt = p.tokens <= 16 ? 16 : p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
   const int64_t tiles = (p.d_ff + few::BF - 1) / few::BF;
   // Shares of k per tile: as many CTAs as run at once, at least two k blocks each.  One token of 4096 x 11264
@@ -490,31 +612,42 @@ template <bool BF16> cudaError_t launch_few_tokens(const GatedProblem &p, unsign
   // f32 accumulator; A (W) is MN-major, B (X) K-major; N >> 3, M >> 4
   f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (static_cast<uint32_t>(nt >> 3) << 17) |
             ((128u >> 4) << 24);
-  if (nt == 16) return launch_few<BF16, 16>(p, f, stream);
-  if (nt == 32) return launch_few<BF16, 32>(p, f, stream);
-  if (nt == 64) return launch_few<BF16, 64>(p, f, stream);
-  return launch_few<BF16, 128>(p, f, stream);
+  if (nt == 16) return launch_few<BF16, 16>(p, q, f, tiles * f.shares, stream);
+  if (nt == 32) return launch_few<BF16, 32>(p, q, f, tiles * f.shares, stream);
+  if (nt == 64) return launch_few<BF16, 64>(p, q, f, tiles * f.shares, stream);
+  return launch_few<BF16, 128>(p, q, f, tiles * f.shares, stream);
 }
 
-template <bool BF16> cudaError_t launch_many_tokens(const GatedProblem &p, unsigned *status, cudaStream_t stream) {
+template <bool BF16>
+cudaError_t launch_tiles(const GatedProblem &p, const Prepared &q, unsigned *status, cudaStream_t stream) {
   CUtensorMap tx, tw;
-  if (!make_map(&tx, p.x, p.dtype, p.d_in, p.tokens, pair::BM, pitch(p.ldx, p.d_in)) ||
-      !make_map(&tw, p.w, p.dtype, 2 * p.d_ff, p.d_in, pair::BK, pitch(p.ldw, 2 * p.d_ff)))
-    return cudaErrorNotSupported;
+  if (!tiles(&tx, &tw, p, q, 128, mid::BK)) return cudaErrorNotSupported;
+  const cudaError_t e = attn::allow_smem<gated_tile_kernel<BF16>>(mid::SMEM);
+  if (e != cudaSuccess) return e;
+  mid::Params f = common<mid::Params>(p, q, mid::BK, status);
+  f.wide = q.wide;
+  f.tiles_f = static_cast<int>((p.d_ff + mid::BF - 1) / mid::BF);
+  const int64_t count = (p.tokens + 127) / 128 * f.tiles_f;
+  // Shares of k: as many CTAs as run at once, at least twenty k blocks each (adding up costs about as much as eight).
+  f.shares = 1;
+  while (f.shares < 8 && count * f.shares * 2 <= 2 * 148 && f.k_blocks >= 40 * f.shares) f.shares *= 2;
+  const uint32_t fmt = BF16 ? 1u : 0u;
+  // f32 accumulator; A (X) is K-major, B (W) MN-major; N >> 3, M >> 4
+  f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  return launch_cluster(gated_tile_kernel<BF16>, tx, tw, f, count * f.shares, mid::THREADS, mid::SMEM, stream);
+}
+
+template <bool BF16>
+cudaError_t launch_pairs(const GatedProblem &p, const Prepared &q, unsigned *status, cudaStream_t stream) {
+  CUtensorMap tx, tw;
+  if (!tiles(&tx, &tw, p, q, pair::BM, pair::BK)) return cudaErrorNotSupported;
   const cudaError_t e = attn::allow_smem<gated_pair_kernel<BF16>>(pair::SMEM_BYTES);
   if (e != cudaSuccess) return e;
-  pair::Params f{};
-  f.h = static_cast<uint16_t *>(p.h);
-  f.gu = static_cast<uint16_t *>(p.gu);
-  f.status = status;
-  f.ldh = pitch(p.ldh, p.d_ff);
-  f.tokens = static_cast<int>(p.tokens);
-  f.d_ff = static_cast<int>(p.d_ff);
-  f.act = p.act;
+  pair::Params f = common<pair::Params>(p, q, pair::BK, status);
+  f.wide = q.wide;
   f.tiles_m = static_cast<int>((p.tokens + 2 * pair::BM - 1) / (2 * pair::BM));
   f.tiles_f = static_cast<int>((p.d_ff + pair::BF - 1) / pair::BF);
   f.num_tiles = f.tiles_m * f.tiles_f;
-  f.k_blocks = static_cast<int>((p.d_in + pair::BK - 1) / pair::BK);
   const uint32_t fmt = BF16 ? 1u : 0u;
   // f32 accumulator; B (W) is MN-major; N = 256, M = 256
   f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
@@ -523,23 +656,31 @@ template <bool BF16> cudaError_t launch_many_tokens(const GatedProblem &p, unsig
   return cudaGetLastError();
 }
 
+template <bool BF16>
+cudaError_t launch_by_tokens(const GatedProblem &p, const Prepared &q, unsigned *status, cudaStream_t stream) {
+  if (p.tokens <= 128) return launch_few_tokens<BF16>(p, q, status, stream);
+  // The small tiles while all of them have an SM of their own.  512 tokens of 4096 x 1024 (16 pair tiles): 18.7 us, 28.9
+  // by pairs; 1000 of 1000 x 1000 (32): 14.8 and 16.7; 256 of 2048 x 5632 (44): 23.3 and 20.8; 512 of 4096 x 4096 (64):
+  // 37.5 and 31.2.
+  const int64_t pairs = (p.tokens + 255) / 256 * ((p.d_ff + 127) / 128);
+  return pairs <= 148 / 4 ? launch_tiles<BF16>(p, q, status, stream) : launch_pairs<BF16>(p, q, status, stream);
+}
+
 } // namespace
 
 cudaError_t launch_gated(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched) {
+  const gated::Layout l(p);
+  Prepared q{p.x, p.w, gated::pitch(p.ldx, p.d_in), gated::pitch(p.ldw, 2 * p.d_ff), gated::pitch(p.ldh, p.d_ff), p.d_ff, true};
   *launched = 1;
-  const bool bf16 = p.dtype == kBF16;
-  if (tma_takes(p)) {
-    if (p.tokens <= 128)
-      return bf16 ? launch_few_tokens<true>(p, status, stream) : launch_few_tokens<false>(p, status, stream);
-    return bf16 ? launch_many_tokens<true>(p, status, stream) : launch_many_tokens<false>(p, status, stream);
+  if (l.padded) {
+    char *ws = static_cast<char *>(p.workspace);
+    cudaError_t e = gated::launch_pad(p.x, q.ldx, ws + l.x, p.tokens, p.d_in, l.d_in, 1, stream);
+    if (e == cudaSuccess) e = gated::launch_pad(p.w, q.ldw, ws + l.w, p.d_in, p.d_ff, l.d_ff, 2, stream);
+    if (e != cudaSuccess) return e;
+    *launched = 3;
+    q = Prepared{ws + l.x, ws + l.w, l.d_in, 2 * l.d_ff, q.ldh, l.d_ff, false};
   }
-  GatedArgs a{static_cast<const uint16_t *>(p.x), static_cast<const uint16_t *>(p.w), static_cast<uint16_t *>(p.h),
-              static_cast<uint16_t *>(p.gu), pitch(p.ldx, p.d_in), pitch(p.ldw, 2 * p.d_ff), pitch(p.ldh, p.d_ff),
-              p.tokens, p.d_in, p.d_ff, p.act};
-  const dim3 grid(static_cast<unsigned>((p.d_ff + 63) / 64), static_cast<unsigned>((p.tokens + 63) / 64));
-  if (bf16) gated_tile_kernel<true><<<grid, 256, 0, stream>>>(a);
-  else gated_tile_kernel<false><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError();
+  return p.dtype == kBF16 ? launch_by_tokens<true>(p, q, status, stream) : launch_by_tokens<false>(p, q, status, stream);
 }
 
 } // namespace imex

@@ -108,7 +108,9 @@ struct GatedProblem {
   void *dx, *dw;   // backward
   void *workspace;
 };
-const char *gated_check(const GatedProblem &p);
+// nullptr, or why the problem is refused.  Pointers are looked at only when `pointers`.
+const char *gated_check(const GatedProblem &p, bool backward, bool pointers);
+size_t gated_workspace_bytes(const GatedProblem &p);      // 0 unless extents or pitches are not multiples of 8
 size_t gated_bwd_workspace_bytes(const GatedProblem &p);
 cudaError_t launch_gated(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched);
 cudaError_t launch_gated_bwd(const GatedProblem &p, unsigned *status, cudaStream_t stream, int *launched);

@@ -28,11 +28,10 @@ __device__ __forceinline__ void leave_row(uint32_t taddr, bool has, uint32_t sum
                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
   }
 }
-// This CTA's part of the rows over all shares, in order, to 16 bits: neighbouring threads write neighbouring
-// 16 bytes of a row.  `thread` of THREADS; rows_left rows and units_left units of eight columns exist; the loads of two steps are in flight together.
-template <bool BF16, int DH, int S, int THREADS>
-__device__ __forceinline__ void add_up_of(uint32_t sums, int rank, float factor, uint16_t *to, int64_t step, int rows_left,
-                                          int units_left, int thread) {
+// This CTA's part of the rows over all shares, in order: put(row of the tile, unit of eight columns, the eight sums),
+// neighbouring threads on neighbouring units.  `thread` of THREADS; the loads of two steps are in flight together.
+template <int DH, int S, int THREADS, typename Put>
+__device__ __forceinline__ void add_up_of(uint32_t sums, int rank, int thread, Put &&put) {
   constexpr int UNITS = TILE / S * (DH / 8), STEPS = (UNITS + THREADS - 1) / THREADS;
 #pragma unroll 2
   for (int k = 0; k < STEPS; ++k) {
@@ -57,20 +56,20 @@ __device__ __forceinline__ void add_up_of(uint32_t sums, int rank, float factor,
         v[0][h].z += v[r][h].z;
         v[0][h].w += v[r][h].w;
       }
-    const float4 x = v[0][0], y = v[0][1];
-    if (u < UNITS && row < rows_left && unit / 2 < units_left)
-      *reinterpret_cast<uint4 *>(to + row * step + unit * 4) =
-          make_uint4(pack2<BF16>(x.x * factor, x.y * factor), pack2<BF16>(x.z * factor, x.w * factor),
-                     pack2<BF16>(y.x * factor, y.y * factor), pack2<BF16>(y.z * factor, y.w * factor));
+    if (u < UNITS) put(row, unit / 2, v[0][0], v[0][1]);
   }
 }
-template <bool BF16, int DH, int THREADS>
-__device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, float factor, uint16_t *to, int64_t step,
-                                       int rows_left, int thread, int units_left = DH / 8) {
-  if (shares == 1) add_up_of<BF16, DH, 1, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
-  else if (shares == 2) add_up_of<BF16, DH, 2, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
-  else if (shares == 4) add_up_of<BF16, DH, 4, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
-  else add_up_of<BF16, DH, 8, THREADS>(sums, rank, factor, to, step, rows_left, units_left, thread);
+template <int DH, int THREADS, typename Put>
+__device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, int thread, Put &&put) {
+  if (shares == 1) add_up_of<DH, 1, THREADS>(sums, rank, thread, put);
+  else if (shares == 2) add_up_of<DH, 2, THREADS>(sums, rank, thread, put);
+  else if (shares == 4) add_up_of<DH, 4, THREADS>(sums, rank, thread, put);
+  else add_up_of<DH, 8, THREADS>(sums, rank, thread, put);
+}
+// Eight sums times a factor as 16-bit values
+template <bool BF16> __device__ __forceinline__ void store_unit(uint16_t *to, float4 x, float4 y, float factor) {
+  *reinterpret_cast<uint4 *>(to) = make_uint4(pack2<BF16>(x.x * factor, x.y * factor), pack2<BF16>(x.z * factor, x.w * factor),
+                                              pack2<BF16>(y.x * factor, y.y * factor), pack2<BF16>(y.z * factor, y.w * factor));
 }
 // The computing warps' sums are in place everywhere / have been read everywhere.  The first warpgroup takes part
 // when there are several CTAs.

@@ -331,7 +331,7 @@ imex::GatedProblem gated_problem(const ImexKernelDesc &d) {
   p.ldx = d.dims[3], p.ldw = d.dims[4], p.ldh = d.dims[5];
   p.dtype = static_cast<int>(d.in_dtype);
   p.act = static_cast<int>(d.epilogue);
-  refuse(d, imex::gated_check(p));
+  refuse(d, imex::gated_check(p, d.op == IMEX_OP_GATED_FFN_BWD, false));
   return p;
 }
 
@@ -340,6 +340,8 @@ size_t workspace_bytes(const ImexKernelDesc &d, const std::string *source) {
   case IMEX_OP_ATTENTION:
   case IMEX_OP_ATTENTION_BWD:
     return imex::attention_workspace_bytes(attention_problem(d, source), d.op == IMEX_OP_ATTENTION_BWD);
+  case IMEX_OP_GATED_FFN:
+    return imex::gated_workspace_bytes(gated_problem(d));
   case IMEX_OP_GATED_FFN_BWD:
     return imex::gated_bwd_workspace_bytes(gated_problem(d));
   }
@@ -564,10 +566,13 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
   }
   case IMEX_OP_GATED_FFN: {
     const bool save = d.flags & IMEX_FLAG_SAVE_GU;
-    need(save ? 4 : 3);
     imex::GatedProblem p = gated_problem(d);
+    const size_t n = save ? 4 : 3, ws = imex::gated_workspace_bytes(p);
+    need(n + (ws ? 1 : 0));
     p.x = ptrs[0], p.w = ptrs[1], p.h = ptrs[2];
     if (save) p.gu = ptrs[3];
+    if (ws) p.workspace = ptrs[n];
+    refuse(d, imex::gated_check(p, false, true));
     s->last_kernel = "gated_ffn";
     err = imex::launch_gated(p, s->status_dev, s->stream, &launches);
     break;
@@ -577,7 +582,7 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
     imex::GatedProblem p = gated_problem(d);
     p.x = ptrs[0], p.w = ptrs[1], p.gu = ptrs[2], p.h = ptrs[3], p.dx = ptrs[4], p.dw = ptrs[5];
     p.workspace = ptrs[6];
-    if (reinterpret_cast<uintptr_t>(p.workspace) & 15) refuse(d, "the workspace must be 16-byte aligned");
+    refuse(d, imex::gated_check(p, true, true));
     s->last_kernel = "gated_ffn_bwd";
     err = imex::launch_gated_bwd(p, s->status_dev, s->stream, &launches);
     break;

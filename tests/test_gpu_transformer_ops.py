@@ -366,6 +366,7 @@ GATED = [
     (16, 264, 1000, "bf16", 2), (17, 256, 256, "f16", 0), (33, 200, 128, "bf16", 2), (64, 1000, 360, "f16", 2),
     (65, 128, 72, "bf16", 1), (127, 64, 8, "f16", 2), (128, 136, 264, "bf16", 2), (129, 520, 392, "f16", 2),
     (300, 1000, 104, "bf16", 2), (513, 72, 513, "bf16", 2), (700, 256, 384, "f16", 2), (40, 33, 65, "bf16", 0),
+    (513, 2600, 200, "bf16", 2), (200, 5201, 70, "f16", 2), (520, 96, 1704, "bf16", 2), (1300, 41, 801, "f16", 1),
 ]
 
 
@@ -411,9 +412,11 @@ def test_gated_ffn_gradients(pkg, sess, case):
         assert ((got.double() - want).abs() <= tol * 1.01).all()
 
 
-@pytest.mark.parametrize("m", [1, 20, 200])
-def test_gated_ffn_row_pitches(pkg, sess, m):
-    d, f, ldx, ldw, ldh = 128, 136, 160, 304, 144
+@pytest.mark.parametrize("m,d,f,ldx,ldw,ldh", [(1, 128, 136, 160, 304, 144), (20, 128, 136, 160, 304, 144),
+                                               (200, 128, 136, 160, 304, 144), (2100, 128, 640, 136, 1288, 648),
+                                               (20, 128, 136, 131, 275, 137), (200, 99, 135, 131, 272, 144),
+                                               (2100, 64, 601, 65, 1210, 603)])
+def test_gated_ffn_row_pitches(pkg, sess, m, d, f, ldx, ldw, ldh):
     x, w = _rand((m, ldx), "bf16", 1), _rand((d, ldw), "bf16", 2, d ** -0.5)
     h = Output(sess, m * ldh, "bf16")
     _launch(sess, pkg.blob.gated_ffn("g", m, d, f, pkg.blob.BF16, ldx=ldx, ldw=ldw, ldh=ldh),
@@ -434,6 +437,33 @@ def test_gated_ffn_row_pitches(pkg, sess, m):
         t = out.get((-1, held))
         assert (t[:, width:].contiguous().view(torch.int16) == SENTINEL).all()
         assert ((t[:, :width].double() - want).abs() <= 1.01 * 2.0 ** -8 * (want.abs() + size) + 1e-5).all()
+
+
+@pytest.mark.parametrize("m", [5, 200])
+def test_gated_ffn_odd_extents_take_arrays_at_any_element(pkg, sess, m):
+    d, f = 33, 69
+    x, w = _rand((m, d), "f16", 1), _rand((d, 2 * f), "f16", 2, d ** -0.5)
+    gu, dh = (x.float() @ w.float()).half(), _rand((m, f), "f16", 3)
+    runs = []
+    for lead in (0, 1, 3):
+        up = lambda t: sess.upload(_bits(torch.cat([torch.zeros(lead, dtype=t.dtype), t.flatten()]))) + 2 * lead
+        outs = [Output(sess, n + lead, "f16") for n in (m * f, m * 2 * f, m * d, d * 2 * f)]
+        at = [o.ptr + 2 * lead for o in outs]
+        _launch(sess, pkg.blob.gated_ffn("g", m, d, f, pkg.blob.F16, save_gu=True), [up(x), up(w), at[0], at[1]])
+        _launch(sess, pkg.blob.gated_ffn_bwd("b", m, d, f, pkg.blob.F16), [up(x), up(w), up(gu), up(dh), at[2], at[3]])
+        runs.append([o.get(-1)[lead:] for o in outs])
+        assert all(o.get(-1)[:lead].view(torch.int16).eq(SENTINEL).all() for o in outs)
+    assert all(torch.isfinite(a).all() and torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
+
+
+@pytest.mark.parametrize("op,d,arg,message", [("gated_ffn", 16, 1, "arrays must be 16-byte"), ("gated_ffn", 15, -1, "the workspace must be"),
+                                              ("gated_ffn_bwd", 16, 5, "arrays must be 16-byte"), ("gated_ffn_bwd", 16, -1, "the workspace must be")])
+def test_misaligned_gated_arrays_are_refused(op, d, arg, message):
+    text = ("from __graft_entry__ import load_package\npkg = load_package()\nB = pkg.blob\ns = pkg.Session(device=0)\n"
+            "k = s.kernel(B.%s('a', 2, %d, 8))\nn = %d\np = [s.alloc(4096) for _ in range(n)]\n"
+            "p[%d] += 8\ns.launch(k, p)\n" % (op, d, 7 if op.endswith("bwd") else 3 + d % 2, arg))
+    r = subprocess.run([sys.executable, "-c", text], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == -6 and message in r.stdout, r.stdout + r.stderr
 
 
 # ------------------------------------------------------------------------------------------- rotary

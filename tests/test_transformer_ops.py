@@ -81,6 +81,11 @@ def test_workspace_bytes():
     assert rt.imexKernelWorkspaceBytes(_kernel(B.softmax("s", 4, 8))) == 0
     assert rt.imexKernelWorkspaceBytes(_kernel(B.attention_bwd("a", 3, 4, 2, 50, 60, 64))) >= 3 * 4 * 50 * 4
     assert rt.imexKernelWorkspaceBytes(_kernel(B.gated_ffn_bwd("g", 30, 64, 72))) >= 30 * 2 * 72 * 2
+    # the gated product wants one only for extents or pitches that are not multiples of eight: its padded operands
+    assert rt.imexKernelWorkspaceBytes(_kernel(B.gated_ffn("g", 30, 64, 72))) == 0
+    for args in (dict(d_in=63, d_ff=72), dict(d_in=64, d_ff=71), dict(d_in=64, d_ff=72, ldx=65), dict(d_in=64, d_ff=72, ldw=145)):
+        d_in = (args["d_in"] + 7) // 8 * 8
+        assert rt.imexKernelWorkspaceBytes(_kernel(B.gated_ffn("g", 30, **args))) >= (30 * d_in + args["d_in"] * 2 * 72) * 2
 
 
 @pytest.mark.parametrize("patch,message", [

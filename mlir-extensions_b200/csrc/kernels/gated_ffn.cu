@@ -661,9 +661,11 @@ cudaError_t launch_by_tokens(const GatedProblem &p, const Prepared &q, unsigned 
   if (p.tokens <= 128) return launch_few_tokens<BF16>(p, q, status, stream);
   // The small tiles while all of them have an SM of their own.  512 tokens of 4096 x 1024 (16 pair tiles): 18.7 us, 28.9
   // by pairs; 1000 of 1000 x 1000 (32): 14.8 and 16.7; 256 of 2048 x 5632 (44): 23.3 and 20.8; 512 of 4096 x 4096 (64):
-  // 37.5 and 31.2.
+  // 37.5 and 31.2.  Results stored value by value cost the pairs more, whose threads have a row each: with k up to 2048
+  // (4096 of 1025 x 2819: 123 us, 166 by pairs; 1000 of 4097 x 2819: 145 and 133).
   const int64_t pairs = (p.tokens + 255) / 256 * ((p.d_ff + 127) / 128);
-  return pairs <= 148 / 4 ? launch_tiles<BF16>(p, q, status, stream) : launch_pairs<BF16>(p, q, status, stream);
+  const bool small = pairs <= 148 / 4 || (!q.wide && p.d_in <= 2048);
+  return small ? launch_tiles<BF16>(p, q, status, stream) : launch_pairs<BF16>(p, q, status, stream);
 }
 
 } // namespace

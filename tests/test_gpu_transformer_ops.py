@@ -366,7 +366,7 @@ GATED = [
     (16, 264, 1000, "bf16", 2), (17, 256, 256, "f16", 0), (33, 200, 128, "bf16", 2), (64, 1000, 360, "f16", 2),
     (65, 128, 72, "bf16", 1), (127, 64, 8, "f16", 2), (128, 136, 264, "bf16", 2), (129, 520, 392, "f16", 2),
     (300, 1000, 104, "bf16", 2), (513, 72, 513, "bf16", 2), (700, 256, 384, "f16", 2), (40, 33, 65, "bf16", 0),
-    (513, 2600, 200, "bf16", 2), (200, 5201, 70, "f16", 2), (520, 96, 1704, "bf16", 2), (1300, 41, 801, "f16", 1),
+    (513, 2600, 200, "bf16", 2), (200, 5201, 70, "f16", 2), (520, 96, 1704, "bf16", 2), (1300, 41, 801, "f16", 1), (520, 2049, 1701, "f16", 2),
 ]
 
 
@@ -415,7 +415,7 @@ def test_gated_ffn_gradients(pkg, sess, case):
 @pytest.mark.parametrize("m,d,f,ldx,ldw,ldh", [(1, 128, 136, 160, 304, 144), (20, 128, 136, 160, 304, 144),
                                                (200, 128, 136, 160, 304, 144), (2100, 128, 640, 136, 1288, 648),
                                                (20, 128, 136, 131, 275, 137), (200, 99, 135, 131, 272, 144),
-                                               (2100, 64, 601, 65, 1210, 603)])
+                                               (2100, 64, 601, 65, 1210, 603), (520, 2056, 1704, 2057, 3409, 1705)])
 def test_gated_ffn_row_pitches(pkg, sess, m, d, f, ldx, ldw, ldh):
     x, w = _rand((m, ldx), "bf16", 1), _rand((d, ldw), "bf16", 2, d ** -0.5)
     h = Output(sess, m * ldh, "bf16")

@@ -812,16 +812,23 @@ int64_t tiles_per_head(const AttentionProblem &p) {
 int64_t tile_count(const AttentionProblem &p) {
   return p.batch * (is_packed(p) ? p.kv_heads : p.q_heads) * tiles_per_head(p);
 }
-// Shares of a tile's key blocks: as many CTAs as run at once, at least four blocks each, none of fewer than twelve.
-// 8 query heads on one key head, one query: 8192 keys 57 us with one share, 17 with 16; 64 tiles of 1000 keys: 12.6 us
-// with one, 14.6 with two.
+// Shares of a tile's key blocks, at least four blocks each, none of fewer than twelve: the number with the shortest sum
+// of rounds, where a CTA's start and end cost about as much as seven blocks (four where two CTAs share an SM and one
+// works on) and the joining as three.  8 query heads on one key head, one query: 8192 keys 57 us with one share, 13
+// with 16; 64 tiles of 1000 keys: 12.6 us with one, 14.6 with two.  One query of 8000 keys, packed: 128 tiles (one
+// round) 84 us with one share, 90 with 2; 160 tiles (two rounds) 139 and 119 with 3; 80 tiles of 4000 keys: 35 with
+// one, 39 with 3.  Tiles that are not packed are split only to fill one round: a share leaves 128 KB in the workspace.
 int split_count(const AttentionProblem &p) {
   const int64_t blocks = (p.n_kv + TILE - 1) / TILE, tiles = tile_count(p);
-  const int64_t slots = p.d_head == 64 ? 2 * SMS : SMS;
-  int64_t s = tiles >= slots ? 1 : slots / tiles;
-  if (s > blocks / 4) s = blocks / 4;
-  if (blocks < 12) s = 1;
-  return static_cast<int>(s < 1 ? 1 : (s > 64 ? 64 : s));
+  const int64_t slots = p.d_head == 64 ? 2 * SMS : SMS, ends = p.d_head == 64 ? 4 : 7;
+  if (blocks < 12 || (tiles >= slots && !is_packed(p))) return 1;
+  int64_t best = 1, best_cost = INT64_MAX;
+  for (int64_t s = 1; s <= 64 && s <= blocks / 4; ++s) {
+    const int64_t rounds = (tiles * s + slots - 1) / slots;
+    const int64_t cost = rounds * ((blocks + s - 1) / s + ends) + (s > 1 ? 3 : 0);
+    if (cost < best_cost && (is_packed(p) || s == 1 || rounds == 1)) best = s, best_cost = cost;
+  }
+  return static_cast<int>(best);
 }
 
 bool aligned(const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }

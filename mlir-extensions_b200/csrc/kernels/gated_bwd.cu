@@ -7,6 +7,8 @@
 // shared out between the CTAs of a cluster where there are few tiles.
 #include "gated_common.cuh"
 
+#include <type_traits>
+
 namespace imex {
 namespace {
 
@@ -67,13 +69,14 @@ template <bool BF16, int V> __global__ void __launch_bounds__(256) gated_grad_ke
 
 // ---- D[128 x 128 tiles] = A . B, f32 sums, 16-bit results
 namespace prod {
-constexpr int BK = 64, STAGES = 3;
+constexpr int BK = 64;
 constexpr int TILE_BYTES = 128 * 128;          // 128 rows or columns x 64 k
 constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-constexpr int SMEM = STAGES * STAGE_BYTES + 256;
+constexpr int smem_bytes(int stages) { return stages * STAGE_BYTES + 256; }
 constexpr int THREADS = 256;                   // TMA, products, two idle warps, four that hand the sums over
-static_assert(128 * 128 * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
-static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+constexpr int FEW = 3, MANY = 6;               // stages: two CTAs per SM, or one
+static_assert(128 * 128 * 4 <= FEW * STAGE_BYTES, "the sums take the ring's place");
+static_assert(2 * (smem_bytes(FEW) + 1024) <= 233472 && smem_bytes(MANY) + 1024 <= 233472, "two CTAs per SM, or one");
 struct Params {
   uint16_t *d;
   unsigned *status;
@@ -88,7 +91,7 @@ struct Params {
 // MN_MAJOR: A is stored [k, rows] and B [k, cols] (X^T dGU); else [rows, k] and [cols, k] (dGU W^T).
 // FIRST: dX's product, which may start while the kernel that writes dGU still runs and lets dW's start beside it once
 // that has ended.
-template <bool BF16, bool MN_MAJOR, bool FIRST>
+template <bool BF16, bool MN_MAJOR, bool FIRST, int STAGES>
 __global__ void __launch_bounds__(prod::THREADS, 2)
 gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const prod::Params p) {
   using namespace prod;
@@ -222,15 +225,13 @@ bool small_product(const GemmProblem &g) {
   return tiles <= 64 || g.K <= 2048 || (tiles <= 148 && g.K <= 4096);
 }
 
-template <auto kernel>
+template <bool BF16, bool MN_MAJOR, bool FIRST>
 cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_t held, unsigned *status, cudaStream_t stream) {
-  const bool mn = g.trans_a;
+  const bool mn = MN_MAJOR;
   CUtensorMap ta, tb;
   if (!(mn ? make_map(&ta, g.A, g.in_dtype, g.M, g.K, prod::BK, g.lda) : make_map(&ta, g.A, g.in_dtype, g.K, g.M, 128, g.lda)) ||
       !(mn ? make_map(&tb, g.B, g.in_dtype, g.N, g.K, prod::BK, g.ldb) : make_map(&tb, g.B, g.in_dtype, g.K, g.N, 128, g.ldb)))
     return cudaErrorNotSupported;
-  const cudaError_t e = allow_smem<kernel>(prod::SMEM);
-  if (e != cudaSuccess) return e;
   prod::Params p{};
   p.d = reinterpret_cast<uint16_t *>(g.C);
   p.status = status;
@@ -253,7 +254,6 @@ cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.shares));
   cfg.blockDim = dim3(prod::THREADS);
-  cfg.dynamicSmemBytes = prod::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -263,7 +263,18 @@ cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  auto launch = [&](auto stages) {
+    constexpr auto kernel = gated_product_kernel<BF16, MN_MAJOR, FIRST, stages()>;
+    cfg.dynamicSmemBytes = prod::smem_bytes(stages());
+    const cudaError_t e = allow_smem<kernel>(prod::smem_bytes(stages()));
+    return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  };
+  // Twice the stages where a CTA walks many blocks with an SM to itself.  300 tokens of 1000 x 2720 (dX: 96 CTAs of 21
+  // blocks): backward 28.7 -> 25.0 us.  Not where dX would keep dW from most SMs: 128 tokens of 2048 x 5632 (128 CTAs)
+  // 53 -> 58 us.
+  if constexpr (FIRST)
+    if (p.shares > 1 && cfg.gridDim.x <= 2 * 148 / 3) return launch(std::integral_constant<int, prod::MANY>());
+  return launch(std::integral_constant<int, prod::FEW>());
 }
 
 } // namespace
@@ -315,7 +326,7 @@ cudaError_t launch_passes(const GatedProblem &p, unsigned *status, cudaStream_t 
   g.lda = 2 * l.d_ff, g.ldb = ldw, g.ldc = ld_dx;
   g.trans_a = false, g.trans_b = true;
   if (l.padded || small_product(g))
-    e = launch_product<gated_product_kernel<BF16, false, true>>(g, !l.padded, gated::eights(g.N), g.N, status, stream);
+    e = launch_product<BF16, false, true>(g, !l.padded, gated::eights(g.N), g.N, status, stream);
   else
     e = launch_gemm_tcgen05_2cta(g, status, stream);
   if (e != cudaSuccess) return e;
@@ -327,7 +338,7 @@ cudaError_t launch_passes(const GatedProblem &p, unsigned *status, cudaStream_t 
   g.lda = ldx, g.ldb = 2 * l.d_ff, g.ldc = ld_dw;
   g.trans_a = true, g.trans_b = false;
   if (l.padded || small_product(g))
-    e = launch_product<gated_product_kernel<BF16, true, false>>(g, !l.padded, l.d_ff, p.d_ff, status, stream);
+    e = launch_product<BF16, true, false>(g, !l.padded, l.d_ff, p.d_ff, status, stream);
   else
     e = launch_gemm_tcgen05_2cta(g, status, stream);
   if (e != cudaSuccess) return e;

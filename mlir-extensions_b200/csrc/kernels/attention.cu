@@ -895,6 +895,8 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
   if (!aligned(p.q) || !aligned(p.k) || !aligned(p.v) || !aligned(p.o) ||
       (backward && (!aligned(p.dout) || !aligned(p.dq) || !aligned(p.dk) || !aligned(p.dv))))
     return "arrays must be 16-byte aligned";
+  if (reinterpret_cast<uintptr_t>(p.lse) % 4 || reinterpret_cast<uintptr_t>(p.key_lens) % 4)
+    return "LSE and key_lens must start on a multiple of 4 bytes";
   if (attention_workspace_bytes(p, backward) && !aligned(p.workspace)) return "the workspace must be 16-byte aligned";
   return nullptr;
 }

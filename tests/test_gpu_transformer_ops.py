@@ -344,13 +344,15 @@ def test_attention_gradients_with_warps_out_of_step(pkg, d, kind):
             assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(first, got))
 
 
-@pytest.mark.parametrize("op,arg,message", [("attention", 0, "16-byte aligned"), ("attention", 3, "16-byte aligned"),
-                                            ("attention_bwd", 7, "16-byte aligned"), ("attention_bwd", -1, "the workspace must be")])
-def test_misaligned_arrays_are_refused(op, arg, message):
+@pytest.mark.parametrize("op,arg,by,message", [
+    ("attention", 0, 8, "16-byte aligned"), ("attention", 3, 8, "16-byte aligned"), ("attention", 4, 2, "multiple of 4 bytes"),
+    ("attention_bwd", 7, 8, "16-byte aligned"), ("attention_bwd", 5, 2, "multiple of 4 bytes"),
+    ("attention_bwd", -1, 8, "the workspace must be")])
+def test_misaligned_arrays_are_refused(op, arg, by, message):
     """Before anything is launched, by the error convention: one line on stdout, then abort()."""
     text = ("from __graft_entry__ import load_package\npkg = load_package()\nB = pkg.blob\ns = pkg.Session(device=0)\n"
             "k = s.kernel(B.%s('a', 1, 1, 1, 8, 8, 64))\nn = %d\np = [s.alloc(4096) for _ in range(n)]\n"
-            "p[%d] += 8\ns.launch(k, p)\n" % (op, 5 if op == "attention" else 10, arg))
+            "p[%d] += %d\ns.launch(k, p)\n" % (op, 5 if op == "attention" else 10, arg, by))
     r = subprocess.run([sys.executable, "-c", text], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == -6 and message in r.stdout, r.stdout + r.stderr
 

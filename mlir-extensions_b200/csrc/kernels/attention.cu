@@ -18,8 +18,9 @@
 //                tiles that share every K and V tile ("paired"), or, packed, both hold the one tile and take
 //                every other key block; they are merged at the end.
 //
-// When there are fewer tiles than SMs the key blocks of a tile are shared out between `splits` CTAs, which
-// leave O (unnormalised), m and l in the workspace; attention_join_kernel adds them up in order.
+// When there are fewer tiles than SMs, or packed ones leave the last round of CTAs nearly empty, the key blocks of a
+// tile are shared out between `splits` CTAs, which leave O (unnormalised), m and l in the workspace;
+// attention_join_kernel adds them up in order.
 //
 //   warp 0      TMA producer: Q, then K and V tiles through one ring in the order the products use them.
 //   warp 1      issues the products.  Per stream and block: wait for P, O += P V, S = Q K^T of the next

@@ -71,7 +71,7 @@ struct BwdParams {
   unsigned *status;
   Strides3 so, sdo, sdq, sdk, sdv;
   int q_heads, kv_heads, group, n_q, n_kv, causal, heads_batch, tiles;
-  int shares;  // CTAs (one cluster) among which a tile's blocks are shared out: 1, 2, 4 or 8
+  int shares;  // CTAs (one cluster) among which a tile's blocks are shared out: 1, 2 or 4
   float scale, scale_log2e;
   uint32_t idesc_s, idesc_o;
 };
@@ -437,7 +437,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(p.shares);
     uint16_t *dq = p.dq + b * p.sdq.batch + head * p.sdq.head + row0 * p.sdq.row;
-    add_up<DH, CT>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT, 4>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (row0 + row < p.n_q) store_unit<BF16>(dq + row * p.sdq.row + unit * 8, x, y, p.scale);
     });
     sums_barrier<CT>(p.shares);
@@ -659,10 +659,10 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     sums_barrier<CT>(p.shares);
     uint16_t *dv = p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row;
     uint16_t *dk = p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key0 * p.sdk.row;
-    add_up<DH, CT>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT, 4>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (key0 + row < p.n_kv) store_unit<BF16>(dv + row * p.sdv.row + unit * 8, x, y, 1.0f);
     });
-    add_up<DH, CT>(L.base + TILE * DH * 4, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT, 4>(L.base + TILE * DH * 4, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (key0 + row < p.n_kv) store_unit<BF16>(dk + row * p.sdk.row + unit * 8, x, y, p.scale);
     });
     sums_barrier<CT>(p.shares);

@@ -59,11 +59,12 @@ __device__ __forceinline__ void add_up_of(uint32_t sums, int rank, int thread, P
     if (u < UNITS) put(row, unit / 2, v[0][0], v[0][1]);
   }
 }
-template <int DH, int THREADS, typename Put>
+// MOST: the largest number of shares
+template <int DH, int THREADS, int MOST, typename Put>
 __device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, int thread, Put &&put) {
   if (shares == 1) add_up_of<DH, 1, THREADS>(sums, rank, thread, put);
   else if (shares == 2) add_up_of<DH, 2, THREADS>(sums, rank, thread, put);
-  else if (shares == 4) add_up_of<DH, 4, THREADS>(sums, rank, thread, put);
+  else if (MOST == 4 || shares == 4) add_up_of<DH, 4, THREADS>(sums, rank, thread, put);
   else add_up_of<DH, 8, THREADS>(sums, rank, thread, put);
 }
 // Eight sums times a factor as 16-bit values

@@ -151,7 +151,7 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       for (int i = max(0, n - STAGES); i < n; ++i)  // everything has been used
         if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1)) break;
       // this kernel's end then also stands for the end of the one it was started beside
-      if (!FIRST) asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (!FIRST && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
     }
   } else if (warp == 1) {
     const uint32_t leader = elect_one();

@@ -704,14 +704,16 @@ cudaError_t launch_shared(const BwdParams &f, int64_t tiles, cudaStream_t stream
   return cudaLaunchKernelEx(&cfg, kernel, maps..., f);
 }
 
-// CTAs a tile's `blocks` are shared out between: as many as fit on the GPU at once, at least `least` blocks each,
-// at most four (clusters of eight CTAs that fill their SMs wait long for a place); one doubling more for the
-// uneven tiles of the causal mask as long as the tiles alone do not fill the GPU.  dK / dV with 1 and 2 shares:
-// 128 tiles of up to 32 blocks (d_head 128) 109 and 99 us, 256 tiles of up to 128 blocks 474 and 497 us; 16 tiles of
-// up to 64 blocks with 1, 2, 4 and 8: 128, 84, 62 and 62 us.
-int share_count(int64_t tiles, int64_t blocks, int64_t slots, int least, bool uneven) {
+// CTAs a tile's `blocks` are shared out between, at least `least` blocks each and at most four (clusters of eight CTAs
+// that fill their SMs wait long for a place): until they are about as long as the part of `total`, the blocks of both
+// kernels, which run beside one another, that one of `slots` CTAs has; two shares sooner for the uneven tiles of the
+// causal mask.  Tiles longer than the other kernel's (shared key heads) come behind all of those, so they are cut finer.
+// 1024 x 1024, 8 heads of 64: 33 us with four shares, 23 with 2; 1000 x 1000 causal, 16 heads on 4 of 128: 47 us with two
+// shares of dQ, 37 with one; 1000 x 1000, 32 on 8 of 64: 70 us with two shares of dK / dV, 56 with 4; 8 of 512 x 512
+// causal, 32 on 4 of 64: 80 with 2, 90 with 4.
+int share_count(int64_t blocks, int64_t total, int64_t slots, int least, bool causal, bool longer) {
   int s = 1;
-  while (s < 4 && blocks >= least * 2 * s && (tiles * s * 2 <= slots || (uneven && s == 1 && tiles <= slots))) s *= 2;
+  while (s < 4 && blocks >= least * 2 * s && 10 * blocks * slots * (causal && s == 1 ? 2 : 1) > (longer ? 11 : 16) * total * s) s *= 2;
   return s;
 }
 
@@ -720,21 +722,22 @@ cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUte
                         BwdParams f, int64_t batch, cudaStream_t stream) {
   using Z = Sizes<DH>;
   const int64_t slots = 148 * Z::CTAS;
-  f.tiles = (f.n_q + TILE - 1) / TILE;
+  const int64_t tiles_q = (f.n_q + TILE - 1) / TILE, tiles_kv = (f.n_kv + TILE - 1) / TILE;
+  const int64_t blocks_kv = (f.n_kv + Z::BN - 1) / Z::BN, blocks_q = static_cast<int64_t>((f.n_q + Z::BN - 1) / Z::BN) * f.group;
+  const int64_t total = batch * (f.q_heads * tiles_q * blocks_kv + f.kv_heads * tiles_kv * blocks_q);
+  f.tiles = static_cast<int>(tiles_q);
   f.heads_batch = static_cast<int>(batch) * f.q_heads;
-  int64_t tiles = static_cast<int64_t>(f.tiles) * f.heads_batch;
-  f.shares = share_count(tiles, (f.n_kv + Z::BN - 1) / Z::BN, slots, DH == 64 ? 2 : 4, f.causal);
+  f.shares = share_count(blocks_kv, total, slots, DH == 64 ? 2 : 4, f.causal, false);
   const int64_t chunks = (f.n_q + 4 * DELTA_ROWS - 1) / (4 * DELTA_ROWS);
   attention_delta_kernel<BF16, DH><<<static_cast<unsigned>(chunks * f.heads_batch), 128, 0, stream>>>(f);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  e = launch_shared<attention_dq_kernel<BF16, DH>, DH>(f, tiles, stream, tq, tk, tv, tdo);
+  e = launch_shared<attention_dq_kernel<BF16, DH>, DH>(f, f.heads_batch * tiles_q, stream, tq, tk, tv, tdo);
   if (e != cudaSuccess) return e;
-  f.tiles = (f.n_kv + TILE - 1) / TILE;
+  f.tiles = static_cast<int>(tiles_kv);
   f.heads_batch = static_cast<int>(batch) * f.kv_heads;
-  tiles = static_cast<int64_t>(f.tiles) * f.heads_batch;
-  f.shares = share_count(tiles, static_cast<int64_t>((f.n_q + Z::BN - 1) / Z::BN) * f.group, slots, DH == 64 ? 2 : 4, f.causal);
-  return launch_shared<attention_dkv_kernel<BF16, DH>, DH>(f, tiles, stream, tq, tk, tv, tdo);
+  f.shares = share_count(blocks_q, total, slots, DH == 64 ? 2 : 4, f.causal, blocks_q > blocks_kv);
+  return launch_shared<attention_dkv_kernel<BF16, DH>, DH>(f, f.heads_batch * tiles_kv, stream, tq, tk, tv, tdo);
 }
 
 } // namespace

@@ -246,7 +246,7 @@ cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_
   const int64_t tiles = (g.M + 127) / 128 * p.tiles_n;
   // Shares of k: as many CTAs as run at once, at least twenty k blocks each (adding up costs about as much as eight).
   // dX of 300 tokens, k 5440 (24 tiles): backward 46 us with one share, 28 with 4, 30 with 8; of 512, k 2048 (32 tiles):
-  // 17 with one, 23 with 2.
+  // 17 with one, 23 with 2 (all with dW waiting for dX).
   p.shares = 1;
   while (p.shares < 8 && tiles * p.shares * 2 <= 2 * 148 && p.k_blocks >= 40 * p.shares) p.shares *= 2;
   const uint32_t fmt = g.in_dtype == kBF16 ? 1u : 0u;
@@ -269,11 +269,11 @@ cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_
     const cudaError_t e = allow_smem<kernel>(prod::smem_bytes(stages()));
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
   };
-  // Twice the stages where a CTA walks many blocks with an SM to itself.  300 tokens of 1000 x 2720 (dX: 96 CTAs of 21
-  // blocks): backward 28.7 -> 25.0 us.  Not where dX would keep dW from most SMs: 128 tokens of 2048 x 5632 (128 CTAs)
-  // 53 -> 58 us.
+  // Twice the stages where a CTA walks many blocks, in half of the SMs at the most (it takes all of an SM's shared memory
+  // and dW's CTAs run beside it).  128 tokens of 1024 x 4096 (dX: 32 CTAs of 32 blocks): backward 24.9 -> 20.8 us; 1000 of
+  // 512 x 1400 (64 CTAs): 20.8 -> 18.7; 300 of 1000 x 2720 (96): 23.0 -> 24.0; 128 of 2048 x 5632 (128): 44 -> 50.
   if constexpr (FIRST)
-    if (p.shares > 1 && cfg.gridDim.x <= 2 * 148 / 3) return launch(std::integral_constant<int, prod::MANY>());
+    if (p.shares > 1 && cfg.gridDim.x <= 148 / 2) return launch(std::integral_constant<int, prod::MANY>());
   return launch(std::integral_constant<int, prod::FEW>());
 }
 

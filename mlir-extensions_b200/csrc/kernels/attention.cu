@@ -269,11 +269,11 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         mbar_expect_tx(q_full, p.n_q * p.group * DH * 2);
         load_tile<DH>(q_smem(0), &tmap_q, 0, w.head * p.group, w.b, q_full);
       } else {
-        const int row0 = w.qt * 2 * TILE;
-        const bool second = row0 + TILE < p.n_q;
-        mbar_expect_tx(q_full, second ? 2 * TB : TB);
-        load_tile<DH>(q_smem(0), &tmap_q, row0, w.head, w.b, q_full);
-        if (second) load_tile<DH>(q_smem(1), &tmap_q, row0 + TILE, w.head, w.b, q_full);
+        // only of the streams that have blocks: the output of one without (under the causal mask the first rows of more
+        // queries than keys see none) takes the place of its Q at once, without a wait for it
+        mbar_expect_tx(q_full, (w.n[0] > 0 ? TB : 0) + (w.n[1] > 0 ? TB : 0));
+        for (int g = 0; g < 2; ++g)
+          if (w.n[g] > 0) load_tile<DH>(q_smem(g), &tmap_q, (w.qt * 2 + g) * TILE, w.head, w.b, q_full);
       }
       mbar_expect_tx(kv_full(0), TB);
       load_tile<DH>(kv_smem(0), &tmap_k, w.kb0 * TILE, PACKED ? w.head : w.head / p.group, w.b, kv_full(0));

@@ -3,20 +3,19 @@
 //   P = 2^(scale log2(e) Q K^T - log2(e) LSE)       dV = sum_group P^T dO
 //   dS = P (dO V^T - delta), delta = rowsum(dO O)   dQ = scale dS K,  dK = scale sum_group dS^T Q
 //
-// Two kernels, each with its accumulators in TMEM to the end, so that nothing is added up in memory: no
+// Two kinds of tiles, each with its accumulators in TMEM to the end, so that nothing is added up in memory: no
 // atomics, no f32 copy of dQ, and the same bits in every run.  The price is that Q K^T and dO V^T are
 // computed twice (7 products instead of 5).
 //
-//   attention_dq_kernel    a CTA owns 128 queries (Q, dO stay in shared memory) and walks the key blocks they
-//                          see.
-//   attention_dkv_kernel   a CTA owns 128 keys (K, V stay) and walks the query blocks that see them, of every
-//                          query head that shares the key head.  It works on the transposed products
-//                          S^T = K Q^T, dP^T = V dO^T (a thread's row is a key), so that P^T and dS^T are A
-//                          operands from TMEM and dO and Q are used as they lie.
+//   dq_tile    a CTA owns 128 queries (Q, dO stay in shared memory) and walks the key blocks they see.
+//   dkv_tile   a CTA owns 128 keys (K, V stay) and walks the query blocks that see them, of every query head
+//              that shares the key head.  It works on the transposed products S^T = K Q^T, dP^T = V dO^T (a
+//              thread's row is a key), so that P^T and dS^T are A operands from TMEM and dO and Q are used as
+//              they lie.
 //
-// attention_delta_kernel leaves -delta in the workspace before them.  So the two do not depend on one another, and
-// dK / dV's tiles fill the SMs that dQ's last round leaves idle (with delta computed by dQ's kernel, and so waited for:
-// padded batch of 64 84.7 us, now 80; 600 x 600, 8 heads of 128: 30 and 23).
+// attention_delta_kernel leaves -delta in the workspace, then one grid (attention_grads_kernel) has dQ's tiles in its
+// first CTAs and those of dK / dV, which do not depend on them, behind: they fill the SMs that dQ's last round leaves
+// idle.  That grid starts while the row sums are still computed; whoever reads them waits for their grid's end itself.
 //
 // The walked blocks are as long as the head is wide: 128 rows for d_head 128; 64 rows for d_head 64, where a CTA
 // then needs half of the TMEM and of the shared memory, so that two run on an SM and fill each other's waits.
@@ -74,8 +73,11 @@ struct BwdParams {
   const int32_t *key_lens;
   unsigned *status;
   Strides3 so, sdo, sdq, sdk, sdv;
-  int q_heads, kv_heads, group, n_q, n_kv, causal, heads_batch, tiles;
-  int shares;  // CTAs (one cluster) among which a tile's blocks are shared out: 1, 2 or 4
+  int batch, q_heads, kv_heads, group, n_q, n_kv, causal;
+  // CTAs among which the blocks of a tile of dQ, and of dK and dV, are shared out: 1, 2 or 4.  The larger is the size
+  // of all clusters of the grid.
+  int shares_q, shares_kv;
+  unsigned dq_ctas;  // the first CTAs, whole clusters
   float scale, scale_log2e;
   uint32_t idesc_s, idesc_o;
 };
@@ -259,6 +261,21 @@ template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_de
   }
 }
 
+// What a CTA does: share `rank` of the `shares` of tile `tile`, which are neighbours in a cluster from its CTA `first` on.
+struct Role {
+  int tile, rank, shares, first;
+  __device__ Role(unsigned cta, int of) : tile(cta / of), rank(cta % of), shares(of), first(0) {
+    if (shares > 1) first = static_cast<int>(cluster_ctarank()) - rank;
+  }
+};
+// CTAs that only fill the last cluster keep step with the two barriers of the others' sums.
+__device__ __forceinline__ void keep_step(int shares) {
+  if (shares > 1) {
+    cluster_sync_all();
+    cluster_sync_all();
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ dQ
 // TMEM, in units of BN columns: S [0,1), dP / dS of even and odd blocks [1,2) [2,3), dQ [3,4).  S is free for the next
 // block as soon as it has been read, dP has two places: the scores and products of block j + 1 run while the
@@ -266,22 +283,24 @@ template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_de
 // of another one, hence a barrier each for the dS of even and odd blocks; two ahead it cannot be, because the dP of
 // block j + 2 comes behind the product over all of dS j.
 template <bool BF16, int DH>
-__global__ void __launch_bounds__(Sizes<DH>::THREADS, Sizes<DH>::CTAS)
-attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
-                    const BwdParams p) {
+__device__ __forceinline__ void dq_tile(const CUtensorMap &tmap_q, const CUtensorMap &tmap_k, const CUtensorMap &tmap_v,
+                                        const CUtensorMap &tmap_do, const BwdParams &p, uint8_t *smem_raw) {
   using T = Layout<DH>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
   const T L(smem_u32(smem_raw));
   constexpr int BN = T::BN, CPT = T::CPT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
-  const int hb = tile % p.heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
-  const int qt = p.tiles - 1 - tile / p.heads_batch;  // under the causal mask the long tiles come first
+  const Role me(blockIdx.x, p.shares_q);
+  const int heads_batch = p.batch * p.q_heads, hb = me.tile % heads_batch, b = hb / p.q_heads, head = hb % p.q_heads;
+  // under the causal mask the long tiles come first
+  const int qt = (p.n_q + TILE - 1) / TILE - 1 - me.tile / heads_batch;
+  if (qt < 0) {
+    keep_step(me.shares);
+    return;
+  }
   const int row0 = qt * TILE;
   const int keys = key_count(p.key_lens, b, p.n_kv);
   const int n_all = (visible_keys(min(row0 + TILE, p.n_q) - 1, keys, p.n_q, p.n_kv, p.causal) + BN - 1) / BN;
-  const int first = share_of(n_all, rank, p.shares), n = share_of(n_all, rank + 1, p.shares) - first;  // key blocks
+  const int first = share_of(n_all, me.rank, me.shares), n = share_of(n_all, me.rank + 1, me.shares) - first;  // key blocks
 
   auto load_a = [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_k, (first + j) * BN, head / p.group, b, bar); };
   auto load_b = [&](int j, uint32_t dst, uint32_t bar) { load_tile<DH, BN>(dst, &tmap_v, (first + j) * BN, head / p.group, b, bar); };
@@ -358,10 +377,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (lane == 0 && !ok) report(p.status, kStatusMmaWaitTimeout);
     }
     __syncwarp();
-    if (p.shares > 1) {  // the computing warps' two barriers
-      cluster_sync_all();
-      cluster_sync_all();
-    }
+    keep_step(me.shares);  // the computing warps' two barriers
   } else {
     take_registers<DH>();
     const int part = (warp - 4) >> 2, lane_group = warp & 3;
@@ -369,9 +385,7 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const bool exists = i < p.n_q;
     const uint32_t lanes = static_cast<uint32_t>(lane_group * 32) << 16;
     float lse2 = INFINITY, neg_d = 0.0f;
-    // the row sums are complete; then the other kernel, which reads them too, may start beside this one
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the row sums are complete
     if (exists) {
       const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head) * p.n_q + i;
       const float lse = p.lse[row];
@@ -440,12 +454,12 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       leave_row<DH, COLS>(dq_tmem + lanes + part * COLS, n > 0, L.base, r, part * COLS);
     }
     constexpr int CT = T::THREADS - 128;
-    sums_barrier<CT>(p.shares);
+    sums_barrier<CT>(me.shares);
     uint16_t *dq = p.dq + b * p.sdq.batch + head * p.sdq.head + row0 * p.sdq.row;
-    add_up<DH, CT, 4>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT, 4>(L.base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (row0 + row < p.n_q) store_unit<BF16>(dq + row * p.sdq.row + unit * 8, x, y, p.scale);
     });
-    sums_barrier<CT>(p.shares);
+    sums_barrier<CT>(me.shares);
   }
 
   __syncwarp();
@@ -460,25 +474,28 @@ attention_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 // ------------------------------------------------------------------------------------------- dK and dV
 // TMEM, in units of BN columns: S^T / P^T, dP^T / dS^T, dV, dK
 template <bool BF16, int DH>
-__global__ void __launch_bounds__(Sizes<DH>::THREADS, Sizes<DH>::CTAS)
-attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                     const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
-                     const BwdParams p) {
+__device__ __forceinline__ void dkv_tile(const CUtensorMap &tmap_q, const CUtensorMap &tmap_k, const CUtensorMap &tmap_v,
+                                         const CUtensorMap &tmap_do, const BwdParams &p, uint8_t *smem_raw) {
   using T = Layout<DH>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
   const T L(smem_u32(smem_raw));
   constexpr int BN = T::BN, CPT = T::CPT;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
-  const int hb = tile % p.heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
-  const int key0 = tile / p.heads_batch * TILE;  // under the causal mask the first keys have the most queries
+  const Role me(blockIdx.x - p.dq_ctas, p.shares_kv);
+  const int heads_batch = p.batch * p.kv_heads, hb = me.tile % heads_batch, b = hb / p.kv_heads, kv_head = hb % p.kv_heads;
+  const int key_tile = me.tile / heads_batch;  // under the causal mask the first keys have the most queries
+  if (key_tile >= (p.n_kv + TILE - 1) / TILE) {
+    keep_step(me.shares);
+    return;
+  }
+  const int key0 = key_tile * TILE;
   const int keys = key_count(p.key_lens, b, p.n_kv);
   // query i sees key j from i = j - (n_kv - n_q) on
   const int shift = p.causal ? p.n_kv - p.n_q : 0;
   const int tiles_q = (p.n_q + BN - 1) / BN;
   const int first_tile = p.causal ? max(0, key0 - shift) / BN : 0;
   const int per_head = key0 < keys ? max(0, tiles_q - first_tile) : 0;
-  const int n_all = per_head * p.group, first = share_of(n_all, rank, p.shares), n = share_of(n_all, rank + 1, p.shares) - first;
+  const int n_all = per_head * p.group, first = share_of(n_all, me.rank, me.shares);
+  const int n = share_of(n_all, me.rank + 1, me.shares) - first;
   auto head_of = [&](int j) { return kv_head * p.group + (first + j) / per_head; };
   auto row_of = [&](int j) { return (first_tile + (first + j) % per_head) * BN; };
 
@@ -551,6 +568,7 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     } else if (warp == 2) {
       // row statistics of the query blocks: -log2(e) LSE and -delta.  Queries that do not exist or see no key
       // get -inf for the first, which makes their probabilities 2^-inf.
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the row sums are complete
       bool ok = true;
       for (int j = 0; j < n && ok; ++j) {
         const int64_t row = (static_cast<int64_t>(b) * p.q_heads + head_of(j)) * p.n_q;
@@ -574,14 +592,9 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         }
         mbar_arrive(L.bar(T::STAT_FULL + j % T::STAT_STAGES));
       }
-      // the end of this kernel then also stands for the end of the one it was started beside
-      if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
     }
     __syncwarp();
-    if (p.shares > 1) {  // the computing warps' two barriers
-      cluster_sync_all();
-      cluster_sync_all();
-    }
+    keep_step(me.shares);  // the computing warps' two barriers
   } else {
     take_registers<DH>();
     const int part = (warp - 4) >> 2, lane_group = warp & 3;
@@ -661,16 +674,16 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       }
     }
     constexpr int CT = T::THREADS - 128;
-    sums_barrier<CT>(p.shares);
+    sums_barrier<CT>(me.shares);
     uint16_t *dv = p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row;
     uint16_t *dk = p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key0 * p.sdk.row;
-    add_up<DH, CT, 4>(L.base, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT, 4>(L.base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (key0 + row < p.n_kv) store_unit<BF16>(dv + row * p.sdv.row + unit * 8, x, y, 1.0f);
     });
-    add_up<DH, CT, 4>(L.base + TILE * DH * 4, rank, p.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT, 4>(L.base + TILE * DH * 4, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (key0 + row < p.n_kv) store_unit<BF16>(dk + row * p.sdk.row + unit * 8, x, y, p.scale);
     });
-    sums_barrier<CT>(p.shares);
+    sums_barrier<CT>(me.shares);
   }
 
   __syncwarp();
@@ -682,35 +695,24 @@ attention_dkv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   }
 }
 
-// May start while the last CTAs of the kernel before it still run.
-template <auto kernel, int DH, typename... Maps>
-cudaError_t launch_shared(const BwdParams &f, int64_t tiles, cudaStream_t stream, const Maps &...maps) {
-  using Z = Sizes<DH>;
-  const cudaError_t e = allow_smem<kernel>(Z::SMEM, Registers<DH>::LAUNCH);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * f.shares));
-  cfg.blockDim = dim3(Z::THREADS);
-  cfg.dynamicSmemBytes = Z::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(f.shares);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, maps..., f);
+// The role is the same throughout a cluster: dq_ctas is a multiple of its size.
+template <bool BF16, int DH>
+__global__ void __launch_bounds__(Sizes<DH>::THREADS, Sizes<DH>::CTAS)
+attention_grads_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
+                       const __grid_constant__ BwdParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];  // swizzled tiles start on 1024 bytes
+  if (blockIdx.x < p.dq_ctas) dq_tile<BF16, DH>(tmap_q, tmap_k, tmap_v, tmap_do, p, smem_raw);
+  else dkv_tile<BF16, DH>(tmap_q, tmap_k, tmap_v, tmap_do, p, smem_raw);
 }
 
 // CTAs a tile's `blocks` are shared out between, at least `least` blocks each and at most four (clusters of eight CTAs
-// that fill their SMs wait long for a place): until they are about as long as the part of `total`, the blocks of both
-// kernels, which run beside one another, that one of `slots` CTAs has; two shares sooner for the uneven tiles of the
-// causal mask.  Tiles longer than the other kernel's (shared key heads) come behind all of those, so they are cut finer.
-// 1024 x 1024, 8 heads of 64: 33 us with four shares, 23 with 2; 1000 x 1000 causal, 16 heads on 4 of 128: 47 us with two
-// shares of dQ, 37 with one; 1000 x 1000, 32 on 8 of 64: 70 us with two shares of dK / dV, 56 with 4; 8 of 512 x 512
-// causal, 32 on 4 of 64: 80 with 2, 90 with 4.
+// that fill their SMs wait long for a place): until they are about as long as the part of `total`, the blocks of dQ and
+// of dK / dV, that one of `slots` CTAs has; two shares sooner for the uneven tiles of the causal mask.  Tiles longer than
+// the other kind's (shared key heads) come behind all of those, so they are cut finer.  Shares of dQ, dK / dV:
+// 1024 x 1024, 8 heads of 64: 32 us with 4, 4, 22.5 with 2, 2; 1000 x 1000 causal, 16 heads on 4 of 128: 49 us with 2, 4,
+// 37 with 1, 4; 1000 x 1000, 32 on 8 of 64: 63 us with 1, 2, 55 with 1, 4; 8 of 512 x 512 causal, 32 on 4 of 64: 86 with
+// 1, 2, 90 with 1, 4.
 int share_count(int64_t blocks, int64_t total, int64_t slots, int least, bool causal, bool longer) {
   int s = 1;
   while (s < 4 && blocks >= least * 2 * s && 10 * blocks * slots * (causal && s == 1 ? 2 : 1) > (longer ? 11 : 16) * total * s) s *= 2;
@@ -725,19 +727,34 @@ cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUte
   const int64_t tiles_q = (f.n_q + TILE - 1) / TILE, tiles_kv = (f.n_kv + TILE - 1) / TILE;
   const int64_t blocks_kv = (f.n_kv + Z::BN - 1) / Z::BN, blocks_q = static_cast<int64_t>((f.n_q + Z::BN - 1) / Z::BN) * f.group;
   const int64_t total = batch * (f.q_heads * tiles_q * blocks_kv + f.kv_heads * tiles_kv * blocks_q);
-  f.tiles = static_cast<int>(tiles_q);
-  f.heads_batch = static_cast<int>(batch) * f.q_heads;
-  f.shares = share_count(blocks_kv, total, slots, DH == 64 ? 2 : 4, f.causal, false);
+  f.shares_q = share_count(blocks_kv, total, slots, DH == 64 ? 2 : 4, f.causal, false);
+  f.shares_kv = share_count(blocks_q, total, slots, DH == 64 ? 2 : 4, f.causal, blocks_q > blocks_kv);
+  const int cluster = f.shares_q > f.shares_kv ? f.shares_q : f.shares_kv;
+  auto ctas = [&](int64_t tiles, int shares) { return (tiles * shares + cluster - 1) / cluster * cluster; };
+  const int64_t dq_ctas = ctas(batch * f.q_heads * tiles_q, f.shares_q);
+  f.dq_ctas = static_cast<unsigned>(dq_ctas);
+
   const int64_t chunks = (f.n_q + 4 * DELTA_ROWS - 1) / (4 * DELTA_ROWS);
-  attention_delta_kernel<BF16, DH><<<static_cast<unsigned>(chunks * f.heads_batch), 128, 0, stream>>>(f);
+  attention_delta_kernel<BF16, DH><<<static_cast<unsigned>(chunks * batch * f.q_heads), 128, 0, stream>>>(f);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  e = launch_shared<attention_dq_kernel<BF16, DH>, DH>(f, f.heads_batch * tiles_q, stream, tq, tk, tv, tdo);
+  // may start while the row sums are still computed
+  e = allow_smem<attention_grads_kernel<BF16, DH>>(Z::SMEM, Registers<DH>::LAUNCH);
   if (e != cudaSuccess) return e;
-  f.tiles = static_cast<int>(tiles_kv);
-  f.heads_batch = static_cast<int>(batch) * f.kv_heads;
-  f.shares = share_count(blocks_q, total, slots, DH == 64 ? 2 : 4, f.causal, blocks_q > blocks_kv);
-  return launch_shared<attention_dkv_kernel<BF16, DH>, DH>(f, f.heads_batch * tiles_kv, stream, tq, tk, tv, tdo);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(dq_ctas + ctas(batch * f.kv_heads * tiles_kv, f.shares_kv)));
+  cfg.blockDim = dim3(Z::THREADS);
+  cfg.dynamicSmemBytes = Z::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, attention_grads_kernel<BF16, DH>, tq, tk, tv, tdo, f);
 }
 
 } // namespace
@@ -762,6 +779,7 @@ cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cu
   f.key_lens = p.key_lens;
   f.status = status;
   f.so = p.so, f.sdo = p.sdo, f.sdq = p.sdq, f.sdk = p.sdk, f.sdv = p.sdv;
+  f.batch = static_cast<int>(p.batch);
   f.q_heads = static_cast<int>(p.q_heads);
   f.kv_heads = static_cast<int>(p.kv_heads);
   f.group = static_cast<int>(p.q_heads / p.kv_heads);
@@ -772,7 +790,7 @@ cudaError_t launch_attention_bwd(const AttentionProblem &p, unsigned *status, cu
   f.scale_log2e = p.scale * LOG2E;
   f.idesc_s = instruction_desc(bf16, false, static_cast<int>(p.d_head));  // BN is d_head
   f.idesc_o = instruction_desc(bf16, true, static_cast<int>(p.d_head));
-  *launched = 3;
+  *launched = 2;
   if (p.d_head == 64)
     return bf16 ? launch_both<true, 64>(tq, tk, tv, tdo, f, p.batch, stream)
                 : launch_both<false, 64>(tq, tk, tv, tdo, f, p.batch, stream);

@@ -190,7 +190,7 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       report(p.status, kStatusEpiWaitTimeout);
     }
     sums_barrier<128>(p.shares);
-    add_up<128, 128, 8>(base, rank, p.shares, threadIdx.x - 128, [&](int r, int unit, float4 x, float4 y) {
+    add_up<128, 128, 8>(base, 0, rank, p.shares, threadIdx.x - 128, [&](int r, int unit, float4 x, float4 y) {
       const int col = col0 + unit * 8;
       if (row0 + r >= p.rows || col >= p.cols) return;
       uint16_t *to = p.d + (row0 + r) * p.ldd;

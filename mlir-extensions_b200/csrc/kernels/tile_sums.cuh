@@ -28,10 +28,11 @@ __device__ __forceinline__ void leave_row(uint32_t taddr, bool has, uint32_t sum
                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
   }
 }
-// This CTA's part of the rows over all shares, in order: put(row of the tile, unit of eight columns, the eight sums),
-// neighbouring threads on neighbouring units.  `thread` of THREADS; the loads of two steps are in flight together.
+// This CTA's part (share `rank`) of the rows over all shares, in order, which are the cluster's CTAs from `first` on:
+// put(row of the tile, unit of eight columns, the eight sums), neighbouring threads on neighbouring units.  `thread` of
+// THREADS; the loads of two steps are in flight together.
 template <int DH, int S, int THREADS, typename Put>
-__device__ __forceinline__ void add_up_of(uint32_t sums, int rank, int thread, Put &&put) {
+__device__ __forceinline__ void add_up_of(uint32_t sums, int first, int rank, int thread, Put &&put) {
   constexpr int UNITS = TILE / S * (DH / 8), STEPS = (UNITS + THREADS - 1) / THREADS;
 #pragma unroll 2
   for (int k = 0; k < STEPS; ++k) {
@@ -45,7 +46,7 @@ __device__ __forceinline__ void add_up_of(uint32_t sums, int rank, int thread, P
         const uint32_t at = sums + sum_offset<DH>(u < UNITS ? row : 0, unit + h);
         asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                      : "=f"(v[r][h].x), "=f"(v[r][h].y), "=f"(v[r][h].z), "=f"(v[r][h].w)
-                     : "r"(S > 1 ? map_to_cta(at, r) : at));
+                     : "r"(S > 1 ? map_to_cta(at, first + r) : at));
       }
 #pragma unroll
     for (int r = 1; r < S; ++r)
@@ -61,11 +62,11 @@ __device__ __forceinline__ void add_up_of(uint32_t sums, int rank, int thread, P
 }
 // MOST: the largest number of shares
 template <int DH, int THREADS, int MOST, typename Put>
-__device__ __forceinline__ void add_up(uint32_t sums, int rank, int shares, int thread, Put &&put) {
-  if (shares == 1) add_up_of<DH, 1, THREADS>(sums, rank, thread, put);
-  else if (shares == 2) add_up_of<DH, 2, THREADS>(sums, rank, thread, put);
-  else if (MOST == 4 || shares == 4) add_up_of<DH, 4, THREADS>(sums, rank, thread, put);
-  else add_up_of<DH, 8, THREADS>(sums, rank, thread, put);
+__device__ __forceinline__ void add_up(uint32_t sums, int first, int rank, int shares, int thread, Put &&put) {
+  if (shares == 1) add_up_of<DH, 1, THREADS>(sums, first, rank, thread, put);
+  else if (shares == 2) add_up_of<DH, 2, THREADS>(sums, first, rank, thread, put);
+  else if (MOST == 4 || shares == 4) add_up_of<DH, 4, THREADS>(sums, first, rank, thread, put);
+  else add_up_of<DH, 8, THREADS>(sums, first, rank, thread, put);
 }
 // Eight sums times a factor as 16-bit values
 template <bool BF16> __device__ __forceinline__ void store_unit(uint16_t *to, float4 x, float4 y, float factor) {

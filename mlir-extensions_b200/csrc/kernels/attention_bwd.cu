@@ -261,21 +261,6 @@ template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_de
   }
 }
 
-// What a CTA does: share `rank` of the `shares` of tile `tile`, which are neighbours in a cluster from its CTA `first` on.
-struct Role {
-  int tile, rank, shares, first;
-  __device__ Role(unsigned cta, int of) : tile(cta / of), rank(cta % of), shares(of), first(0) {
-    if (shares > 1) first = static_cast<int>(cluster_ctarank()) - rank;
-  }
-};
-// CTAs that only fill the last cluster keep step with the two barriers of the others' sums.
-__device__ __forceinline__ void keep_step(int shares) {
-  if (shares > 1) {
-    cluster_sync_all();
-    cluster_sync_all();
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ dQ
 // TMEM, in units of BN columns: S [0,1), dP / dS of even and odd blocks [1,2) [2,3), dQ [3,4).  S is free for the next
 // block as soon as it has been read, dP has two places: the scores and products of block j + 1 run while the
@@ -456,7 +441,7 @@ __device__ __forceinline__ void dq_tile(const CUtensorMap &tmap_q, const CUtenso
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(me.shares);
     uint16_t *dq = p.dq + b * p.sdq.batch + head * p.sdq.head + row0 * p.sdq.row;
-    add_up<DH, CT, 4>(L.base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT>(L.base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (row0 + row < p.n_q) store_unit<BF16>(dq + row * p.sdq.row + unit * 8, x, y, p.scale);
     });
     sums_barrier<CT>(me.shares);
@@ -677,10 +662,10 @@ __device__ __forceinline__ void dkv_tile(const CUtensorMap &tmap_q, const CUtens
     sums_barrier<CT>(me.shares);
     uint16_t *dv = p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row;
     uint16_t *dk = p.dk + b * p.sdk.batch + kv_head * p.sdk.head + key0 * p.sdk.row;
-    add_up<DH, CT, 4>(L.base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT>(L.base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (key0 + row < p.n_kv) store_unit<BF16>(dv + row * p.sdv.row + unit * 8, x, y, 1.0f);
     });
-    add_up<DH, CT, 4>(L.base + TILE * DH * 4, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
+    add_up<DH, CT>(L.base + TILE * DH * 4, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int row, int unit, float4 x, float4 y) {
       if (key0 + row < p.n_kv) store_unit<BF16>(dk + row * p.sdk.row + unit * 8, x, y, p.scale);
     });
     sums_barrier<CT>(me.shares);

@@ -4,10 +4,8 @@
 // into the workspace, rounded once to the 16-bit type; because W holds both projections side by side,
 // dX = [dG dU] W^T and dW = X^T [dG dU] are then one product each.  Large ones go to the framework's CTA-pair GEMM;
 // small ones, and extents that are not multiples of eight, to gated_product_kernel: 128 x 128 tiles, two CTAs per SM, k
-// shared out between the CTAs of a cluster where there are few tiles.
+// shared out between the CTAs of a cluster where there are few tiles, both products in one grid.
 #include "gated_common.cuh"
-
-#include <type_traits>
 
 namespace imex {
 namespace {
@@ -72,39 +70,44 @@ namespace prod {
 constexpr int BK = 64;
 constexpr int TILE_BYTES = 128 * 128;          // 128 rows or columns x 64 k
 constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-constexpr int smem_bytes(int stages) { return stages * STAGE_BYTES + 256; }
+constexpr int STAGES = 3;
+constexpr int SMEM = STAGES * STAGE_BYTES + 256;
 constexpr int THREADS = 256;                   // TMA, products, two idle warps, four that hand the sums over
-constexpr int FEW = 3, MANY = 6;               // stages: two CTAs per SM, or one
-static_assert(128 * 128 * 4 <= FEW * STAGE_BYTES, "the sums take the ring's place");
-static_assert(2 * (smem_bytes(FEW) + 1024) <= 233472 && smem_bytes(MANY) + 1024 <= 233472, "two CTAs per SM, or one");
-struct Params {
+static_assert(128 * 128 * 4 <= STAGES * STAGE_BYTES, "the sums take the ring's place");
+static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+struct Product {
   uint16_t *d;
-  unsigned *status;
   long long ldd;
   int rows, cols, tiles_n, k_blocks, shares;
   int wide;        // results may be stored 16 bytes at a time
   int half, held;  // columns come in halves of `half`, of which `held` exist and are stored side by side
   uint32_t idesc;
 };
+struct Params {
+  Product of[2];      // dX, dW
+  unsigned dx_ctas;   // the first CTAs, whole clusters; clusters have the size of the larger number of shares
+  unsigned *status;
+};
 } // namespace prod
 
 // MN_MAJOR: A is stored [k, rows] and B [k, cols] (X^T dGU); else [rows, k] and [cols, k] (dGU W^T).
-// FIRST: dX's product, which may start while the kernel that writes dGU still runs and lets dW's start beside it once
-// that has ended.
-template <bool BF16, bool MN_MAJOR, bool FIRST, int STAGES>
-__global__ void __launch_bounds__(prod::THREADS, 2)
-gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const prod::Params p) {
+template <bool BF16, bool MN_MAJOR>
+__device__ __forceinline__ void product_tile(const CUtensorMap &tmap_a, const CUtensorMap &tmap_b, const prod::Product &p,
+                                             unsigned cta, unsigned *status, uint8_t *smem_raw) {
   using namespace prod;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw), bars = base + STAGES * STAGE_BYTES;
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
   const uint32_t done = bars + 8u * (2 * STAGES), slot = done + 8;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = p.shares > 1 ? static_cast<int>(cluster_ctarank()) : 0, tile = blockIdx.x / p.shares;
-  const int row0 = tile / p.tiles_n * 128, col0 = tile % p.tiles_n * 128;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.shares);
-  const int n = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / p.shares) - kb0;
+  const Role me(cta, p.shares);
+  const int row0 = me.tile / p.tiles_n * 128, col0 = me.tile % p.tiles_n * 128;
+  if (row0 >= p.rows) {
+    keep_step(me.shares);
+    return;
+  }
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * me.rank / me.shares);
+  const int n = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (me.rank + 1) / me.shares) - kb0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -125,15 +128,12 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem_raw + (slot - base));
 
   if (warp == 0) {
-    if (FIRST) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // dGU is complete
     if (lane == 0) {
       for (int i = 0; i < n; ++i) {
         const int s = i % STAGES, k = (kb0 + i) * BK;
         if (i >= STAGES && !mbar_wait(empty_bar(s), (i / STAGES - 1) & 1)) {
-          report(p.status, kStatusTmaWaitTimeout);
+          report(status, kStatusTmaWaitTimeout);
           break;
         }
         mbar_expect_tx(full_bar(s), STAGE_BYTES);
@@ -150,8 +150,6 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
       for (int i = max(0, n - STAGES); i < n; ++i)  // everything has been used
         if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1)) break;
-      // this kernel's end then also stands for the end of the one it was started beside
-      if (!FIRST && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
     }
   } else if (warp == 1) {
     const uint32_t leader = elect_one();
@@ -172,14 +170,11 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       commit(empty_bar(s), leader);
     }
     if (ok) commit(done, leader);
-    else if (lane == 0) report(p.status, kStatusMmaWaitTimeout);
+    else if (lane == 0) report(status, kStatusMmaWaitTimeout);
   }
   if (warp < 4) {
-    if (p.shares > 1) {  // the other warps' two barriers
-      __syncwarp();
-      cluster_sync_all();
-      cluster_sync_all();
-    }
+    __syncwarp();
+    keep_step(me.shares);  // the other warps' two barriers
   } else {
     const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0));
     if (ok) {
@@ -187,10 +182,10 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const int lane_group = warp & 3;
       leave_row<128, 128>(tmem + (static_cast<uint32_t>(lane_group * 32) << 16), true, base, lane_group * 32 + lane, 0);
     } else if (lane == 0) {
-      report(p.status, kStatusEpiWaitTimeout);
+      report(status, kStatusEpiWaitTimeout);
     }
-    sums_barrier<128>(p.shares);
-    add_up<128, 128, 8>(base, 0, rank, p.shares, threadIdx.x - 128, [&](int r, int unit, float4 x, float4 y) {
+    sums_barrier<128>(me.shares);
+    add_up<128, 128>(base, me.first, me.rank, me.shares, threadIdx.x - 128, [&](int r, int unit, float4 x, float4 y) {
       const int col = col0 + unit * 8;
       if (row0 + r >= p.rows || col >= p.cols) return;
       uint16_t *to = p.d + (row0 + r) * p.ldd;
@@ -205,7 +200,7 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         }
       }
     });
-    sums_barrier<128>(p.shares);
+    sums_barrier<128>(me.shares);
   }
   __syncwarp();
   tcgen05_fence_before();
@@ -216,65 +211,81 @@ gated_product_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   }
 }
 
+// The role is the same throughout a cluster: dx_ctas is a multiple of its size.
+template <bool BF16>
+__global__ void __launch_bounds__(prod::THREADS, 2)
+gated_product_kernel(const __grid_constant__ CUtensorMap dx_a, const __grid_constant__ CUtensorMap dx_b,
+                     const __grid_constant__ CUtensorMap dw_a, const __grid_constant__ CUtensorMap dw_b,
+                     const __grid_constant__ prod::Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  if (blockIdx.x < p.dx_ctas) product_tile<BF16, false>(dx_a, dx_b, p.of[0], blockIdx.x, p.status, smem_raw);
+  else product_tile<BF16, true>(dw_a, dw_b, p.of[1], blockIdx.x - p.dx_ctas, p.status, smem_raw);
+}
+
 // The pair GEMM's 256 x 256 tiles move half as much through shared memory per operation, but they need many tiles and
 // a long k to pay: 4096 tokens of 4096 x 11264 (256 and 1408 tiles, k 22528 and 4096): 1.20 ms, 1.38 and 1.57 with dX
-// or dW by the small kernel.  300 of 1000 x 2720: 58 us and 30; one of 4096 x 11264 (k of dW 1): 397 and 137; 2048 of
+// or dW by the small kernel.  300 of 1000 x 2720: 58 us and 23; one of 4096 x 11264 (k of dW 1): 397 and 131; 2048 of
 // 4096 x 4096 (512 tiles, k 2048): dW saves 40 of 300 us; 4096 of 2048 x 2048 (128 tiles, k 4096): the same.
 bool small_product(const GemmProblem &g) {
   const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
   return tiles <= 64 || g.K <= 2048 || (tiles <= 148 && g.K <= 4096);
 }
 
-template <bool BF16, bool MN_MAJOR, bool FIRST>
-cudaError_t launch_product(const GemmProblem &g, bool wide, int64_t half, int64_t held, unsigned *status, cudaStream_t stream) {
-  const bool mn = MN_MAJOR;
-  CUtensorMap ta, tb;
-  if (!(mn ? make_map(&ta, g.A, g.in_dtype, g.M, g.K, prod::BK, g.lda) : make_map(&ta, g.A, g.in_dtype, g.K, g.M, 128, g.lda)) ||
-      !(mn ? make_map(&tb, g.B, g.in_dtype, g.N, g.K, prod::BK, g.ldb) : make_map(&tb, g.B, g.in_dtype, g.K, g.N, 128, g.ldb)))
-    return cudaErrorNotSupported;
-  prod::Params p{};
-  p.d = reinterpret_cast<uint16_t *>(g.C);
-  p.status = status;
-  p.ldd = g.ldc;
-  p.rows = static_cast<int>(g.M);
-  p.cols = static_cast<int>(g.N);
-  p.wide = wide;
-  p.half = static_cast<int>(half);
-  p.held = static_cast<int>(held);
-  p.tiles_n = static_cast<int>((g.N + 127) / 128);
-  p.k_blocks = static_cast<int>((g.K + prod::BK - 1) / prod::BK);
-  const int64_t tiles = (g.M + 127) / 128 * p.tiles_n;
-  // Shares of k: as many CTAs as run at once, at least twenty k blocks each (adding up costs about as much as eight).
-  // dX of 300 tokens, k 5440 (24 tiles): backward 46 us with one share, 28 with 4, 30 with 8; of 512, k 2048 (32 tiles):
-  // 17 with one, 23 with 2 (all with dW waiting for dX).
-  p.shares = 1;
-  while (p.shares < 8 && tiles * p.shares * 2 <= 2 * 148 && p.k_blocks >= 40 * p.shares) p.shares *= 2;
+// Shares of k of a tile: as many CTAs as run at once, at least twenty k blocks each (adding up costs about as much as
+// eight), at most four (the clusters of both products have one size).  300 tokens of 1000 x 2720 (dX: 24 tiles, k 5440):
+// 28.7 us with two, 22.6 with 4; 128 of 2048 x 5632 (16 tiles, k 11264): 47 us with 8, 43 with 4; one of 4096 x 11264: 150
+// and 132; 300 of 640 x 8192 (15 tiles): 36 and 39.
+bool prepare_product(CUtensorMap *a, CUtensorMap *b, prod::Product *p, const GemmProblem &g, bool mn_major, bool wide,
+                     int64_t half, int64_t held) {
+  p->d = reinterpret_cast<uint16_t *>(g.C);
+  p->ldd = g.ldc;
+  p->rows = static_cast<int>(g.M);
+  p->cols = static_cast<int>(g.N);
+  p->wide = wide;
+  p->half = static_cast<int>(half);
+  p->held = static_cast<int>(held);
+  p->tiles_n = static_cast<int>((g.N + 127) / 128);
+  p->k_blocks = static_cast<int>((g.K + prod::BK - 1) / prod::BK);
+  const int64_t tiles = (g.M + 127) / 128 * p->tiles_n;
+  p->shares = 1;
+  while (p->shares < 4 && tiles * p->shares * 2 <= 2 * 148 && p->k_blocks >= 40 * p->shares) p->shares *= 2;
   const uint32_t fmt = g.in_dtype == kBF16 ? 1u : 0u;
-  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 3u << 15 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  p->idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn_major ? 3u << 15 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  return mn_major ? make_map(a, g.A, g.in_dtype, g.M, g.K, prod::BK, g.lda) && make_map(b, g.B, g.in_dtype, g.N, g.K, prod::BK, g.ldb)
+                  : make_map(a, g.A, g.in_dtype, g.K, g.M, 128, g.lda) && make_map(b, g.B, g.in_dtype, g.K, g.N, 128, g.ldb);
+}
+// The products that `dx` and `dw` ask for, in one grid: dW's CTAs, which do not depend on dX's, fill the places that those
+// leave.  after_grad: the grid may start while the kernel that writes dGU, the one before it in the stream, still runs.
+template <bool BF16>
+cudaError_t launch_products(const GemmProblem *dx, const GemmProblem *dw, bool wide, int64_t d_in, int64_t d_ff_wide, int64_t d_ff,
+                            bool after_grad, unsigned *status, cudaStream_t stream) {
+  CUtensorMap maps[4] = {};
+  prod::Params p{};
+  p.status = status;
+  p.of[0].shares = p.of[1].shares = 1;
+  if ((dx && !prepare_product(&maps[0], &maps[1], &p.of[0], *dx, false, wide, gated::eights(d_in), d_in)) ||
+      (dw && !prepare_product(&maps[2], &maps[3], &p.of[1], *dw, true, wide, d_ff_wide, d_ff)))
+    return cudaErrorNotSupported;
+  const int cluster = p.of[0].shares > p.of[1].shares ? p.of[0].shares : p.of[1].shares;
+  auto ctas = [&](const prod::Product &q) {
+    return ((q.rows + 127ll) / 128 * q.tiles_n * q.shares + cluster - 1) / cluster * cluster;
+  };
+  p.dx_ctas = static_cast<unsigned>(ctas(p.of[0]));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.shares));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas(p.of[0]) + ctas(p.of[1])));
   cfg.blockDim = dim3(prod::THREADS);
+  cfg.dynamicSmemBytes = prod::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.shares);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  auto launch = [&](auto stages) {
-    constexpr auto kernel = gated_product_kernel<BF16, MN_MAJOR, FIRST, stages()>;
-    cfg.dynamicSmemBytes = prod::smem_bytes(stages());
-    const cudaError_t e = allow_smem<kernel>(prod::smem_bytes(stages()));
-    return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
-  };
-  // Twice the stages where a CTA walks many blocks, in half of the SMs at the most (it takes all of an SM's shared memory
-  // and dW's CTAs run beside it).  128 tokens of 1024 x 4096 (dX: 32 CTAs of 32 blocks): backward 24.9 -> 20.8 us; 1000 of
-  // 512 x 1400 (64 CTAs): 20.8 -> 18.7; 300 of 1000 x 2720 (96): 23.0 -> 24.0; 128 of 2048 x 5632 (128): 44 -> 50.
-  if constexpr (FIRST)
-    if (p.shares > 1 && cfg.gridDim.x <= 148 / 2) return launch(std::integral_constant<int, prod::MANY>());
-  return launch(std::integral_constant<int, prod::FEW>());
+  cfg.numAttrs = after_grad ? 2 : 1;
+  const cudaError_t e = allow_smem<gated_product_kernel<BF16>>(prod::SMEM);
+  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, gated_product_kernel<BF16>, maps[0], maps[1], maps[2], maps[3], p);
 }
 
 } // namespace
@@ -312,37 +323,40 @@ cudaError_t launch_passes(const GatedProblem &p, unsigned *status, cudaStream_t 
   ++*launched;
 
   int n = 1;
-  GemmProblem g;
-  g.in_dtype = g.out_dtype = p.dtype;
-  g.epilogue = kEpiNone;
-  g.accumulate = false;
-  g.bias = nullptr;
-  g.workspace = ws + l.rest;
-  g.workspace_bytes = gemm_tcgen05_workspace_bytes();
-  g.launched = &n;
+  GemmProblem dx;
+  dx.in_dtype = dx.out_dtype = p.dtype;
+  dx.epilogue = kEpiNone;
+  dx.accumulate = false;
+  dx.bias = nullptr;
+  dx.workspace = ws + l.rest;
+  dx.workspace_bytes = gemm_tcgen05_workspace_bytes();
+  dx.launched = &n;
+  GemmProblem dw = dx;
   // dX[tokens, d_in] = dGU[tokens, 2 d_ff] . W^T, W stored [d_in, 2 d_ff]
-  g.A = dgu, g.B = w, g.C = static_cast<float *>(p.dx);
-  g.M = p.tokens, g.N = p.d_in, g.K = 2 * l.d_ff;
-  g.lda = 2 * l.d_ff, g.ldb = ldw, g.ldc = ld_dx;
-  g.trans_a = false, g.trans_b = true;
-  if (l.padded || small_product(g))
-    e = launch_product<BF16, false, true>(g, !l.padded, gated::eights(g.N), g.N, status, stream);
-  else
-    e = launch_gemm_tcgen05_2cta(g, status, stream);
-  if (e != cudaSuccess) return e;
-  *launched += n;
+  dx.A = dgu, dx.B = w, dx.C = static_cast<float *>(p.dx);
+  dx.M = p.tokens, dx.N = p.d_in, dx.K = 2 * l.d_ff;
+  dx.lda = 2 * l.d_ff, dx.ldb = ldw, dx.ldc = ld_dx;
+  dx.trans_a = false, dx.trans_b = true;
   // dW[d_in, 2 d_ff] = X^T . dGU, X stored [tokens, d_in]
-  n = 1;
-  g.A = x, g.B = dgu, g.C = static_cast<float *>(p.dw);
-  g.M = p.d_in, g.N = 2 * l.d_ff, g.K = p.tokens;
-  g.lda = ldx, g.ldb = 2 * l.d_ff, g.ldc = ld_dw;
-  g.trans_a = true, g.trans_b = false;
-  if (l.padded || small_product(g))
-    e = launch_product<BF16, true, false>(g, !l.padded, l.d_ff, p.d_ff, status, stream);
-  else
-    e = launch_gemm_tcgen05_2cta(g, status, stream);
-  if (e != cudaSuccess) return e;
-  *launched += n;
+  dw.A = x, dw.B = dgu, dw.C = static_cast<float *>(p.dw);
+  dw.M = p.d_in, dw.N = 2 * l.d_ff, dw.K = p.tokens;
+  dw.lda = ldx, dw.ldb = 2 * l.d_ff, dw.ldc = ld_dw;
+  dw.trans_a = true, dw.trans_b = false;
+  const bool small_dx = l.padded || small_product(dx), small_dw = l.padded || small_product(dw);
+  if (!small_dx) {
+    if ((e = launch_gemm_tcgen05_2cta(dx, status, stream)) != cudaSuccess) return e;
+    *launched += n;
+  }
+  if (small_dx || small_dw) {
+    e = launch_products<BF16>(small_dx ? &dx : nullptr, small_dw ? &dw : nullptr, !l.padded, p.d_in, l.d_ff, p.d_ff, small_dx, status, stream);
+    if (e != cudaSuccess) return e;
+    ++*launched;
+  }
+  if (!small_dw) {
+    n = 1;
+    if ((e = launch_gemm_tcgen05_2cta(dw, status, stream)) != cudaSuccess) return e;
+    *launched += n;
+  }
   return cudaSuccess;
 }
 } // namespace

@@ -7,6 +7,21 @@
 namespace imex {
 namespace attn {
 
+// What a CTA does: share `rank` of the `shares` of tile `tile`, which are neighbours in a cluster from its CTA `first` on.
+struct Role {
+  int tile, rank, shares, first;
+  __device__ Role(unsigned cta, int of) : tile(cta / of), rank(cta % of), shares(of), first(0) {
+    if (shares > 1) first = static_cast<int>(cluster_ctarank()) - rank;
+  }
+};
+// CTAs that only fill the last cluster keep step with the two barriers of the others' sums.
+__device__ __forceinline__ void keep_step(int shares) {
+  if (shares > 1) {
+    cluster_sync_all();
+    cluster_sync_all();
+  }
+}
+
 // f32 rows of DH values in shared memory, 16-byte units swizzled by the row
 template <int DH> __device__ __forceinline__ uint32_t sum_offset(int row, int unit) {
   return row * (DH * 4) + ((unit ^ (row & 7)) * 16);
@@ -60,13 +75,11 @@ __device__ __forceinline__ void add_up_of(uint32_t sums, int first, int rank, in
     if (u < UNITS) put(row, unit / 2, v[0][0], v[0][1]);
   }
 }
-// MOST: the largest number of shares
-template <int DH, int THREADS, int MOST, typename Put>
+template <int DH, int THREADS, typename Put>
 __device__ __forceinline__ void add_up(uint32_t sums, int first, int rank, int shares, int thread, Put &&put) {
   if (shares == 1) add_up_of<DH, 1, THREADS>(sums, first, rank, thread, put);
   else if (shares == 2) add_up_of<DH, 2, THREADS>(sums, first, rank, thread, put);
-  else if (MOST == 4 || shares == 4) add_up_of<DH, 4, THREADS>(sums, first, rank, thread, put);
-  else add_up_of<DH, 8, THREADS>(sums, first, rank, thread, put);
+  else add_up_of<DH, 4, THREADS>(sums, first, rank, thread, put);
 }
 // Eight sums times a factor as 16-bit values
 template <bool BF16> __device__ __forceinline__ void store_unit(uint16_t *to, float4 x, float4 y, float factor) {

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from __graft_entry__ import load_package
-from test_gpu_transformer_ops import Attention, Output, _bits, _dt
+from test_gpu_transformer_ops import HALF_STEP, TORCH, Attention, Output, _bits, _dt
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,87 @@ def test_attention_gradients_by_shares(pkg, sess, case, lens):
         sess.launch(kernel, args + [work])
         for x, n, t in zip(outs, first, (a.q, a.k, a.v)):
             assert torch.equal(a.back(x.get(-1), t.shape), first[n]), n
+
+
+# --------------------------------------------------------------------------------------- gated product
+class Gated:
+    """A problem on the GPU with rows behind one another or `pitch` elements further apart, exact results and tolerances
+    as in test_gpu_transformer_ops.py."""
+
+    def __init__(self, m, d, f, kind, pitch=0):
+        self.m, self.d, self.f, self.kind = m, d, f, kind
+        self.u = HALF_STEP[kind]
+        self.pitches = dict(ldx=d + pitch, ldw=2 * f + pitch, ldh=f + pitch) if pitch else {}
+        self.x, self.w, self.dh = self.new(m, d, 1, pitch), self.new(d, 2 * f, 2, pitch, d ** -0.5), self.new(m, f, 3, pitch)
+
+    def new(self, rows, cols, seed, pitch, std=1.0):
+        g = torch.Generator("cuda").manual_seed(seed)
+        return (torch.randn((rows, cols + pitch), generator=g, device="cuda") * std).to(TORCH[self.kind])[:, :cols]
+
+    def like(self, t):
+        """A result of t's shape and pitch, NaN, also between its rows."""
+        whole = torch.full((t.shape[0], t.stride(0)), float("nan"), dtype=t.dtype, device="cuda")
+        return whole, whole[:, :t.shape[1]]
+
+    def launches(self, pkg, desc, tensors, outs, times=1):
+        """The results of `times` launches, each with NaN in the workspace before it; the same bits each time."""
+        with pkg.Session(device=0, adopt_stream=1) as s:
+            kernel = s.kernel(desc)
+            need = s.workspace_bytes(kernel)
+            work = [torch.empty(need, dtype=torch.uint8, device="cuda")] if need else []
+            run = s.bind(kernel, [t.data_ptr() for t in tensors + [o[1] for o in outs] + work])
+            first = None
+            for _ in range(times):
+                for t in work + [o[0] for o in outs]:
+                    t.fill_(255 if t.dtype == torch.uint8 else float("nan"))
+                run()
+                got = [o[1].clone() for o in outs]
+                first = first or got
+                assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(first, got))
+            for whole, t in outs:
+                assert torch.isnan(whole[:, t.shape[1]:]).all(), "written between the rows"
+            s.wait()
+        return first
+
+    def forward(self, pkg, save=True, times=1):
+        outs = [self.like(self.dh)] + ([self.like(torch.empty((self.m, 2 * self.f), dtype=self.x.dtype, device="cuda"))] if save else [])
+        desc = pkg.blob.gated_ffn("g", self.m, self.d, self.f, _dt(pkg, self.kind), save_gu=save, **self.pitches)
+        got = self.launches(pkg, desc, [self.x, self.w], outs, times)
+        x, w, f = self.x.double(), self.w.double(), self.f
+        z = x @ w
+        acc = 2.0 ** -24 * (self.d + 8) * (x.abs() @ w.abs()) + 2.0 ** -25
+        a, up = torch.nn.functional.silu(z[:, :f]), z[:, f:]
+        want = a * up
+        tol = 1.1 * acc[:, :f] * (up.abs() + acc[:, f:]) + a.abs() * acc[:, f:] + (self.u + 4e-6) * want.abs() + 2.0 ** -25
+        assert ((got[0].double() - want).abs() <= tol * 1.01).all()
+        if save:
+            assert ((got[1].double() - z).abs() <= (acc + self.u * z.abs()) * 1.01).all()
+
+    def backward(self, pkg, times=3):
+        f, tiny = self.f, 2.0 ** -25
+        gu = (self.x.float() @ self.w.float()).to(TORCH[self.kind])
+        desc = pkg.blob.gated_ffn_bwd("gb", self.m, self.d, f, _dt(pkg, self.kind), **self.pitches)
+        dx, dw = self.launches(pkg, desc, [self.x, self.w, gu, self.dh], [self.like(self.x), self.like(self.w)], times)
+        z = gu.double().requires_grad_(True)
+        dz, = torch.autograd.grad(torch.nn.functional.silu(z[:, :f]) * z[:, f:], z, self.dh.double())
+        x, w = self.x.double(), self.w.double()
+        e = (self.u + 1e-5) * dz.abs() + tiny
+        for got, want, size, terms in ((dx, dz @ w.t(), e @ w.abs().t(), dz.abs() @ w.abs().t()),
+                                       (dw, x.t() @ dz, x.abs().t() @ e, x.abs().t() @ dz.abs())):
+            tol = size + self.u * want.abs() + 2.0 ** -24 * (max(self.m, 2 * f) + 8) * terms + tiny
+            assert ((got.double() - want).abs() <= tol * 1.01).all()
+
+
+@pytest.mark.parametrize("m,d,f,kind,pitch", [
+    (2048, 4096, 2064, "bf16", 0),   # dX by CTA pairs, then dW's small tiles
+    (2305, 1000, 4808, "f16", 0),    # dX by small tiles, then dW by CTA pairs
+    (2400, 2056, 2200, "bf16", 0),   # both by CTA pairs
+    (2400, 2056, 2200, "f16", 8),
+    (300, 1000, 2720, "f16", 0),     # both by small tiles in one grid, dX's k in four shares
+    (257, 520, 2600, "bf16", 0),     # fifteen tiles of dX
+    (150, 296, 1400, "bf16", 16),    # dX's k in two
+    (2600, 256, 104, "f16", 0),      # dW's k in two
+    (70, 4100, 30, "f16", 3),        # copied operands
+])
+def test_gated_gradients_by_products(pkg, m, d, f, kind, pitch):
+    Gated(m, d, f, kind, pitch).backward(pkg)

@@ -9,12 +9,11 @@
 #include "tcgen05_host.h"
 #include "tcgen05_ptx.cuh"
 
-#include <atomic>
-
 namespace imex {
 namespace attn {
 
 using namespace tc;
+using tc_host::allow_smem;
 
 constexpr int TILE = 128;              // rows of a query or key tile
 constexpr int BOX_BYTES = TILE * 128;  // 128 rows x 64 columns
@@ -200,26 +199,6 @@ inline bool make_map_4d(CUtensorMap *m, const void *base, int dtype, int64_t d, 
              const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Dynamic shared memory beyond 48 KB has to be asked for on every device a kernel runs on.
-// `kernel` is a template argument so that each has its own record of where that was done.  registers: what its
-// warpgroups hand over by setmaxnreg adds up to this many a thread, so it must have been built with them.
-template <auto kernel> cudaError_t allow_smem(int bytes, int registers = 0) {
-  static std::atomic<uint64_t> done{0};  // a bit per device
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && registers) {
-    cudaFuncAttributes built;
-    e = cudaFuncGetAttributes(&built, reinterpret_cast<const void *>(kernel));
-    if (e == cudaSuccess && built.numRegs != registers) e = cudaErrorInvalidKernelImage;
-  }
-  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-  return e;
 }
 
 } // namespace attn

@@ -40,7 +40,6 @@
 
 #include <cstdio>
 #include <cstdlib>
-#include <mutex>
 #include <string>
 
 namespace imex {
@@ -530,16 +529,9 @@ cudaError_t launch_flash_attention_fwd(const void *q, const void *k, const void 
                                        int64_t n_ctx, int64_t d_head, float sm_scale, int dtype,
                                        unsigned *status, cudaStream_t stream) {
   if (!flash_attention_supported(heads, n_ctx, d_head, dtype, q, k, v, o)) return cudaErrorNotSupported;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    cudaError_t a = cudaFuncSetAttribute(flash_attention_fwd_kernel<false>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    cudaError_t b = cudaFuncSetAttribute(flash_attention_fwd_kernel<true>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    attr_err = a != cudaSuccess ? a : b;
-  });
-  if (attr_err != cudaSuccess) return attr_err;
+  const cudaError_t smem_err = dtype == kBF16 ? allow_smem<flash_attention_fwd_kernel<true>>(SMEM_BYTES)
+                                              : allow_smem<flash_attention_fwd_kernel<false>>(SMEM_BYTES);
+  if (smem_err != cudaSuccess) return smem_err;
   // heads are a dimension of the tensor maps: a tile that runs past the last key (or query) of
   // its head is filled with zeros, not with the next head's first rows (whose values, were they
   // Inf or NaN, would reach this head's output through 0 x V)

@@ -36,7 +36,6 @@
 #include <cstdio>
 #include <cstdlib>
 #include <map>
-#include <mutex>
 #include <tuple>
 
 namespace imex {
@@ -289,13 +288,8 @@ bool gemm_tcgen05_supported(const GemmProblem &p) {
 
 cudaError_t launch_gemm_tcgen05(const GemmProblem &g, unsigned *status, cudaStream_t stream) {
   if (!gemm_tcgen05_supported(g)) return cudaErrorInvalidValue;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(gemm_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    SMEM_BYTES);
-  });
-  if (attr_err != cudaSuccess) return attr_err;
+  const cudaError_t smem_err = allow_smem<gemm_tcgen05_kernel>(SMEM_BYTES);
+  if (smem_err != cudaSuccess) return smem_err;
 
   CUtensorMap ta, tb;
   // cudaErrorNotSupported: the driver refused this shape for a tensor map; the

@@ -37,7 +37,7 @@
 
 #include <cstdio>
 #include <cstdlib>
-#include <mutex>
+#include <type_traits>
 
 namespace imex {
 namespace {
@@ -574,26 +574,9 @@ bool gemm_tcgen05_2cta_preferred(const GemmProblem &p) {
 
 cudaError_t launch_gemm_tcgen05_2cta(const GemmProblem &g, unsigned *status, cudaStream_t stream) {
   if (!gemm_tcgen05_2cta_supported(g)) return cudaErrorInvalidValue;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  static bool with_stats = false;
-  std::call_once(once, [] {
-    with_stats = getenv("IMEX_GEMM_STATS") != nullptr;
-    auto set = [](const void *fn, int bytes) {
-      return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    };
-    const cudaError_t e[] = {
-        set((const void *)gemm_tcgen05_2cta_kernel<3, 128, false, false, false>, smem_bytes(3, 128)),
-        set((const void *)gemm_tcgen05_2cta_kernel<3, 128, true, false, false>, smem_bytes(3, 128)),
-        set((const void *)gemm_tcgen05_2cta_kernel<3, 128, false, true, false>, smem_bytes(3, 128)),
-        set((const void *)gemm_tcgen05_2cta_kernel<3, 128, false, false, true>, smem_bytes(3, 128)),
-        set((const void *)gemm_tcgen05_2cta_kernel<3, 128, false, true, true>, smem_bytes(3, 128))};
-    for (cudaError_t x : e)
-      if (x != cudaSuccess && attr_err == cudaSuccess) attr_err = x;
-  });
+  static const bool with_stats = getenv("IMEX_GEMM_STATS") != nullptr;
   const bool transposed = g.trans_a || g.trans_b;
   const int BK = 128;  // 3 stages of 128 k (see the header of this file)
-  if (attr_err != cudaSuccess) return attr_err;
 
   const int64_t lda = g.lda > 0 ? g.lda : (g.trans_a ? g.M : g.K);
   const int64_t ldb = g.ldb > 0 ? g.ldb : (g.trans_b ? g.K : g.N);
@@ -673,16 +656,20 @@ cudaError_t launch_gemm_tcgen05_2cta(const GemmProblem &g, unsigned *status, cud
   const int clusters = p.num_items < max_clusters ? p.num_items : max_clusters;
   const dim3 grid(2 * clusters), block(NUM_THREADS);
   const int sm3 = smem_bytes(3, 128);
-  if (g.trans_a && g.trans_b)
-    gemm_tcgen05_2cta_kernel<3, 128, false, true, true><<<grid, block, sm3, stream>>>(ta, tb, tc_, tp, p);
-  else if (g.trans_a)
-    gemm_tcgen05_2cta_kernel<3, 128, false, true, false><<<grid, block, sm3, stream>>>(ta, tb, tc_, tp, p);
-  else if (g.trans_b)
-    gemm_tcgen05_2cta_kernel<3, 128, false, false, true><<<grid, block, sm3, stream>>>(ta, tb, tc_, tp, p);
-  else if (with_stats)
-    gemm_tcgen05_2cta_kernel<3, 128, true, false, false><<<grid, block, sm3, stream>>>(ta, tb, tc_, tp, p);
-  else
-    gemm_tcgen05_2cta_kernel<3, 128, false, false, false><<<grid, block, sm3, stream>>>(ta, tb, tc_, tp, p);
+  auto launch = [&](auto with, auto trans_a, auto trans_b) {
+    constexpr auto kernel = gemm_tcgen05_2cta_kernel<3, 128, with(), trans_a(), trans_b()>;
+    const cudaError_t e = allow_smem<kernel>(sm3);
+    if (e == cudaSuccess) kernel<<<grid, block, sm3, stream>>>(ta, tb, tc_, tp, p);
+    return e;
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  const cudaError_t smem_err = g.trans_a && g.trans_b ? launch(No(), Yes(), Yes())
+                               : g.trans_a            ? launch(No(), Yes(), No())
+                               : g.trans_b            ? launch(No(), No(), Yes())
+                               : with_stats           ? launch(Yes(), No(), No())
+                                                      : launch(No(), No(), No());
+  if (smem_err != cudaSuccess) return smem_err;
   if (p.split_tiles) {
     cudaError_t le = cudaGetLastError();
     if (le != cudaSuccess) return le;

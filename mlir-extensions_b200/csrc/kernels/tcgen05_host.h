@@ -1,10 +1,12 @@
-// Host helpers shared by the tcgen05 GEMM launchers: tensor-map encoding
-// through the driver entry point (no link-time dependency on libcuda) and the
-// SM count of the current device.
+// Host helpers shared by the tcgen05 launchers: tensor-map encoding through the
+// driver entry point (no link-time dependency on libcuda), the SM count of the
+// current device, and the request for dynamic shared memory.
 #pragma once
 #include "kernels.h"
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 namespace imex {
 namespace tc_host {
@@ -87,6 +89,25 @@ inline int sm_count() {
   return n;
 }
 
+// Dynamic shared memory beyond 48 KB has to be asked for on every device a kernel runs on.
+// `kernel` is a template argument so that each has its own record of where that was done.  registers: what its
+// warpgroups hand over by setmaxnreg adds up to this many a thread, so it must have been built with them.
+template <auto kernel> cudaError_t allow_smem(int bytes, int registers = 0) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && registers) {
+    cudaFuncAttributes built;
+    e = cudaFuncGetAttributes(&built, reinterpret_cast<const void *>(kernel));
+    if (e == cudaSuccess && built.numRegs != registers) e = cudaErrorInvalidKernelImage;
+  }
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 } // namespace tc_host
 } // namespace imex

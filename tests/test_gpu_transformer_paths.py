@@ -120,7 +120,7 @@ class Gated:
 
     def launches(self, pkg, desc, tensors, outs, times=1):
         """The results of `times` launches, each with NaN in the workspace before it; the same bits each time."""
-        with pkg.Session(device=0, adopt_stream=1) as s:
+        with pkg.Session(device=torch.cuda.current_device(), adopt_stream=1) as s:
             kernel = s.kernel(desc)
             need = s.workspace_bytes(kernel)
             work = [torch.empty(need, dtype=torch.uint8, device="cuda")] if need else []
@@ -180,3 +180,12 @@ class Gated:
 ])
 def test_gated_gradients_by_products(pkg, m, d, f, kind, pitch):
     Gated(m, d, f, kind, pitch).backward(pkg)
+
+
+def test_large_products_on_a_second_device(pkg):
+    """Sessions on two devices in one process: what a kernel needs is asked for on each."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one CUDA device")
+    for device in (0, 1):
+        with torch.cuda.device(device):
+            Gated(2400, 2056, 2200, "bf16").backward(pkg, times=1)

@@ -201,8 +201,9 @@ def attention(name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype=BF16, sm_
     Key j is visible to query i of batch b when j < key_lens[b] and, when causal, j <= i + n_kv - n_q
     (the last query sees every key).  O = softmax(sm_scale Q K^T) V over the visible keys, LSE = log of
     the sum of exponentials; a row that sees no key gets O = 0 and LSE = -inf.  Keys and values at and
-    behind key_lens[b] may hold anything, NaN included; elsewhere values must be finite (under the causal
-    mask a non-finite value of a later key of the same tile reaches earlier queries as 0 * inf).
+    behind key_lens[b] may hold anything, NaN included; elsewhere a NaN or infinite score makes the rows that see
+    it NaN, LSE included (and under the causal mask a non-finite V of a later key of the same tile reaches earlier
+    queries as 0 * inf).  P is rounded to the element type in between; sums stay in 32 bits.
     q_heads / kv_heads query heads share a key head.  sm_scale: 1 / sqrt(d_head) unless given.
     layout: "heads" for [batch, heads, rows, d] arrays, "tokens" for [batch, rows, heads, d];
     strides: {"q" | "k" | "v" | "o": (batch, head, row)} in elements overrides it per array."""

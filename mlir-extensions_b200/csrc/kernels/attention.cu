@@ -177,8 +177,10 @@ __device__ __forceinline__ float exponentials(const uint32_t (&s)[4][32], float 
   unpack_f32x2(add_f32x2(sum[0], sum[1]), lo, hi);
   return lo + hi;
 }
+// A row sees no key where the sum is 0; where a score is NaN or +inf it is NaN, and so are LSE and the row.
+__device__ __forceinline__ bool sees_any(float l) { return !(l == 0.0f); }
 __device__ __forceinline__ float row_lse(float m, float l) {
-  return l > 0.0f ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
+  return sees_any(l) ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
 }
 // Results go out through shared memory, where Q was: a thread puts its row there as 16-bit units of 16 bytes
 // (swizzled by the row), then the warp writes its 32 rows with neighbouring lanes on neighbouring units.
@@ -482,7 +484,7 @@ attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     } else {
       tcgen05_fence_after();
       const bool has0 = PACKED ? w.n[0] > 0 : n > 0, has1 = PACKED && w.n[1] > 0;
-      const bool some = l > 0.0f;
+      const bool some = sees_any(l);
       const float inv = p.splits > 1 ? 1.0f : (some ? 1.0f / l : 0.0f);
       a0 *= inv;
       a1 *= inv;
@@ -716,7 +718,7 @@ attention_solo_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_c
     } else {
       tcgen05_fence_after();
       const int64_t row = exists ? (static_cast<int64_t>(b) * p.q_heads + head_of(r)) * p.n_q + i : 0;
-      const bool some = l > 0.0f;
+      const bool some = sees_any(l);
       const float f = p.splits > 1 ? 1.0f : (some ? 1.0f / l : 0.0f);
       if (exists) {
         if (p.splits > 1) p.part_ml[split * p.rows + row] = make_float2(m, l);
@@ -790,7 +792,7 @@ template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_jo
         for (int c = 0; c < V; ++c) x[c] = fmaf(e[c], a, x[c]);
       }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = sees_any(l) ? 1.0f / l : 0.0f;
   const int i = static_cast<int>(row % p.n_q);
   const int64_t bh = row / p.n_q;
   uint16_t *to = p.o + (bh / p.q_heads) * p.so.batch + (bh % p.q_heads) * p.so.head + i * p.so.row + lane * V;

@@ -189,3 +189,44 @@ def test_large_products_on_a_second_device(pkg):
     for device in (0, 1):
         with torch.cuda.device(device):
             Gated(2400, 2056, 2200, "bf16").backward(pkg, times=1)
+
+
+# ----------------------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("q_heads,kv_heads,n_q,n_kv,d,causal", [
+    (2, 2, 140, 140, 64, True), (4, 2, 300, 300, 128, True), (2, 1, 3, 260, 64, False), (4, 1, 2, 515, 128, True),
+    (4, 1, 1, 3000, 128, False), (2, 1, 2, 2500, 64, True), (1, 1, 200, 2000, 128, True)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 1e38], ids=str)
+def test_scores_that_are_not_finite_make_their_rows_nan(pkg, sess, q_heads, kv_heads, n_q, n_kv, d, causal, bad):
+    """A NaN or infinite key, or one whose scores overflow (the sum of products leaves f32): O and LSE of the rows that
+    see it are NaN, the other rows are what they are without it.  A query of NaN: its row alone."""
+    a = Attention(1, q_heads, kv_heads, n_q, n_kv, d, "bf16", causal)
+    a.q[0, 0] = a.q[0, 0].abs() + 4.0
+    key = n_kv - n_q + n_q // 2 if causal else n_kv // 2
+    a.k[0, 0, key] = bad
+    row = n_q // 3
+    a.q[0, 1 % q_heads, row] = float("nan")
+    got = a.run(pkg, sess, backward=False)
+    sees = torch.arange(n_q) >= (key - (n_kv - n_q) if causal else 0)
+    nan = torch.zeros((q_heads, n_q), dtype=torch.bool)
+    nan[:q_heads // kv_heads] |= sees
+    if bad != bad or bad == float("inf"):
+        touched = nan.clone()
+    else:  # the overflow of the head whose queries are positive; the others' may cancel
+        touched = torch.zeros_like(nan)
+        touched[0] = nan[0]
+    touched[1 % q_heads, row] = True
+    nan[1 % q_heads, row] = True
+    assert torch.isnan(got["lse"][0][touched]).all() and torch.isnan(got["o"][0][touched]).all()
+    a.k[0, 0, key], a.q[0, 1 % q_heads, row] = 0.0, 0.0
+    ref, tol = a.exact()
+    off = (got["o"].double() - ref["o"]).abs()[0] / tol["o"][0]
+    assert (off[~nan] <= 1.0).all()
+    assert (got["lse"].double() - ref["lse"]).abs()[0][~nan].le(2e-5 + 1e-6 * ref["lse"][0][~nan].abs()).all()
+
+
+@pytest.mark.parametrize("d,n_q,n_kv", [(64, 140, 140), (128, 1, 2000)])
+def test_a_score_of_minus_infinity_has_no_weight(pkg, sess, d, n_q, n_kv):
+    a = Attention(1, 2, 1, n_q, n_kv, d, "bf16")
+    a.q = a.q.abs() + 1.0
+    a.k[0, 0, 7] = -3e38
+    a.check(a.run(pkg, sess, backward=False))

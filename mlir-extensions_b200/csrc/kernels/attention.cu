@@ -886,6 +886,7 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
     return "too many sequences, heads or rows";
   const Strides3 *s[8] = {&p.sq, &p.sk, &p.sv, &p.so, &p.sdo, &p.sdq, &p.sdk, &p.sdv};
   const bool of_keys[8] = {false, true, true, false, false, false, true, true};
+  const bool written[8] = {false, false, false, !backward, false, true, true, true};
   for (int i = 0; i < (backward ? 8 : 4); ++i) {
     const int64_t extent[3] = {p.batch, of_keys[i] ? p.kv_heads : p.q_heads, of_keys[i] ? p.n_kv : p.n_q};
     const int64_t step[3] = {s[i]->batch, s[i]->head, s[i]->row};
@@ -893,6 +894,8 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
       if (step[j] < 0 || step[j] % 8 || step[j] >= (1ll << 38)) return "strides are multiples of 8 elements, below 2^38";
       if (extent[j] > 1 && step[j] == 0) return "strides of extents above 1 are not zero";
     }
+    if (written[i] && rows_overlap(p.d_head, {{step[0], extent[0]}, {step[1], extent[1]}, {step[2], extent[2]}}))
+      return "the rows of an output overlap";
   }
   if (!pointers) return nullptr;
   if (!aligned(p.q) || !aligned(p.k) || !aligned(p.v) || !aligned(p.o) ||

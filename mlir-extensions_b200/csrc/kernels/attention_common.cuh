@@ -5,8 +5,23 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <cstdint>
+#include <utility>
+
 namespace imex {
 namespace attn {
+
+// Whether rows of `width` elements that N (stride, extent) pairs repeat may share elements.
+template <int N> bool rows_overlap(int64_t width, std::pair<int64_t, int64_t> (&&steps)[N]) {
+  std::sort(steps, steps + N);
+  for (const auto &s : steps) {
+    if (s.second <= 1) continue;
+    if (s.first < width) return true;
+    width = s.first > (INT64_MAX - width) / (s.second - 1) ? INT64_MAX : width + s.first * (s.second - 1);
+  }
+  return false;
+}
 
 // Both masks leave a row a prefix of the keys: j < min(key_lens[b], i + n_kv - n_q + 1).
 __device__ __forceinline__ int key_count(const int32_t *key_lens, int b, int n_kv) {

@@ -125,9 +125,10 @@ struct RotaryProblem {
   const void *x;
   const int32_t *positions;
   void *y;
-  const double *turns;  // host memory, rot_dims / 2
+  double turns[128];    // of the first rot_dims / 2
 };
-const char *rotary_check(const RotaryProblem &p);
+// nullptr, or why the problem is refused.  Pointers are looked at only when `pointers`.
+const char *rotary_check(const RotaryProblem &p, bool pointers);
 cudaError_t launch_rotary(const RotaryProblem &p, cudaStream_t stream);
 
 // One thread waits (bounded, ~1 ms) on a barrier nothing signals and reports

@@ -204,13 +204,15 @@ template <typename T> cudaError_t launch_typed(RotaryArgs &a, const RotaryProble
 
 } // namespace
 
-const char *rotary_check(const RotaryProblem &p) {
+const char *rotary_check(const RotaryProblem &p, bool pointers) {
   if (p.dtype != kF32 && p.dtype != kF16 && p.dtype != kBF16) return "the element type is f32, f16 or bf16";
   if (p.tokens < 1 || p.heads < 1 || p.d_head < 1) return "extents are at least 1";
   if (p.rot_dims < 2 || p.rot_dims % 2 || p.rot_dims > 256 || p.rot_dims > p.d_head)
     return "rot_dims is even, 2..256 and at most d_head";
   if (p.tokens > INT32_MAX || p.heads > 65535 || p.d_head > 512) return "at most 2^31 - 1 tokens, 65535 heads of 512 dimensions";
   if (p.x_token < 0 || p.x_head < 0 || p.y_token < 0 || p.y_head < 0) return "strides are not negative";
+  if (attn::rows_overlap(p.d_head, {{p.y_token, p.tokens}, {p.y_head, p.heads}})) return "the rows of Y overlap";
+  if (!pointers) return nullptr;
   const int64_t e = p.dtype == kF32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(p.x) % e || reinterpret_cast<uintptr_t>(p.y) % e ||
       reinterpret_cast<uintptr_t>(p.positions) % 4)

@@ -335,6 +335,22 @@ imex::GatedProblem gated_problem(const ImexKernelDesc &d) {
   return p;
 }
 
+imex::RotaryProblem rotary_problem(const ImexKernelDesc &d, const std::string *source) {
+  const ImexRotaryShape r = payload_as<ImexRotaryShape>(d, source);
+  if (d.in_dtype != d.out_dtype) refuse(d, "rotary positions keep the element type");
+  imex::RotaryProblem p{};
+  p.tokens = r.tokens, p.heads = r.heads, p.d_head = r.d_head, p.rot_dims = r.rot_dims;
+  p.x_token = r.x_token, p.x_head = r.x_head, p.y_token = r.y_token, p.y_head = r.y_head;
+  p.dtype = static_cast<int>(d.in_dtype);
+  p.interleaved = d.flags & IMEX_FLAG_INTERLEAVED;
+  p.inverse = d.flags & IMEX_FLAG_INVERSE;
+  p.factor = d.fparams[0];
+  static_assert(sizeof p.turns == sizeof r.turns, "turns per pair");
+  memcpy(p.turns, r.turns, sizeof p.turns);
+  refuse(d, imex::rotary_check(p, false));
+  return p;
+}
+
 size_t workspace_bytes(const ImexKernelDesc &d, const std::string *source) {
   switch (d.op) {
   case IMEX_OP_ATTENTION:
@@ -344,6 +360,9 @@ size_t workspace_bytes(const ImexKernelDesc &d, const std::string *source) {
     return imex::gated_workspace_bytes(gated_problem(d));
   case IMEX_OP_GATED_FFN_BWD:
     return imex::gated_bwd_workspace_bytes(gated_problem(d));
+  case IMEX_OP_ROTARY:
+    rotary_problem(d, source);
+    break;
   }
   return 0;
 }
@@ -589,18 +608,9 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
   }
   case IMEX_OP_ROTARY: {
     need(3);
-    const ImexRotaryShape r = payload_as<ImexRotaryShape>(d, source);
-    if (d.in_dtype != d.out_dtype) refuse(d, "rotary positions keep the element type");
-    imex::RotaryProblem p{};
-    p.tokens = r.tokens, p.heads = r.heads, p.d_head = r.d_head, p.rot_dims = r.rot_dims;
-    p.x_token = r.x_token, p.x_head = r.x_head, p.y_token = r.y_token, p.y_head = r.y_head;
-    p.dtype = static_cast<int>(d.in_dtype);
-    p.interleaved = d.flags & IMEX_FLAG_INTERLEAVED;
-    p.inverse = d.flags & IMEX_FLAG_INVERSE;
-    p.factor = d.fparams[0];
+    imex::RotaryProblem p = rotary_problem(d, source);
     p.x = ptrs[0], p.positions = static_cast<const int32_t *>(ptrs[1]), p.y = ptrs[2];
-    p.turns = r.turns;
-    refuse(d, imex::rotary_check(p));
+    refuse(d, imex::rotary_check(p, true));
     s->last_kernel = "rotary";
     err = imex::launch_rotary(p, s->stream);
     break;

@@ -1,6 +1,10 @@
 """Checks of the attention, gated feed-forward and rotary operators that need no GPU, beyond test_transformer_ops.py."""
 import glob
 import os
+import subprocess
+import sys
+
+import pytest
 
 from __graft_entry__ import ROOT, load_package
 
@@ -20,3 +24,35 @@ def test_dynamic_shared_memory_is_asked_for_on_every_device():
             owners.append(os.path.basename(path))
             assert "call_once" not in text, path
     assert owners == ["tcgen05_host.h"]
+
+
+@pytest.mark.parametrize("make,patch,message", [
+    # strides of dq, dk, dv and o are words 6 + 3 * (5, 6, 7, 3) of the payload: batch, head, row
+    ("B.attention('a', 2, 2, 1, 8, 8, 64)", "put(17, 56)", "the rows of an output overlap"),
+    ("B.attention('a', 2, 2, 1, 8, 8, 64)", "put(15, 512)", "the rows of an output overlap"),
+    ("B.attention_bwd('a', 2, 2, 1, 8, 8, 64)", "put(23, 8)", "the rows of an output overlap"),
+    ("B.attention_bwd('a', 2, 2, 1, 8, 8, 64)", "put(26, 32)", "the rows of an output overlap"),
+    ("B.attention_bwd('a', 2, 2, 1, 8, 8, 64)", "put(27, 64)", "the rows of an output overlap"),
+    ("B.attention_bwd('a', 2, 2, 1, 8, 8, 64)", "put(15, 512), put(17, 56)", None),   # O is only read
+    ("B.attention('a', 1, 2, 2, 1, 8, 64, layout='tokens')", "put(15, 0), put(17, 0)", None),  # of extents of 1
+    ("B.attention_bwd('a', 1, 1, 1, 1 << 30, 8, 64)", "put(21, 1 << 37), put(23, 1 << 37)", None),
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(6, 100)", "the rows of Y overlap"),
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(7, 63)", "the rows of Y overlap"),
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(7, 0)", "the rows of Y overlap"),
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(4, 0), put(5, 0)", None),                 # X may be broadcast
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(6, 64), put(7, 320)", None),              # heads outside
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(3, 5)", "rot_dims is even"),
+    ("B.rotary('a', 5, 2, 64, [1.0])", "put(2, 513)", "512 dimensions"),
+])
+def test_problems_the_builders_refuse_are_refused_by_the_library(make, patch, message):
+    """Descriptors of another program: the library makes the checks itself, before a launch."""
+    text = ("import struct\nfrom __graft_entry__ import load_package\npkg = load_package()\nB, rt = pkg.blob, pkg.runtime\n"
+            "d = %s\n"
+            "def put(word, value):\n    d.payload = d.payload[:8 * word] + struct.pack('<q', value) + d.payload[8 * word + 8:]\n"
+            "%s\nblob = B.Blob([d])\nk = rt.gpuKernelGet(None, rt.gpuModuleLoad(None, blob.address, blob.size), b'a')\n"
+            "rt.imexKernelWorkspaceBytes(k)\n" % (make, patch))
+    r = subprocess.run([sys.executable, "-c", text], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    if message is None:
+        assert r.returncode == 0, r.stdout + r.stderr
+    else:
+        assert r.returncode == -6 and message in r.stdout, r.stdout + r.stderr

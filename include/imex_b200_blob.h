@@ -106,6 +106,9 @@ extern "C" {
  *                   payload; fparams[0] = factor on the turned dimensions.  Pairs are
  *                   (i, i + rot_dims/2), or (2i, 2i + 1) with IMEX_FLAG_INTERLEAVED;
  *                   IMEX_FLAG_INVERSE turns the other way (the gradient).  Y may be X.
+ *   Outputs of the last five share no element with one another or with an input, except ATTENTION's
+ *   O with Q and ROTARY's Y with X (same address, same strides); ATTENTION_BWD's gradients may take
+ *   the place of O, and GATED_FFN_BWD's of GU and dH.
  *   FILL_UNIFORM    Y[n]  dims = {n, seed, first}; fparams = {lo, hi}
  *   FILL_NORMAL     Y[n]  dims = {n, seed, first}; fparams = {mean, stddev}
  */

@@ -206,7 +206,8 @@ def attention(name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype=BF16, sm_
     queries as 0 * inf).  P is rounded to the element type in between; sums stay in 32 bits.
     q_heads / kv_heads query heads share a key head.  sm_scale: 1 / sqrt(d_head) unless given.
     layout: "heads" for [batch, heads, rows, d] arrays, "tokens" for [batch, rows, heads, d];
-    strides: {"q" | "k" | "v" | "o": (batch, head, row)} in elements overrides it per array."""
+    strides: {"q" | "k" | "v" | "o": (batch, head, row)} in elements overrides it per array.  O may be Q (with the
+    same strides) and otherwise shares no element with an input."""
     return _attention(OP_ATTENTION, name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype, sm_scale, causal,
                       key_lens, layout, strides)
 
@@ -217,7 +218,8 @@ def attention_bwd(name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype=BF16,
     O, dO, LSE, dQ, dK, dV, then key_lens and the workspace as in `attention`.  Gradients of shared key
     heads are summed over their query heads; masked keys and rows that see no key get zeros.  P and
     dS = P (dO V^T - rowsum(dO O)) are rounded to the element type in between, so with F16 |dS| has to stay
-    below 65504.  The result does not change from run to run (no atomics).  strides also takes "do", "dq", "dk", "dv"."""
+    below 65504.  The result does not change from run to run (no atomics).  strides also takes "do", "dq", "dk", "dv".
+    The gradients share no element with Q, K, V, dO or one another."""
     return _attention(OP_ATTENTION_BWD, name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype, sm_scale, causal,
                       key_lens, layout, strides)
 
@@ -240,13 +242,15 @@ def gated_ffn(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, save_gu=False,
     the up projection's), H [tokens, d_ff], and with save_gu GU [tokens, 2 * d_ff] = X W for the backward
     pass, then the workspace when Session.workspace_bytes says so (extents or pitches that are not multiples
     of 8).  f32 accumulation; H and GU are rounded once.  ldx / ldw / ldh: row pitches in elements (0 = dense;
-    GU is dense).  Arrays start on 16-byte boundaries unless the extents need the workspace."""
+    GU is dense).  Arrays start on 16-byte boundaries unless the extents need the workspace.  H and GU share no element
+    with X, W or one another."""
     return _gated(OP_GATED_FFN, name, tokens, d_in, d_ff, dtype, act, FLAG_SAVE_GU if save_gu else 0, ldx, ldw, ldh)
 
 
 def gated_ffn_bwd(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, ldx=0, ldw=0, ldh=0):
     """The gradients of `gated_ffn` for dH.  Pointers X, W, GU (as the forward pass kept it), dH, dX, dW,
-    workspace (Session.workspace_bytes).  dX has X's shape and pitch, dW those of W, dH those of H."""
+    workspace (Session.workspace_bytes).  dX has X's shape and pitch, dW those of W, dH those of H.  dX
+    and dW share no element with X, W or one another."""
     return _gated(OP_GATED_FFN_BWD, name, tokens, d_in, d_ff, dtype, act, 0, ldx, ldw, ldh)
 
 
@@ -275,8 +279,8 @@ def rotary(name, tokens, heads, d_head, frequencies, dtype=BF16, interleaved=Fal
     2 * len(frequencies) dimensions of every head are turned in pairs by position * frequency (angles are
     reduced in 64 bits, so far positions keep their precision) and multiplied by `factor`; the others are
     copied.  Pairs are (i, i + n) of the n frequencies, or (2i, 2i + 1) when interleaved.  inverse turns
-    the other way: the gradient.  Y may be X.  x_strides / y_strides: (token, head) in elements, for
-    heads inside a packed projection."""
+    the other way: the gradient.  Y may be X (with the same strides) and otherwise
+    shares no element with it.  x_strides / y_strides: (token, head) in elements, for heads inside a packed projection."""
     freqs = [float(f) for f in frequencies]
     if min(tokens, heads, d_head) < 1:
         raise ValueError("rotary: extents are at least 1")

@@ -834,6 +834,7 @@ int split_count(const AttentionProblem &p) {
   return static_cast<int>(best);
 }
 
+bool same(const Strides3 &a, const Strides3 &b) { return a.batch == b.batch && a.head == b.head && a.row == b.row; }
 bool aligned(const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
 template <auto kernel>
@@ -904,6 +905,13 @@ const char *attention_check(const AttentionProblem &p, bool backward, bool point
   if (reinterpret_cast<uintptr_t>(p.lse) % 4 || reinterpret_cast<uintptr_t>(p.key_lens) % 4)
     return "LSE and key_lens must start on a multiple of 4 bytes";
   if (attention_workspace_bytes(p, backward) && !aligned(p.workspace)) return "the workspace must be 16-byte aligned";
+  // Arrays that start at one address share their first row at least.  A tile's O goes out after its Q has been read;
+  // everything else is read by tiles that may run later.
+  if (!backward && (p.o == p.k || p.o == p.v || (p.o == p.q && !same(p.so, p.sq)))) return "O may not be K or V, nor Q with other strides";
+  if (backward)
+    for (const void *d : {p.dq, p.dk, p.dv})
+      if (d == p.q || d == p.k || d == p.v || d == p.dout || (d == p.dq) + (d == p.dk) + (d == p.dv) > 1)
+        return "dQ, dK and dV may not be Q, K, V, dO or one another";
   return nullptr;
 }
 

@@ -538,6 +538,9 @@ const char *gated_check(const GatedProblem &p, bool backward, bool pointers) {
     if (reinterpret_cast<uintptr_t>(q) % unit)
       return padded ? "arrays must be aligned to their elements" : "arrays must be 16-byte aligned";
   if ((padded || backward) && reinterpret_cast<uintptr_t>(p.workspace) % 16) return "the workspace must be 16-byte aligned";
+  // arrays that start at one address: a tile's results go out while others still read X and W
+  if (!backward && (p.h == p.x || p.h == p.w || p.gu == p.x || p.gu == p.w || p.gu == p.h)) return "H and GU may not be X, W or one another";
+  if (backward && (p.dx == p.x || p.dx == p.w || p.dw == p.x || p.dw == p.w || p.dx == p.dw)) return "dX and dW may not be X, W or one another";
   return nullptr;
 }
 

@@ -217,6 +217,8 @@ const char *rotary_check(const RotaryProblem &p, bool pointers) {
   if (reinterpret_cast<uintptr_t>(p.x) % e || reinterpret_cast<uintptr_t>(p.y) % e ||
       reinterpret_cast<uintptr_t>(p.positions) % 4)
     return "arrays must start on a multiple of their element size";
+  if (p.x == p.y && ((p.tokens > 1 && p.x_token != p.y_token) || (p.heads > 1 && p.x_head != p.y_head)))
+    return "in place, X and Y have the same strides";
   return nullptr;
 }
 

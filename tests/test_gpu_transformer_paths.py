@@ -1,10 +1,13 @@
 """The ways through the attention and gated feed-forward kernels that only some shapes take, each against its formula in
 64 bits; the tolerances are those of test_gpu_transformer_ops.py."""
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
-from __graft_entry__ import load_package
+from __graft_entry__ import ROOT, load_package
 from test_gpu_transformer_ops import HALF_STEP, TORCH, Attention, Output, _bits, _dt
 
 pytestmark = pytest.mark.gpu
@@ -230,3 +233,71 @@ def test_a_score_of_minus_infinity_has_no_weight(pkg, sess, d, n_q, n_kv):
     a.q = a.q.abs() + 1.0
     a.k[0, 0, 7] = -3e38
     a.check(a.run(pkg, sess, backward=False))
+
+
+# ------------------------------------------------------------------------------------ arrays in one another's place
+def _refusals(cases):
+    """(builder call, number of pointers, what is done to them, message): refused before anything is launched, by one line
+    on stdout and abort().  A process each, side by side."""
+    runs = []
+    for make, n, patch, message in cases:
+        text = ("from __graft_entry__ import load_package\npkg = load_package()\nB = pkg.blob\ns = pkg.Session(device=0)\n"
+                "k = s.kernel(B.%s)\np = [s.alloc(1 << 16) for _ in range(%d)]\n%s\ns.launch(k, p)\n" % (make, n, patch))
+        runs.append((subprocess.Popen([sys.executable, "-c", text], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True),
+                     make, patch, message))
+    for process, make, patch, message in runs:
+        out, _ = process.communicate(timeout=300)
+        assert process.returncode == -6 and message in out, (make, patch, out)
+
+
+def test_outputs_in_the_place_of_inputs_are_refused():
+    """No value is looked at: all buffers are large enough for what would run."""
+    attention, wide = "attention('a', 2, 2, 2, 8, 8, 64%s)", ", strides={'o': (2048, 1024, 128)}"
+    back, grads = "attention_bwd('a', 1, 1, 1, 8, 8, 64)", "dQ, dK and dV may not be"
+    _refusals([
+        (attention % "", 5, "p[3] = p[1]", "O may not be K or V"),
+        (attention % "", 5, "p[3] = p[2]", "O may not be K or V"),
+        (attention % wide, 5, "p[3] = p[0]", "nor Q with other strides"),
+        (back, 10, "p[6] = p[0]", grads), (back, 10, "p[7] = p[4]", grads), (back, 10, "p[8] = p[2]", grads), (back, 10, "p[8] = p[7]", grads),
+        ("gated_ffn('a', 4, 16, 16)", 3, "p[2] = p[0]", "H and GU may not be"),
+        ("gated_ffn('a', 4, 16, 16, save_gu=True)", 4, "p[3] = p[2]", "H and GU may not be"),
+        ("gated_ffn_bwd('a', 4, 16, 16)", 7, "p[6] = s.alloc(s.workspace_bytes(k)); p[4] = p[0]", "dX and dW may not be"),
+        ("gated_ffn_bwd('a', 4, 16, 16)", 7, "p[6] = s.alloc(s.workspace_bytes(k)); p[5] = p[1]", "dX and dW may not be"),
+        ("rotary('a', 4, 2, 64, [1.0], x_strides=(192, 64))", 3, "p[2] = p[0]", "in place, X and Y have the same strides"),
+    ])
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,n_q,n_kv,d", [(4, 2, 300, 300, 64), (4, 2, 300, 300, 128), (4, 1, 1, 3000, 128), (2, 2, 200, 2000, 64)])
+def test_attention_output_in_the_place_of_q(pkg, sess, q_heads, kv_heads, n_q, n_kv, d):
+    a = Attention(1, q_heads, kv_heads, n_q, n_kv, d, "bf16", True)
+    want = a.run(pkg, sess, backward=False)
+    kernel = sess.kernel(pkg.blob.attention("in_place", *a.dims, causal=True))
+    q, k, v = (sess.upload(_bits(t)) for t in (a.q, a.k, a.v))
+    lse = Output(sess, q_heads * n_q, "f32")
+    need = sess.workspace_bytes(kernel)
+    sess.launch(kernel, [q, k, v, q, lse.ptr] + ([sess.alloc(need)] if need else []))
+    assert np.array_equal(sess.download(q, a.q.shape, np.int16), _bits(want["o"]))
+
+
+def test_gradients_in_the_place_of_what_is_read_before_them(pkg):
+    """The gated product's GU and dH, and attention's O, have been read when the gradients are written."""
+    a = Gated(300, 264, 264, "bf16")
+    gu = (a.x.float() @ a.w.float()).to(torch.bfloat16)
+    desc = pkg.blob.gated_ffn_bwd("gb", 300, 264, 264)
+    outs = [a.like(a.x), a.like(a.w)]
+    want = a.launches(pkg, desc, [a.x, a.w, gu, a.dh], outs)
+    with pkg.Session(device=0, adopt_stream=1) as s:
+        kernel = s.kernel(desc)
+        work, dh = torch.empty(s.workspace_bytes(kernel), dtype=torch.uint8, device="cuda"), a.dh.clone()
+        s.launch(kernel, [t.data_ptr() for t in (a.x, a.w, gu, dh, dh, outs[1][1], work)])
+    assert torch.equal(dh, want[0]) and torch.equal(outs[1][1], want[1])
+    t = lambda *shape: torch.randn(shape, device="cuda").to(torch.bfloat16)  # noqa: E731
+    q, k, v, o, do = (t(2, 4, 333, 128) for _ in range(5))
+    lse = torch.full((2, 4, 333), 6.0, device="cuda")
+    grads = [torch.empty_like(q) for _ in range(3)]
+    with pkg.Session(device=0, adopt_stream=1) as s:
+        kernel = s.kernel(pkg.blob.attention_bwd("b", 2, 4, 4, 333, 333, 128))
+        work = torch.empty(s.workspace_bytes(kernel), dtype=torch.uint8, device="cuda")
+        s.launch(kernel, [x.data_ptr() for x in [q, k, v, o, do, lse] + grads + [work]])
+        s.launch(kernel, [x.data_ptr() for x in [q, k, v, o, do, lse, o] + grads[1:] + [work]])
+    assert torch.equal(o, grads[0])

@@ -375,6 +375,13 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
                                ") needs " + std::to_string(n) + " pointer arguments, got " +
                                std::to_string(nptrs));
   };
+  // An operand more than an op with a workspace takes would shift another array into the workspace's place.
+  auto need_workspace = [&](size_t n) {
+    need(n);
+    if (nptrs > n)
+      throw std::runtime_error(std::string("gpuLaunchKernel: '") + d.name + "' (" + op_name(d.op) + ") takes " + std::to_string(n) +
+                               " pointer arguments, the last its workspace, got " + std::to_string(nptrs));
+  };
   const bool acc = d.flags & IMEX_FLAG_ACCUMULATE;
   cudaError_t err = cudaSuccess;
   int launches = 1;
@@ -567,7 +574,9 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
     imex::AttentionProblem p = attention_problem(d, source);
     const size_t ws = imex::attention_workspace_bytes(p, backward);
     size_t n = backward ? 9 : 5;
-    need(n + ((d.flags & IMEX_FLAG_KEY_LENS) ? 1 : 0) + (ws ? 1 : 0));
+    const size_t arrays = n + ((d.flags & IMEX_FLAG_KEY_LENS) ? 1 : 0);
+    if (ws) need_workspace(arrays + 1);
+    else need(arrays);
     p.q = ptrs[0], p.k = ptrs[1], p.v = ptrs[2], p.o = ptrs[3];
     if (backward) {
       p.dout = ptrs[4], p.lse = static_cast<float *>(ptrs[5]);
@@ -587,7 +596,8 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
     const bool save = d.flags & IMEX_FLAG_SAVE_GU;
     imex::GatedProblem p = gated_problem(d);
     const size_t n = save ? 4 : 3, ws = imex::gated_workspace_bytes(p);
-    need(n + (ws ? 1 : 0));
+    if (ws) need_workspace(n + 1);
+    else need(n);
     p.x = ptrs[0], p.w = ptrs[1], p.h = ptrs[2];
     if (save) p.gu = ptrs[3];
     if (ws) p.workspace = ptrs[n];
@@ -597,7 +607,7 @@ void enqueue(Stream *s, const ImexKernelDesc &d, void **ptrs, size_t nptrs, cons
     break;
   }
   case IMEX_OP_GATED_FFN_BWD: {
-    need(7);
+    need_workspace(7);
     imex::GatedProblem p = gated_problem(d);
     p.x = ptrs[0], p.w = ptrs[1], p.gu = ptrs[2], p.h = ptrs[3], p.dx = ptrs[4], p.dw = ptrs[5];
     p.workspace = ptrs[6];

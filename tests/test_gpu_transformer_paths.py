@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from __graft_entry__ import ROOT, load_package
-from test_gpu_transformer_ops import HALF_STEP, TORCH, Attention, Output, _bits, _dt
+from test_gpu_transformer_ops import HALF_STEP, SENTINEL, TORCH, Attention, Output, _bits, _dt
 
 pytestmark = pytest.mark.gpu
 
@@ -301,3 +301,29 @@ def test_gradients_in_the_place_of_what_is_read_before_them(pkg):
         s.launch(kernel, [x.data_ptr() for x in [q, k, v, o, do, lse] + grads + [work]])
         s.launch(kernel, [x.data_ptr() for x in [q, k, v, o, do, lse, o] + grads[1:] + [work]])
     assert torch.equal(o, grads[0])
+
+
+def test_missing_and_surplus_arrays_are_refused():
+    """A null is no array; one array too many would take the workspace's place."""
+    split, back = "attention('a', 1, 1, 1, 1, 3000, 64%s)", "attention_bwd('a', 1, 1, 1, 8, 8, 64%s)"
+    _refusals([
+        ("attention('a', 1, 1, 1, 8, 8, 64, key_lens=True)", 6, "p[5] = 0", "needs 6 pointer arguments, got 5"),
+        ("gated_ffn('a', 4, 16, 16, save_gu=True)", 4, "p[3] = 0", "needs 4 pointer arguments, got 3"),
+        (split % "", 6, "p[5] = 0", "needs 6 pointer arguments, got 5"),
+        (split % "", 7, "", "takes 6 pointer arguments, the last its workspace, got 7"),
+        (split % ", key_lens=True", 8, "", "takes 7 pointer arguments, the last its workspace, got 8"),
+        (back % "", 11, "", "takes 10 pointer arguments, the last its workspace, got 11"),
+        ("gated_ffn('a', 4, 15, 16)", 5, "", "takes 4 pointer arguments, the last its workspace, got 5"),
+        ("gated_ffn_bwd('a', 4, 16, 16)", 8, "", "takes 7 pointer arguments, the last its workspace, got 8"),
+        ("rotary('a', 4, 2, 64, [1.0])", 3, "p[1] = 0", "needs 3 pointer arguments, got 2"),
+    ])
+
+
+def test_a_workspace_where_none_is_needed_is_not_used(pkg, sess):
+    a = Attention(1, 2, 2, 20, 30, 64, "bf16")
+    kernel = sess.kernel(pkg.blob.attention("a", *a.dims))
+    assert sess.workspace_bytes(kernel) == 0
+    o, lse, spare = Output(sess, a.q.numel(), "bf16"), Output(sess, 40, "f32"), Output(sess, 64, "f32")
+    sess.launch(kernel, [sess.upload(_bits(t)) for t in (a.q, a.k, a.v)] + [o.ptr, lse.ptr, spare.ptr])
+    a.check({"o": o.get(a.q.shape), "lse": lse.get((1, 2, 20))})
+    assert (_bits(spare.get(-1)) == SENTINEL).all()

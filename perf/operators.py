@@ -161,10 +161,11 @@ _sessions = {}
 def _framework():
     from __graft_entry__ import load_package
     pkg = load_package()
-    stream = torch.cuda.current_stream().cuda_stream or 1  # 1: the handle of the legacy default stream
-    if stream not in _sessions:
-        _sessions[stream] = pkg.Session(device=torch.cuda.current_device(), adopt_stream=stream)
-    return pkg.blob, _sessions[stream]
+    # 1: the handle of the legacy default stream, which every device has
+    at = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream or 1
+    if at not in _sessions:
+        _sessions[at] = pkg.Session(device=at[0], adopt_stream=at[1])
+    return pkg.blob, _sessions[at]
 
 
 def _bind(s):

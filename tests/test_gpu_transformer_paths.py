@@ -327,3 +327,44 @@ def test_a_workspace_where_none_is_needed_is_not_used(pkg, sess):
     sess.launch(kernel, [sess.upload(_bits(t)) for t in (a.q, a.k, a.v)] + [o.ptr, lse.ptr, spare.ptr])
     a.check({"o": o.get(a.q.shape), "lse": lse.get((1, 2, 20))})
     assert (_bits(spare.get(-1)) == SENTINEL).all()
+
+
+# -------------------------------------------------------------------------- keys shared out between CTAs, and joined
+SPLIT = [
+    # batch, q_heads, kv_heads, n_q, n_kv, d, kind, causal, lens, layout
+    (4, 4, 2, 1, 3000, 64, "bf16", False, [3000, 0, 1, 300], "heads"),        # six shares, most of them empty
+    (4, 4, 2, 1, 3000, 128, "f16", True, [3000, 0, 1, 300], "tokens"),
+    (3, 8, 1, 5, 2600, 64, "f16", True, [2600, 130, 1999], "tokens"),         # the last key inside a later share's block
+    (3, 8, 1, 5, 2600, 128, "bf16", False, [2600, 130, 1999], "heads"),
+    (1, 1, 1, 1, 33000, 64, "bf16", False, None, "heads"),                    # 52 shares
+    (1, 2, 1, 1, 33000, 128, "bf16", True, None, "heads"),
+    (2, 1, 1, 1, 33000, 128, "f16", False, [31111, 5], "heads"),
+    (1, 2, 2, 300, 2000, 64, "bf16", True, None, "heads"),                    # a tile per 128 queries
+    (1, 2, 2, 300, 2000, 128, "f16", True, None, "tokens"),
+    (2, 3, 1, 140, 1800, 128, "bf16", False, [1800, 500], "tokens"),
+    (2, 3, 1, 140, 1800, 64, "f16", True, [0, 1733], "heads"),
+    (1, 1, 1, 700, 5000, 128, "bf16", True, None, "heads"),                   # ten shares of pairs that end unequally
+    (1, 1, 1, 3000, 2600, 128, "bf16", True, None, "heads"),                  # the first queries see no key
+]
+
+
+@pytest.mark.parametrize("case", SPLIT, ids=lambda c: "-".join(str(x) for x in c).replace(" ", ""))
+def test_attention_with_keys_shared_out(pkg, sess, case):
+    a = Attention(*case)
+    if a.lens is not None:
+        a.poison_padding()
+    desc = pkg.blob.attention("a", *a.dims, dtype=_dt(pkg, a.kind), causal=a.causal, key_lens=a.lens is not None, layout=a.layout)
+    assert sess.workspace_bytes(sess.kernel(desc)) > 0, "one share"
+    a.check(a.run(pkg, sess))
+
+
+@pytest.mark.parametrize("m,d,f,kind,pitch", [
+    (2100, 136, 2824, "bf16", 0),    # 207 tiles on 74 pairs of CTAs, two k blocks
+    (4200, 264, 2824, "f16", 0),     # 391 tiles, three bands of row blocks, three k blocks
+    (5000, 8, 1160, "bf16", 0),      # one k block
+    (2600, 1000, 2000, "bf16", 8),   # rows with a pitch
+    (2500, 2051, 1301, "f16", 0),    # copied operands, results stored value by value
+])
+@pytest.mark.parametrize("save", [False, True], ids=["", "kept"])
+def test_gated_pairs_of_ctas_walk_several_tiles(pkg, m, d, f, kind, pitch, save):
+    Gated(m, d, f, kind, pitch).forward(pkg, save, times=3)

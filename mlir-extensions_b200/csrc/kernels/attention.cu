@@ -804,8 +804,6 @@ template <bool BF16, int DH> __global__ void __launch_bounds__(128) attention_jo
   if (lane == 0) p.lse[row] = row_lse(m, l);
 }
 
-constexpr int SMS = 148;
-
 bool is_packed(const AttentionProblem &p) { return p.n_q * (p.q_heads / p.kv_heads) <= TILE; }
 int64_t tiles_per_head(const AttentionProblem &p) {
   if (is_packed(p)) return 1;
@@ -823,7 +821,7 @@ int64_t tile_count(const AttentionProblem &p) {
 // one, 39 with 3.  Tiles that are not packed are split only to fill one round: a share leaves 128 KB in the workspace.
 int split_count(const AttentionProblem &p) {
   const int64_t blocks = (p.n_kv + TILE - 1) / TILE, tiles = tile_count(p);
-  const int64_t slots = p.d_head == 64 ? 2 * SMS : SMS, ends = p.d_head == 64 ? 4 : 7;
+  const int64_t slots = (p.d_head == 64 ? 2 : 1) * tc_host::sm_count(), ends = p.d_head == 64 ? 4 : 7;
   if (blocks < 12 || (tiles >= slots && !is_packed(p))) return 1;
   int64_t best = 1, best_cost = INT64_MAX;
   for (int64_t s = 1; s <= 64 && s <= blocks / 4; ++s) {

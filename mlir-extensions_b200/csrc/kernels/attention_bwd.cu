@@ -708,7 +708,7 @@ template <bool BF16, int DH>
 cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tdo,
                         BwdParams f, int64_t batch, cudaStream_t stream) {
   using Z = Sizes<DH>;
-  const int64_t slots = 148 * Z::CTAS;
+  const int64_t slots = tc_host::sm_count() * Z::CTAS;
   const int64_t tiles_q = (f.n_q + TILE - 1) / TILE, tiles_kv = (f.n_kv + TILE - 1) / TILE;
   const int64_t blocks_kv = (f.n_kv + Z::BN - 1) / Z::BN, blocks_q = static_cast<int64_t>((f.n_q + Z::BN - 1) / Z::BN) * f.group;
   const int64_t total = batch * (f.q_heads * tiles_q * blocks_kv + f.kv_heads * tiles_kv * blocks_q);

@@ -228,7 +228,7 @@ gated_product_kernel(const __grid_constant__ CUtensorMap dx_a, const __grid_cons
 // 4096 x 4096 (512 tiles, k 2048): dW saves 40 of 300 us; 4096 of 2048 x 2048 (128 tiles, k 4096): the same.
 bool small_product(const GemmProblem &g) {
   const int64_t tiles = ((g.M + 255) / 256) * ((g.N + 255) / 256);
-  return tiles <= 64 || g.K <= 2048 || (tiles <= 148 && g.K <= 4096);
+  return tiles <= 64 || g.K <= 2048 || (tiles <= sm_count() && g.K <= 4096);
 }
 
 // Shares of k of a tile: as many CTAs as run at once, at least twenty k blocks each (adding up costs about as much as
@@ -248,7 +248,7 @@ bool prepare_product(CUtensorMap *a, CUtensorMap *b, prod::Product *p, const Gem
   p->k_blocks = static_cast<int>((g.K + prod::BK - 1) / prod::BK);
   const int64_t tiles = (g.M + 127) / 128 * p->tiles_n;
   p->shares = 1;
-  while (p->shares < 4 && tiles * p->shares * 2 <= 2 * 148 && p->k_blocks >= 40 * p->shares) p->shares *= 2;
+  while (p->shares < 4 && tiles * p->shares * 2 <= 2 * sm_count() && p->k_blocks >= 40 * p->shares) p->shares *= 2;
   const uint32_t fmt = g.in_dtype == kBF16 ? 1u : 0u;
   p->idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn_major ? 3u << 15 : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
   return mn_major ? make_map(a, g.A, g.in_dtype, g.M, g.K, prod::BK, g.lda) && make_map(b, g.B, g.in_dtype, g.N, g.K, prod::BK, g.ldb)
@@ -315,7 +315,7 @@ cudaError_t launch_passes(const GatedProblem &p, unsigned *status, cudaStream_t 
   }
   const GradArgs a{static_cast<const uint16_t *>(p.gu), static_cast<const uint16_t *>(p.h), dgu, ldh, p.tokens, p.d_ff, l.d_ff, p.act};
   const int64_t items = p.tokens * (l.padded ? l.d_ff : l.d_ff / 8);
-  const int64_t most = 148 * 8 * 4;  // resident blocks, four rounds each at the most
+  const int64_t most = sm_count() * 8 * 4;  // resident blocks, four rounds each at the most
   const unsigned blocks = static_cast<unsigned>((items + 255) / 256 < most ? (items + 255) / 256 : most);
   if (l.padded) gated_grad_kernel<BF16, 1><<<blocks, 256, 0, stream>>>(a);
   else gated_grad_kernel<BF16, 8><<<blocks, 256, 0, stream>>>(a);

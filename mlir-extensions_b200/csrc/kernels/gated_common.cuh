@@ -43,7 +43,7 @@ gated_pad_kernel(const uint16_t *from, int64_t ld, uint16_t *to, int64_t rows, i
 }
 inline cudaError_t launch_pad(const void *from, int64_t ld, void *to, int64_t rows, int64_t cols, int64_t wide, int segments,
                               cudaStream_t stream) {
-  const int64_t blocks = (rows * segments * wide / 8 + 255) / 256, most = 148 * 8 * 4;
+  const int64_t blocks = (rows * segments * wide / 8 + 255) / 256, most = tc_host::sm_count() * 8 * 4;
   gated_pad_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(
       static_cast<const uint16_t *>(from), ld, static_cast<uint16_t *>(to), rows, cols, wide, segments);
   return cudaGetLastError();

@@ -607,7 +607,7 @@ cudaError_t launch_few_tokens(const GatedProblem &p, const Prepared &q, unsigned
   const int64_t tiles = (p.d_ff + few::BF - 1) / few::BF;
   // Shares of k per tile: as many CTAs as run at once, at least two k blocks each.  One token of 4096 x 11264
   // (176 tiles): 31.5 us with one share, 38 with 2; of 8192 x 1024 (16 tiles): 35 us with one, 10.3 with 8.
-  int64_t shares = 2 * 148 / tiles;
+  int64_t shares = 2 * sm_count() / tiles;
   if (shares > 8) shares = 8;
   if (shares > f.k_blocks / 2) shares = f.k_blocks / 2;
   f.shares = shares < 1 ? 1 : static_cast<int>(shares);
@@ -633,7 +633,7 @@ cudaError_t launch_tiles(const GatedProblem &p, const Prepared &q, unsigned *sta
   const int64_t count = (p.tokens + 127) / 128 * f.tiles_f;
   // Shares of k: as many CTAs as run at once, at least twenty k blocks each (adding up costs about as much as eight).
   f.shares = 1;
-  while (f.shares < 8 && count * f.shares * 2 <= 2 * 148 && f.k_blocks >= 40 * f.shares) f.shares *= 2;
+  while (f.shares < 8 && count * f.shares * 2 <= 2 * sm_count() && f.k_blocks >= 40 * f.shares) f.shares *= 2;
   const uint32_t fmt = BF16 ? 1u : 0u;
   // f32 accumulator; A (X) is K-major, B (W) MN-major; N >> 3, M >> 4
   f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -654,7 +654,7 @@ cudaError_t launch_pairs(const GatedProblem &p, const Prepared &q, unsigned *sta
   const uint32_t fmt = BF16 ? 1u : 0u;
   // f32 accumulator; B (W) is MN-major; N = 256, M = 256
   f.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-  const int clusters = f.num_tiles < 74 ? f.num_tiles : 74;  // a pair of SMs each
+  const int clusters = f.num_tiles < sm_count() / 2 ? f.num_tiles : sm_count() / 2;  // a pair of SMs each
   gated_pair_kernel<BF16><<<2 * clusters, pair::THREADS, pair::SMEM_BYTES, stream>>>(tx, tw, f);
   return cudaGetLastError();
 }
@@ -667,7 +667,7 @@ cudaError_t launch_by_tokens(const GatedProblem &p, const Prepared &q, unsigned 
   // 37.5 and 31.2.  Results stored value by value cost the pairs more, whose threads have a row each: with k up to 2048
   // (4096 of 1025 x 2819: 123 us, 166 by pairs; 1000 of 4097 x 2819: 145 and 133).
   const int64_t pairs = (p.tokens + 255) / 256 * ((p.d_ff + 127) / 128);
-  const bool small = pairs <= 148 / 4 || (!q.wide && p.d_in <= 2048);
+  const bool small = pairs <= sm_count() / 4 || (!q.wide && p.d_in <= 2048);
   return small ? launch_tiles<BF16>(p, q, status, stream) : launch_pairs<BF16>(p, q, status, stream);
 }
 

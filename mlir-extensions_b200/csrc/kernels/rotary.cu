@@ -7,6 +7,7 @@
 // heads.  Bound by memory: what counts is that enough blocks are resident to cover the chain position - angle -
 // barrier - values - store, so a thread holds one item at a time in few registers.
 #include "attention_common.cuh"
+#include "tcgen05_host.h"
 
 namespace imex {
 namespace {
@@ -180,7 +181,7 @@ template <typename T> cudaError_t launch_typed(RotaryArgs &a, const RotaryProble
   a.per_head = a.pairs / n + a.rest / n;
   // the heads of a token are shared out between blocks until there are two blocks per SM
   int64_t splits = 1;
-  while (splits < p.heads && p.tokens * splits < 2 * 148) ++splits;
+  while (splits < p.heads && p.tokens * splits < 2 * tc_host::sm_count()) ++splits;
   a.heads_per_block = static_cast<int>((p.heads + splits - 1) / splits);
   const int64_t gy = (p.heads + a.heads_per_block - 1) / a.heads_per_block;
   // about 256 threads (more only where one head has more items), as few rounds over the heads as that allows, evenly
@@ -192,7 +193,7 @@ template <typename T> cudaError_t launch_typed(RotaryArgs &a, const RotaryProble
   a.lanes = at_once * a.per_head;
   a.tokens_per_block = a.lanes > 256 ? 1 : 256 / a.lanes;
   if (a.tokens_per_block > 16) a.tokens_per_block = 16;
-  while (a.tokens_per_block > 1 && (p.tokens + a.tokens_per_block - 1) / a.tokens_per_block * gy < 4 * 148) --a.tokens_per_block;
+  while (a.tokens_per_block > 1 && (p.tokens + a.tokens_per_block - 1) / a.tokens_per_block * gy < 4 * tc_host::sm_count()) --a.tokens_per_block;
   const int threads = (a.lanes * a.tokens_per_block + 31) / 32 * 32;
   const dim3 grid(static_cast<unsigned>((p.tokens + a.tokens_per_block - 1) / a.tokens_per_block), static_cast<unsigned>(gy));
   if constexpr (sizeof(T) == 2)

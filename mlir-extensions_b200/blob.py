@@ -46,6 +46,12 @@ class KernelDesc:
         return _DESC.pack(self.name.encode(), self.op, self.in_dtype, self.out_dtype,
                           self.epilogue, self.flags, self.sm_margin, *self.dims, *self.fparams)
 
+    def key(self):
+        """Equal for descriptors of the same kernel (where in a blob the payload lies is not part of it)."""
+        dims = self.dims[:1] + (0, 0) + tuple(self.dims[3:]) if self.payload else self.dims
+        return _DESC.pack(self.name.encode(), self.op, self.in_dtype, self.out_dtype, self.epilogue, self.flags,
+                          self.sm_margin, *dims, *self.fparams), bytes(self.payload)
+
 
 def pack_blob(descs):
     """bytes of a blob holding `descs` (list of KernelDesc): header, descriptor table, then

@@ -28,7 +28,7 @@ class Session:
             self._dev = C.c_int32(int(device))
             dev = C.addressof(self._dev)
         self.stream = rt.gpuCreateStream(dev, adopt_stream)
-        self._blobs = []
+        self._kernels = {}
         self._allocs = []
 
     # ---- memory -------------------------------------------------------------
@@ -56,11 +56,14 @@ class Session:
 
     # ---- kernels ------------------------------------------------------------
     def kernel(self, desc):
-        """Module with one descriptor -> kernel handle."""
-        blob = B.Blob([desc])
-        self._blobs.append(blob)  # the module cache is keyed by this address
-        mod = rt.gpuModuleLoad(self.stream, blob.address, blob.size)
-        return rt.gpuKernelGet(self.stream, mod, desc.name.encode())
+        """Module with one descriptor -> kernel handle.  Equal descriptors share one: blobs and modules live to
+        the end of the process, so a program that asks again in every step must not make new ones."""
+        key = desc.key()
+        if key not in self._kernels:
+            blob = B.Blob([desc])  # the module cache is keyed by its address
+            mod = rt.gpuModuleLoad(self.stream, blob.address, blob.size)
+            self._kernels[key] = rt.gpuKernelGet(self.stream, mod, desc.name.encode())
+        return self._kernels[key]
 
     def launch(self, kernel, pointer_args, wait=True, deps=()):
         # grid/block: what the reference's one-work-item-per-element lowering

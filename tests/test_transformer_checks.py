@@ -56,3 +56,20 @@ def test_problems_the_builders_refuse_are_refused_by_the_library(make, patch, me
         assert r.returncode == 0, r.stdout + r.stderr
     else:
         assert r.returncode == -6 and message in r.stdout, r.stdout + r.stderr
+
+
+def test_equal_descriptors_share_a_kernel_handle():
+    """In a session; descriptors that differ in anything have handles of their own."""
+    s = object.__new__(pkg.Session)   # no stream: loading a module needs none
+    s.stream, s._kernels = None, {}
+    attention = lambda **kw: B.attention("a", 1, 2, 2, kw.pop("n_q", 8), 8, 64, **kw)  # noqa: E731
+    desc = attention()
+    first, kept = s.kernel(desc), len(B._KEEP)
+    assert s.kernel(desc) == first and s.kernel(attention()) == first and len(B._KEEP) == kept
+    others = [attention(n_q=9), attention(causal=True), attention(sm_scale=0.5), attention(dtype=B.F16),
+              B.attention_bwd("a", 1, 2, 2, 8, 8, 64), B.gated_ffn("a", 3, 8, 8), B.gated_ffn("a", 4, 8, 8),
+              B.rotary("a", 3, 1, 64, [1.0]), B.rotary("a", 3, 1, 64, [0.5]), B.gemm("a", 8, 8, 8, B.BF16), B.gemm("b", 8, 8, 8, B.BF16)]
+    handles = [s.kernel(d) for d in others]
+    assert len(set(handles + [first])) == len(others) + 1
+    assert [s.kernel(d) for d in others] == handles
+    assert rt.imexKernelWorkspaceBytes(handles[4]) > 0

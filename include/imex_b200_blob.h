@@ -86,7 +86,7 @@ extern "C" {
  *                   (dims[1], dims[2] = its offset and bytes); fparams[0] = sm_scale.
  *                   Key j is visible to query i of batch b when j < key_lens[b]
  *                   (IMEX_FLAG_KEY_LENS: int32[batch], values clamped to [0, n_kv]; all keys
- *                   without) and, with IMEX_FLAG_CAUSAL, j <= i + n_kv - n_q.
+ *                   without) and, with IMEX_FLAG_CAUSAL, j <= i + n_kv - n_q (n_kv, not key_lens[b]).
  *                   S = sm_scale Q K^T, LSE = log sum_visible exp S (f32 [batch, q_heads, n_q]),
  *                   O = exp(S - LSE) V; a row that sees no key gets O = 0, LSE = -inf.
  *                   Query head h reads key head h / (q_heads / kv_heads).

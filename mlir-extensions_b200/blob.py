@@ -205,7 +205,9 @@ def attention(name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype=BF16, sm_
     key_lens (int32 [batch]) when asked for, then the workspace when Session.workspace_bytes says so.
 
     Key j is visible to query i of batch b when j < key_lens[b] and, when causal, j <= i + n_kv - n_q
-    (the last query sees every key).  O = softmax(sm_scale Q K^T) V over the visible keys, LSE = log of
+    (the last query sees every key: the diagonal belongs to n_kv, not to key_lens[b], so that causal with key_lens
+    fits prompts that start at position 0 and single new tokens, not chunks behind caches of different
+    lengths).  O = softmax(sm_scale Q K^T) V over the visible keys, LSE = log of
     the sum of exponentials; a row that sees no key gets O = 0 and LSE = -inf.  Keys and values at and
     behind key_lens[b] may hold anything, NaN included; elsewhere a NaN or infinite score makes the rows that see
     it NaN, LSE included (and under the causal mask a non-finite V of a later key of the same tile reaches earlier
@@ -224,7 +226,7 @@ def attention_bwd(name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype=BF16,
     O, dO, LSE, dQ, dK, dV, then key_lens and the workspace as in `attention`.  Gradients of shared key
     heads are summed over their query heads; masked keys and rows that see no key get zeros.  P and
     dS = P (dO V^T - rowsum(dO O)) are rounded to the element type in between, so with F16 |dS| has to stay
-    below 65504.  The result does not change from run to run (no atomics).  strides also takes "do", "dq", "dk", "dv".
+    below 65504, and what of it is below 2^-14 loses bits (scale the loss).  The result does not change from run to run (no atomics).  strides also takes "do", "dq", "dk", "dv".
     The gradients share no element with Q, K, V, dO or one another."""
     return _attention(OP_ATTENTION_BWD, name, batch, q_heads, kv_heads, n_q, n_kv, d_head, dtype, sm_scale, causal,
                       key_lens, layout, strides)
@@ -255,7 +257,8 @@ def gated_ffn(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, save_gu=False,
 
 def gated_ffn_bwd(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, ldx=0, ldw=0, ldh=0):
     """The gradients of `gated_ffn` for dH.  Pointers X, W, GU (as the forward pass kept it), dH, dX, dW,
-    workspace (Session.workspace_bytes).  dX has X's shape and pitch, dW those of W, dH those of H.  dX
+    workspace (Session.workspace_bytes).  [dG dU] is rounded to the element type in between, so with F16 |dG| and
+    |dU| have to stay below 65504, and what of them is below 2^-14 loses bits (scale the loss).  dX has X's shape and pitch, dW those of W, dH those of H.  dX
     and dW share no element with X, W or one another."""
     return _gated(OP_GATED_FFN_BWD, name, tokens, d_in, d_ff, dtype, act, 0, ldx, ldw, ldh)
 

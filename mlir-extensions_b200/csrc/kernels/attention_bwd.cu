@@ -658,6 +658,8 @@ __device__ __forceinline__ void dkv_tile(const CUtensorMap &tmap_q, const CUtens
         leave_row<DH, (DH < COLS ? DH : COLS)>(dv_tmem + lanes + col, n > 0, L.base + col / DH * (TILE * DH * 4), r, col % DH);
       }
     }
+    // dK and dV may have the place of O, which the row sums' kernel reads: a tile that no query sees gets here at once
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int CT = T::THREADS - 128;
     sums_barrier<CT>(me.shares);
     uint16_t *dv = p.dv + b * p.sdv.batch + kv_head * p.sdv.head + key0 * p.sdv.row;

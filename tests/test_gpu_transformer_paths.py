@@ -368,3 +368,27 @@ def test_attention_with_keys_shared_out(pkg, sess, case):
 @pytest.mark.parametrize("save", [False, True], ids=["", "kept"])
 def test_gated_pairs_of_ctas_walk_several_tiles(pkg, m, d, f, kind, pitch, save):
     Gated(m, d, f, kind, pitch).forward(pkg, save, times=3)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("place", [0, 1, 2], ids=["dq", "dk", "dv"])
+def test_attention_gradients_in_the_place_of_o(pkg, d, place):
+    """Also those of keys that no query sees, whose zeros depend on nothing: they go out when O has been read.  Cold caches
+    before every launch."""
+    t = lambda *shape: torch.randn(shape, device="cuda").to(torch.bfloat16)  # noqa: E731
+    dims = (8, 16, 16, 600, 600, d)
+    q, k, v, kept, do = (t(8, 16, 600, d) for _ in range(5))
+    lse, lens = torch.full((8, 16, 600), 6.0, device="cuda"), torch.tensor([0, 600, 1, 0, 100, 0, 0, 599], dtype=torch.int32, device="cuda")
+    want, o, spoil = [torch.empty_like(q) for _ in range(3)], torch.empty_like(q), torch.empty(64 << 20, device="cuda")
+    got = [o if i == place else torch.empty_like(q) for i in range(3)]
+    with pkg.Session(device=0, adopt_stream=1) as s:
+        kernel = s.kernel(pkg.blob.attention_bwd("b", *dims, key_lens=True))
+        work = torch.empty(s.workspace_bytes(kernel), dtype=torch.uint8, device="cuda")
+        s.launch(kernel, [x.data_ptr() for x in [q, k, v, kept, do, lse] + want + [lens, work]])
+        run = s.bind(kernel, [x.data_ptr() for x in [q, k, v, o, do, lse] + got + [lens, work]])
+        for _ in range(10):
+            o.copy_(kept)
+            spoil.fill_(1.0)
+            run()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        s.wait()

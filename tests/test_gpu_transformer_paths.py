@@ -392,3 +392,180 @@ def test_attention_gradients_in_the_place_of_o(pkg, d, place):
             run()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
         s.wait()
+
+
+# ------------------------------------------------------------------------------------------------ far offsets
+def test_offsets_beyond_32_bits(pkg):
+    """Sequences, rows and tokens more than 2^31 elements apart: the same bits as side by side."""
+    B, step = pkg.blob, 2 ** 30 + 8
+    big = torch.zeros(3 * step + 4096 * 64, dtype=torch.bfloat16, device="cuda")   # 6.5 GB
+    at = lambda offset, shape, strides: torch.as_strided(big, shape, strides, offset)  # noqa: E731
+    new = lambda *shape: torch.randn(shape, device="cuda").to(torch.bfloat16)  # noqa: E731
+    with pkg.Session(device=0, adopt_stream=1) as s:
+        def launch(desc, tensors):
+            kernel = s.kernel(desc)
+            need = s.workspace_bytes(kernel)
+            work = [torch.empty(need, dtype=torch.uint8, device="cuda")] if need else []
+            s.launch(kernel, [t.data_ptr() for t in tensors + work])
+
+        # attention: four sequences of 40 rows of 64, each array in a part of its own of every 2^30
+        dims, far = (4, 2, 2, 40, 40, 64), (step, 40 * 64, 64)
+        near = {n: new(4, 2, 40, 64) for n in ("q", "k", "v", "do")}
+        outs = {n: torch.empty_like(near["q"]) for n in ("o", "dq", "dk", "dv")}
+        lse = torch.empty((4, 2, 40), device="cuda")
+        names = ("q", "k", "v", "o", "do", "dq", "dk", "dv")
+        wide = {n: at(i * 8192, (4, 2, 40, 64), (step, 40 * 64, 64, 1)) for i, n in enumerate(names)}
+        for n, t in near.items():
+            wide[n].copy_(t)
+        strides = {n: far for n in names}
+        both = dict(near, **outs)
+        for t, kw in ((both, {}), (wide, {"strides": strides})):
+            launch(B.attention("a", *dims, causal=True, **kw), [t[n] for n in ("q", "k", "v", "o")] + [lse])
+            launch(B.attention_bwd("b", *dims, causal=True, **kw), [t[n] for n in ("q", "k", "v", "o", "do")] + [lse] + [t[n] for n in ("dq", "dk", "dv")])
+        for n in outs:
+            assert torch.equal(outs[n], wide[n]), n
+        # gated product: X, H and dH with their rows 2^30 apart (dX has X's pitch)
+        m, d, f = 4, 128, 136
+        x, w, dh, gu = new(m, d), new(d, 2 * f), new(m, f), torch.empty((m, 2 * f), dtype=torch.bfloat16, device="cuda")
+        h, dx, dw = torch.empty_like(dh), torch.empty_like(x), torch.empty_like(w)
+        xs, hs, dhs, dxs = (at(i * 8192, (m, c), (step, 1)) for i, c in enumerate((d, f, f, d)))
+        xs.copy_(x), dhs.copy_(dh)
+        dw2, gu2 = torch.empty_like(dw), torch.empty_like(gu)
+        launch(B.gated_ffn("g", m, d, f, save_gu=True), [x, w, h, gu])
+        launch(B.gated_ffn_bwd("gb", m, d, f), [x, w, gu, dh, dx, dw])
+        launch(B.gated_ffn("g", m, d, f, save_gu=True, ldx=step, ldh=step), [xs, w, hs, gu2])
+        launch(B.gated_ffn_bwd("gb", m, d, f, ldx=step, ldh=step), [xs, w, gu, dhs, dxs, dw2])
+        for a, b in ((h, hs), (gu, gu2), (dx, dxs), (dw, dw2)):
+            assert torch.equal(a, b)
+        # rotary: tokens 2^30 apart
+        x, y, pos = new(4, 3, 64), torch.empty((4, 3, 64), dtype=torch.bfloat16, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+        xs, ys = (at(i * 8192, (4, 3, 64), (step, 64, 1)) for i in range(2))
+        xs.copy_(x)
+        freqs = B.rotary_frequencies(64)
+        launch(B.rotary("r", 4, 3, 64, freqs), [x, pos, y])
+        launch(B.rotary("r", 4, 3, 64, freqs, x_strides=(step, 64), y_strides=(step, 64)), [xs, pos, ys])
+        assert torch.equal(y, ys)
+
+
+def test_many_rows_of_one_head_pass_32_bits(pkg):
+    """2^24 + 100 keys of 128: offsets inside one head beyond 2^31 elements, one query, by shares.  All weights are equal but
+    for the last keys', so O is known."""
+    n, d = 2 ** 24 + 100, 128
+    k, v = torch.zeros((1, 1, n, d), dtype=torch.bfloat16, device="cuda"), torch.ones((1, 1, n, d), dtype=torch.bfloat16, device="cuda")
+    q = torch.ones((1, 1, 1, d), dtype=torch.bfloat16, device="cuda")
+    k[0, 0, -3:] = 2.0           # scores 256 / sqrt(128) = 22.6: three keys against 2^24 of weight 1
+    v[0, 0, -3:] = -3.0
+    o, lse = torch.empty_like(q), torch.empty((1, 1, 1), device="cuda")
+    with pkg.Session(device=0, adopt_stream=1) as s:
+        kernel = s.kernel(pkg.blob.attention("a", 1, 1, 1, 1, n, d))
+        work = torch.empty(s.workspace_bytes(kernel), dtype=torch.uint8, device="cuda")
+        s.launch(kernel, [t.data_ptr() for t in (q, k, v, o, lse, work)])
+    heavy = 3 * np.exp(256 / np.sqrt(128.0))
+    total = n - 3 + heavy
+    want = (n - 3 - 3 * heavy) / total
+    # P of the heavy keys is 1 (the reference maximum) and exact; those of the light ones e^-22.6 rounded to bf16, all
+    # the same way: half a step of their share of the sum; then O's own half step
+    assert abs(o.double().cpu() - want).max() <= 2.0 ** -8 * ((n - 3) / total + abs(want)) + 1e-4
+    assert abs(lse.item() - np.log(total)) <= 2e-5 + 1e-6 * np.log(total) + 1e-4
+
+
+# ---------------------------------------------------------------------------------------------- several at once
+def test_sessions_on_several_streams_at_once(pkg):
+    """Three streams with a session, buffers and workspaces each, all operators back to back on each: the results of
+    every stream are those of the calls alone."""
+    B, chains = pkg.blob, []
+    new = lambda *shape: torch.randn(shape, device="cuda").to(torch.bfloat16)  # noqa: E731
+    torch.manual_seed(5)
+    torch.cuda.synchronize()
+    for i, (d, n, heads, kv) in enumerate([(64, 520, 12, 3), (128, 400, 8, 2), (64, 300, 16, 16)]):
+        stream = torch.cuda.Stream()
+        s = pkg.Session(device=0, adopt_stream=stream.cuda_stream)
+        q, do, k, v = new(2, heads, n, d), new(2, heads, n, d), new(2, kv, n, d), new(2, kv, n, d)
+        q1, k1, v1 = new(2, heads, 1, d), new(2, kv, 2500, d), new(2, kv, 2500, d)
+        x, w, dh = new(n, 256), new(256, 2 * 520), new(n, 520)
+        out = {name: torch.empty_like(t) for name, t in dict(o=q, dq=q, dk=k, dv=v, o1=q1, dx=x, dw=w, h=dh, turned=q).items()}
+        out["gu"] = torch.empty((n, 2 * 520), dtype=torch.bfloat16, device="cuda")
+        out["lse"], out["lse1"] = torch.empty((2, heads, n), device="cuda"), torch.empty((2, heads, 1), device="cuda")
+        pos = torch.arange(2 * heads * n, dtype=torch.int32, device="cuda")
+        dims, dims1 = (2, heads, kv, n, n, d), (2, heads, kv, 1, 2500, d)
+        calls = [(B.rotary("r", 2 * heads * n, 1, d, B.rotary_frequencies(d)), [q, pos, out["turned"]]),
+                 (B.attention("a", *dims, causal=True), [q, k, v, out["o"], out["lse"]]),
+                 (B.attention("a1", *dims1), [q1, k1, v1, out["o1"], out["lse1"]]),
+                 (B.gated_ffn("g", n, 256, 520, save_gu=True), [x, w, out["h"], out["gu"]]),
+                 (B.attention_bwd("b", *dims, causal=True), [q, k, v, out["o"], do, out["lse"], out["dq"], out["dk"], out["dv"]]),
+                 (B.gated_ffn_bwd("gb", n, 256, 520), [x, w, out["gu"], dh, out["dx"], out["dw"]])]
+        launches, keep = [], [stream]
+        for desc, args in calls:
+            kernel = s.kernel(desc)
+            need = s.workspace_bytes(kernel)
+            args = args + ([torch.empty(need, dtype=torch.uint8, device="cuda")] if need else [])
+            keep.append(args)
+            launches.append(s.bind(kernel, [t.data_ptr() for t in args]))
+        chains.append((s, launches, out, keep))
+    torch.cuda.synchronize()
+    alone = []
+    for s, launches, out, _ in chains:
+        for run in launches:
+            run()
+        s.wait()
+        alone.append({n: t.clone() for n, t in out.items()})
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for j in range(len(chains[0][1])):
+            for s, launches, _, _ in chains:
+                launches[j]()
+    for (s, _, out, _), want in zip(chains, alone):
+        s.wait()
+        for n in out:
+            assert torch.equal(out[n], want[n]), n
+        s.close()
+
+
+def test_captured_gradients_by_products_and_shares(pkg):
+    """The mixed orders of the gated backward pass and clusters of attention's, captured and replayed on other inputs: the
+    bits of direct launches."""
+    B, stream = pkg.blob, torch.cuda.Stream()
+    with torch.cuda.stream(stream), pkg.Session(device=0, adopt_stream=stream.cuda_stream) as s:
+        new = lambda *shape: torch.randn(shape, device="cuda").to(torch.bfloat16)  # noqa: E731
+        ins, outs, launches, keep = [], [], [], []
+
+        def bind(desc, args):
+            kernel = s.kernel(desc)
+            need = s.workspace_bytes(kernel)
+            keep.append(args + ([torch.empty(need, dtype=torch.uint8, device="cuda")] if need else []))
+            launches.append(s.bind(kernel, [t.data_ptr() for t in keep[-1]]))
+        for m, d, f in ((2048, 4096, 2064), (2305, 1000, 4808), (2400, 2056, 2200), (300, 1000, 2720), (70, 410, 30), (33, 41, 65)):
+            x, w, gu, dh = new(m, d), new(d, 2 * f), new(m, 2 * f), new(m, f)
+            h, kept, dx, dw = torch.empty_like(dh), torch.empty_like(gu), torch.empty_like(x), torch.empty_like(w)
+            bind(B.gated_ffn("g", m, d, f, save_gu=True), [x, w, h, kept])
+            bind(B.gated_ffn_bwd("gb", m, d, f), [x, w, gu, dh, dx, dw])
+            ins += [x, w, gu, dh]
+            outs += [h, kept, dx, dw]
+        for q_heads, kv_heads, n_q, n_kv, d, causal in SHARES:
+            q, do, o = (new(1, n_q, q_heads, d) for _ in range(3))
+            k, v = (new(1, n_kv, kv_heads, d) for _ in range(2))
+            lse = torch.full((1, q_heads, n_q), 5.0, device="cuda")
+            grads = [torch.empty_like(t) for t in (q, k, v)]
+            bind(B.attention_bwd("b", 1, q_heads, kv_heads, n_q, n_kv, d, causal=causal, layout="tokens"), [q, k, v, o, do, lse] + grads)
+            ins += [q, k, v, o, do]
+            outs += grads
+        for run in launches:
+            run()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            for run in launches:
+                run()
+        for t in ins:
+            t.copy_(new(*t.shape))
+        for run in launches:
+            run()
+        stream.synchronize()
+        want = [t.clone() for t in outs]
+        for t in outs:
+            t.zero_()
+        for _ in range(3):
+            graph.replay()
+        stream.synchronize()
+        s.wait()
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(outs, want))

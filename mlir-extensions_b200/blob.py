@@ -258,8 +258,9 @@ def gated_ffn(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, save_gu=False,
 def gated_ffn_bwd(name, tokens, d_in, d_ff, dtype=BF16, act=EPI_SILU, ldx=0, ldw=0, ldh=0):
     """The gradients of `gated_ffn` for dH.  Pointers X, W, GU (as the forward pass kept it), dH, dX, dW,
     workspace (Session.workspace_bytes).  [dG dU] is rounded to the element type in between, so with F16 |dG| and
-    |dU| have to stay below 65504, and what of them is below 2^-14 loses bits (scale the loss).  dX has X's shape and pitch, dW those of W, dH those of H.  dX
-    and dW share no element with X, W or one another."""
+    |dU| have to stay below 65504, and what of them is below 2^-14 loses bits (scale the loss).  relu's slope at
+    0 is 0.  dX has X's shape and pitch, dW those of W, dH those of H.  dX and dW share no element with X, W or one
+    another."""
     return _gated(OP_GATED_FFN_BWD, name, tokens, d_in, d_ff, dtype, act, 0, ldx, ldw, ldh)
 
 

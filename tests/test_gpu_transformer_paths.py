@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from __graft_entry__ import ROOT, load_package
-from test_gpu_transformer_ops import HALF_STEP, SENTINEL, TORCH, Attention, Output, _bits, _dt
+from test_gpu_transformer_ops import HALF_STEP, SENTINEL, TORCH, Attention, Output, _bits, _dt, _launch, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -569,3 +569,21 @@ def test_captured_gradients_by_products_and_shares(pkg):
         stream.synchronize()
         s.wait()
         assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("m,d,f", [(130, 64, 72), (130, 33, 41)])
+def test_the_slope_of_relu_at_zero_is_zero(pkg, sess, m, d, f):
+    x, w = _rand((m, d), "f16", 1), _rand((d, 2 * f), "f16", 2, d ** -0.5)
+    gu, dh = _rand((m, 2 * f), "f16", 3), _rand((m, f), "f16", 4)
+    gu[:, :f][::2] = 0.0
+    gu[:, :f][::4] = -0.0
+    dx, dw = Output(sess, m * d, "f16"), Output(sess, d * 2 * f, "f16")
+    _launch(sess, pkg.blob.gated_ffn_bwd("gb", m, d, f, pkg.blob.F16, pkg.blob.EPI_RELU),
+            [sess.upload(_bits(t)) for t in (x, w, gu, dh)] + [dx.ptr, dw.ptr])
+    g, u = gu[:, :f].double(), gu[:, f:].double()
+    dz = torch.cat([dh.double() * u * (g > 0), dh.double() * g.clamp(min=0)], 1)
+    e = (2.0 ** -11 + 1e-5) * dz.abs() + 2.0 ** -25
+    for got, want, size, terms in ((dx.get((m, d)), dz @ w.double().t(), e @ w.double().abs().t(), dz.abs() @ w.double().abs().t()),
+                                   (dw.get((d, 2 * f)), x.double().t() @ dz, x.double().abs().t() @ e, x.double().abs().t() @ dz.abs())):
+        tol = size + 2.0 ** -11 * want.abs() + 2.0 ** -24 * (max(m, 2 * f) + 8) * terms + 2.0 ** -25
+        assert ((got.double() - want).abs() <= tol * 1.01).all()

@@ -725,7 +725,8 @@ cudaError_t launch_both(const CUtensorMap &tq, const CUtensorMap &tk, const CUte
   attention_delta_kernel<BF16, DH><<<static_cast<unsigned>(chunks * batch * f.q_heads), 128, 0, stream>>>(f);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // may start while the row sums are still computed
+  // May start while the row sums are still computed.  Its first tiles of Q, K, V and dO are loaded before its wait for
+  // them: the row sums' kernel is an ordinary launch, so whatever wrote those was complete before it began.
   e = allow_smem<attention_grads_kernel<BF16, DH>>(Z::SMEM, Registers<DH>::LAUNCH);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
